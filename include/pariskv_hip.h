@@ -50,7 +50,8 @@ int pkv_version(void);
 const char *pkv_last_error(void);
 /* sizeof of the argument structs as this library was compiled, for a binding to
  * compare with its own mirror: 0 pkv_attn_segment, 1 pkv_attn_args,
- * 2 pkv_retrieve_args, 3 pkv_adaptive_args, 5 pkv_prefill_args, 6 pkv_append_args (0 for any other number).
+ * 2 pkv_retrieve_args, 3 pkv_adaptive_args, 5 pkv_prefill_args, 6 pkv_append_args, 7 pkv_path_layer, 8 pkv_path_args,
+ * 9 pkv_tree_args (0 for any other number).
  * No counterpart in the reference. */
 size_t pkv_struct_bytes(int which);
 
@@ -289,6 +290,30 @@ typedef struct pkv_append_args {
 int pkv_append_kv_run(const pkv_append_args *args, const void *k_new, int64_t k_stride_b, int64_t k_stride_h,
                       const void *v_new, int64_t v_stride_b, int64_t v_stride_h, int64_t slot, void *stream);
 
+/* The accepted path of a tree of drafted tokens into the K/V stores of all layers: what n calls of pkv_append_kv a layer would
+ * write (decode_update_kv_cache, cache_hub/polar_cache.py:848-856, a token at a time; drafting has no counterpart in the
+ * reference), in one launch for up to 48 layers.  Row (b, h) of layer l: for i < n, t = path[b*path_stride_b + i]:
+ *   dst_k[b*dst_stride_b + h*dst_stride_h + (slot + i)*row_bytes] = draft_k[b*k_stride_b + h*k_stride_h + t*k_stride_t]
+ * and likewise for V; t outside [0, n_draft): the row (and its norm) stays as it is, so that sequences that accepted fewer
+ * tokens are padded with -1.  vnorm (all layers or none; rows of 128 bf16 or fp32 elements): the value norm as pkv_append_kv
+ * writes it, at [b*vn_stride_b + h*vn_stride_h + slot + i].  Strides of rows in BYTES, multiples of 16; of norms in elements;
+ * path int64 on the device; `layers` is host memory, read before the call returns.  Drafted rows must not overlap the
+ * destination rows. */
+typedef struct pkv_path_layer {
+  const void *draft_k, *draft_v;
+  void *dst_k, *dst_v;
+  float *vnorm;
+  int64_t slot;
+} pkv_path_layer;
+typedef struct pkv_path_args {
+  const int64_t *path;
+  int64_t path_stride_b;
+  int bs, n_kv_heads, n, n_draft, row_bytes;
+  int64_t k_stride_b, k_stride_h, k_stride_t, v_stride_b, v_stride_h, v_stride_t;
+  int64_t dst_stride_b, dst_stride_h, dst_len; /* bytes, bytes, rows */
+  int64_t vn_stride_b, vn_stride_h;
+} pkv_path_args;
+int pkv_append_path(const pkv_path_args *args, const pkv_path_layer *layers, int n_layers, void *stream);
 
 /* The oldest tokens of a layer leave the GPU: replaces the copy_() of staged
  * [bs][h][n][d] tensors into slices of the pinned host tensors on the side
@@ -467,6 +492,37 @@ int pkv_decode_attention(const void *q, int dtype, int bs, int n_kv_heads, int g
                          const int32_t *row_keys, float scale,
                          void *out, void *ws, size_t ws_bytes, void *stream);
 
+/* Attention of a tree of drafted tokens (speculative decoding; no counterpart in the reference, whose decode step takes one token
+ * a sequence): n_draft query tokens per sequence attend to the cached keys and to each other.
+ *   out[b][t][hq] = sum_j softmax_j(scale q[b][t][hq] . k_j) v_j   over the keys j that token t of sequence b sees:
+ *   - of the concatenation of the segments (see pkv_attn_segment; 0 segments: nothing is cached yet) the first
+ *     row_keys[b*n_kv_heads + h] keys, all of them where row_keys is NULL, none where it is <= 0;
+ *   - drafted token u (K and V rows draft_k / draft_v) where mask[b*mask_stride_b + t*mask_stride_t + u] is not zero;
+ *     mask NULL: u <= t (a chain).
+ * A token that sees nothing gets zeros.  What a token does not see does not touch it, infinities and NaN included.
+ * q [bs][n_draft][n_kv_heads*group][128], heads side by side, of `dtype`; out the same, contiguous; q_stride_* and the drafted
+ * rows' strides in elements (rows 128 contiguous elements, 16-byte multiples); mask strides in bytes, 0 allowed.
+ * 1 <= n_draft <= 1024, group >= 1 with n_draft * group <= 8192, fewer than 2^23 cached keys.
+ * fp32 sums and statistics; bf16: probabilities are rounded to bf16 for the product with V.
+ * ws: pkv_tree_attention_ws_bytes(dtype, bs, n_kv_heads, group, n_draft, cached keys) bytes for the partial results (0: none needed). */
+typedef struct pkv_tree_args {
+  const void *q;
+  int dtype, bs, n_kv_heads, group, n_draft;
+  int64_t q_stride_b, q_stride_t;
+  pkv_attn_segment segments[PKV_ATTN_MAX_SEGMENTS];
+  int n_segments;
+  const int32_t *row_keys;  /* or NULL */
+  const void *draft_k, *draft_v;
+  int64_t dk_stride_b, dk_stride_h, dk_stride_t, dv_stride_b, dv_stride_h, dv_stride_t;
+  const uint8_t *mask;      /* or NULL */
+  int64_t mask_stride_b, mask_stride_t;
+  float scale;
+  void *out, *ws;
+  size_t ws_bytes;
+} pkv_tree_args;
+size_t pkv_tree_attention_ws_bytes(int dtype, int bs, int n_kv_heads, int group, int n_draft, int64_t total_keys);
+int pkv_tree_attention(const pkv_tree_args *args, void *stream);
+
 /* ------------------------------------------------- decode glue (model side) */
 
 /* One decode token per sequence between the fused QKV projection and the cache:
@@ -494,6 +550,45 @@ int pkv_add_rmsnorm(const void *x, const void *residual, const void *weight, flo
  * MLP (model_hub/qwen.py:377-381, flashinfer.activation.silu_and_mul there).
  * gate_up bf16 [rows][row_stride >= 2*inter]; out bf16 [rows][inter]. */
 int pkv_silu_mul(const void *gate_up, int64_t row_stride, int rows, int inter, void *out, void *stream);
+
+/* ---------------------------------------------------------- 4-bit weights */
+
+/* Matrices of the model in 4 bits (no counterpart in the reference, whose projections are bf16 GEMMs, model_hub/qwen.py:327-383):
+ * weight[n][k] = scale[n][k/group] * (code[n][k] - zero[n][k/group]), codes and zeros whole numbers 0..15, scales bf16,
+ * group 32, 64 or 128, k a multiple of the group, any n.
+ *
+ * Stored for the matrix instructions that read it (pkv_w4_bytes bytes, 16-byte aligned, no counterpart in the reference):
+ * tiles of 16 rows x 128 columns, padded with zero weights, 1024 bytes each, [n/16][k/128]; of a tile's 64 16-byte vectors vector
+ * j*16 + r (j < 4) holds row r, columns 32 s + 8 j .. +7 in its word s < 4.  Column pair (2 i, 2 i + 1) of those eight has its codes
+ * in bits 3 + 4 i .. 6 + 4 i and 19 + 4 i .. 22 + 4 i (modulo 32), so that a rotation by 4 i, an AND and an OR make them the bf16
+ * numbers 16 + code.  Behind all tiles the groups' words [n/16][k/group][16 rows]: scale in the upper half, 16 + zero as
+ * bf16 in the lower. */
+size_t pkv_w4_bytes(int64_t n, int64_t k, int group);
+
+/* Codes u8 [n][k], scales bf16 [n][k/group], zeros u8 [n][k/group], all contiguous, into that form (no counterpart in the
+ * reference); bits above the lowest four of a code or zero are ignored. */
+int pkv_w4_pack(const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, int64_t n, int64_t k, int group, void *packed,
+                void *stream);
+
+/* Nearest codes of a matrix w [n][k] of `dtype` (row stride in elements; finite values; no counterpart in the reference).  Per
+ * group: lo = min(0, w), hi = max(0, w), scale = bf16((hi - lo) / 15), zero = rint(-lo / scale), code = rint(w / scale) + zero
+ * clamped to 0..15 (a group of zeros, or one whose scale would be below the smallest normal number: scale, zero and codes 0). */
+int pkv_w4_quantize(const void *w, int dtype, int64_t row_stride, int64_t n, int64_t k, int group, uint8_t *codes, uint16_t *scales,
+                    uint8_t *zeros, void *stream);
+
+/* The matrix back from its stored form, fp32 [n][k] contiguous (no counterpart in the reference). */
+int pkv_w4_unpack(const void *packed, int64_t n, int64_t k, int group, float *w, void *stream);
+
+/* y[m][n] = sum_k x[m][k] weight[n][k] + bias[n] (no counterpart in the reference): x bf16 [rows][k] (row stride in elements, a
+ * multiple of 8, 16-byte aligned), bias bf16 [n] or NULL, y [rows][n] contiguous of out_dtype.  Sums in fp32, one rounding. */
+int pkv_w4_linear(const void *x, int64_t x_stride, int64_t rows, const void *packed, int64_t n, int64_t k, int group,
+                  const void *bias, void *y, int out_dtype, void *stream);
+
+/* y[m][j] = silu(x[m] . gate[j]) * (x[m] . up[j]), bf16 [rows][n] contiguous: both projections of the gated feed-forward block,
+ * the activation and the product in one launch (model_hub/qwen.py:365-383 with 4-bit weights).  gate and up: two matrices
+ * [n][k] as stored above, of one group size.  fp32 until the one rounding of y. */
+int pkv_w4_silu_mul(const void *x, int64_t x_stride, int64_t rows, const void *gate, const void *up, int64_t n, int64_t k, int group,
+                    void *y, void *stream);
 
 /* ------------------------------------------------------- fused decode step */
 

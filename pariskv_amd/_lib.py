@@ -42,6 +42,31 @@ class AppendArgs(C.Structure):
                 ("bs", _i), ("n_kv_heads", _i), ("row_bytes", _i), ("vnorm", _vp), ("vn_stride_b", _i64), ("vn_stride_h", _i64)]
 
 
+class PathLayer(C.Structure):
+    """Mirror of ``pkv_path_layer``."""
+
+    _fields_ = [("draft_k", _vp), ("draft_v", _vp), ("dst_k", _vp), ("dst_v", _vp), ("vnorm", _vp), ("slot", _i64)]
+
+
+class PathArgs(C.Structure):
+    """Mirror of ``pkv_path_args``."""
+
+    _fields_ = [("path", _vp), ("path_stride_b", _i64), ("bs", _i), ("n_kv_heads", _i), ("n", _i), ("n_draft", _i), ("row_bytes", _i),
+                ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_t", _i64), ("v_stride_b", _i64), ("v_stride_h", _i64),
+                ("v_stride_t", _i64), ("dst_stride_b", _i64), ("dst_stride_h", _i64), ("dst_len", _i64), ("vn_stride_b", _i64),
+                ("vn_stride_h", _i64)]
+
+
+class TreeArgs(C.Structure):
+    """Mirror of ``pkv_tree_args``."""
+
+    _fields_ = [("q", _vp), ("dtype", _i), ("bs", _i), ("n_kv_heads", _i), ("group", _i), ("n_draft", _i), ("q_stride_b", _i64),
+                ("q_stride_t", _i64), ("segments", AttnSegment * 4), ("n_segments", _i), ("row_keys", _vp), ("draft_k", _vp),
+                ("draft_v", _vp), ("dk_stride_b", _i64), ("dk_stride_h", _i64), ("dk_stride_t", _i64), ("dv_stride_b", _i64),
+                ("dv_stride_h", _i64), ("dv_stride_t", _i64), ("mask", _vp), ("mask_stride_b", _i64), ("mask_stride_t", _i64),
+                ("scale", C.c_float), ("out", _vp), ("ws", _vp), ("ws_bytes", _sz)]
+
+
 class KvAppend(C.Structure):
     """Mirror of ``pkv_kv_append``."""
 
@@ -155,6 +180,15 @@ PROTOTYPES = {
     "pkv_decode_attention_run": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnArgs), _vp]),
     "pkv_decode_attention_counted": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnArgs), _vp, _i, _vp]),
     "pkv_append_kv_run": (_i, [C.POINTER(AppendArgs), _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp]),
+    "pkv_append_path": (_i, [C.POINTER(PathArgs), _vp, _i, _vp]),
+    "pkv_tree_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i64]),
+    "pkv_tree_attention": (_i, [C.POINTER(TreeArgs), _vp]),
+    "pkv_w4_bytes": (_sz, [_i64, _i64, _i]),
+    "pkv_w4_pack": (_i, [_vp, _vp, _vp, _i64, _i64, _i, _vp, _vp]),
+    "pkv_w4_quantize": (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp]),
+    "pkv_w4_unpack": (_i, [_vp, _i64, _i64, _i, _vp, _vp]),
+    "pkv_w4_linear": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i, _vp]),
+    "pkv_w4_silu_mul": (_i, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i, _vp, _vp]),
     "pkv_decode_attention": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnSegment), _i, _vp, C.c_float, _vp, _vp, _sz, _vp]),
     "pkv_qk_norm_rope": (_i, [_vp, _i64, _i, _i, _i, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp]),
     "pkv_add_rmsnorm": (_i, [_vp, _vp, _vp, C.c_float, _i, _i, _vp, _vp, _vp]),
@@ -203,7 +237,7 @@ def lib():
             fn.restype = res
             fn.argtypes = args
         for which, mirror in ((0, AttnSegment), (1, AttnArgs), (2, RetrieveArgs), (3, AdaptiveArgs), (5, PrefillArgs),
-                              (6, AppendArgs)):
+                              (6, AppendArgs), (7, PathLayer), (8, PathArgs), (9, TreeArgs)):
             if os.environ.get("PARISKV_HIP_SO") and handle.pkv_struct_bytes(which) == 0:
                 continue
             if handle.pkv_struct_bytes(which) != C.sizeof(mirror):

@@ -40,50 +40,6 @@ constexpr int kAttKeysPerIter = kAttThreads / 16;  // 16 keys per workgroup step
 constexpr int kWholeSplits = 16, kWholeWorkgroups = 256;
 constexpr int kAttUnroll = 2;                      // keys per 16-lane group per step
 
-struct AttSegs {
-  const void *k[PKV_ATTN_MAX_SEGMENTS];
-  const void *v[PKV_ATTN_MAX_SEGMENTS];
-  int64_t stride_b[PKV_ATTN_MAX_SEGMENTS], stride_h[PKV_ATTN_MAX_SEGMENTS];
-  int64_t row0[PKV_ATTN_MAX_SEGMENTS];
-  int64_t end[PKV_ATTN_MAX_SEGMENTS];  // exclusive end of the segment in the concatenated key order
-  const int64_t *idx[PKV_ATTN_MAX_SEGMENTS];  // per segment: selected rows (relative to row0) or nullptr
-  int64_t idx_stride[PKV_ATTN_MAX_SEGMENTS], idx_limit[PKV_ATTN_MAX_SEGMENTS];
-  int n;
-};
-
-// A field of a segment as a value in scalar registers.  Without this a field picked by a lane's segment number becomes a pick among
-// the fields' addresses, for which the compiler lays the whole argument out in scratch memory: 168 and 264 bytes a lane.  Keys in
-// two tensors, us with that / without: 8 rows x 1600 8.1 / 6.7, 64 x 1600 21.6 / 14.5, 8 x 8000 18.2 / 13.0, fp32 32 x 1600 24.8 / 19.8.
-template <typename T>
-__device__ __forceinline__ T att_field(T v) {
-  asm("" : "+s"(v));
-  return v;
-}
-
-// Row (inside the (b, h) slab of its segment, row0 included) and segment of concatenated key jj, packed as
-// row | segment << 29.  Indexed segments cost one dependent 8-byte load.
-__device__ __forceinline__ uint32_t att_resolve_row(const AttSegs &segs, int row, uint32_t jj) {
-  int s = 0;
-  uint32_t first = 0;
-#pragma unroll
-  for (int t = 1; t < PKV_ATTN_MAX_SEGMENTS; ++t)
-    if (t < segs.n && jj >= (uint32_t)segs.end[t - 1]) s = t, first = (uint32_t)segs.end[t - 1];
-  const int64_t *ip = att_field(segs.idx[0]);
-  int64_t stride = att_field(segs.idx_stride[0]), limit = att_field(segs.idx_limit[0]), row0 = att_field(segs.row0[0]);
-#pragma unroll
-  for (int t = 1; t < PKV_ATTN_MAX_SEGMENTS; ++t) {
-    const int64_t *const ip_t = att_field(segs.idx[t]);
-    const int64_t stride_t = att_field(segs.idx_stride[t]), limit_t = att_field(segs.idx_limit[t]), row0_t = att_field(segs.row0[t]);
-    if (s == t) ip = ip_t, stride = stride_t, limit = limit_t, row0 = row0_t;
-  }
-  int64_t r = jj - first;
-  if (ip) {
-    r = ip[(int64_t)row * stride + r];
-    r = r < 0 ? 0 : (r >= limit ? limit - 1 : r);
-  }
-  return (uint32_t)(r + row0) | ((uint32_t)s << 29);
-}
-
 // Keys row `row` attends to: all `total`, its own row_keys[row], or with uniform > 0 the largest of row_keys[0 .. uniform)
 // (the dense form of the adaptive-k step, where a launch of its own for the maximum took 4.5 us at 24 rows).
 __device__ __forceinline__ int64_t att_row_total(int64_t total, const int32_t *__restrict__ row_keys, int row, int uniform) {
@@ -100,27 +56,6 @@ __device__ __forceinline__ int64_t att_row_total(int64_t total, const int32_t *_
     rk = row_keys[row];
   }
   return rk < total ? (rk > 0 ? rk : 1) : total;
-}
-
-// The addresses of key jj's K and V rows; ROW: bytes of a row.
-template <bool INDEXED, uint32_t ROW>
-__device__ __forceinline__ AttPlace<false> att_place(const AttSegs &a, int row, int b, int h, uint32_t jj) {
-  int s = 0;
-  uint32_t first = 0;
-#pragma unroll
-  for (int t = 1; t < PKV_ATTN_MAX_SEGMENTS; ++t)
-    if (t < a.n && jj >= (uint32_t)a.end[t - 1]) s = t, first = (uint32_t)a.end[t - 1];
-  const char *k = (const char *)att_field(a.k[0]), *v = (const char *)att_field(a.v[0]);
-  int64_t sb = att_field(a.stride_b[0]), sh = att_field(a.stride_h[0]), row0 = att_field(a.row0[0]);
-#pragma unroll
-  for (int t = 1; t < PKV_ATTN_MAX_SEGMENTS; ++t) {
-    const char *const k_t = (const char *)att_field(a.k[t]), *const v_t = (const char *)att_field(a.v[t]);
-    const int64_t sb_t = att_field(a.stride_b[t]), sh_t = att_field(a.stride_h[t]), row0_t = att_field(a.row0[t]);
-    if (s == t) k = k_t, v = v_t, sb = sb_t, sh = sh_t, row0 = row0_t;
-  }
-  const int64_t r = INDEXED ? (int64_t)(att_resolve_row(a, row, jj) & 0x1fffffffu) : row0 + (int64_t)(jj - first);
-  const int64_t off = ((int64_t)b * sb + (int64_t)h * sh) * (ROW / 128) + r * ROW;
-  return {(uint64_t)(k + off), (uint64_t)(v + off)};
 }
 
 // Eight consecutive elements as loaded.  Kept apart from their use so that a load can be issued a whole step before its data is
@@ -471,31 +406,6 @@ int pick_splits_mfma(int rows, int64_t total) {
   return (int)s;
 }
 
-// The segments as offsets into one (b, h) slab: false where they lie in different tensors, more than one is indexed or a
-// row's byte offset would not fit 32 bits (2^24 rows of 256 bytes, 2^23 of 512).
-bool as_one_tensor(const AttSegs &sg, int es, AttOne &one) {
-  memset(&one, 0, sizeof one);
-  one.k = (const char *)sg.k[0], one.v = (const char *)sg.v[0];
-  one.stride_b = sg.stride_b[0] * es, one.stride_h = sg.stride_h[0] * es;
-  for (int i = 0; i < PKV_ATTN_MAX_SEGMENTS; ++i) one.end[i] = 0xffffffffu;
-  int64_t first = 0;
-  for (int i = 0; i < sg.n; ++i) {
-    if (sg.k[i] != sg.k[0] || sg.v[i] != sg.v[0] || sg.stride_b[i] != sg.stride_b[0] || sg.stride_h[i] != sg.stride_h[0])
-      return false;
-    const int64_t n = sg.end[i] - first, rows = sg.row0[i] + (sg.idx[i] ? sg.idx_limit[i] : n);
-    if (rows > ((int64_t)1 << 32) / (128 * es)) return false;
-    one.end[i] = (uint32_t)sg.end[i];
-    one.delta[i] = (int32_t)(sg.row0[i] - first);
-    if (sg.idx[i]) {
-      if (one.idx) return false;
-      one.idx = sg.idx[i], one.idx_stride = sg.idx_stride[i], one.idx_limit = sg.idx_limit[i];
-      one.idx_lo = (uint32_t)first, one.idx_hi = (uint32_t)sg.end[i], one.idx_row0 = (uint32_t)sg.row0[i];
-    }
-    first = sg.end[i];
-  }
-  return true;
-}
-
 }  // namespace
 
 // One CU fetches scattered rows at 35 to 40 GB/s, 2.7 us for 200 of them and as much as the merge's launch: up to six blocks of 32
@@ -517,36 +427,6 @@ extern "C" size_t pkv_decode_attention_ws_bytes(int bs, int n_kv_heads, int grou
   if (bs <= 0 || n_kv_heads <= 0 || group <= 0 || total_keys <= 0) return 256;
   // room for the largest split count either path uses (64), whatever the key count and dtype
   return pkv_align_up((size_t)bs * n_kv_heads * 64 * group * kPartStride * sizeof(float), 256);
-}
-
-// The segments that have rows, checked, one behind the other.
-static int collect_segments(int dtype, const pkv_attn_segment *segments, int n_segments, AttSegs &sg, int64_t &total, bool &indexed) {
-  const int64_t vec = dtype == PKV_DTYPE_BF16 ? 8 : 4;
-  memset(&sg, 0, sizeof sg);
-  total = 0;
-  indexed = false;
-  for (int i = 0; i < n_segments; ++i) {
-    const pkv_attn_segment &s = segments[i];
-    PKV_REQUIRE(s.n_rows >= 0 && s.row0 >= 0, "segment %d: negative extent", i);
-    if (s.n_rows == 0) continue;
-    PKV_REQUIRE(s.k && s.v, "segment %d: null K/V", i);
-    PKV_REQUIRE(pkv_aligned(s.k, 16) && pkv_aligned(s.v, 16) && s.stride_b % vec == 0 && s.stride_h % vec == 0,
-                "segment %d: K/V must be 16-byte aligned with 16-byte-multiple strides", i);
-    sg.k[sg.n] = s.k, sg.v[sg.n] = s.v;
-    sg.stride_b[sg.n] = s.stride_b, sg.stride_h[sg.n] = s.stride_h;
-    sg.row0[sg.n] = s.row0;
-    if (s.idx) {
-      PKV_REQUIRE(pkv_aligned(s.idx, 8) && s.idx_stride >= s.n_rows && s.idx_limit > 0 &&
-                      s.row0 + s.idx_limit < ((int64_t)1 << 29),
-                  "segment %d: indexed rows need idx_stride >= n_rows and 0 < idx_limit (row0 + idx_limit < 2^29)", i);
-      sg.idx[sg.n] = s.idx, sg.idx_stride[sg.n] = s.idx_stride, sg.idx_limit[sg.n] = s.idx_limit;
-      indexed = true;
-    }
-    total += s.n_rows;
-    sg.end[sg.n] = total;
-    ++sg.n;
-  }
-  return PKV_OK;
 }
 
 static int decode_attention(const void *q, int dtype, int bs, int n_kv_heads, int group, const pkv_attn_segment *segments,

@@ -73,13 +73,39 @@ __global__ __launch_bounds__(kGatherThreads) void pkv_gather_packed_kernel(
   (kv ? dst_v : dst_k)[drow * vpr + lane] = val;
 }
 
+// Euclidean norm of a row of 128 elements (VNORM 1 bf16, 2 fp32) whose 16-byte vectors lie in neighbouring lanes: a lane adds the
+// squares of its 16 bytes in order, the lanes of the row meet in a pairwise tree (lane ^ 1, 2, 4, ...), then the square root,
+// rounded to bf16 for bf16 rows (the norm of a bf16 tensor is a bf16 tensor).  Every lane of a row must be here.
+template <int VNORM>
+__device__ __forceinline__ float value_row_norm(pkv_u32x4 val) {
+  const uint32_t w[4] = {val.x, val.y, val.z, val.w};
+  float acc;
+  if (VNORM == 1) {
+    float e[8];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) e[2 * p] = __uint_as_float(w[p] << 16), e[2 * p + 1] = __uint_as_float(w[p] & 0xffff0000u);
+    acc = e[0] * e[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) acc = acc + e[j] * e[j];
+  } else {
+    acc = __uint_as_float(w[0]) * __uint_as_float(w[0]);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) acc = acc + __uint_as_float(w[j]) * __uint_as_float(w[j]);
+  }
+  acc = acc + pkv_lane_xor_f<1>(acc);
+  acc = acc + pkv_lane_xor_f<2>(acc);
+  acc = acc + pkv_lane_xor_f<4>(acc);
+  acc = acc + pkv_lane_xor_f<8>(acc);
+  if (VNORM == 2) acc = acc + pkv_lane_xor_f<16>(acc);
+  const float n = sqrtf(acc);
+  return VNORM == 1 ? pkv_bf16_round(n) : n;
+}
+
 // One new token per sequence: row (b, h) of k_new / v_new goes to row `slot` of
 // the [bs][h][dst_len] K and V stores.  Lane g: (task, lane) = divmod(g, vpr),
 // kv = task & 1, (b, h) = divmod(task >> 1, n_heads).  Strides in 16-byte vectors.
 // VNORM (0 off, 1 bf16 rows, 2 fp32 rows): the value row's Euclidean norm also goes to
-// vnorm[b*vn_stride_b + h*vn_stride_h + slot] as fp32: a lane adds the squares of its 16 bytes in
-// order, the vpr lanes of the row meet in a pairwise tree (lane ^ 1, 2, 4, ...), then the square
-// root, rounded to bf16 for bf16 rows (the norm of a bf16 tensor is a bf16 tensor).
+// vnorm[b*vn_stride_b + h*vn_stride_h + slot] as fp32, see value_row_norm.
 template <int VNORM>
 __global__ __launch_bounds__(kGatherThreads) void pkv_append_rows_kernel(
     const pkv_u32x4 *__restrict__ k_new, const pkv_u32x4 *__restrict__ v_new, int64_t k_stride_b, int64_t k_stride_h,
@@ -94,29 +120,39 @@ __global__ __launch_bounds__(kGatherThreads) void pkv_append_rows_kernel(
   const pkv_u32x4 val = kv ? v_new[b * v_stride_b + h * v_stride_h + lane] : k_new[b * k_stride_b + h * k_stride_h + lane];
   (kv ? dst_v : dst_k)[b * dst_stride_b + h * dst_stride_h + slot * vpr + lane] = val;
   if (VNORM != 0) {  // tasks are whole groups of vpr lanes inside a wave: every lane of a row is here
-    const uint32_t w[4] = {val.x, val.y, val.z, val.w};
-    float acc;
-    if (VNORM == 1) {
-      float e[8];
-#pragma unroll
-      for (int p = 0; p < 4; ++p) e[2 * p] = __uint_as_float(w[p] << 16), e[2 * p + 1] = __uint_as_float(w[p] & 0xffff0000u);
-      acc = e[0] * e[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) acc = acc + e[j] * e[j];
-    } else {
-      acc = __uint_as_float(w[0]) * __uint_as_float(w[0]);
-#pragma unroll
-      for (int j = 1; j < 4; ++j) acc = acc + __uint_as_float(w[j]) * __uint_as_float(w[j]);
-    }
-    acc = acc + pkv_lane_xor_f<1>(acc);
-    acc = acc + pkv_lane_xor_f<2>(acc);
-    acc = acc + pkv_lane_xor_f<4>(acc);
-    acc = acc + pkv_lane_xor_f<8>(acc);
-    if (VNORM == 2) acc = acc + pkv_lane_xor_f<16>(acc);
-    if (kv && lane == 0) {
-      const float n = sqrtf(acc);
-      vnorm[b * vn_stride_b + h * vn_stride_h + slot] = VNORM == 1 ? pkv_bf16_round(n) : n;
-    }
+    const float n = value_row_norm<VNORM>(val);
+    if (kv && lane == 0) vnorm[b * vn_stride_b + h * vn_stride_h + slot] = n;
+  }
+}
+
+// The accepted path of a drafted tree into the K/V rows of up to kPathLayers layers: row (b, h) of layer l gets, at rows
+// slot .. slot + n - 1, the drafted rows path[b][0 .. n-1]; a path entry outside [0, n_draft) leaves its row (and its norm) as it
+// is, so that sequences that accepted fewer tokens are padded.  grid (vectors of a layer / 256, layers); strides in 16-byte
+// vectors.  The norm as above, to the same bits.
+// Moves a few rows of 256 or 512 bytes: bound by its launch, so that all layers take one.
+constexpr int kPathLayers = 48;
+struct PathLayers {
+  pkv_path_layer layer[kPathLayers];
+};
+template <int VNORM>
+__global__ __launch_bounds__(kGatherThreads) void pkv_append_path_kernel(
+    const int64_t *__restrict__ path, int64_t path_stride_b, int n, int n_draft, int n_heads, int n_tasks, int vpr,
+    int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t,
+    int64_t dst_stride_b, int64_t dst_stride_h, int64_t vn_stride_b, int64_t vn_stride_h, PathLayers layers) {
+  const pkv_path_layer &l = layers.layer[blockIdx.y];
+  const int g = blockIdx.x * kGatherThreads + threadIdx.x;
+  const int task = g / vpr, lane = g % vpr;
+  if (task >= n_tasks) return;
+  const int kv = task & 1, i = (task >> 1) % n, bh = (task >> 1) / n;
+  const int b = bh / n_heads, h = bh % n_heads;
+  const int64_t t = path[b * path_stride_b + i];
+  if (t < 0 || t >= n_draft) return;  // uniform over the lanes of a row
+  const pkv_u32x4 val = kv ? ((const pkv_u32x4 *)l.draft_v)[b * v_stride_b + h * v_stride_h + t * v_stride_t + lane]
+                           : ((const pkv_u32x4 *)l.draft_k)[b * k_stride_b + h * k_stride_h + t * k_stride_t + lane];
+  ((pkv_u32x4 *)(kv ? l.dst_v : l.dst_k))[b * dst_stride_b + h * dst_stride_h + (l.slot + i) * vpr + lane] = val;
+  if (VNORM != 0) {
+    const float norm = value_row_norm<VNORM>(val);
+    if (kv && lane == 0) l.vnorm[b * vn_stride_b + h * vn_stride_h + l.slot + i] = norm;
   }
 }
 
@@ -271,6 +307,48 @@ extern "C" int pkv_append_kv_run(const pkv_append_args *a, const void *k_new, in
   return pkv_append_kv(k_new, k_stride_b, k_stride_h, v_new, v_stride_b, v_stride_h, a->dst_k, a->dst_v, a->dst_stride_b,
                        a->dst_stride_h, a->dst_len, slot, a->bs, a->n_kv_heads, a->row_bytes, a->vnorm, a->vn_stride_b,
                        a->vn_stride_h, stream);
+}
+
+extern "C" int pkv_append_path(const pkv_path_args *a, const pkv_path_layer *layers, int n_layers, void *stream) {
+  PKV_REQUIRE(a && layers && a->path, "append_path: null pointer");
+  PKV_REQUIRE(n_layers > 0 && a->bs > 0 && a->n_kv_heads > 0 && a->n > 0 && a->n_draft > 0, "append_path: bad counts");
+  PKV_REQUIRE(a->row_bytes > 0 && a->row_bytes % 16 == 0 && a->row_bytes <= 4096, "row_bytes must be a multiple of 16 (got %d)",
+              a->row_bytes);
+  PKV_REQUIRE((int64_t)a->bs * a->n_kv_heads * a->n * 2 * (a->row_bytes / 16) < ((int64_t)1 << 31), "append_path: too many rows");
+  PKV_REQUIRE(pkv_aligned(a->path, 8) && a->path_stride_b >= (a->bs > 1 ? a->n : 0), "append_path: path must be int64 [bs][n]");
+  const int64_t strides[] = {a->k_stride_b, a->k_stride_h, a->k_stride_t, a->v_stride_b, a->v_stride_h, a->v_stride_t,
+                             a->dst_stride_b, a->dst_stride_h};
+  for (int64_t x : strides) PKV_REQUIRE(x % 16 == 0 && x >= 0, "append_path: strides are bytes, multiples of 16");
+  PKV_REQUIRE(a->dst_len > 0 && a->dst_stride_h >= a->dst_len * a->row_bytes, "append_path: rows must not overlap");
+  const bool norms = layers[0].vnorm != nullptr;
+  PKV_REQUIRE(!norms || ((a->row_bytes == 256 || a->row_bytes == 512) && a->vn_stride_b >= 0 && a->vn_stride_h >= 0),
+              "append_path: value norms need rows of 128 bf16 or fp32 elements");
+  for (int i = 0; i < n_layers; ++i) {
+    const pkv_path_layer &l = layers[i];
+    PKV_REQUIRE(l.draft_k && l.draft_v && l.dst_k && l.dst_v, "append_path: null pointer of layer %d", i);
+    PKV_REQUIRE(pkv_aligned(l.draft_k, 16) && pkv_aligned(l.draft_v, 16) && pkv_aligned(l.dst_k, 16) && pkv_aligned(l.dst_v, 16),
+                "append_path: buffers must be 16-byte aligned");
+    PKV_REQUIRE((l.vnorm != nullptr) == norms, "append_path: all layers keep value norms, or none");
+    PKV_REQUIRE(l.slot >= 0 && l.slot + a->n <= a->dst_len && (!norms || a->vn_stride_h >= l.slot + a->n),
+                "append_path: rows %lld .. of layer %d do not fit %lld", (long long)l.slot, i, (long long)a->dst_len);
+  }
+  const int vpr = a->row_bytes / 16, n_tasks = a->bs * a->n_kv_heads * a->n * 2;
+  for (int at = 0; at < n_layers; at += kPathLayers) {
+    const int count = n_layers - at < kPathLayers ? n_layers - at : kPathLayers;
+    PathLayers part;
+    memset(&part, 0, sizeof part);
+    memcpy(part.layer, layers + at, (size_t)count * sizeof *layers);
+    const dim3 grid((unsigned)(((int64_t)n_tasks * vpr + kGatherThreads - 1) / kGatherThreads), (unsigned)count);
+#define PKV_PATH(VN)                                                                                                         \
+  hipLaunchKernelGGL(pkv_append_path_kernel<VN>, grid, dim3(kGatherThreads), 0, (hipStream_t)stream, a->path,                \
+                     a->path_stride_b, a->n, a->n_draft, a->n_kv_heads, n_tasks, vpr, a->k_stride_b / 16, a->k_stride_h / 16, \
+                     a->k_stride_t / 16, a->v_stride_b / 16, a->v_stride_h / 16, a->v_stride_t / 16, a->dst_stride_b / 16,   \
+                     a->dst_stride_h / 16, a->vn_stride_b, a->vn_stride_h, part)
+    if (!norms) PKV_PATH(0); else if (a->row_bytes == 256) PKV_PATH(1); else PKV_PATH(2);
+#undef PKV_PATH
+    PKV_LAUNCH_CHECK("pkv_append_path_kernel");
+  }
+  return PKV_OK;
 }
 
 extern "C" int pkv_offload_rows(const void *src_k, const void *src_v, int64_t src_stride_b, int64_t src_stride_h,

@@ -32,6 +32,9 @@ extern "C" size_t pkv_struct_bytes(int which) {
     case 3: return sizeof(pkv_adaptive_args);
     case 5: return sizeof(pkv_prefill_args);
     case 6: return sizeof(pkv_append_args);
+    case 7: return sizeof(pkv_path_layer);
+    case 8: return sizeof(pkv_path_args);
+    case 9: return sizeof(pkv_tree_args);
     default: return 0;
   }
 }

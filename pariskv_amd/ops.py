@@ -597,6 +597,86 @@ def append_kv(key_states, value_states, dst_k, dst_v, slot: int, vnorm: Optional
         _p(vnorm), vn_b, vn_h, _stream(dst_k)))
 
 
+class PathAppend:
+    """The accepted path of a tree of drafted tokens into the K/V rows of all layers, one launch for up to 48 of them: what a
+    layer's :class:`BoundAppend` writes a token at a time.  ``dst_k`` / ``dst_v``: a layer's [bs,Hkv,rows,D] each, contiguous
+    rows, all of one shape and layout; ``vnorms``: each layer's fp32 [bs,Hkv,rows'] norms (contiguous), or None."""
+
+    def __init__(self, dst_k: Sequence[torch.Tensor], dst_v: Sequence[torch.Tensor], vnorms: Optional[Sequence[torch.Tensor]] = None):
+        import numpy as np
+
+        dst_k, dst_v = list(dst_k), list(dst_v)
+        _need(len(dst_k) == len(dst_v) > 0 and (vnorms is None or len(vnorms) == len(dst_k)), "one K, one V (and one norm) tensor a layer")
+        _cuda(*dst_k, *dst_v)
+        _one_device(dst_k[0], *dst_k, *dst_v, *(vnorms or ()))
+        k0 = dst_k[0]
+        _need(k0.dim() == 4, "dst_k, dst_v: [bs,Hkv,rows,D]")
+        bs, H, rows, D = k0.shape
+        for t in dst_k + dst_v:
+            _need(t.dtype == k0.dtype and t.shape == k0.shape and t.stride() == k0.stride() and t.stride(3) == 1 and t.stride(2) == D,
+                  "dst_k, dst_v: [bs,Hkv,rows,D] of one type, shape and layout, with contiguous rows")
+        es = k0.element_size()
+        self._a = _lib.PathArgs()
+        self._a.bs, self._a.n_kv_heads, self._a.row_bytes = bs, H, D * es
+        self._a.dst_stride_b, self._a.dst_stride_h, self._a.dst_len = k0.stride(0) * es, k0.stride(1) * es, rows
+        if vnorms is not None:
+            vnorms = list(vnorms)
+            for t in vnorms:
+                _need(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.shape == vnorms[0].shape and
+                      tuple(t.shape[:2]) == (bs, H), "vnorms: contiguous fp32 [bs,Hkv,rows] a layer")
+            self._a.vn_stride_b, self._a.vn_stride_h = vnorms[0].stride()[:2]
+        self._np = np
+        self._layers = np.zeros(len(dst_k), dtype=[(f, np.int64) for f, _ in _lib.PathLayer._fields_])
+        self._layers["dst_k"], self._layers["dst_v"] = [t.data_ptr() for t in dst_k], [t.data_ptr() for t in dst_v]
+        if vnorms is not None:
+            self._layers["vnorm"] = [t.data_ptr() for t in vnorms]
+        self.keep = (dst_k, dst_v, vnorms)
+        self._like = k0
+
+    def _rows_of(self, draft):
+        """(addresses of the layers' drafted rows, shape [bs,T,Hkv,D], strides) of a stacked tensor or one tensor a layer."""
+        n = len(self._layers)
+        if isinstance(draft, torch.Tensor):
+            _need(draft.dim() == 5 and draft.shape[0] == n, "drafted rows: [layers,bs,T,Hkv,D], or one [bs,T,Hkv,D] a layer")
+            first, shape, strides = draft, tuple(draft.shape[1:]), draft.stride()[1:]
+            at = draft.data_ptr() + self._np.arange(n, dtype=self._np.int64) * (draft.stride(0) * draft.element_size())
+        else:
+            _need(len(draft) == n, "drafted rows: one [bs,T,Hkv,D] a layer")
+            first = draft[0]
+            shape, strides = tuple(first.shape), first.stride()
+            for t in draft:
+                _need(tuple(t.shape) == shape and t.stride() == strides and t.dtype == first.dtype, "drafted rows: one shape, layout and type")
+            _cuda(*draft)
+            _one_device(self._like, *draft)
+            at = [t.data_ptr() for t in draft]
+        like = self._like
+        _need(first.is_cuda and first.dtype == like.dtype and len(shape) == 4 and shape[0] == like.shape[0] and shape[2] == like.shape[1] and
+              shape[3] == like.shape[3] and strides[3] == 1, "drafted rows: [bs,T,Hkv,D] of the cache's type with contiguous rows")
+        _one_device(like, first)
+        return at, shape, strides
+
+    def launch(self, draft_k, draft_v, path: torch.Tensor, slots) -> None:
+        """draft_k, draft_v: the drafted rows, [layers,bs,T,Hkv,D] or a sequence of [bs,T,Hkv,D]; path int64 [bs,n] on the GPU: the
+        accepted tokens of each sequence in order, -1 where it accepted fewer (such a row stays as it is); slots: the cache row of the
+        path's first token, one int or one a layer."""
+        layers, a = self._layers.copy(), _lib.PathArgs.from_buffer_copy(self._a)
+        layers["draft_k"], shape, ks = self._rows_of(draft_k)
+        layers["draft_v"], v_shape, vs = self._rows_of(draft_v)
+        layers["slot"] = slots
+        _need(v_shape == shape, "drafted K and V rows differ in shape")
+        _cuda(path)
+        _one_device(self._like, path)
+        _need(path.dtype == torch.int64 and path.dim() == 2 and path.shape[0] == shape[0] and (path.shape[1] == 0 or path.stride(1) == 1),
+              "path: int64 [bs,n]")
+        if path.shape[1] == 0 or shape[0] == 0:
+            return
+        es = self._like.element_size()
+        a.path, a.path_stride_b, a.n, a.n_draft = path.data_ptr(), path.stride(0), path.shape[1], shape[1]
+        a.k_stride_b, a.k_stride_t, a.k_stride_h = (x * es for x in ks[:3])
+        a.v_stride_b, a.v_stride_t, a.v_stride_h = (x * es for x in vs[:3])
+        _lib.check(_lib.lib().pkv_append_path(C.byref(a), layers.ctypes.data, len(layers), _stream(self._like)))
+
+
 OFFLOAD_ONE_COMMAND = 1
 
 
@@ -643,6 +723,34 @@ def gather_uva_packed(src_k, src_v, k_packed, v_packed, indices_packed, cu_seqle
 # --------------------------------------------------------- decode attention
 
 
+def _fill_segments(segs, segments, bs: int, H: int, dtype: torch.dtype, least: int) -> int:
+    """Validate the rows an attention reads and fill the C segment array ``segs``; returns how many there are."""
+    _need(least <= len(segments) <= 4, f"{least}..4 key segments")
+    total = 0
+    for i, seg in enumerate(segments):
+        k, v, row0, n_rows = seg[:4]
+        idx = seg[4] if len(seg) > 4 else None
+        _cuda(k, v)
+        _need(k.dtype == dtype and v.dtype == dtype, "q, k, v must share a dtype")
+        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.shape[3] == HEAD_DIM and
+              k.stride(3) == 1 and k.stride(2) == HEAD_DIM and tuple(k.shape[:2]) == (bs, H),
+              "k, v: [bs,Hkv,rows,128] with contiguous rows")
+        segs[i].k, segs[i].v = _p(k), _p(v)
+        segs[i].stride_b, segs[i].stride_h = k.stride(0), k.stride(1)
+        segs[i].row0, segs[i].n_rows = row0, n_rows
+        total += n_rows
+        if idx is None:
+            _need(0 <= row0 and row0 + n_rows <= k.shape[2], "segment rows out of range")
+            segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = None, 0, 0
+        else:  # the segment's rows are row0 + idx[b, h, :n_rows], read where they lie
+            _cuda(idx)
+            _need(idx.dtype == torch.int64 and idx.is_contiguous() and idx.dim() == 3 and
+                  tuple(idx.shape[:2]) == (bs, H) and idx.shape[2] >= n_rows and 0 <= row0 < k.shape[2],
+                  "segment indices: contiguous int64 [bs,Hkv,>=n_rows]")
+            segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = _p(idx), idx.shape[2], k.shape[2] - row0
+    return total
+
+
 class DecodeAttention:
     """softmax(q k^T * scale) v for one query token per sequence over up to four row segments of
     [bs, Hkv, rows, 128] K/V tensors, read in place (cache_hub/polar_cache.py:1084-1105)."""
@@ -676,27 +784,7 @@ class DecodeAttention:
         """Validate and fill the C segment array `segs`; returns (segs, out, scale)."""
         _cuda(q)
         _need(q.shape[-1] == HEAD_DIM and q.numel() == self.bs * self.H * self.G * HEAD_DIM, "queries: [bs,1,Hq,128]")
-        _need(1 <= len(segments) <= 4, "1..4 key segments")
-        for i, seg in enumerate(segments):
-            k, v, row0, n_rows = seg[:4]
-            idx = seg[4] if len(seg) > 4 else None
-            _cuda(k, v)
-            _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v must share a dtype")
-            _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.shape[3] == HEAD_DIM and
-                  k.stride(3) == 1 and k.stride(2) == HEAD_DIM and tuple(k.shape[:2]) == (self.bs, self.H),
-                  "k, v: [bs,Hkv,rows,128] with contiguous rows")
-            segs[i].k, segs[i].v = _p(k), _p(v)
-            segs[i].stride_b, segs[i].stride_h = k.stride(0), k.stride(1)
-            segs[i].row0, segs[i].n_rows = row0, n_rows
-            if idx is None:
-                _need(0 <= row0 and row0 + n_rows <= k.shape[2], "segment rows out of range")
-                segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = None, 0, 0
-            else:  # the segment's rows are row0 + idx[b, h, :n_rows], read where they lie
-                _cuda(idx)
-                _need(idx.dtype == torch.int64 and idx.is_contiguous() and idx.dim() == 3 and
-                      tuple(idx.shape[:2]) == (self.bs, self.H) and idx.shape[2] >= n_rows and 0 <= row0 < k.shape[2],
-                      "segment indices: contiguous int64 [bs,Hkv,>=n_rows]")
-                segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = _p(idx), idx.shape[2], k.shape[2] - row0
+        _fill_segments(segs, segments, self.bs, self.H, q.dtype, 1)
         if out is None:
             out = torch.empty_like(q)
         if scale is None:
@@ -714,6 +802,86 @@ class DecodeAttention:
         a.n_segments, a.row_keys, a.scale = len(segments), _p(row_keys), float(scale)
         a.out, a.ws, a.ws_bytes = _p(out), _p(self.ws), self.ws.numel()
         return a, out
+
+
+def tree_mask(parents) -> torch.Tensor:
+    """Which drafted tokens each token of a tree sees: itself and the tokens it descends from.  ``parents`` int64 [T] or [bs,T]
+    (tensor or list): the token before each one, -1 for tokens that follow the cached ones; a parent comes before its children.
+    Returns bool [T,T] or [bs,T,T] (row t: what t sees) on the device of ``parents``."""
+    p = torch.as_tensor(parents, dtype=torch.int64)
+    T = p.shape[-1]
+    at = torch.arange(T, device=p.device)
+    if p.device.type == "cpu":
+        _need(bool(((p < at) & (p >= -1)).all()), "parents: -1 or the number of an earlier token")
+    m = p.unsqueeze(-1) == at
+    steps = 1
+    while steps < T:  # ancestors up to `steps` away -> up to twice as far
+        m = m | (m.to(torch.float32) @ m.to(torch.float32) > 0)
+        steps *= 2
+    return m | (at.unsqueeze(-1) == at)
+
+
+class TreeAttention:
+    """Attention of the drafted tokens of a tree (speculative decoding) over the cached rows and over each other: :class:`DecodeAttention`
+    for several query tokens a sequence.  Partial results are allocated with every call, so that calls on several
+    streams, or of several captured graphs, do not share any."""
+
+    def __init__(self, bs: int, n_kv_heads: int, group: int, max_draft: int, max_keys: int, device):
+        _need(bs > 0 and n_kv_heads > 0 and group > 0 and 1 <= max_draft <= 1024 and max_draft * group <= 8192,
+              "1..1024 drafted tokens, at most 8192 query rows a KV head")
+        self.bs, self.H, self.G, self.max_draft, self.max_keys = bs, n_kv_heads, group, max_draft, max_keys
+        self.device = torch.device(device)
+
+    def run(self, queries: torch.Tensor, segments, draft_k: torch.Tensor, draft_v: torch.Tensor, mask: Optional[torch.Tensor] = None,
+            scale: Optional[float] = None, out: Optional[torch.Tensor] = None, row_keys: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """queries [bs,T,Hq,128]; segments: the cached rows as :meth:`DecodeAttention.run` takes them (an empty list: none yet);
+        draft_k, draft_v [bs,T,Hkv,128]: the drafted tokens' own rows; mask bool [T,T] or [bs,T,T]: row t holds what token t sees of the
+        draft (see :func:`tree_mask`; None: itself and the tokens before it); row_keys int32 [bs,Hkv]: how many of the cached keys,
+        in their concatenated order, a row sees (0 or less: none).  Returns [bs,T,Hq,128]; a token that sees nothing gets zeros, and
+        what a token does not see does not touch it, whatever it holds."""
+        bs, H, G = self.bs, self.H, self.G
+        _need(queries.dim() == 4 and queries.shape[0] == bs and queries.shape[2:] == (H * G, HEAD_DIM) and
+              1 <= queries.shape[1] <= self.max_draft, "queries: [bs,T,Hq,128], 1 <= T <= max_draft")
+        T, dt = queries.shape[1], queries.dtype
+        _need(tuple(draft_k.shape) == (bs, T, H, HEAD_DIM) and draft_v.shape == draft_k.shape and draft_k.dtype == dt and
+              draft_v.dtype == dt, "draft_k, draft_v: [bs,T,Hkv,128] of the queries' type")
+        _cuda(queries, draft_k, draft_v, mask, row_keys, out)
+        _one_device(queries, draft_k, draft_v, mask, row_keys, out, *(t for seg in segments for t in (seg[0], seg[1], *seg[4:])))
+        vec = 16 // queries.element_size()
+
+        def rows(t, heads_apart):  # 16-byte aligned rows, or a copy
+            if t.stride(3) != 1 or t.data_ptr() % 16 or any(x % vec for x in t.stride()[:3]) or (heads_apart and t.stride(2) != HEAD_DIM):
+                t = t.clone(memory_format=torch.contiguous_format)
+            return t
+
+        q, dk, dv = rows(queries, True), rows(draft_k, False), rows(draft_v, False)
+        a = _lib.TreeArgs()
+        a.q, a.dtype, a.bs, a.n_kv_heads, a.group, a.n_draft = q.data_ptr(), _dt(dt), bs, H, G, T
+        a.q_stride_b, a.q_stride_t = q.stride()[:2]
+        a.draft_k, a.draft_v = dk.data_ptr(), dv.data_ptr()
+        a.dk_stride_b, a.dk_stride_t, a.dk_stride_h = dk.stride()[:3]
+        a.dv_stride_b, a.dv_stride_t, a.dv_stride_h = dv.stride()[:3]
+        total = _fill_segments(a.segments, segments, bs, H, dt, 0)
+        _need(total <= self.max_keys, "more cached keys than max_keys")
+        a.n_segments = len(segments)
+        if mask is not None:
+            _need(mask.dtype == torch.bool and tuple(mask.shape) in ((T, T), (bs, T, T)), "mask: bool [T,T] or [bs,T,T]")
+            if mask.stride(-1) != 1:
+                mask = mask.contiguous()
+            a.mask, a.mask_stride_b, a.mask_stride_t = mask.data_ptr(), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2)
+        if row_keys is not None:
+            _need(row_keys.dtype == torch.int32 and row_keys.is_contiguous() and row_keys.numel() == bs * H, "row_keys: contiguous int32 [bs,Hkv]")
+            a.row_keys = row_keys.data_ptr()
+        if out is None:
+            out = torch.empty(bs, T, H * G, HEAD_DIM, dtype=dt, device=queries.device)
+        _need(tuple(out.shape) == (bs, T, H * G, HEAD_DIM) and out.dtype == dt and out.is_contiguous(), "out: contiguous, like queries")
+        a.scale, a.out = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale), out.data_ptr()
+        lib = _lib.lib()
+        a.ws_bytes = lib.pkv_tree_attention_ws_bytes(a.dtype, bs, H, G, T, total)
+        ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=queries.device) if a.ws_bytes else None
+        a.ws = _p(ws)
+        _lib.check(lib.pkv_tree_attention(C.byref(a), _stream(queries)))
+        return out
 
 
 def qk_norm_rope(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, q_weight, k_weight, eps: float,
@@ -785,6 +953,106 @@ def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
     out = torch.empty(*gate_up.shape[:-1], inter, dtype=gate_up.dtype, device=gate_up.device)
     _lib.check(_lib.lib().pkv_silu_mul(_p(gate_up), width, rows, inter, _p(out), _stream(gate_up)))
     return out
+
+
+class W4Weight:
+    """A matrix [n,k] in 4 bits, laid out once for the kernels that read it: weight = scale * (code - zero) with whole codes and zeros
+    0..15 and a bf16 scale and a zero for every ``group_size`` (32, 64 or 128) columns of a row; k a multiple of that, any n."""
+
+    __slots__ = ("packed", "n", "k", "group_size")
+
+    def __init__(self, packed: torch.Tensor, n: int, k: int, group_size: int):
+        _need(packed.dtype == torch.uint8 and packed.is_cuda and packed.is_contiguous() and
+              packed.numel() == _lib.lib().pkv_w4_bytes(n, k, group_size) > 0, "packed: what from_codes or quantize laid out")
+        self.packed, self.n, self.k, self.group_size = packed, int(n), int(k), int(group_size)
+
+    @property
+    def shape(self):
+        return (self.n, self.k)
+
+    @property
+    def device(self):
+        return self.packed.device
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor) -> "W4Weight":
+        """codes u8 [n,k], scales bf16 [n,k/g], zeros u8 [n,k/g] (0..15; higher bits are ignored): a quantized checkpoint's."""
+        _need(codes.dim() == 2 and scales.dim() == 2 and zeros.shape == scales.shape and codes.shape[0] == scales.shape[0] and
+              scales.shape[1] > 0 and codes.shape[1] % scales.shape[1] == 0, "codes [n,k], scales and zeros [n,k/g]")
+        _need(codes.dtype == torch.uint8 and scales.dtype == torch.bfloat16 and zeros.dtype == torch.uint8, "codes u8, scales bf16, zeros u8")
+        _cuda(codes, scales, zeros)
+        _one_device(codes, scales, zeros)
+        (n, k), g = codes.shape, codes.shape[1] // scales.shape[1]
+        nbytes = _lib.lib().pkv_w4_bytes(n, k, g)
+        _need(nbytes > 0, f"groups of 32, 64 or 128 columns, n >= 1 (got n={n} k={k} group={g})")
+        packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+        codes, scales, zeros = codes.contiguous(), scales.contiguous(), zeros.contiguous()
+        _lib.check(_lib.lib().pkv_w4_pack(_p(codes), _p(scales), _p(zeros), n, k, g, _p(packed), _stream(codes)))
+        return cls(packed, n, k, g)
+
+    @classmethod
+    def quantize(cls, weight: torch.Tensor, group_size: int = 128) -> "W4Weight":
+        """Nearest codes of a finite matrix [n,k] (bf16 or fp32), see :func:`w4_quantize`."""
+        return cls.from_codes(*w4_quantize(weight, group_size))
+
+    def dequantize(self) -> torch.Tensor:
+        """fp32 [n,k]."""
+        w = torch.empty(self.n, self.k, dtype=torch.float32, device=self.device)
+        _lib.check(_lib.lib().pkv_w4_unpack(_p(self.packed), self.n, self.k, self.group_size, _p(w), _stream(w)))
+        return w
+
+
+def w4_quantize(weight: torch.Tensor, group_size: int = 128):
+    """(codes u8 [n,k], scales bf16 [n,k/g], zeros u8 [n,k/g]) of a finite matrix [n,k], bf16 or fp32.  Per group, with lo = min(0, w)
+    and hi = max(0, w): scale = bf16((hi - lo) / 15), zero = rint(-lo / scale), code = rint(w / scale) + zero within 0..15."""
+    _cuda(weight)
+    _need(weight.dim() == 2 and weight.numel() > 0, "weight: [n,k]")
+    n, k = weight.shape
+    _need(group_size in (32, 64, 128) and k % group_size == 0, "groups of 32, 64 or 128 columns that divide k")
+    if weight.stride(1) != 1 or weight.stride(0) < k:
+        weight = weight.contiguous()
+    codes = torch.empty(n, k, dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(n, k // group_size, dtype=torch.bfloat16, device=weight.device)
+    zeros = torch.empty(n, k // group_size, dtype=torch.uint8, device=weight.device)
+    _lib.check(_lib.lib().pkv_w4_quantize(_p(weight), _dt(weight.dtype), weight.stride(0), n, k, group_size, _p(codes), _p(scales),
+                                          _p(zeros), _stream(weight)))
+    return codes, scales, zeros
+
+
+def _w4_rows(x: torch.Tensor, k: int):
+    """x [..., k] as rows that the kernels can read: 16-byte aligned, a multiple of 8 elements apart."""
+    _need(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] == k, f"x: bf16 [..., {k}] on the GPU")
+    x = x if x.dim() == 2 else x.reshape(-1, k)
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x [..., k] (bf16) times the transpose of a 4-bit matrix, plus ``bias`` (bf16 [n]): [..., n] in ``out_dtype`` (bf16, the default,
+    or fp32).  fp32 sums, one rounding; for the few rows of a decode step or of its drafted tokens."""
+    rows = _w4_rows(x, weight.k)
+    _one_device(rows, weight.packed, bias)
+    _need(bias is None or (bias.is_cuda and bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == weight.n), "bias: contiguous bf16 [n]")
+    y = torch.empty(*x.shape[:-1], weight.n, dtype=out_dtype or torch.bfloat16, device=x.device)
+    dt = _dt(y.dtype)
+    if rows.shape[0] > 0:
+        _lib.check(_lib.lib().pkv_w4_linear(_p(rows), rows.stride(0), rows.shape[0], _p(weight.packed), weight.n, weight.k,
+                                            weight.group_size, _p(bias), _p(y), dt, _stream(rows)))
+    return y
+
+
+def w4_silu_mul(x: torch.Tensor, gate: W4Weight, up: W4Weight) -> torch.Tensor:
+    """silu(x gate^T) * (x up^T), bf16 [..., n]: both projections of the gated feed-forward block, the activation and the product in one
+    launch (model_hub/qwen.py:365-383 with 4-bit weights); nothing is rounded in between, unlike :func:`silu_mul` of a bf16 product."""
+    rows = _w4_rows(x, gate.k)
+    _one_device(rows, gate.packed, up.packed)
+    _need(gate.shape == up.shape and gate.group_size == up.group_size, "gate and up: matrices of one shape and group size")
+    y = torch.empty(*x.shape[:-1], gate.n, dtype=torch.bfloat16, device=x.device)
+    if rows.shape[0] > 0:
+        _lib.check(_lib.lib().pkv_w4_silu_mul(_p(rows), rows.stride(0), rows.shape[0], _p(gate.packed), _p(up.packed), gate.n, gate.k,
+                                              gate.group_size, _p(y), _stream(rows)))
+    return y
 
 
 def alloc_pinned(shape, dtype: torch.dtype, zero: bool = False) -> torch.Tensor:
