@@ -182,7 +182,7 @@ PROTOTYPES = {
     "pkv_append_kv_run": (_i, [C.POINTER(AppendArgs), _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp]),
     "pkv_append_path": (_i, [C.POINTER(PathArgs), _vp, _i, _vp]),
     "pkv_tree_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i64]),
-    "pkv_tree_attention": (_i, [C.POINTER(TreeArgs), _vp]),
+    "pkv_tree_attention": (_i, [_vp, _vp]),
     "pkv_w4_bytes": (_sz, [_i64, _i64, _i]),
     "pkv_w4_pack": (_i, [_vp, _vp, _vp, _i64, _i64, _i, _vp, _vp]),
     "pkv_w4_quantize": (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp]),

@@ -2,31 +2,28 @@
 // decoding.  (No counterpart in the reference, whose decode step takes one token a sequence.)
 //
 // A KV head's T * G query rows (T drafted tokens, G query heads) share its keys, so K and V (2 * 128 elements a key) are read once for
-// all of them: up to some 64 rows the bytes bound it, beyond 256 the matrix instructions.  Rows go to the matrix cores 16 at
-// a time, a wave holds NT such tiles; the four waves of a workgroup take keys in turns of their own and merge through LDS; the key axis is
-// split over workgroups, whose partial results a second launch joins.  Nothing but the merge goes through LDS:
+// all of them: up to some 64 rows the bytes bound it, beyond 256 the instructions of the softmax and the matrix products.  Rows go to the
+// matrix cores 16 at a time; the key axis is split over waves and workgroups, whose partial results a second launch joins.
 //   scores   S^T[key][row] = K[key][dim] . Q^T[dim][row]: lane (n, j) receives the scores of row n for four keys 4j .. 4j+3 of a
 //            tile of 16 ...
-//   output   O[row][dim] += P[row][key] . V[key][dim]: ... which is where this product wants the probabilities.
-//            Columns n of instruction m are the dims 8n + m, so that rows of V are read whole.
-// bf16: v_mfma_f32_16x16x32_bf16, 32 keys a step (see pkv_attn.h, whose one-token step this is for many rows); the probabilities
-//       are rounded to bf16 for the second product, half a step of their own type each, and summed unrounded.
+//   output   O[row][dim] += P[row][key] . V[key][dim]: ... which is where this product wants the weights: nothing is moved.
+// bf16: v_mfma_f32_16x16x32_bf16, 32 keys a step; the weights are rounded to bf16 for the second product (half a step of 2^-8 each) and
+//       the normaliser is the sum of the same rounded weights, from one more product with ones.
 // fp32: v_mfma_f32_16x16x4_f32, 16 keys a step; no rounding.
-// Softmax over all keys a row sees in one pass with the running maximum and sum, fp32.
+// Softmax over all keys a row sees in one pass with a running base and sum, fp32.
 #include "pkv_attn.h"
 
 #pragma clang fp contract(fast)
 
 namespace {
 
-constexpr int kTreeWaves = 4, kTreeMaxSplits = 64;
+constexpr int kTreeWaves = 4, kWideWaves = 8, kTreeMaxSplits = 64, kTreeWorkgroups = 256;
 
 struct TreeCall {
   const void *q;
   int64_t q_stride_b, q_stride_t;  // elements
   int n_kv_heads, group, n_draft;
   uint32_t total;                  // cached keys
-  uint32_t per_split;              // a multiple of what the waves take in one step
   const int32_t *row_keys;
   const char *dk, *dv;
   int64_t dk_b, dk_h, dk_t, dv_b, dv_h, dv_t;  // bytes
@@ -35,7 +32,21 @@ struct TreeCall {
   float scale_log2e;
   float *ws_o, *ws_ml;  // [row of (b, h)][split][query row][128], [..][2]
   void *out;
+  int n_splits, row_tiles, n_pairs;  // (b, h) times splits
 };
+
+// A workgroup's part: a split of the keys of one (b, h), and a tile of its query rows.  Workgroups go to the eight dies in turn, and the tiles of
+// one split read the same keys: they are eight numbers apart, so that a die's L2 reads the keys once for all.  us, 256 query rows (four tiles),
+// tiles side by side / on one die: see pkv_tree_wide_kernel.
+struct TreePart {
+  int bh, split, tile;
+  bool any;
+};
+__device__ __forceinline__ TreePart tree_part(const TreeCall &a) {
+  const int per = 8 * a.row_tiles, x = (int)blockIdx.x, in = x % per, pair = x / per * 8 + in % 8;
+  return {pair / a.n_splits, pair % a.n_splits, in / 8, pair < a.n_pairs};
+}
+static unsigned tree_grid(const TreeCall &a) { return (unsigned)((a.n_pairs + 7) / 8 * 8 * a.row_tiles); }
 
 template <bool BF16, int NT>
 struct TreeWave {
@@ -44,114 +55,83 @@ struct TreeWave {
   static constexpr int kKeys = BF16 ? 32 : 16;
   static constexpr uint32_t kRow = BF16 ? 256 : 512;
   pkv_u32x4 q[NT][kQ];
-  float m[NT], l[NT];
-  pkv_f32x4 o[NT][8];
+  // Weights are 2^(score - use): use is the largest score of some step, not of all.  It moves (and the sums with it) when a score is above
+  // it by more than lim = 8, so that most steps neither look for the row's maximum across lanes nor touch the sums: exact all the same, as
+  // a weight of 2^8 has the precision of one below 1.  lim = -inf: the row has seen nothing yet.
+  float use[NT], lim[NT];
+  pkv_f32x4 l[NT];     // sums: of rows 4j + i (bf16); of row n, this lane's keys, in the first element (fp32)
+  pkv_f32x4 o[NT][8];  // o[m][i]: row 4j + i, dim tree_dim(n, m)
 };
 
 __device__ __forceinline__ pkv_f32x4 mfma_f32(float a, float b, pkv_f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// Two numbers as bf16 in one instruction.
+__device__ __forceinline__ uint32_t tree_pack(float lo, float hi) {
+  const pkv_f32x2 v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, pkv_bf16x2));
+}
+
 // Key of the step that element e of lane (., j) belongs to.
 __device__ __forceinline__ int tree_key(int e, int j) { return 16 * (e >> 2) + 4 * j + (e & 3); }
 
-// One step's keys into the wave's rows.  kv_at(key of the step, address of K, of V); sees(tile, e): whether the lane's row sees its key
-// e; count: keys of the step that there are (the others are read again and count for nothing).
-template <bool BF16, int NT, bool DRAFT, typename At, typename Sees>
-__device__ __forceinline__ void tree_step(TreeWave<BF16, NT> &w, At at, Sees sees, int count, float scale_log2e) {
-  using W = TreeWave<BF16, NT>;
-  const int lane = pkv_lane(), n = lane & 15, j = lane >> 4;
-  pkv_u32x4 k[8], v[8];
+// Dim of column n of the m-th product with V, chosen so that rows of V are read whole: 16 bytes a lane, or (TURNED) as the transposing
+// LDS read delivers them.
+template <bool BF16, bool TURNED>
+__device__ __forceinline__ int tree_dim(int n, int m) {
+  return !BF16 ? 4 * n + (m & 3) + 64 * (m >> 2) : TURNED ? 16 * m + n : 8 * n + m;
+}
+
+// The scores of tile t.
+template <bool BF16, int NT>
+__device__ __forceinline__ void tree_scores(const TreeWave<BF16, NT> &w, const pkv_u32x4 (&k)[8], int t, float (&s)[TreeWave<BF16, NT>::kE]) {
+  pkv_f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
   if constexpr (BF16) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const char *kp, *vp;
-      at(16 * t + n, kp, vp);
+    for (int c = 0; c < 4; ++c) s0 = mfma_bf16(k[c], w.q[t][c], s0), s1 = mfma_bf16(k[4 + c], w.q[t][c], s1);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) k[4 * t + c] = *(const pkv_u32x4 *)(kp + 64 * c + 16 * j);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const char *kp, *vp;
-      at(tree_key(e, j), kp, vp);
-      v[e] = *(const pkv_u32x4 *)(vp + 16 * n);
-    }
+    for (int e = 0; e < 8; ++e) s[e] = e < 4 ? s0[e & 3] : s1[e & 3];
   } else {
-    const char *kp, *vp;
-    at(n, kp, vp);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) k[c] = *(const pkv_u32x4 *)(kp + 64 * c + 16 * j);
+    for (int c = 0; c < 8; ++c)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      at(tree_key(e, j), kp, vp);
-      v[2 * e] = *(const pkv_u32x4 *)(vp + 32 * n);
-      v[2 * e + 1] = *(const pkv_u32x4 *)(vp + 32 * n + 16);
-    }
+      for (int i = 0; i < 4; ++i) s0 = mfma_f32(__uint_as_float(k[c][i]), __uint_as_float(w.q[t][c][i]), s0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = s0[e];
   }
-  // Keys that are not there: zeros, so that nothing of a key read again reaches the sums.
-  if (count < W::kKeys) {
+}
+
+// Scores into weights 2^(scale s - use) of the keys in `bits` (MASKED; else of all), as the operand of the second product; the sum and
+// the base of the sums kept.
+template <bool MASKED, bool BF16, int NT>
+__device__ __forceinline__ pkv_u32x4 tree_weights(TreeWave<BF16, NT> &w, int t, const float (&s)[TreeWave<BF16, NT>::kE], uint32_t bits,
+                                                  float scale_log2e) {
+  constexpr int kE = TreeWave<BF16, NT>::kE;
+  const int j = pkv_lane() >> 4;
+  float p[kE], top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < W::kE; ++e)
-      if (tree_key(e, j) >= count) {
-        if constexpr (BF16) v[e] = pkv_u32x4{0u, 0u, 0u, 0u};
-        else v[2 * e] = v[2 * e + 1] = pkv_u32x4{0u, 0u, 0u, 0u};
-      }
-  }
-  // A drafted value that is not finite belongs to the rows that see it and to no other; in the product it would reach all of the
-  // tile as 0 * inf.  It is taken out there and added for its rows below.
-  pkv_u32x4 odd[8];
-  bool any_odd = false;
-  if constexpr (DRAFT) {
-    uint32_t found = 0;
+  for (int e = 0; e < kE; ++e) p[e] = fmaf(s[e], scale_log2e, -w.use[t]);
+  if (MASKED) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      odd[i] = v[i];
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const uint32_t x = v[i][d];
-        if constexpr (BF16) {
-          const uint32_t lo = (x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u, hi = (x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
-          v[i][d] = x & ~(lo | hi), odd[i][d] = x & (lo | hi), found |= lo | hi;
-        } else {
-          const uint32_t bad = (x & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
-          v[i][d] = x & ~bad, odd[i][d] = x & bad, found |= bad;
-        }
-      }
-    }
-    any_odd = __any(found != 0);
+    for (int e = 0; e < kE; ++e) p[e] = (bits >> e) & 1u ? p[e] : -INFINITY;
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float s[W::kE];
-    if constexpr (BF16) {
-      pkv_f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+  for (int e = 0; e < kE; ++e) top = fmaxf(top, p[e]);
+  if (__any(top > w.lim[t])) {
+    // From here the scores as rounded numbers: the largest is the base itself, and its weight 1, however large they are.
+    float x[kE];
+    top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s0 = mfma_bf16(k[c], w.q[t][c], s0), s1 = mfma_bf16(k[4 + c], w.q[t][c], s1);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = e < 4 ? s0[e & 3] : s1[e & 3];
-    } else {
-      pkv_f32x4 s0 = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s0 = mfma_f32(__uint_as_float(k[c][i]), __uint_as_float(w.q[t][c][i]), s0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = s0[e];
+    for (int e = 0; e < kE; ++e) {
+      x[e] = att_scaled(s[e], scale_log2e);
+      if (MASKED) x[e] = (bits >> e) & 1u ? x[e] : -INFINITY;
+      top = fmaxf(top, x[e]);
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < W::kE; ++e) {
-      s[e] = (DRAFT ? sees(t, e) : tree_key(e, j) < count) ? s[e] * scale_log2e : -INFINITY;
-      mx = fmaxf(mx, s[e]);
-    }
-    const float m_new = fmaxf(w.m[t], pkv_pair_max<32>(pkv_pair_max<16>(mx)));
-    const float base = m_new == -INFINITY ? 0.f : m_new;  // a row that has seen nothing yet
-    const float corr = __builtin_amdgcn_exp2f(w.m[t] - base);
-    w.m[t] = m_new;
-    float p[W::kE], sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < W::kE; ++e) p[e] = __builtin_amdgcn_exp2f(s[e] - base), sum += p[e];
-    w.l[t] = fmaf(w.l[t], corr, sum);
+    top = pkv_pair_max<32>(pkv_pair_max<16>(top));
+    const bool fresh = w.lim[t] < 0.f, moves = top > -INFINITY && (fresh || top > w.use[t]);
+    const float next = moves ? top : w.use[t], corr = fresh ? 0.f : __builtin_amdgcn_exp2f(w.use[t] - next);
+    w.use[t] = next, w.lim[t] = moves ? 8.f : w.lim[t];
     float cr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) cr[i] = __shfl(corr, 4 * j + i, PKV_WAVE);
@@ -160,163 +140,550 @@ __device__ __forceinline__ void tree_step(TreeWave<BF16, NT> &w, At at, Sees see
 #pragma unroll
       for (int i = 0; i < 4; ++i) w.o[t][m][i] *= cr[i];
     if constexpr (BF16) {
-      const pkv_u32x4 pa = {pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])};
 #pragma unroll
-      for (int m = 0; m < 8; ++m) {
-        const uint32_t sel = (m & 1) ? 0x07060302u : 0x05040100u;  // element m of each of the eight rows
-        pkv_u32x4 b;
+      for (int i = 0; i < 4; ++i) w.l[t][i] *= cr[i];
+    } else {
+      w.l[t][0] *= corr;
+    }
 #pragma unroll
-        for (int d = 0; d < 4; ++d) b[d] = __builtin_amdgcn_perm(v[2 * d + 1][m >> 1], v[2 * d][m >> 1], sel);
-        w.o[t][m] = mfma_bf16(pa, b, w.o[t][m]);
-      }
+    for (int e = 0; e < kE; ++e) p[e] = x[e] - next;
+  }
+#pragma unroll
+  for (int e = 0; e < kE; ++e) p[e] = __builtin_amdgcn_exp2f(p[e]);
+  if constexpr (BF16) {
+    const pkv_u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    const pkv_u32x4 a = {tree_pack(p[0], p[1]), tree_pack(p[2], p[3]), tree_pack(p[4], p[5]), tree_pack(p[6], p[7])};
+    w.l[t] = mfma_bf16(a, ones, w.l[t]);
+    return a;
+  } else {
+    w.l[t][0] += (p[0] + p[1]) + (p[2] + p[3]);
+    return pkv_u32x4{__float_as_uint(p[0]), __float_as_uint(p[1]), __float_as_uint(p[2]), __float_as_uint(p[3])};
+  }
+}
+
+// O += P V.  v_of(m): the operand of the m-th product, rows of V for the lane's keys: element e in half e % 2 of word e / 2 (bf16), or in word e.
+template <bool BF16, int NT, typename Of>
+__device__ __forceinline__ void tree_output(TreeWave<BF16, NT> &w, const pkv_u32x4 (&p)[NT], Of v_of) {
+#pragma unroll
+  for (int m = 0; m < 8; ++m) {
+    const pkv_u32x4 v = v_of(m);
+    if constexpr (BF16) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) w.o[t][m] = mfma_bf16(p[t], v, w.o[t][m]);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int m = 0; m < 8; ++m) w.o[t][m] = mfma_f32(p[e], __uint_as_float(v[2 * e + (m >> 2)][m & 3]), w.o[t][m]);
+        for (int t = 0; t < NT; ++t) w.o[t][m] = mfma_f32(__uint_as_float(p[t][e]), __uint_as_float(v[e]), w.o[t][m]);
     }
-    if constexpr (DRAFT) {
-      if (any_odd) {  // the whole wave
+  }
+}
+
+// The m-th operand out of rows of V as loaded, 16 bytes a key (bf16) or twice 16 (fp32).
+template <bool BF16>
+__device__ __forceinline__ pkv_u32x4 tree_turn(const pkv_u32x4 (&v)[8], int m) {
+  pkv_u32x4 b;
+  if constexpr (BF16) {
+    const uint32_t sel = (m & 1) ? 0x07060302u : 0x05040100u;  // element m of each of the eight rows
 #pragma unroll
-        for (int e = 0; e < W::kE; ++e)
-          for (int from = 0; from < 4; ++from) {  // key tree_key(e, from): its value in the lanes (n, from), row r's weight in lane (r, from)
-            float x[8];
+    for (int d = 0; d < 4; ++d) b[d] = __builtin_amdgcn_perm(v[2 * d + 1][m >> 1], v[2 * d][m >> 1], sel);
+  } else {
 #pragma unroll
-            for (int m = 0; m < 8; ++m) {
-              if constexpr (BF16) {
-                const uint32_t d = (uint32_t)__shfl((int)odd[e][m >> 1], n + 16 * from, PKV_WAVE);
-                x[m] = __uint_as_float(m & 1 ? d & 0xffff0000u : d << 16);
-              } else {
-                x[m] = __uint_as_float((uint32_t)__shfl((int)odd[2 * e + (m >> 2)][m & 3], n + 16 * from, PKV_WAVE));
-              }
-            }
+    for (int e = 0; e < 4; ++e) b[e] = v[2 * e + (m >> 2)][m & 3];
+  }
+  return b;
+}
+
+// A step with keys that the rows do not all see: its first `here` keys are there; drafted ones (dv not null: the drafted V rows of this
+// (b, h)), the tokens from u0 on, only for the rows whose token sees them.  v_of as in tree_output; weight: room of this wave's own.
+template <bool BF16, bool TURNED, int NT, typename Of>
+__device__ __forceinline__ void tree_masked_step(TreeWave<BF16, NT> &w, const TreeCall &a, int b, const char *dv, int u0, int here,
+                                                 const int (&token)[NT], float (*weight)[33], const pkv_u32x4 (&k)[8], Of v_of) {
+  using W = TreeWave<BF16, NT>;
+  const int lane = pkv_lane(), n = lane & 15, j = lane >> 4;
+  const bool draft = dv != nullptr;
+  uint32_t there = 0, bits[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float pr = __shfl(p[e], 4 * j + i + 16 * from, PKV_WAVE);
+  for (int e = 0; e < W::kE; ++e) there |= tree_key(e, j) < here ? 1u << e : 0u;
 #pragma unroll
-              for (int m = 0; m < 8; ++m)
-                if (pr != 0.f && x[m] != 0.f) w.o[t][m][i] += pr * x[m];
-            }
-          }
+  for (int t = 0; t < NT; ++t) {
+    bits[t] = there;
+    if (draft && a.mask) {
+      const uint8_t *const row = a.mask + (int64_t)b * a.mask_b + (int64_t)token[t] * a.mask_t + u0;
+      uint32_t x = 0;
+#pragma unroll
+      for (int e = 0; e < W::kE; ++e) {
+        const int key = tree_key(e, j);
+        x |= (row[key < here ? key : here - 1] != 0 ? 1u : 0u) << e;
+      }
+      bits[t] &= x;
+    } else if (draft) {
+      uint32_t x = 0;
+#pragma unroll
+      for (int e = 0; e < W::kE; ++e) x |= (u0 + tree_key(e, j) <= token[t] ? 1u : 0u) << e;
+      bits[t] &= x;
+    }
+  }
+  pkv_u32x4 p[NT], keep;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    float s[W::kE];
+    tree_scores(w, k, t, s);
+    p[t] = tree_weights<true>(w, t, s, bits[t], a.scale_log2e);
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    if constexpr (BF16) keep[d] = ((there >> (2 * d)) & 1u ? 0xffffu : 0u) | ((there >> (2 * d + 1)) & 1u ? 0xffff0000u : 0u);
+    else keep[d] = (there >> d) & 1u ? 0xffffffffu : 0u;
+  }
+  // Keys that are not there were read again: zeros, so that nothing of them reaches the sums.  A drafted value that is not finite is for the
+  // rows that see it and for no other, but in the product it would be 0 * inf for all: zero there, and added below.
+  uint32_t found = 0;
+  tree_output(w, p, [&](int m) {
+    pkv_u32x4 v = v_of(m);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      uint32_t x = v[d] & keep[d], bad;
+      if constexpr (BF16) bad = ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+      else bad = (x & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
+      if (!draft) bad = 0;
+      found |= bad, v[d] = x & ~bad;
+    }
+    return v;
+  });
+  if (__any(found != 0)) {  // the whole wave: drafted values that are not finite, one key at a time
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < W::kE; ++e) {
+        const uint32_t d = BF16 ? p[t][e >> 1] : p[t][e & 3];
+        weight[n][tree_key(e, j)] = __uint_as_float(!BF16 ? d : e & 1 ? d & 0xffff0000u : d << 16);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int key = 0; key < here; ++key) {
+        const char *vp = dv + (int64_t)(u0 + key) * a.dv_t;
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = weight[4 * j + i][key];
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          const int d = tree_dim<BF16, TURNED>(n, m);
+          float x;
+          if constexpr (BF16) x = pkv_bf16_bits_to_f32(((const uint16_t *)vp)[d]);
+          else x = ((const float *)vp)[d];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w.o[t][m][i] += f[i] != 0.f && !(fabsf(x) < INFINITY) ? f[i] * x : 0.f;
+        }
       }
     }
   }
 }
 
-// grid (splits, tiles of 16 NT query rows, rows of (b, h))
-template <bool BF16, int NT, bool INDEXED, typename SEGS>
-__global__ __launch_bounds__(kTreeWaves * PKV_WAVE) void pkv_tree_partial_kernel(TreeCall a, SEGS segs) {
-  using W = TreeWave<BF16, NT>;
-  constexpr bool ONE = __is_same(SEGS, AttOne);
-  const int split = blockIdx.x, n_splits = gridDim.x, r0 = blockIdx.y * 16 * NT, bh = blockIdx.z;
-  const int b = bh / a.n_kv_heads, h = bh % a.n_kv_heads, rows = a.n_draft * a.group;
-  const int tid = threadIdx.x, lane = tid & (PKV_WAVE - 1), wave = tid / PKV_WAVE, n = lane & 15, j = lane >> 4;
-  constexpr int es = BF16 ? 2 : 4;
-
-  uint32_t total = a.total;
-  if (a.row_keys) {
-    const int rk = a.row_keys[bh];
-    total = rk <= 0 ? 0u : (uint32_t)rk < total ? (uint32_t)rk : total;
-  }
-  const uint32_t per_wave = a.per_split / kTreeWaves;  // a multiple of a step's keys
-  const uint32_t k0 = (uint32_t)split * a.per_split + (uint32_t)wave * per_wave;
-  const uint32_t k1 = k0 + per_wave < total ? k0 + per_wave : total;  // k1 <= k0: nothing for this wave
-
-  W w;
-  int token[NT];
+// The waves that took keys of the same rows meet, a tile of 16 rows at a time, and leave their result, or the split's part of it.
+template <bool BF16, bool TURNED, int NT, int RW, int WAVES>
+__device__ __forceinline__ void tree_finish(const TreeWave<BF16, NT> &w, const TreeCall &a, const TreePart &part, float (&s_m)[WAVES][16],
+                                            float (&s_l)[WAVES][16], float (&s_o)[WAVES][16][132]) {
+  constexpr int KW = WAVES / RW;
+  const int tid = threadIdx.x, lane = pkv_lane(), wave = tid / PKV_WAVE, n = lane & 15, j = lane >> 4;
+  const int bh = part.bh, n_splits = a.n_splits, rows = a.n_draft * a.group, b = bh / a.n_kv_heads, h = bh % a.n_kv_heads;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int r = r0 + 16 * t + n, rr = r < rows ? r : rows - 1;  // rows past the last repeat it and are not stored
+    __syncthreads();
+    if (j == 0) s_m[wave][n] = w.lim[t] < 0.f ? -INFINITY : w.use[t];
+    if constexpr (BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n == 0) s_l[wave][4 * j + i] = w.l[t][i];
+    } else {
+      const float l = pkv_pair_add<32>(pkv_pair_add<16>(w.l[t][0]));
+      if (j == 0) s_l[wave][n] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float *const row = s_o[wave][4 * j + i];
+      if constexpr (BF16 && TURNED) {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) row[tree_dim<BF16, TURNED>(n, m)] = w.o[t][m][i];
+      } else {
+        *(float4 *)(row + tree_dim<BF16, TURNED>(n, 0)) = float4{w.o[t][0][i], w.o[t][1][i], w.o[t][2][i], w.o[t][3][i]};
+        *(float4 *)(row + tree_dim<BF16, TURNED>(n, 4)) = float4{w.o[t][4][i], w.o[t][5][i], w.o[t][6][i], w.o[t][7][i]};
+      }
+    }
+    __syncthreads();
+    for (int e = tid; e < RW * 16 * 32; e += WAVES * PKV_WAVE) {  // four dims at a time
+      const int rw = e >> 9, r = (e >> 5) & 15, d = 4 * (e & 31), row = (part.tile * RW + rw) * 16 * NT + 16 * t + r;
+      if (row >= rows) continue;
+      float mx = s_m[rw][r];
+#pragma unroll
+      for (int i = 1; i < KW; ++i) mx = fmaxf(mx, s_m[rw + i * RW][r]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float ls = 0.f;
+      pkv_f32x4 os = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KW; ++i) {
+        const float c = __builtin_amdgcn_exp2f(s_m[rw + i * RW][r] - base);
+        const pkv_f32x4 x = *(const pkv_f32x4 *)&s_o[rw + i * RW][r][d];
+        ls = fmaf(s_l[rw + i * RW][r], c, ls);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) os[u] = fmaf(x[u], c, os[u]);
+      }
+      if (n_splits == 1) {
+        const int64_t to = (((int64_t)b * a.n_draft + row / a.group) * a.n_kv_heads * a.group + h * a.group + row % a.group) * 128 + d;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) os[u] = ls == 0.f ? 0.f : os[u] / ls;  // 0: nothing seen
+        if constexpr (BF16) *(pkv_u32x2 *)((uint16_t *)a.out + to) = pkv_u32x2{tree_pack(os[0], os[1]), tree_pack(os[2], os[3])};
+        else *(pkv_f32x4 *)((float *)a.out + to) = os;
+      } else {
+        const int64_t at = ((int64_t)bh * n_splits + part.split) * rows + row;
+        *(pkv_f32x4 *)(a.ws_o + at * 128 + d) = os;
+        if (d == 0) *(float2 *)(a.ws_ml + at * 2) = float2{mx, ls};
+      }
+    }
+  }
+}
+
+// Query rows r0 .. of this wave (those past the last repeat it and are not stored), and sums of nothing.
+template <bool BF16, int NT>
+__device__ __forceinline__ void tree_begin(TreeWave<BF16, NT> &w, const TreeCall &a, int b, int h, int r0, int (&token)[NT]) {
+  const int lane = pkv_lane(), n = lane & 15, j = lane >> 4, rows = a.n_draft * a.group;
+  constexpr int es = BF16 ? 2 : 4;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int r = r0 + 16 * t + n, rr = r < rows ? r : rows - 1;
     token[t] = rr / a.group;
     const char *qp = (const char *)a.q + ((int64_t)b * a.q_stride_b + (int64_t)token[t] * a.q_stride_t +
                                           (int64_t)(h * a.group + rr % a.group) * 128) * es + 16 * j;
 #pragma unroll
-    for (int c = 0; c < W::kQ; ++c) w.q[t][c] = *(const pkv_u32x4 *)(qp + 64 * c);
-    w.m[t] = -INFINITY, w.l[t] = 0.f;
+    for (int c = 0; c < TreeWave<BF16, NT>::kQ; ++c) w.q[t][c] = *(const pkv_u32x4 *)(qp + 64 * c);
+    w.use[t] = 0.f, w.lim[t] = -INFINITY, w.l[t] = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int m = 0; m < 8; ++m) w.o[t][m] = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
   }
+}
 
-  const char *kbase = nullptr, *vbase = nullptr;
-  if constexpr (ONE) {
-    const int64_t slab = (int64_t)b * segs.stride_b + (int64_t)h * segs.stride_h;
-    kbase = segs.k + slab, vbase = segs.v + slab;
+// Cached keys of row bh.
+__device__ __forceinline__ uint32_t tree_total(const TreeCall &a, int bh) {
+  if (!a.row_keys) return a.total;
+  const int rk = a.row_keys[bh];
+  return rk <= 0 ? 0u : (uint32_t)rk < a.total ? (uint32_t)rk : a.total;
+}
+
+// Places of cached keys of one (b, h).  The fields of segments in one tensor are held in registers and added up: a field picked by a lane
+// would be loaded from memory, and the wait for it would be for all keys under way too.
+template <bool BF16, bool INDEXED, typename SEGS>
+struct TreePlaces {
+  static constexpr uint32_t kRow = BF16 ? 256 : 512;
+  const SEGS &segs;
+  int bh, b, h;
+  __device__ __forceinline__ TreePlaces(const SEGS &s, int bh_, int b_, int h_) : segs(s), bh(bh_), b(b_), h(h_) {}
+  __device__ __forceinline__ AttPlace<false> of(uint32_t at) const { return att_place<INDEXED, kRow>(segs, bh, b, h, at); }
+};
+template <bool BF16, bool INDEXED>
+struct TreePlaces<BF16, INDEXED, AttOne> {
+  static constexpr uint32_t kRow = BF16 ? 256 : 512;
+  static_assert(PKV_ATTN_MAX_SEGMENTS == 4, "segments one by one");
+  const char *k, *v;
+  uint32_t end0, end1, end2;
+  uint32_t delta0, more1, more2, more3;
+  const int64_t *idx;
+  int64_t limit;
+  uint32_t lo, hi, row0;
+  __device__ __forceinline__ TreePlaces(const AttOne &s, int bh, int b, int h) {
+    const int64_t slab = (int64_t)b * s.stride_b + (int64_t)h * s.stride_h;
+    k = s.k + slab, v = s.v + slab;
+    end0 = att_field(s.end[0]), end1 = att_field(s.end[1]), end2 = att_field(s.end[2]);
+    const uint32_t d0 = (uint32_t)att_field(s.delta[0]), d1 = (uint32_t)att_field(s.delta[1]), d2 = (uint32_t)att_field(s.delta[2]);
+    delta0 = d0, more1 = d1 - d0, more2 = d2 - d1, more3 = (uint32_t)att_field(s.delta[3]) - d2;
+    if (INDEXED) idx = s.idx + (int64_t)bh * s.idx_stride, limit = s.idx_limit, lo = s.idx_lo, hi = s.idx_hi, row0 = s.idx_row0;
   }
-  AttPlace<ONE> mine;  // of key (block of 64) + lane
-  for (uint32_t at = k0; at < k1; at += W::kKeys) {
-    const int in_block = (int)(at - k0) & (PKV_WAVE - 1);
-    if (in_block == 0) mine = att_place<INDEXED, W::kRow>(segs, bh, b, h, at + lane < k1 ? at + lane : k1 - 1);
-    const int count = k1 - at < (uint32_t)W::kKeys ? (int)(k1 - at) : W::kKeys;
-    tree_step<BF16, NT, false>(
-        w,
-        [&](int key, const char *&kp, const char *&vp) {
-          if constexpr (ONE) {
-            const uint64_t off = mine.from(in_block + key).off;
-            kp = kbase + off, vp = vbase + off;
-          } else {
-            kp = mine.k_from(in_block + key), vp = mine.v_from(in_block + key);
-          }
-        },
-        [](int, int) { return true; }, count, a.scale_log2e);
-  }
-  if (split == n_splits - 1) {  // the drafted tokens, a step's keys a wave in turn
-    for (int u0 = wave * W::kKeys; u0 < a.n_draft; u0 += kTreeWaves * W::kKeys) {
-      const int count = a.n_draft - u0 < W::kKeys ? a.n_draft - u0 : W::kKeys;
-      tree_step<BF16, NT, true>(
-          w,
-          [&](int key, const char *&kp, const char *&vp) {
-            const int64_t u = u0 + (key < count ? key : count - 1);
-            kp = a.dk + (int64_t)b * a.dk_b + (int64_t)h * a.dk_h + u * a.dk_t;
-            vp = a.dv + (int64_t)b * a.dv_b + (int64_t)h * a.dv_h + u * a.dv_t;
-          },
-          [&](int t, int e) {
-            const int key = tree_key(e, j), u = u0 + (key < count ? key : count - 1);
-            const bool on = a.mask ? a.mask[(int64_t)b * a.mask_b + (int64_t)token[t] * a.mask_t + u] != 0 : u <= token[t];
-            return on && key < count;
-          },
-          count, a.scale_log2e);
+  __device__ __forceinline__ AttPlace<true> of(uint32_t at) const {
+    uint32_t r = at + delta0 + (at >= end0 ? more1 : 0u) + (at >= end1 ? more2 : 0u) + (at >= end2 ? more3 : 0u);
+    if (INDEXED && at >= lo && at < hi) {
+      const int64_t x = idx[at - lo];
+      r = row0 + (uint32_t)(x < 0 ? 0 : (x >= limit ? limit - 1 : x));
     }
+    return {r * kRow};
+  }
+};
+
+// Lane `key`'s place, key = a constant plus what the lane adds: the constant goes into the instruction.
+__device__ __forceinline__ AttPlace<true> tree_from(const AttPlace<true> &p, int base4, int key) {
+  return {(uint32_t)__builtin_amdgcn_ds_bpermute(base4 + 4 * key, (int)p.off)};
+}
+
+// at(what the lane adds, constant part): address of that key's row.
+template <bool BF16, typename At>
+__device__ __forceinline__ void tree_load_k(pkv_u32x4 (&k)[8], At at) {
+  const int lane = pkv_lane(), n = lane & 15, j = lane >> 4;
+  constexpr int kTiles = BF16 ? 2 : 1, kVecs = BF16 ? 4 : 8;
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const char *kp = at(n, 16 * t);
+#pragma unroll
+    for (int c = 0; c < kVecs; ++c) k[kVecs * t + c] = *(const pkv_u32x4 *)(kp + 64 * c + 16 * j);
+  }
+}
+template <bool BF16, typename At>
+__device__ __forceinline__ void tree_load_v(pkv_u32x4 (&v)[8], At at) {
+  const int lane = pkv_lane(), n = lane & 15, j = lane >> 4;
+  constexpr int kE = BF16 ? 8 : 4, kVecs = BF16 ? 1 : 2;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    const char *vp = at(4 * j, tree_key(e, 0));
+#pragma unroll
+    for (int c = 0; c < kVecs; ++c) v[kVecs * e + c] = *(const pkv_u32x4 *)(vp + 16 * n + 256 * c);
+  }
+}
+
+// Workgroups of a launch: one to a compute unit (kTreeWorkgroups).  us, 128 / 256 / 512 / 1024 workgroups: 4 x 8 heads x 65536 keys, 16 rows
+// a head 226 / 191 / 195 / 212, 64 rows 260 / 178 / 189 / 222; 1 x 8 x 32768, 32 rows 39.5 / 35.4 / 46.2 / 46.3; 3 x 4 x 9001 fp32, 49 rows 78 / 50 / 59 / 67.
+//
+// Up to 16 query rows.  The four waves of a workgroup take steps of keys in turns, straight from memory into the operands' registers.
+// Full steps go round the waves of all splits, so that what the chip reads at one time lies side by side; the steps that not all rows see in
+// full, the cached keys behind the last full step and the drafted tokens, are dealt out behind them.
+template <bool BF16, bool INDEXED, typename SEGS>
+__global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_kernel(TreeCall a, SEGS segs) {
+  using W = TreeWave<BF16, 1>;
+  constexpr bool ONE = __is_same(SEGS, AttOne);
+  const TreePart part = tree_part(a);
+  if (!part.any) return;  // the whole workgroup
+  const int split = part.split, n_splits = a.n_splits, bh = part.bh;
+  const int b = bh / a.n_kv_heads, h = bh % a.n_kv_heads;
+  const int lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PKV_WAVE);
+
+  const uint32_t total = tree_total(a, bh);
+  const int turns = kTreeWaves * n_splits, turn0 = split * kTreeWaves + wave;
+  const int all_full = (int)(total / W::kKeys), rest = (int)(total % W::kKeys);
+  const int n_full = turn0 < all_full ? (all_full - 1 - turn0) / turns + 1 : 0;
+
+  // Where the keys of a step lie: lane l knows key l's place.  Found two steps ahead, since a selected row's number is read from memory.
+  const TreePlaces<BF16, INDEXED, SEGS> places(segs, bh, b, h);
+  auto find = [&](int first, int keys) {
+    const int key = lane & (W::kKeys - 1);
+    return places.of((uint32_t)(first + (key < keys ? key : keys - 1)));
+  };
+  auto k_at = [&](const AttPlace<ONE> &place) {
+    return [&](int base, int key) -> const char * {
+      if constexpr (ONE) return places.k + (uint64_t)tree_from(place, 4 * base, key).off;
+      else return (const char *)place.pull(place.k, base + key);
+    };
+  };
+  auto v_at = [&](const AttPlace<ONE> &place) {
+    return [&](int base, int key) -> const char * {
+      if constexpr (ONE) return places.v + (uint64_t)tree_from(place, 4 * base, key).off;
+      else return (const char *)place.pull(place.v, base + key);
+    };
+  };
+
+  W w;
+  pkv_u32x4 k[8], v[8];
+  int token[1];
+  tree_begin<BF16, 1>(w, a, b, h, 0, token);
+  // In the order of the loop, so that a wait there is for what it needs alone: K, the place of the next step, V.
+  AttPlace<ONE> mine, next;
+  if (n_full > 0) {
+    mine = find(turn0 * W::kKeys, W::kKeys);
+    tree_load_k<BF16>(k, k_at(mine));
+    next = find((n_full > 1 ? turn0 + turns : turn0) * W::kKeys, W::kKeys);
+    tree_load_v<BF16>(v, v_at(mine));
+  }
+  // Keys and values of the next step are requested where the registers of this one's are free again.
+  for (int i = 0; i < n_full; ++i) {
+    float s[W::kE];
+    tree_scores(w, k, 0, s);
+    mine = next;
+    if (i + 1 < n_full) tree_load_k<BF16>(k, k_at(mine));
+    if (i + 2 < n_full) next = find((turn0 + (i + 2) * turns) * W::kKeys, W::kKeys);
+    const pkv_u32x4 p[1] = {tree_weights<false>(w, 0, s, 0u, a.scale_log2e)};
+    tree_output(w, p, [&](int m) { return tree_turn<BF16>(v, m); });
+    if (i + 1 < n_full) tree_load_v<BF16>(v, v_at(mine));
   }
 
-  // the waves of the workgroup, a tile of rows at a time
   __shared__ float s_m[kTreeWaves][16], s_l[kTreeWaves][16];
   __shared__ alignas(16) float s_o[kTreeWaves][16][128 + 4];
+  const char *const dk = a.dk + (int64_t)b * a.dk_b + (int64_t)h * a.dk_h, *const dv = a.dv + (int64_t)b * a.dv_b + (int64_t)h * a.dv_h;
+  const int n_tail = rest > 0 ? 1 : 0, n_more = n_tail + (a.n_draft - 1) / W::kKeys + 1;
+  for (int i = (turn0 - all_full % turns + turns) % turns; i < n_more; i += turns) {
+    const bool draft = i >= n_tail;
+    const int u0 = (i - n_tail) * W::kKeys, left = draft ? a.n_draft - u0 : rest, here = left < W::kKeys ? left : W::kKeys;
+    if (draft) {
+      tree_load_k<BF16>(k, [&](int base, int key) { return dk + (int64_t)(u0 + (base + key < here ? base + key : here - 1)) * a.dk_t; });
+      tree_load_v<BF16>(v, [&](int base, int key) { return dv + (int64_t)(u0 + (base + key < here ? base + key : here - 1)) * a.dv_t; });
+    } else {
+      mine = find(all_full * W::kKeys, rest);
+      tree_load_k<BF16>(k, k_at(mine));
+      tree_load_v<BF16>(v, v_at(mine));
+    }
+    tree_masked_step<BF16, false, 1>(w, a, b, draft ? dv : nullptr, u0, here, token, (float(*)[33]) & s_o[wave][0][0], k,
+                                     [&](int m) { return tree_turn<BF16>(v, m); });
+  }
+  tree_finish<BF16, false, 1, 1, kTreeWaves>(w, a, part, s_m, s_l, s_o);
+}
+
+typedef short tree_s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) tree_s16x4 tree_lds_s16x4;
+
+// More than 16 query rows: the waves of a workgroup share the keys, which go through LDS once for all of them.
+// RW of the eight waves take 16 NT rows each; the 8 / RW groups of such waves take neighbouring steps of keys, a turn of them at a time.  Rows of K and V
+// are requested two turns ahead into registers, written to one of two LDS buffers a turn ahead, and read from there as operands; one
+// barrier a turn.  us, straight from memory with each wave's own loads (two tiles a wave) / through LDS: 4 x 8 x 65536 keys, 64 rows 240 / 170;
+// 8 x 8 x 1617 selected keys, 256 rows 54 / 46.  A 16-byte vector c of a row r lies at c ^ (r mod 16), so that the 16 rows of an operand of K are on different banks.
+template <bool BF16, int NT, int RW, bool INDEXED, typename SEGS>
+__global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel(TreeCall a, SEGS segs) {
+  using W = TreeWave<BF16, NT>;
+  constexpr bool ONE = __is_same(SEGS, AttOne);
+  constexpr int KW = kWideWaves / RW, kTurnKeys = KW * W::kKeys, kRow = W::kRow, kVecs = kRow / 16;
+  constexpr int kRowsAt = kWideWaves * PKV_WAVE / kVecs, kLoads = kTurnKeys / kRowsAt;  // rows a load of the workgroup covers; loads a turn
+  constexpr int kTensor = kTurnKeys * kRow;
+  const TreePart part = tree_part(a);
+  if (!part.any) return;  // the whole workgroup
+  const int split = part.split, n_splits = a.n_splits, bh = part.bh;
+  const int b = bh / a.n_kv_heads, h = bh % a.n_kv_heads;
+  const int tid = threadIdx.x, lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(tid / PKV_WAVE), n = lane & 15, j = lane >> 4;
+  const int row_wave = wave % RW, key_wave = wave / RW, r0 = (part.tile * RW + row_wave) * 16 * NT;
+  constexpr int kEnd = kWideWaves * (16 * 132 + 32) * 4, kLds = 4 * kTensor > kEnd ? 4 * kTensor : kEnd;
+  static_assert(2 * kTensor + kWideWaves * 16 * 33 * 4 <= kLds, "room for the weights of drafted tokens behind a turn");
+  __shared__ alignas(16) char lds[kLds];
+
+  const uint32_t total = tree_total(a, bh);
+  const int all_full = (int)(total / kTurnKeys), rest = (int)(total % kTurnKeys);
+  const int n_mine = split < all_full ? (all_full - 1 - split) / n_splits + 1 : 0, n_full = n_mine > 1 ? n_mine : 0;  // a single turn: not piped
+  const TreePlaces<BF16, INDEXED, SEGS> places(segs, bh, b, h);
+  const char *const dk = a.dk + (int64_t)b * a.dk_b + (int64_t)h * a.dk_h, *const dv = a.dv + (int64_t)b * a.dv_b + (int64_t)h * a.dv_h;
+
+  // What this thread brings in: vector my_vec of rows my_row + kRowsAt u.
+  const int my_row = tid / kVecs, my_vec = tid % kVecs;
+  struct Rows {
+    pkv_u32x4 k[kLoads], v[kLoads];
+  };
+  auto find = [&](int first, int count, AttPlace<ONE> (&at)[kLoads]) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const float l = pkv_pair_add<32>(pkv_pair_add<16>(w.l[t]));
-    if (t > 0) __syncthreads();
-    if (j == 0) s_m[wave][n] = w.m[t], s_l[wave][n] = l;
+    for (int u = 0; u < kLoads; ++u) {
+      const int r = my_row + kRowsAt * u;
+      at[u] = places.of((uint32_t)(first + (r < count ? r : count - 1)));
+    }
+  };
+  auto fetch = [&](const AttPlace<ONE> (&at)[kLoads], Rows &r) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *(float4 *)&s_o[wave][4 * j + i][8 * n] = float4{w.o[t][0][i], w.o[t][1][i], w.o[t][2][i], w.o[t][3][i]};
-      *(float4 *)&s_o[wave][4 * j + i][8 * n + 4] = float4{w.o[t][4][i], w.o[t][5][i], w.o[t][6][i], w.o[t][7][i]};
+    for (int u = 0; u < kLoads; ++u) {
+      const char *kp, *vp;
+      if constexpr (ONE) kp = places.k + (uint64_t)at[u].off, vp = places.v + (uint64_t)at[u].off;
+      else kp = (const char *)at[u].k, vp = (const char *)at[u].v;
+      r.k[u] = __builtin_nontemporal_load((const pkv_u32x4 *)kp + my_vec);
+      r.v[u] = __builtin_nontemporal_load((const pkv_u32x4 *)vp + my_vec);
+    }
+  };
+  auto put = [&](const Rows &r, int buffer) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int row = my_row + kRowsAt * u, at = buffer * 2 * kTensor + row * kRow + 16 * (my_vec ^ (row & 15));
+      *(pkv_u32x4 *)(lds + at) = r.k[u];
+      *(pkv_u32x4 *)(lds + at + kTensor) = r.v[u];
+    }
+  };
+  W w;
+  pkv_u32x4 k[8];
+  auto get_k = [&](int buffer) {
+    constexpr int kTiles = BF16 ? 2 : 1, kC = BF16 ? 4 : 8;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+        k[kC * t + c] = *(const pkv_u32x4 *)(lds + buffer * 2 * kTensor + (key_wave * W::kKeys + 16 * t + n) * kRow + 16 * ((4 * c + j) ^ n));
+  };
+  // bf16: a transposing read takes four rows times 16 dims with 16 lanes, eight bytes of a row each, and gives a lane one dim of the four.
+  auto v_of = [&](int buffer) {
+    return [&, buffer](int m) {
+      const char *const rows = lds + buffer * 2 * kTensor + kTensor + key_wave * W::kKeys * kRow;
+      pkv_u32x4 x;
+      if constexpr (BF16) {
+        const int r = 4 * j + (n >> 2), at = r * (int)kRow + 16 * ((2 * m + ((n >> 1) & 1)) ^ r) + 8 * (n & 1);
+        const tree_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tree_lds_s16x4 *)(rows + at));
+        const tree_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tree_lds_s16x4 *)(rows + at + 16 * kRow));
+        const pkv_u32x2 a2 = __builtin_bit_cast(pkv_u32x2, lo), b2 = __builtin_bit_cast(pkv_u32x2, hi);
+        x = pkv_u32x4{a2.x, a2.y, b2.x, b2.y};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = tree_key(e, j);
+          x[e] = *(const uint32_t *)(rows + r * kRow + 16 * ((16 * (m >> 2) + n) ^ r) + 4 * (m & 3));
+        }
+      }
+      return x;
+    };
+  };
+
+  int token[NT];
+  tree_begin<BF16, NT>(w, a, b, h, r0, token);
+  AttPlace<ONE> next[kLoads], later[kLoads];
+  Rows ahead[2];
+  auto first_of = [&](int i) { return (split + (i < n_full ? i : n_full - 1) * n_splits) * kTurnKeys; };  // past the last: read again, never used
+  if (n_full > 0) {
+    find(first_of(0), kTurnKeys, next);
+    fetch(next, ahead[0]);
+    find(first_of(1), kTurnKeys, next);
+    fetch(next, ahead[1]);
+    find(first_of(2), kTurnKeys, later);
+    find(first_of(3), kTurnKeys, next);
+    put(ahead[0], 0);
+    fetch(later, ahead[0]);
+  }
+  // Turn i is in LDS or on its way there, turn i + 1 in registers, turn i + 2 requested, the places of turn i + 3 known.  Places are asked
+  // for before rows: a wait for them is then not for the rows as well.
+  auto turn = [&](int i, Rows &after) {
+    __syncthreads();  // turn i is there, and everybody is done with turn i - 1
+    put(after, (i + 1) & 1);
+    find(first_of(i + 4), kTurnKeys, later);
+    fetch(next, after);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) next[u] = later[u];
+    float s[NT][W::kE];
+    get_k(i & 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) tree_scores(w, k, t, s[t]);
+    pkv_u32x4 p[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) p[t] = tree_weights<false>(w, t, s[t], 0u, a.scale_log2e);
+    tree_output(w, p, v_of(i & 1));
+  };
+  for (int i = 0; i < n_full; i += 2) {
+    turn(i, ahead[1]);
+    if (i + 1 < n_full) turn(i + 1, ahead[0]);
+  }
+
+  // The cached keys behind the last full turn, and the drafted tokens, a turn of them at a time, dealt out behind the full ones.
+  const int n_tail = rest > 0 ? 1 : 0, n_more = n_tail + (a.n_draft - 1) / kTurnKeys + 1;
+  for (int i = n_mine > n_full ? -1 : 0, turn0 = (split - all_full % n_splits + n_splits) % n_splits; i < 0 || turn0 < n_more; ++i) {
+    const bool whole = i < 0, draft = !whole && turn0 >= n_tail;
+    const int first = whole ? split * kTurnKeys : draft ? (turn0 - n_tail) * kTurnKeys : all_full * kTurnKeys, left = (draft ? a.n_draft : (int)total) - first;
+    const int count = left < kTurnKeys ? left : kTurnKeys;
+    if (draft) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const int r = my_row + kRowsAt * u, at = first + (r < count ? r : count - 1);
+        ahead[0].k[u] = ((const pkv_u32x4 *)(dk + (int64_t)at * a.dk_t))[my_vec];
+        ahead[0].v[u] = ((const pkv_u32x4 *)(dv + (int64_t)at * a.dv_t))[my_vec];
+      }
+    } else {
+      find(first, count, next);
+      fetch(next, ahead[0]);
     }
     __syncthreads();
-    for (int e = tid; e < 16 * 128; e += kTreeWaves * PKV_WAVE) {
-      const int r = e >> 7, d = e & 127, row = r0 + 16 * t + r;
-      if (row >= rows) break;  // rows come in order
-      float mx = s_m[0][r];
-#pragma unroll
-      for (int i = 1; i < kTreeWaves; ++i) mx = fmaxf(mx, s_m[i][r]);
-      const float base = mx == -INFINITY ? 0.f : mx;
-      float ls = 0.f, os = 0.f;
-#pragma unroll
-      for (int i = 0; i < kTreeWaves; ++i) {
-        const float c = __builtin_amdgcn_exp2f(s_m[i][r] - base);
-        ls = fmaf(s_l[i][r], c, ls), os = fmaf(s_o[i][r][d], c, os);
-      }
-      if (n_splits == 1) {
-        const float y = ls == 0.f ? 0.f : os / ls;  // nothing seen
-        const int64_t to = (((int64_t)b * a.n_draft + row / a.group) * a.n_kv_heads * a.group + h * a.group + row % a.group) * 128 + d;
-        if constexpr (BF16) ((uint16_t *)a.out)[to] = pkv_f32_to_bf16_bits(y);
-        else ((float *)a.out)[to] = y;
-      } else {
-        const int64_t at = ((int64_t)bh * n_splits + split) * rows + row;
-        a.ws_o[at * 128 + d] = os;
-        if (d == 0) a.ws_ml[at * 2] = mx, a.ws_ml[at * 2 + 1] = ls;
-      }
+    put(ahead[0], 0);
+    __syncthreads();
+    const int here = count - key_wave * W::kKeys < W::kKeys ? count - key_wave * W::kKeys : W::kKeys;
+    if (here > 0) {
+      get_k(0);
+      tree_masked_step<BF16, true, NT>(w, a, b, draft ? dv : nullptr, first + key_wave * W::kKeys, here, token,
+                                       (float(*)[33])(lds + 2 * kTensor + wave * 2112), k, v_of(0));
     }
+    if (!whole) turn0 += n_splits;
   }
+  tree_finish<BF16, true, NT, RW, kWideWaves>(w, a, part, *(float(*)[kWideWaves][16])lds, *(float(*)[kWideWaves][16])(lds + kWideWaves * 64),
+                                        *(float(*)[kWideWaves][16][132])(lds + kWideWaves * 128));
 }
 
 // One wave a query row: lane l weighs split l and holds dims 2 l, 2 l + 1 of the output.
@@ -336,36 +703,45 @@ __global__ __launch_bounds__(256) void pkv_tree_merge_kernel(const float *__rest
   const float c = __builtin_amdgcn_exp2f(m - base), all = pkv_wave_sum(l * c);
   const float weight = all == 0.f ? 0.f : c / all;
   float x = 0.f, y = 0.f;
-  for (int s = 0; s < n_splits; ++s) {
-    const float2 o = *(const float2 *)(ws_o + (first + (int64_t)s * rows) * 128 + 2 * lane);
-    const float f = __shfl(weight, s, PKV_WAVE);
-    x = fmaf(o.x, f, x), y = fmaf(o.y, f, y);
+  for (int s = 0; s < n_splits; s += 16) {
+    float2 o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      o[i] = s + i < n_splits ? *(const float2 *)(ws_o + (first + (int64_t)(s + i) * rows) * 128 + 2 * lane) : float2{0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float f = s + i < n_splits ? __shfl(weight, s + i, PKV_WAVE) : 0.f;
+      x = fmaf(o[i].x, f, x), y = fmaf(o[i].y, f, y);
+    }
   }
   const int64_t to = (((int64_t)b * n_draft + row / group) * n_kv_heads * group + h * group + row % group) * 128 + 2 * lane;
-  if constexpr (BF16) *(uint32_t *)((uint16_t *)out + to) = pack_bf16x2(x, y);
+  if constexpr (BF16) *(uint32_t *)((uint16_t *)out + to) = tree_pack(x, y);
   else *(float2 *)((float *)out + to) = float2{x, y};
 }
 
 struct TreePlan {
-  int nt, row_tiles, n_splits;
-  uint32_t per_split;
+  int nt, rw, row_tiles, n_splits;
 };
 
 TreePlan tree_plan(int dtype, int bs, int n_kv_heads, int rows, int64_t total) {
   TreePlan p;
   const bool bf = dtype == PKV_DTYPE_BF16;
-  p.nt = 1;
-  p.row_tiles = (rows + 16 * p.nt - 1) / (16 * p.nt);
-  const int step = kTreeWaves * (bf ? 32 : 16);
-  int64_t s = 1024 / ((int64_t)bs * n_kv_heads * p.row_tiles), most = (total + step - 1) / step;
-  if (s > most) s = most;
-  if (s > kTreeMaxSplits) s = kTreeMaxSplits;
-  if (s < 1) s = 1;
-  int64_t per = (total + s - 1) / s;
-  per = (per + step - 1) / step * step;
-  if (per < step) per = step;
-  p.per_split = (uint32_t)per;
-  p.n_splits = (int)(total > 0 ? (total + per - 1) / per : 1);
+  p.rw = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t bh = (int64_t)bs * n_kv_heads;
+  auto split = [&](int nt) {
+    p.nt = nt;
+    const int per_wg = 16 * nt * p.rw, turn = (p.rw == 1 ? kTreeWaves : kWideWaves / p.rw) * (bf ? 32 : 16);  // keys a workgroup takes at a time
+    p.row_tiles = (rows + per_wg - 1) / per_wg;
+    int64_t s = kTreeWorkgroups / (bh * p.row_tiles), most = (total + turn - 1) / turn;
+    if (s > most) s = most;
+    if (s > kTreeMaxSplits) s = kTreeMaxSplits;
+    p.n_splits = (int)(s < 1 ? 1 : s);
+  };
+  split(1);
+  if (bf && rows > 64) {
+    split(2);
+    if (total / p.n_splits < 1024) split(1);
+  }
   return p;
 }
 
@@ -397,6 +773,8 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
   const int64_t strides[] = {a->q_stride_b, a->q_stride_t, a->dk_stride_b, a->dk_stride_h, a->dk_stride_t,
                              a->dv_stride_b, a->dv_stride_h, a->dv_stride_t};
   for (int64_t x : strides) PKV_REQUIRE(x % vec == 0 && x >= 0, "pkv_tree_attention: strides must be multiples of 16 bytes");
+  PKV_REQUIRE((a->n_draft - 1) * a->dk_stride_t * es < ((int64_t)1 << 32) && (a->n_draft - 1) * a->dv_stride_t * es < ((int64_t)1 << 32),
+              "pkv_tree_attention: a sequence's drafted rows must lie within 4 GiB");
   PKV_REQUIRE(!a->mask || (a->mask_stride_b >= 0 && a->mask_stride_t >= 0), "pkv_tree_attention: bad mask strides");
   PKV_REQUIRE(!a->row_keys || pkv_aligned(a->row_keys, 4), "pkv_tree_attention: row_keys must be int32");
   AttSegs sg;
@@ -417,7 +795,7 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
   memset(&c, 0, sizeof c);
   c.q = a->q, c.q_stride_b = a->q_stride_b, c.q_stride_t = a->q_stride_t;
   c.n_kv_heads = a->n_kv_heads, c.group = a->group, c.n_draft = a->n_draft;
-  c.total = (uint32_t)total, c.per_split = p.per_split, c.row_keys = a->row_keys;
+  c.total = (uint32_t)total, c.row_keys = a->row_keys;
   c.dk = (const char *)a->draft_k, c.dk_b = a->dk_stride_b * es, c.dk_h = a->dk_stride_h * es, c.dk_t = a->dk_stride_t * es;
   c.dv = (const char *)a->draft_v, c.dv_b = a->dv_stride_b * es, c.dv_h = a->dv_stride_h * es, c.dv_t = a->dv_stride_t * es;
   c.mask = a->mask, c.mask_b = a->mask_stride_b, c.mask_t = a->mask_stride_t;
@@ -427,16 +805,31 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
   AttOne one;
   const bool is_one = as_one_tensor(sg, (int)es, one);
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)p.n_splits, (unsigned)p.row_tiles, (unsigned)(a->bs * a->n_kv_heads)), block(kTreeWaves * PKV_WAVE);
-#define PKV_TREE(BF, NT, IDX, S) hipLaunchKernelGGL((pkv_tree_partial_kernel<BF, NT, IDX, decltype(S)>), grid, block, 0, s, c, S)
-#define PKV_TREE_S(BF, NT)                                                            \
-  do {                                                                                \
-    if (is_one) { if (indexed) PKV_TREE(BF, NT, true, one); else PKV_TREE(BF, NT, false, one); } \
-    else { if (indexed) PKV_TREE(BF, NT, true, sg); else PKV_TREE(BF, NT, false, sg); }          \
+  c.n_splits = p.n_splits, c.row_tiles = p.row_tiles, c.n_pairs = a->bs * a->n_kv_heads * p.n_splits;
+  const dim3 grid(tree_grid(c));
+  const dim3 block((p.rw == 1 ? kTreeWaves : kWideWaves) * PKV_WAVE);
+#define PKV_TREE(IDX, S)                                                                                             \
+  do {                                                                                                               \
+    if (p.rw == 1) PKV_TREE_LAUNCH((pkv_tree_partial_kernel<BF, IDX, decltype(S)>), S);                              \
+    else if (p.rw == 2) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 2, IDX, decltype(S)>), S);                      \
+    else if (p.nt == 1) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 4, IDX, decltype(S)>), S);                      \
+    else PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 2, 4, IDX, decltype(S)>), S);                                     \
   } while (0)
-  if (bf) PKV_TREE_S(true, 1);
-  else PKV_TREE_S(false, 1);
+#define PKV_TREE_LAUNCH(KERNEL, S) hipLaunchKernelGGL(KERNEL, grid, block, 0, s, c, S)
+#define PKV_TREE_S                                                              \
+  do {                                                                          \
+    if (is_one) { if (indexed) PKV_TREE(true, one); else PKV_TREE(false, one); } \
+    else { if (indexed) PKV_TREE(true, sg); else PKV_TREE(false, sg); }          \
+  } while (0)
+  if (bf) {
+    constexpr bool BF = true;
+    PKV_TREE_S;
+  } else {
+    constexpr bool BF = false;
+    PKV_TREE_S;
+  }
 #undef PKV_TREE_S
+#undef PKV_TREE_LAUNCH
 #undef PKV_TREE
   PKV_LAUNCH_CHECK("pkv_tree_partial_kernel");
   if (p.n_splits == 1) return PKV_OK;

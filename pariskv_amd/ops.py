@@ -10,6 +10,7 @@ streams only; every computation happens in ``libpariskv_hip.so``.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional, Sequence
 
 import math
@@ -723,34 +724,6 @@ def gather_uva_packed(src_k, src_v, k_packed, v_packed, indices_packed, cu_seqle
 # --------------------------------------------------------- decode attention
 
 
-def _fill_segments(segs, segments, bs: int, H: int, dtype: torch.dtype, least: int) -> int:
-    """Validate the rows an attention reads and fill the C segment array ``segs``; returns how many there are."""
-    _need(least <= len(segments) <= 4, f"{least}..4 key segments")
-    total = 0
-    for i, seg in enumerate(segments):
-        k, v, row0, n_rows = seg[:4]
-        idx = seg[4] if len(seg) > 4 else None
-        _cuda(k, v)
-        _need(k.dtype == dtype and v.dtype == dtype, "q, k, v must share a dtype")
-        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.shape[3] == HEAD_DIM and
-              k.stride(3) == 1 and k.stride(2) == HEAD_DIM and tuple(k.shape[:2]) == (bs, H),
-              "k, v: [bs,Hkv,rows,128] with contiguous rows")
-        segs[i].k, segs[i].v = _p(k), _p(v)
-        segs[i].stride_b, segs[i].stride_h = k.stride(0), k.stride(1)
-        segs[i].row0, segs[i].n_rows = row0, n_rows
-        total += n_rows
-        if idx is None:
-            _need(0 <= row0 and row0 + n_rows <= k.shape[2], "segment rows out of range")
-            segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = None, 0, 0
-        else:  # the segment's rows are row0 + idx[b, h, :n_rows], read where they lie
-            _cuda(idx)
-            _need(idx.dtype == torch.int64 and idx.is_contiguous() and idx.dim() == 3 and
-                  tuple(idx.shape[:2]) == (bs, H) and idx.shape[2] >= n_rows and 0 <= row0 < k.shape[2],
-                  "segment indices: contiguous int64 [bs,Hkv,>=n_rows]")
-            segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = _p(idx), idx.shape[2], k.shape[2] - row0
-    return total
-
-
 class DecodeAttention:
     """softmax(q k^T * scale) v for one query token per sequence over up to four row segments of
     [bs, Hkv, rows, 128] K/V tensors, read in place (cache_hub/polar_cache.py:1084-1105)."""
@@ -784,7 +757,27 @@ class DecodeAttention:
         """Validate and fill the C segment array `segs`; returns (segs, out, scale)."""
         _cuda(q)
         _need(q.shape[-1] == HEAD_DIM and q.numel() == self.bs * self.H * self.G * HEAD_DIM, "queries: [bs,1,Hq,128]")
-        _fill_segments(segs, segments, self.bs, self.H, q.dtype, 1)
+        _need(1 <= len(segments) <= 4, "1..4 key segments")
+        for i, seg in enumerate(segments):
+            k, v, row0, n_rows = seg[:4]
+            idx = seg[4] if len(seg) > 4 else None
+            _cuda(k, v)
+            _need(k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v must share a dtype")
+            _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.shape[3] == HEAD_DIM and
+                  k.stride(3) == 1 and k.stride(2) == HEAD_DIM and tuple(k.shape[:2]) == (self.bs, self.H),
+                  "k, v: [bs,Hkv,rows,128] with contiguous rows")
+            segs[i].k, segs[i].v = _p(k), _p(v)
+            segs[i].stride_b, segs[i].stride_h = k.stride(0), k.stride(1)
+            segs[i].row0, segs[i].n_rows = row0, n_rows
+            if idx is None:
+                _need(0 <= row0 and row0 + n_rows <= k.shape[2], "segment rows out of range")
+                segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = None, 0, 0
+            else:  # the segment's rows are row0 + idx[b, h, :n_rows], read where they lie
+                _cuda(idx)
+                _need(idx.dtype == torch.int64 and idx.is_contiguous() and idx.dim() == 3 and
+                      tuple(idx.shape[:2]) == (self.bs, self.H) and idx.shape[2] >= n_rows and 0 <= row0 < k.shape[2],
+                      "segment indices: contiguous int64 [bs,Hkv,>=n_rows]")
+                segs[i].idx, segs[i].idx_stride, segs[i].idx_limit = _p(idx), idx.shape[2], k.shape[2] - row0
         if out is None:
             out = torch.empty_like(q)
         if scale is None:
@@ -840,48 +833,97 @@ class TreeAttention:
         in their concatenated order, a row sees (0 or less: none).  Returns [bs,T,Hq,128]; a token that sees nothing gets zeros, and
         what a token does not see does not touch it, whatever it holds."""
         bs, H, G = self.bs, self.H, self.G
-        _need(queries.dim() == 4 and queries.shape[0] == bs and queries.shape[2:] == (H * G, HEAD_DIM) and
-              1 <= queries.shape[1] <= self.max_draft, "queries: [bs,T,Hq,128], 1 <= T <= max_draft")
-        T, dt = queries.shape[1], queries.dtype
-        _need(tuple(draft_k.shape) == (bs, T, H, HEAD_DIM) and draft_v.shape == draft_k.shape and draft_k.dtype == dt and
-              draft_v.dtype == dt, "draft_k, draft_v: [bs,T,Hkv,128] of the queries' type")
-        _cuda(queries, draft_k, draft_v, mask, row_keys, out)
-        _one_device(queries, draft_k, draft_v, mask, row_keys, out, *(t for seg in segments for t in (seg[0], seg[1], *seg[4:])))
-        vec = 16 // queries.element_size()
+        shape, dt, at = tuple(queries.shape), queries.dtype, queries.get_device()
+        T = shape[1] if len(shape) == 4 else 0
+        if shape != (bs, T, H * G, HEAD_DIM) or not 1 <= T <= self.max_draft:
+            raise RuntimeError("queries: [bs,T,Hq,128], 1 <= T <= max_draft")
+        code = _dt(dt)
+        rows = (bs, T, H, HEAD_DIM)
+        if tuple(draft_k.shape) != rows or tuple(draft_v.shape) != rows or draft_k.dtype != dt or draft_v.dtype != dt:
+            raise RuntimeError("draft_k, draft_v: [bs,T,Hkv,128] of the queries' type")
+        if at < 0 or draft_k.get_device() != at or draft_v.get_device() != at:
+            _cuda(queries, draft_k, draft_v)
+            _one_device(queries, draft_k, draft_v)
+        odd = 7 if code == _lib.DTYPE_BF16 else 3  # strides that are not multiples of 16 bytes
 
-        def rows(t, heads_apart):  # 16-byte aligned rows, or a copy
-            if t.stride(3) != 1 or t.data_ptr() % 16 or any(x % vec for x in t.stride()[:3]) or (heads_apart and t.stride(2) != HEAD_DIM):
-                t = t.clone(memory_format=torch.contiguous_format)
-            return t
-
-        q, dk, dv = rows(queries, True), rows(draft_k, False), rows(draft_v, False)
-        a = _lib.TreeArgs()
-        a.q, a.dtype, a.bs, a.n_kv_heads, a.group, a.n_draft = q.data_ptr(), _dt(dt), bs, H, G, T
-        a.q_stride_b, a.q_stride_t = q.stride()[:2]
-        a.draft_k, a.draft_v = dk.data_ptr(), dv.data_ptr()
-        a.dk_stride_b, a.dk_stride_t, a.dk_stride_h = dk.stride()[:3]
-        a.dv_stride_b, a.dv_stride_t, a.dv_stride_h = dv.stride()[:3]
-        total = _fill_segments(a.segments, segments, bs, H, dt, 0)
+        q, qs = queries, queries.stride()
+        if qs[3] != 1 or qs[2] != HEAD_DIM or (qs[0] | qs[1]) & odd or q.data_ptr() & 15:
+            q = q.clone(memory_format=torch.contiguous_format)
+            qs = q.stride()
+        dk, ks = draft_k, draft_k.stride()
+        if ks[3] != 1 or (ks[0] | ks[1] | ks[2]) & odd or dk.data_ptr() & 15:
+            dk = dk.clone(memory_format=torch.contiguous_format)
+            ks = dk.stride()
+        dv, vs = draft_v, draft_v.stride()
+        if vs[3] != 1 or (vs[0] | vs[1] | vs[2]) & odd or dv.data_ptr() & 15:
+            dv = dv.clone(memory_format=torch.contiguous_format)
+            vs = dv.stride()
+        n_seg = len(segments)
+        _need(n_seg <= 4, "0..4 key segments")
+        segs, total = [], 0
+        for i, seg in enumerate(segments):
+            k, v, row0, n_rows = seg[:4]
+            idx = seg[4] if len(seg) > 4 else None
+            ss, kshape = k.stride(), k.shape
+            if k.get_device() != at or v.get_device() != at:
+                _cuda(k, v)
+                _one_device(queries, k, v)
+            if k.dtype != dt or v.dtype != dt:
+                raise RuntimeError("q, k, v must share a dtype")
+            if (len(kshape) != 4 or v.shape != kshape or v.stride() != ss or kshape[3] != HEAD_DIM or ss[3] != 1 or ss[2] != HEAD_DIM or
+                    kshape[0] != bs or kshape[1] != H):
+                raise RuntimeError("k, v: [bs,Hkv,rows,128] with contiguous rows")
+            total += n_rows
+            if idx is None:
+                if row0 < 0 or n_rows < 0 or row0 + n_rows > kshape[2]:
+                    raise RuntimeError("segment rows out of range")
+                segs += (k.data_ptr(), v.data_ptr(), ss[0], ss[1], row0, n_rows, 0, 0, 0)
+            else:  # the segment's rows are row0 + idx[b, h, :n_rows], read where they lie
+                _cuda(idx)
+                _one_device(queries, idx)
+                _need(idx.dtype == torch.int64 and idx.is_contiguous() and idx.dim() == 3 and tuple(idx.shape[:2]) == (bs, H) and
+                      0 <= n_rows <= idx.shape[2] and 0 <= row0 < kshape[2], "segment indices: contiguous int64 [bs,Hkv,>=n_rows]")
+                segs += (k.data_ptr(), v.data_ptr(), ss[0], ss[1], row0, n_rows, idx.data_ptr(), idx.shape[2], kshape[2] - row0)
+        segs += _NO_SEGMENTS[9 * n_seg:]
         _need(total <= self.max_keys, "more cached keys than max_keys")
-        a.n_segments = len(segments)
+        mask_at = mask_b = mask_t = keys_at = 0
         if mask is not None:
-            _need(mask.dtype == torch.bool and tuple(mask.shape) in ((T, T), (bs, T, T)), "mask: bool [T,T] or [bs,T,T]")
+            mshape = tuple(mask.shape)
+            _need(mask.dtype == torch.bool and mshape in ((bs, T, T), (T, T)), "mask: bool [T,T] or [bs,T,T]")
+            if mask.get_device() != at:
+                _cuda(mask)
+                _one_device(queries, mask)
             if mask.stride(-1) != 1:
                 mask = mask.contiguous()
-            a.mask, a.mask_stride_b, a.mask_stride_t = mask.data_ptr(), mask.stride(0) if mask.dim() == 3 else 0, mask.stride(-2)
+            mask_at, mask_t, mask_b = mask.data_ptr(), mask.stride(-2), mask.stride(0) if len(mshape) == 3 else 0
         if row_keys is not None:
+            _cuda(row_keys)
+            _one_device(queries, row_keys)
             _need(row_keys.dtype == torch.int32 and row_keys.is_contiguous() and row_keys.numel() == bs * H, "row_keys: contiguous int32 [bs,Hkv]")
-            a.row_keys = row_keys.data_ptr()
+            keys_at = row_keys.data_ptr()
         if out is None:
-            out = torch.empty(bs, T, H * G, HEAD_DIM, dtype=dt, device=queries.device)
-        _need(tuple(out.shape) == (bs, T, H * G, HEAD_DIM) and out.dtype == dt and out.is_contiguous(), "out: contiguous, like queries")
-        a.scale, a.out = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale), out.data_ptr()
+            out = queries.new_empty(shape)
+        else:
+            _cuda(out)
+            _one_device(queries, out)
+            _need(tuple(out.shape) == shape and out.dtype == dt and out.is_contiguous() and out.data_ptr() % 16 == 0, "out: contiguous, like queries")
         lib = _lib.lib()
-        a.ws_bytes = lib.pkv_tree_attention_ws_bytes(a.dtype, bs, H, G, T, total)
-        ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=queries.device) if a.ws_bytes else None
-        a.ws = _p(ws)
-        _lib.check(lib.pkv_tree_attention(C.byref(a), _stream(queries)))
+        need = lib.pkv_tree_attention_ws_bytes(code, bs, H, G, T, total)
+        ws = queries.new_empty(need, dtype=torch.uint8) if need else None
+        block = _TREE_BLOCK.pack(q.data_ptr(), code, bs, H, G, T, qs[0], qs[1], *segs, n_seg, keys_at, dk.data_ptr(), dv.data_ptr(),
+                                 ks[0], ks[2], ks[1], vs[0], vs[2], vs[1], mask_at, mask_b, mask_t,
+                                 _SCALE if scale is None else scale, out.data_ptr(), ws.data_ptr() if need else 0, need)
+        rc = lib.pkv_tree_attention(block, _stream(queries))
+        if rc != 0:
+            _lib.check(rc)
         return out
+
+
+# pkv_tree_args as one packed block: filled field by field it takes the host 9 us of a call that the GPU answers in 15.
+_TREE_BLOCK = struct.Struct("@P5i2q" + "PP4qP2q" * 4 + "iPPP6qPqqfPPN")
+assert _TREE_BLOCK.size == C.sizeof(_lib.TreeArgs)
+_NO_SEGMENTS = (0,) * 36
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
 def qk_norm_rope(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, q_weight, k_weight, eps: float,
@@ -1019,39 +1061,53 @@ def w4_quantize(weight: torch.Tensor, group_size: int = 128):
     return codes, scales, zeros
 
 
-def _w4_rows(x: torch.Tensor, k: int):
-    """x [..., k] as rows that the kernels can read: 16-byte aligned, a multiple of 8 elements apart."""
-    _need(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() >= 1 and x.shape[-1] == k, f"x: bf16 [..., {k}] on the GPU")
-    x = x if x.dim() == 2 else x.reshape(-1, k)
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < k)):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+def _w4_rows(x: torch.Tensor, k: int, at: int):
+    """x [..., k] as rows that the kernels can read (16-byte aligned, a multiple of 8 elements apart), and their shape and stride."""
+    shape = x.shape
+    if x.dtype != torch.bfloat16 or len(shape) < 1 or shape[-1] != k or x.get_device() != at:
+        _need(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() >= 1 and shape[-1] == k, f"x: bf16 [..., {k}] on the GPU")
+        raise RuntimeError("tensors of one launch are on different GPUs")
+    rows = x if len(shape) == 2 else x.reshape(-1, k)
+    n, (step, unit) = rows.shape[0], rows.stride()
+    if unit != 1 or rows.data_ptr() & 15 or (n > 1 and (step & 7 or step < k)):
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        step = k
+    return rows, n, step, shape
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., k] (bf16) times the transpose of a 4-bit matrix, plus ``bias`` (bf16 [n]): [..., n] in ``out_dtype`` (bf16, the default,
     or fp32).  fp32 sums, one rounding; for the few rows of a decode step or of its drafted tokens."""
-    rows = _w4_rows(x, weight.k)
-    _one_device(rows, weight.packed, bias)
-    _need(bias is None or (bias.is_cuda and bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == weight.n), "bias: contiguous bf16 [n]")
-    y = torch.empty(*x.shape[:-1], weight.n, dtype=out_dtype or torch.bfloat16, device=x.device)
-    dt = _dt(y.dtype)
-    if rows.shape[0] > 0:
-        _lib.check(_lib.lib().pkv_w4_linear(_p(rows), rows.stride(0), rows.shape[0], _p(weight.packed), weight.n, weight.k,
-                                            weight.group_size, _p(bias), _p(y), dt, _stream(rows)))
+    packed = weight.packed
+    rows, m, step, shape = _w4_rows(x, weight.k, packed.get_device())
+    n = weight.n
+    if bias is not None:
+        _one_device(packed, bias)
+        _need(bias.is_cuda and bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == n, "bias: contiguous bf16 [n]")
+    code = _lib.DTYPE_BF16 if out_dtype is None else _dt(out_dtype)
+    y = x.new_empty((*shape[:-1], n)) if code == _lib.DTYPE_BF16 else x.new_empty((*shape[:-1], n), dtype=torch.float32)
+    if m > 0:
+        rc = _lib.lib().pkv_w4_linear(rows.data_ptr(), step, m, packed.data_ptr(), n, weight.k, weight.group_size,
+                                      None if bias is None else bias.data_ptr(), y.data_ptr(), code, _stream(packed))
+        if rc != 0:
+            _lib.check(rc)
     return y
 
 
 def w4_silu_mul(x: torch.Tensor, gate: W4Weight, up: W4Weight) -> torch.Tensor:
     """silu(x gate^T) * (x up^T), bf16 [..., n]: both projections of the gated feed-forward block, the activation and the product in one
     launch (model_hub/qwen.py:365-383 with 4-bit weights); nothing is rounded in between, unlike :func:`silu_mul` of a bf16 product."""
-    rows = _w4_rows(x, gate.k)
-    _one_device(rows, gate.packed, up.packed)
-    _need(gate.shape == up.shape and gate.group_size == up.group_size, "gate and up: matrices of one shape and group size")
-    y = torch.empty(*x.shape[:-1], gate.n, dtype=torch.bfloat16, device=x.device)
-    if rows.shape[0] > 0:
-        _lib.check(_lib.lib().pkv_w4_silu_mul(_p(rows), rows.stride(0), rows.shape[0], _p(gate.packed), _p(up.packed), gate.n, gate.k,
-                                              gate.group_size, _p(y), _stream(rows)))
+    packed = gate.packed
+    rows, m, step, shape = _w4_rows(x, gate.k, packed.get_device())
+    if gate.n != up.n or gate.k != up.k or gate.group_size != up.group_size:
+        raise RuntimeError("gate and up: matrices of one shape and group size")
+    _one_device(packed, up.packed)
+    y = x.new_empty((*shape[:-1], gate.n))
+    if m > 0:
+        rc = _lib.lib().pkv_w4_silu_mul(rows.data_ptr(), step, m, packed.data_ptr(), up.packed.data_ptr(), gate.n, gate.k, gate.group_size,
+                                        y.data_ptr(), _stream(packed))
+        if rc != 0:
+            _lib.check(rc)
     return y
 
 

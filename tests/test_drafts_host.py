@@ -99,12 +99,12 @@ def test_tree_attention_entry_point_checks_its_arguments():
                                 (dict(q_stride_t=1028), _lib.EINVAL, b"strides"), (dict(dk_stride_b=-8), _lib.EINVAL, b"strides"),
                                 (dict(mask=8, mask_stride_t=-5), _lib.EINVAL, b"mask"), (dict(row_keys=6), _lib.EINVAL, b"row_keys")):
         a = args(**change)
-        assert L.pkv_tree_attention(a, None) == code and words in L.pkv_last_error(), (change, L.pkv_last_error())
+        assert L.pkv_tree_attention(ctypes.byref(a), None) == code and words in L.pkv_last_error(), (change, L.pkv_last_error())
     a = args()
     a.segments[0].n_rows = 1 << 23
-    assert L.pkv_tree_attention(a, None) == _lib.EINVAL and b"2^23" in L.pkv_last_error()
+    assert L.pkv_tree_attention(ctypes.byref(a), None) == _lib.EINVAL and b"2^23" in L.pkv_last_error()
     a.segments[0].n_rows, a.segments[0].stride_h = 5000, 4
-    assert L.pkv_tree_attention(a, None) == _lib.EINVAL
+    assert L.pkv_tree_attention(ctypes.byref(a), None) == _lib.EINVAL
     assert L.pkv_tree_attention_ws_bytes(1, 1, 1, 1, 1, 0) == 0 and L.pkv_tree_attention_ws_bytes(1, 0, 1, 1, 1, 100) == 0
     assert L.pkv_tree_attention_ws_bytes(1, 1, 8, 4, 5, 100000) > 0
 
