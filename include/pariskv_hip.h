@@ -580,15 +580,17 @@ int pkv_w4_quantize(const void *w, int dtype, int64_t row_stride, int64_t n, int
 int pkv_w4_unpack(const void *packed, int64_t n, int64_t k, int group, float *w, void *stream);
 
 /* y[m][n] = sum_k x[m][k] weight[n][k] + bias[n] (no counterpart in the reference): x bf16 [rows][k] (row stride in elements, a
- * multiple of 8, 16-byte aligned), bias bf16 [n] or NULL, y [rows][n] contiguous of out_dtype.  Sums in fp32, one rounding. */
+ * multiple of 8, 16-byte aligned), bias bf16 [n] or NULL, y [rows][n] contiguous of out_dtype.  Sums in fp32, one rounding.
+ * ws: pkv_w4_ws_bytes(rows, n, k, group, 0) bytes for the shares of columns that several workgroups take (0: none needed). */
+size_t pkv_w4_ws_bytes(int64_t rows, int64_t n, int64_t k, int group, int gated);
 int pkv_w4_linear(const void *x, int64_t x_stride, int64_t rows, const void *packed, int64_t n, int64_t k, int group,
-                  const void *bias, void *y, int out_dtype, void *stream);
+                  const void *bias, void *y, int out_dtype, void *ws, size_t ws_bytes, void *stream);
 
 /* y[m][j] = silu(x[m] . gate[j]) * (x[m] . up[j]), bf16 [rows][n] contiguous: both projections of the gated feed-forward block,
  * the activation and the product in one launch (model_hub/qwen.py:365-383 with 4-bit weights).  gate and up: two matrices
- * [n][k] as stored above, of one group size.  fp32 until the one rounding of y. */
+ * [n][k] as stored above, of one group size.  fp32 until the one rounding of y.  ws: pkv_w4_ws_bytes(rows, n, k, group, 1). */
 int pkv_w4_silu_mul(const void *x, int64_t x_stride, int64_t rows, const void *gate, const void *up, int64_t n, int64_t k, int group,
-                    void *y, void *stream);
+                    void *y, void *ws, size_t ws_bytes, void *stream);
 
 /* ------------------------------------------------------- fused decode step */
 

@@ -187,8 +187,9 @@ PROTOTYPES = {
     "pkv_w4_pack": (_i, [_vp, _vp, _vp, _i64, _i64, _i, _vp, _vp]),
     "pkv_w4_quantize": (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _vp]),
     "pkv_w4_unpack": (_i, [_vp, _i64, _i64, _i, _vp, _vp]),
-    "pkv_w4_linear": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i, _vp]),
-    "pkv_w4_silu_mul": (_i, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i, _vp, _vp]),
+    "pkv_w4_ws_bytes": (_sz, [_i64, _i64, _i64, _i, _i]),
+    "pkv_w4_linear": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i, _vp, _sz, _vp]),
+    "pkv_w4_silu_mul": (_i, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i, _vp, _vp, _sz, _vp]),
     "pkv_decode_attention": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnSegment), _i, _vp, C.c_float, _vp, _vp, _sz, _vp]),
     "pkv_qk_norm_rope": (_i, [_vp, _i64, _i, _i, _i, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp]),
     "pkv_add_rmsnorm": (_i, [_vp, _vp, _vp, C.c_float, _i, _i, _vp, _vp, _vp]),

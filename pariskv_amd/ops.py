@@ -1087,8 +1087,11 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     code = _lib.DTYPE_BF16 if out_dtype is None else _dt(out_dtype)
     y = x.new_empty((*shape[:-1], n)) if code == _lib.DTYPE_BF16 else x.new_empty((*shape[:-1], n), dtype=torch.float32)
     if m > 0:
-        rc = _lib.lib().pkv_w4_linear(rows.data_ptr(), step, m, packed.data_ptr(), n, weight.k, weight.group_size,
-                                      None if bias is None else bias.data_ptr(), y.data_ptr(), code, _stream(packed))
+        lib = _lib.lib()
+        need = lib.pkv_w4_ws_bytes(m, n, weight.k, weight.group_size, 0)
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
+        rc = lib.pkv_w4_linear(rows.data_ptr(), step, m, packed.data_ptr(), n, weight.k, weight.group_size,
+                               None if bias is None else bias.data_ptr(), y.data_ptr(), code, _p(ws), need, _stream(packed))
         if rc != 0:
             _lib.check(rc)
     return y
@@ -1104,8 +1107,11 @@ def w4_silu_mul(x: torch.Tensor, gate: W4Weight, up: W4Weight) -> torch.Tensor:
     _one_device(packed, up.packed)
     y = x.new_empty((*shape[:-1], gate.n))
     if m > 0:
-        rc = _lib.lib().pkv_w4_silu_mul(rows.data_ptr(), step, m, packed.data_ptr(), up.packed.data_ptr(), gate.n, gate.k, gate.group_size,
-                                        y.data_ptr(), _stream(packed))
+        lib = _lib.lib()
+        need = lib.pkv_w4_ws_bytes(m, gate.n, gate.k, gate.group_size, 1)
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
+        rc = lib.pkv_w4_silu_mul(rows.data_ptr(), step, m, packed.data_ptr(), up.packed.data_ptr(), gate.n, gate.k, gate.group_size,
+                                 y.data_ptr(), _p(ws), need, _stream(packed))
         if rc != 0:
             _lib.check(rc)
     return y

@@ -171,12 +171,12 @@ def test_w4_refusals():
             ops.w4_quantize(m, g)
     L = _lib.lib()
     A = 1 << 20
-    for args, words in (((A, 128, 4, None, 16, 128, 128, None, A, 1, None), b"weights"), ((A, 128, 4, A, 16, 100, 32, None, A, 1, None), b"groups"),
-                        ((A, 128, 4, A, 16, 128, 128, None, A, 5, None), b"dtype"), ((A, 128, 0, A, 16, 128, 128, None, A, 1, None), b"row count"),
-                        ((A, 120, 4, A, 16, 128, 128, None, A, 1, None), b"overlap"), ((A, 129, 4, A, 16, 128, 128, None, A, 1, None), b"aligned"),
-                        ((A + 2, 128, 4, A, 16, 128, 128, None, A, 1, None), b"aligned"), ((None, 128, 4, A, 16, 128, 128, None, A, 1, None), b"null")):
+    for args, words in (((A, 128, 4, None, 16, 128, 128, None, A, 1, None, 0, None), b"weights"), ((A, 128, 4, A, 16, 100, 32, None, A, 1, None, 0, None), b"groups"),
+                        ((A, 128, 4, A, 16, 128, 128, None, A, 5, None, 0, None), b"dtype"), ((A, 128, 0, A, 16, 128, 128, None, A, 1, None, 0, None), b"row count"),
+                        ((A, 120, 4, A, 16, 128, 128, None, A, 1, None, 0, None), b"overlap"), ((A, 129, 4, A, 16, 128, 128, None, A, 1, None, 0, None), b"aligned"),
+                        ((A + 2, 128, 4, A, 16, 128, 128, None, A, 1, None, 0, None), b"aligned"), ((None, 128, 4, A, 16, 128, 128, None, A, 1, None, 0, None), b"null")):
         assert L.pkv_w4_linear(*args) == _lib.EINVAL and words in L.pkv_last_error(), (args, L.pkv_last_error())
-    assert L.pkv_w4_silu_mul(A, 128, 4, A, None, 16, 128, 128, A, None) == _lib.EINVAL
+    assert L.pkv_w4_silu_mul(A, 128, 4, A, None, 16, 128, 128, A, None, 0, None) == _lib.EINVAL
     assert L.pkv_w4_pack(A, A, A, 16, 128, 48, A, None) == _lib.EINVAL and L.pkv_w4_unpack(A, 16, 128, 128, None, None) == _lib.EINVAL
     assert L.pkv_w4_quantize(A, 0, 100, 16, 128, 128, A, A, A, None) == _lib.EINVAL
 

@@ -368,6 +368,27 @@ def test_w4_linear_sizes(n, k, group, m):
         assert (y.double().cpu() - want).norm() <= 2.0 ** -20 * want.norm()
 
 
+# a few rows that stay in LDS: all of it, more than a workgroup's share of row tiles, tiles shared by fewer waves; rows that do not fit; columns
+# split over workgroups, with an odd run of chunks at the end and with rows of the result that are not a multiple of four long
+@pytest.mark.parametrize("m,n,k,group", [(13, 50, 4096, 128), (3, 16500, 1024, 128), (2, 20011, 256, 32), (16, 5000, 640, 64), (5, 100, 16384, 128),
+                                         (40, 64, 4224, 128), (20, 131, 8192, 32), (64, 4096, 2048, 64)])
+def test_w4_ways(m, n, k, group):
+    from pariskv_amd import ops
+
+    a, b = w4_case(n + k, n, k, group), w4_case(n, n, k, group)
+    g = torch.Generator().manual_seed(k)
+    x, bias = _randn(g, m, k), _randn(g, n)
+    gx, ha, hb = x.to(DEV), handle(a), handle(b)
+    y = ops.w4_linear(gx, ha, bias.to(DEV), F32)
+    check(y, *exact_linear(x, a, bias, F32))
+    z = ops.w4_silu_mul(gx, ha, hb)
+    (ya, ta), (yb, tb) = exact_linear(x, a, None, F32), exact_linear(x, b, None, F32)
+    want = ya * torch.sigmoid(ya) * yb
+    check(z, want, 1.1 * ta * (yb.abs() + tb) + ya.abs() * tb + 8 * U * want.abs() + HALF[BF] * want.abs() + 1e-37)
+    for _ in range(2):
+        assert torch.equal(y, ops.w4_linear(gx, ha, bias.to(DEV), F32)) and torch.equal(z, ops.w4_silu_mul(gx, ha, hb))
+
+
 def test_w4_linear_layouts_and_odd_values():
     from pariskv_amd import ops
 
