@@ -297,7 +297,8 @@ int pkv_append_kv_run(const pkv_append_args *args, const void *k_new, int64_t k_
  * and likewise for V; t outside [0, n_draft): the row (and its norm) stays as it is, so that sequences that accepted fewer
  * tokens are padded with -1.  vnorm (all layers or none; rows of 128 bf16 or fp32 elements): the value norm as pkv_append_kv
  * writes it, at [b*vn_stride_b + h*vn_stride_h + slot + i].  Strides of rows in BYTES, multiples of 16; of norms in elements;
- * path int64 on the device; `layers` is host memory, read before the call returns.  Drafted rows must not overlap the
+ * path int64 on the device; `layers` is host memory, read before the call returns; layer l's drafted rows are l*k_stride_l (v_) bytes
+ * behind its draft_k (draft_v), so that layers of one tensor can all name its start.  Drafted rows must not overlap the
  * destination rows. */
 typedef struct pkv_path_layer {
   const void *draft_k, *draft_v;
@@ -309,6 +310,7 @@ typedef struct pkv_path_args {
   const int64_t *path;
   int64_t path_stride_b;
   int bs, n_kv_heads, n, n_draft, row_bytes;
+  int64_t k_stride_l, v_stride_l;
   int64_t k_stride_b, k_stride_h, k_stride_t, v_stride_b, v_stride_h, v_stride_t;
   int64_t dst_stride_b, dst_stride_h, dst_len; /* bytes, bytes, rows */
   int64_t vn_stride_b, vn_stride_h;

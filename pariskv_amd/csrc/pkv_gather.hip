@@ -316,7 +316,7 @@ extern "C" int pkv_append_path(const pkv_path_args *a, const pkv_path_layer *lay
               a->row_bytes);
   PKV_REQUIRE((int64_t)a->bs * a->n_kv_heads * a->n * 2 * (a->row_bytes / 16) < ((int64_t)1 << 31), "append_path: too many rows");
   PKV_REQUIRE(pkv_aligned(a->path, 8) && a->path_stride_b >= (a->bs > 1 ? a->n : 0), "append_path: path must be int64 [bs][n]");
-  const int64_t strides[] = {a->k_stride_b, a->k_stride_h, a->k_stride_t, a->v_stride_b, a->v_stride_h, a->v_stride_t,
+  const int64_t strides[] = {a->k_stride_l, a->v_stride_l, a->k_stride_b, a->k_stride_h, a->k_stride_t, a->v_stride_b, a->v_stride_h, a->v_stride_t,
                              a->dst_stride_b, a->dst_stride_h};
   for (int64_t x : strides) PKV_REQUIRE(x % 16 == 0 && x >= 0, "append_path: strides are bytes, multiples of 16");
   PKV_REQUIRE(a->dst_len > 0 && a->dst_stride_h >= a->dst_len * a->row_bytes, "append_path: rows must not overlap");
@@ -338,6 +338,10 @@ extern "C" int pkv_append_path(const pkv_path_args *a, const pkv_path_layer *lay
     PathLayers part;
     memset(&part, 0, sizeof part);
     memcpy(part.layer, layers + at, (size_t)count * sizeof *layers);
+    for (int i = 0; i < count; ++i) {
+      part.layer[i].draft_k = (const char *)part.layer[i].draft_k + (at + i) * a->k_stride_l;
+      part.layer[i].draft_v = (const char *)part.layer[i].draft_v + (at + i) * a->v_stride_l;
+    }
     const dim3 grid((unsigned)(((int64_t)n_tasks * vpr + kGatherThreads - 1) / kGatherThreads), (unsigned)count);
 #define PKV_PATH(VN)                                                                                                         \
   hipLaunchKernelGGL(pkv_append_path_kernel<VN>, grid, dim3(kGatherThreads), 0, (hipStream_t)stream, a->path,                \

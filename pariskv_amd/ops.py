@@ -617,65 +617,78 @@ class PathAppend:
             _need(t.dtype == k0.dtype and t.shape == k0.shape and t.stride() == k0.stride() and t.stride(3) == 1 and t.stride(2) == D,
                   "dst_k, dst_v: [bs,Hkv,rows,D] of one type, shape and layout, with contiguous rows")
         es = k0.element_size()
-        self._a = _lib.PathArgs()
-        self._a.bs, self._a.n_kv_heads, self._a.row_bytes = bs, H, D * es
-        self._a.dst_stride_b, self._a.dst_stride_h, self._a.dst_len = k0.stride(0) * es, k0.stride(1) * es, rows
+        vn_strides = (0, 0)
         if vnorms is not None:
             vnorms = list(vnorms)
             for t in vnorms:
                 _need(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.shape == vnorms[0].shape and
                       tuple(t.shape[:2]) == (bs, H), "vnorms: contiguous fp32 [bs,Hkv,rows] a layer")
-            self._a.vn_stride_b, self._a.vn_stride_h = vnorms[0].stride()[:2]
-        self._np = np
-        self._layers = np.zeros(len(dst_k), dtype=[(f, np.int64) for f, _ in _lib.PathLayer._fields_])
-        self._layers["dst_k"], self._layers["dst_v"] = [t.data_ptr() for t in dst_k], [t.data_ptr() for t in dst_v]
+            vn_strides = vnorms[0].stride()[:2]
+        # what a call adds to the layers' table are its first two columns and its last
+        fields = [f for f, _ in _lib.PathLayer._fields_]
+        self._table = np.zeros((len(dst_k), len(fields)), dtype=np.int64)
+        self._table[:, fields.index("dst_k")] = [t.data_ptr() for t in dst_k]
+        self._table[:, fields.index("dst_v")] = [t.data_ptr() for t in dst_v]
         if vnorms is not None:
-            self._layers["vnorm"] = [t.data_ptr() for t in vnorms]
+            self._table[:, fields.index("vnorm")] = [t.data_ptr() for t in vnorms]
+        self._shape, self._es = (bs, H, D), es
+        self._tail = (k0.stride(0) * es, k0.stride(1) * es, rows, *vn_strides)
         self.keep = (dst_k, dst_v, vnorms)
         self._like = k0
 
     def _rows_of(self, draft):
-        """(addresses of the layers' drafted rows, shape [bs,T,Hkv,D], strides) of a stacked tensor or one tensor a layer."""
-        n = len(self._layers)
+        """(address of the layers' drafted rows, or one a layer, T, strides in bytes: layer, batch, head, token) of a stacked tensor or
+        of one tensor a layer."""
+        like, es = self._like, self._es
         if isinstance(draft, torch.Tensor):
-            _need(draft.dim() == 5 and draft.shape[0] == n, "drafted rows: [layers,bs,T,Hkv,D], or one [bs,T,Hkv,D] a layer")
-            first, shape, strides = draft, tuple(draft.shape[1:]), draft.stride()[1:]
-            at = draft.data_ptr() + self._np.arange(n, dtype=self._np.int64) * (draft.stride(0) * draft.element_size())
+            first, shape, strides, at = draft, draft.shape, draft.stride(), draft.data_ptr()
+            if len(shape) != 5 or shape[0] != len(self._table):
+                raise RuntimeError("drafted rows: [layers,bs,T,Hkv,D], or one [bs,T,Hkv,D] a layer")
         else:
-            _need(len(draft) == n, "drafted rows: one [bs,T,Hkv,D] a layer")
+            _need(len(draft) == len(self._table), "drafted rows: one [bs,T,Hkv,D] a layer")
             first = draft[0]
-            shape, strides = tuple(first.shape), first.stride()
+            shape, strides, at = (0, *first.shape), (0, *first.stride()), []
             for t in draft:
-                _need(tuple(t.shape) == shape and t.stride() == strides and t.dtype == first.dtype, "drafted rows: one shape, layout and type")
+                if t.shape != shape[1:] or t.stride() != strides[1:] or t.dtype != like.dtype:
+                    raise RuntimeError("drafted rows: one shape, layout and type")
+                at.append(t.data_ptr())
             _cuda(*draft)
-            _one_device(self._like, *draft)
-            at = [t.data_ptr() for t in draft]
-        like = self._like
-        _need(first.is_cuda and first.dtype == like.dtype and len(shape) == 4 and shape[0] == like.shape[0] and shape[2] == like.shape[1] and
-              shape[3] == like.shape[3] and strides[3] == 1, "drafted rows: [bs,T,Hkv,D] of the cache's type with contiguous rows")
-        _one_device(like, first)
-        return at, shape, strides
+            _one_device(like, *draft)
+        bs, H, D = self._shape
+        if (first.dtype != like.dtype or not first.is_cuda or len(shape) != 5 or shape[1] != bs or shape[3] != H or shape[4] != D or
+                strides[4] != 1):
+            raise RuntimeError("drafted rows: GPU [bs,T,Hkv,D] of the cache's type with contiguous rows")
+        if first.get_device() != like.get_device():
+            _one_device(like, first)
+        return at, shape[2], strides[0] * es, (strides[1] * es, strides[3] * es, strides[2] * es)
 
     def launch(self, draft_k, draft_v, path: torch.Tensor, slots) -> None:
         """draft_k, draft_v: the drafted rows, [layers,bs,T,Hkv,D] or a sequence of [bs,T,Hkv,D]; path int64 [bs,n] on the GPU: the
         accepted tokens of each sequence in order, -1 where it accepted fewer (such a row stays as it is); slots: the cache row of the
         path's first token, one int or one a layer."""
-        layers, a = self._layers.copy(), _lib.PathArgs.from_buffer_copy(self._a)
-        layers["draft_k"], shape, ks = self._rows_of(draft_k)
-        layers["draft_v"], v_shape, vs = self._rows_of(draft_v)
-        layers["slot"] = slots
-        _need(v_shape == shape, "drafted K and V rows differ in shape")
+        table = self._table.copy()
+        table[:, 0], n_draft, k_layer, ks = self._rows_of(draft_k)
+        table[:, 1], n_v, v_layer, vs = self._rows_of(draft_v)
+        table[:, -1] = slots
+        if n_v != n_draft:
+            raise RuntimeError("drafted K and V rows differ in shape")
         _cuda(path)
         _one_device(self._like, path)
-        _need(path.dtype == torch.int64 and path.dim() == 2 and path.shape[0] == shape[0] and (path.shape[1] == 0 or path.stride(1) == 1),
-              "path: int64 [bs,n]")
-        if path.shape[1] == 0 or shape[0] == 0:
+        bs, H, D = self._shape
+        if path.dtype != torch.int64 or path.dim() != 2 or path.shape[0] != bs or (path.shape[1] > 0 and path.stride(1) != 1):
+            raise RuntimeError("path: int64 [bs,n]")
+        n = path.shape[1]
+        if n == 0 or bs == 0:
             return
-        es = self._like.element_size()
-        a.path, a.path_stride_b, a.n, a.n_draft = path.data_ptr(), path.stride(0), path.shape[1], shape[1]
-        a.k_stride_b, a.k_stride_t, a.k_stride_h = (x * es for x in ks[:3])
-        a.v_stride_b, a.v_stride_t, a.v_stride_h = (x * es for x in vs[:3])
-        _lib.check(_lib.lib().pkv_append_path(C.byref(a), layers.ctypes.data, len(layers), _stream(self._like)))
+        block = _PATH_BLOCK.pack(path.data_ptr(), path.stride(0), bs, H, n, n_draft, D * self._es, k_layer, v_layer, *ks, *vs, *self._tail)
+        rc = _lib.lib().pkv_append_path(block, table.tobytes(), len(table), _stream(self._like))
+        if rc != 0:
+            _lib.check(rc)
+
+
+# pkv_path_args as one packed block
+_PATH_BLOCK = struct.Struct("@Pq5i13q")
+assert _PATH_BLOCK.size == C.sizeof(_lib.PathArgs)
 
 
 OFFLOAD_ONE_COMMAND = 1
@@ -1001,12 +1014,21 @@ class W4Weight:
     """A matrix [n,k] in 4 bits, laid out once for the kernels that read it: weight = scale * (code - zero) with whole codes and zeros
     0..15 and a bf16 scale and a zero for every ``group_size`` (32, 64 or 128) columns of a row; k a multiple of that, any n."""
 
-    __slots__ = ("packed", "n", "k", "group_size")
+    __slots__ = ("packed", "n", "k", "group_size", "_ws_bytes")
 
     def __init__(self, packed: torch.Tensor, n: int, k: int, group_size: int):
         _need(packed.dtype == torch.uint8 and packed.is_cuda and packed.is_contiguous() and
               packed.numel() == _lib.lib().pkv_w4_bytes(n, k, group_size) > 0, "packed: what from_codes or quantize laid out")
         self.packed, self.n, self.k, self.group_size = packed, int(n), int(k), int(group_size)
+        self._ws_bytes = {}
+
+    def ws_bytes(self, rows: int, gated: bool = False) -> int:
+        """Bytes of workspace for a product with so many rows; 0 for most of them."""
+        key = -rows if gated else rows
+        need = self._ws_bytes.get(key)
+        if need is None:
+            need = self._ws_bytes[key] = _lib.lib().pkv_w4_ws_bytes(rows, self.n, self.k, self.group_size, int(gated))
+        return need
 
     @property
     def shape(self):
@@ -1087,10 +1109,9 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     code = _lib.DTYPE_BF16 if out_dtype is None else _dt(out_dtype)
     y = x.new_empty((*shape[:-1], n)) if code == _lib.DTYPE_BF16 else x.new_empty((*shape[:-1], n), dtype=torch.float32)
     if m > 0:
-        lib = _lib.lib()
-        need = lib.pkv_w4_ws_bytes(m, n, weight.k, weight.group_size, 0)
+        need = weight.ws_bytes(m)
         ws = x.new_empty(need, dtype=torch.uint8) if need else None
-        rc = lib.pkv_w4_linear(rows.data_ptr(), step, m, packed.data_ptr(), n, weight.k, weight.group_size,
+        rc = _lib.lib().pkv_w4_linear(rows.data_ptr(), step, m, packed.data_ptr(), n, weight.k, weight.group_size,
                                None if bias is None else bias.data_ptr(), y.data_ptr(), code, _p(ws), need, _stream(packed))
         if rc != 0:
             _lib.check(rc)
@@ -1107,10 +1128,9 @@ def w4_silu_mul(x: torch.Tensor, gate: W4Weight, up: W4Weight) -> torch.Tensor:
     _one_device(packed, up.packed)
     y = x.new_empty((*shape[:-1], gate.n))
     if m > 0:
-        lib = _lib.lib()
-        need = lib.pkv_w4_ws_bytes(m, gate.n, gate.k, gate.group_size, 1)
+        need = gate.ws_bytes(m, gated=True)
         ws = x.new_empty(need, dtype=torch.uint8) if need else None
-        rc = lib.pkv_w4_silu_mul(rows.data_ptr(), step, m, packed.data_ptr(), up.packed.data_ptr(), gate.n, gate.k, gate.group_size,
+        rc = _lib.lib().pkv_w4_silu_mul(rows.data_ptr(), step, m, packed.data_ptr(), up.packed.data_ptr(), gate.n, gate.k, gate.group_size,
                                  y.data_ptr(), _p(ws), need, _stream(packed))
         if rc != 0:
             _lib.check(rc)
