@@ -190,6 +190,7 @@ class polar_cache(KV_Cache):
         self._dense_bound = [None] * layer_num
         self._out_ids = torch.empty((bs, H, max(1, final_topk)), dtype=torch.int64, device=dev)
         self._attention = ops.DecodeAttention(bs, H, self.group_size, self.unified_kv_capacity, dev)
+        self._tree = self._path_plans = None  # made with the first drafted tokens
         self.last_topk_indices = None  # [bs, H, K] of the most recent retrieval (zone-relative), for inspection
 
     # ------------------------------------------------------------- helpers
@@ -620,6 +621,105 @@ class polar_cache(KV_Cache):
         step = (n_keys, bound, topk, out_ids, local_seg)
         self._bound[layer_idx] = step
         return step
+
+    # ------------------------------------------------------------- drafted tokens (no counterpart in the reference)
+    def draft_attend(self, queries, key_states, value_states, layer_idx, mask=None):
+        """Attention of T drafted tokens a sequence that are not in the cache: each attends to what a decode step would attend to (every
+        stored token, or sink, selected and recent ones) and to the drafted tokens its row of ``mask`` names (bool [T,T] or
+        [bs,T,T], :func:`ops.tree_mask`; None: itself and those before it).  queries [bs,T,Hq,D], key_states and value_states
+        [bs,T,Hkv,D] -> [bs,T,Hq,D].  The retrieval runs once for all of a KV head's drafted queries, on their mean: one token alone
+        selects what :meth:`compute` selects for it (except the token that fills the update buffer, which a decode step attends from with
+        the refreshed index).  The cache stays as it is: see :meth:`commit_draft`."""
+        if queries.dim() != 4 or queries.shape[1] == 0:
+            raise RuntimeError("queries: [bs,T,Hq,D] of at least one drafted token")
+        if key_states.dtype != self.dtype or value_states.dtype != self.dtype:
+            key_states, value_states = key_states.to(self.dtype), value_states.to(self.dtype)
+        if self._tree is None:
+            self._tree = ops.TreeAttention(self.batch_size, self.kv_head, self.group_size, min(1024, 8192 // self.group_size),
+                                           self.unified_kv_capacity, self.device)
+        z = self._zones[layer_idx]
+        n_keys = self.cpu_valid_end[layer_idx] if self._layer_offload[layer_idx] else z.encoded
+        if z.seq_len + 1 < self._min_total() or n_keys <= 0:  # as with the first of them appended
+            segments = self._full_kv(layer_idx)
+            if self._short_kv[layer_idx] is not None:
+                self._record_short_rows(self._short_kv[layer_idx])
+        else:
+            segments = self._draft_segments(queries, layer_idx, z)
+        return self._tree.run(queries, [s for s in segments if s[3] > 0], key_states, value_states, mask)
+
+    def _draft_segments(self, queries, layer_idx, z):
+        """What the drafted tokens attend to of a cache that retrieves, the selected rows found and, from a host store, fetched."""
+        if self._dense_bound[layer_idx] is not None or self._short_kv[layer_idx] is not None:
+            self._drop_short_rows(layer_idx)
+        bs, T, H, G, D = self.batch_size, queries.shape[1], self.kv_head, self.group_size, self.head_dim
+        if tuple(queries.shape) != (bs, T, H * G, D):
+            raise RuntimeError("queries: [bs,T,Hq,D]")
+        q = queries.reshape(bs, T, H, G, D).transpose(1, 2).contiguous()
+        n_keys, n_cand, topk, tiers = self.retrieval_shape(layer_idx)
+        kg, vg = self.unified_keys_gpu[layer_idx], self.unified_values_gpu[layer_idx]
+        gather, prefix = None, z.gpu_prefix_rows
+        if self._layer_offload[layer_idx]:
+            self._wait_offload(layer_idx)
+            gather = dict(src_k=self.unified_keys_cpu[layer_idx], src_v=self.unified_values_cpu[layer_idx], from_host=True,
+                          idx_offset=0, dst_k=kg, dst_v=vg, dst_row0=prefix)
+        ids = self._plan.run(q, self._srht_signs, self._mag_centers, self.cluster_key_counts_gpu[layer_idx],
+                             self._codes_km[layer_idx], self._nib_km[layer_idx], self._w_km[layer_idx], self.sink_size, n_keys, tiers,
+                             n_cand, topk, gather=gather, any_order=True, group=T * G)
+        self.last_topk_indices = ids
+        if gather is not None:
+            return [(kg, vg, 0, prefix + topk)]
+        return [(kg, vg, 0, self.sink_size), (kg, vg, self.sink_size, topk, ids), (kg, vg, z.local_start, z.dense_tail_len)]
+
+    def commit_draft(self, draft_k, draft_v, path) -> None:
+        """Append the accepted tokens of a draft to every layer: what :meth:`decode_update_kv_cache` does a token and a layer at a time,
+        index refreshes included.  draft_k, draft_v: the drafted rows, [bs,T,Hkv,D] a layer (a sequence, or one stacked tensor); path:
+        host integers [bs][n], the accepted tokens of each sequence in order.  The sequences of a batch share one length, so all of
+        them accept the same number of tokens."""
+        lengths = {len(row) for row in path} if isinstance(path, (list, tuple)) and all(hasattr(row, "__len__") for row in path) else None
+        path = torch.as_tensor(path) if lengths is None or len(lengths) == 1 else torch.empty(0)
+        if path.dim() != 2 or path.shape[0] != self.batch_size or (path.numel() > 0 and path.is_floating_point()) or path.device.type != "cpu":
+            raise RuntimeError("path: integers [bs][n] on the host, as many for every sequence")
+        if len(draft_k) != self.layer_num or len(draft_v) != self.layer_num:
+            raise RuntimeError("one tensor of drafted rows a layer")
+        n = path.shape[1]
+        if n == 0:
+            return
+        T = draft_k[0].shape[1]
+        if int(path.min()) < 0 or int(path.max()) >= T:
+            raise RuntimeError(f"path: drafted tokens 0..{T - 1}")
+        if max(z.seq_len for z in self._zones) + n > self.unified_kv_capacity:
+            raise RuntimeError("the accepted tokens do not fit into the cache")
+        if self.enable_offload and (self._prefill_stage[0] is not None or self._prefill_stage[1] is not None):
+            self.release_prefill_staging()  # as the first decoded token does
+        if not isinstance(draft_k, torch.Tensor):
+            draft_k, draft_v = ([t.to(self.dtype) for t in d] for d in (draft_k, draft_v))
+        if self._path_plans is None:  # a launch takes layers whose rows are laid out alike
+            norms, alike = self._path_norms(), {}
+            for l, t in enumerate(self.unified_keys_gpu):
+                alike.setdefault((t.shape, t.stride()), []).append(l)
+            pick = lambda ts, ls: [ts[l] for l in ls]
+            self._path_plans = [(ls, ops.PathAppend(pick(self.unified_keys_gpu, ls), pick(self.unified_values_gpu, ls),
+                                                    pick(norms, ls) if norms is not None else None)) for ls in alike.values()]
+        path = path.to(torch.int64).to(self.device)
+        done = 0
+        while done < n:  # up to the next index refresh, which moves rows about
+            run = min(n - done, min(z.tokens_to_refresh() for z in self._zones))
+            for ls, plan in self._path_plans:
+                dk, dv = ((d if len(ls) == self.layer_num else [d[l] for l in ls]) for d in (draft_k, draft_v))
+                plan.launch(dk, dv, path[:, done:done + run], [self._zones[l].append_slot() for l in ls])
+            for l, z in enumerate(self._zones):
+                for _ in range(run):
+                    refresh = z.appended()
+                self.current_seq_len[l] = z.seq_len
+                if refresh is not None:
+                    with ranges.span("update_polar_index"):
+                        self._update_polar_index(l, refresh)
+            done += run
+        self.context += n
+
+    def _path_norms(self):
+        """The value norms that go with every layer's rows, for subclasses that keep them."""
+        return None
 
     def sync(self, layer_idx, batch_idx):
         """No-op, as in the reference (:1310-1312)."""

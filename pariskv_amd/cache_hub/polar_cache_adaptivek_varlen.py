@@ -107,6 +107,13 @@ class polar_cache(_polar_cache_base):
         """K/V rows and the value norm of the new token (:1179) in one launch."""
         super()._append(layer_idx, slot, key_states, value_states, vnorm=self._sl_vnorm_cache[layer_idx])
 
+    def _path_norms(self):
+        return self._sl_vnorm_cache
+
+    def _draft_segments(self, queries, layer_idx, z):
+        raise RuntimeError("drafted tokens: this cache chooses how many keys one token attends to; from the length at which it retrieves "
+                           "on, decode token by token")
+
     def _on_refresh(self, layer_idx, r):
         S0, n, L = self.sink_size, r.n_new, self.local_size
         sl = self._sl_vnorm_cache[layer_idx]

@@ -86,6 +86,10 @@ class LayerZones:
         """Whether the next ``appended()`` will return a Refresh (the token that fills the update buffer)."""
         return self.seq_len >= self.steady and self.buffered + 1 >= self.interval
 
+    def tokens_to_refresh(self) -> int:
+        """How many ``appended()`` until one returns a Refresh, itself included; their slots follow one another."""
+        return max(0, self.steady - self.seq_len) + self.interval - self.buffered
+
     # ---------------------------------------------------------------- regions
     @property
     def retrieval_start(self) -> int:

@@ -1352,34 +1352,35 @@ class RetrievePlan:
         return cand, scores
 
     def _fill(self, queries, signs, centers, cluster_counts, codes_km, nib_km, w_km, key0, n_keys, tier_counts, n_cand, k,
-              out_ids, out_scores, gather, candidates_only, any_order=False, record_word_offset=0):
+              out_ids, out_scores, gather, candidates_only, any_order=False, record_word_offset=0, group=None):
         """Validate one retrieval's operands and return its C argument block (the workspace grows if it must)."""
         need = _lib.lib().pkv_retrieve_ws_bytes(self.rows, n_keys, n_cand, k)
         _need(need > 0, "need 0 < k <= n_cand <= n_keys")
         if need > self.ws.numel():
             self.ws = torch.empty(int(need), dtype=torch.uint8, device=self.device)
-        a = _retrieve_args(self.bs, self.H, self.group, self.cap, queries, signs, centers, cluster_counts, codes_km,
+        a = _retrieve_args(self.bs, self.H, self.group if group is None else group, self.cap, queries, signs, centers, cluster_counts, codes_km,
                            nib_km, w_km, key0, n_keys, tier_counts, n_cand, k, out_ids, out_scores, gather,
                            candidates_only, any_order, record_word_offset)
         a.launch_plan, a.skip_vote_counts = int(self.launch_plan), int(bool(self.skip_vote_counts))
         return a
 
     def run(self, queries, signs, centers, cluster_counts, codes_km, nib_km, w_km, key0, n_keys, tier_counts, n_cand, k,
-            out_ids=None, out_scores=None, gather=None, candidates_only=False, attention=None, any_order=False):
+            out_ids=None, out_scores=None, gather=None, candidates_only=False, attention=None, any_order=False, group=None):
         """Returns out_ids int64 [bs,H,k] in descending score order, or, with ``any_order``, the same ids in an
         unspecified fixed order (the final sort is left out; enough for gather + attention).  ``gather`` = dict(src_k, src_v, from_host, idx_offset, dst_k, dst_v, dst_row0).
         ``attention`` = (DecodeAttention, segments, out or None): the attention over those segments is launched by the
-        same C call, after the gather (pkv_decode_step); the output tensor is then in ``self.attn_out``."""
+        same C call, after the gather (pkv_decode_step); the output tensor is then in ``self.attn_out``.  ``group``: query rows to a KV
+        head where they are not the plan's (the heads of several drafted tokens; not with ``attention``)."""
         lib = _lib.lib()
         if out_ids is None and not candidates_only:
             out_ids = torch.empty(self.bs, self.H, k, dtype=torch.int64, device=self.device)
         a = self._fill(queries, signs, centers, cluster_counts, codes_km, nib_km, w_km, key0, n_keys, tier_counts, n_cand, k,
-                       out_ids, out_scores, gather, candidates_only, any_order)
+                       out_ids, out_scores, gather, candidates_only, any_order, group=group)
         if attention is None:
             _lib.check(lib.pkv_retrieve(C.byref(a), _p(self.ws), self.ws.numel(), _stream(self.ws)))
         else:
             att, segments, att_out = attention
-            _need(not candidates_only, "attention needs the final top-k")
+            _need(not candidates_only and group in (None, self.group), "attention needs the final top-k and the plan's own group")
             qq = queries if queries.is_contiguous() else queries.contiguous()
             aa, self.attn_out = att.c_args(qq, segments, out=att_out)
             _lib.check(lib.pkv_decode_step(C.byref(a), _p(self.ws), self.ws.numel(), C.byref(aa), _stream(self.ws)))

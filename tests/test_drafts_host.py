@@ -214,3 +214,20 @@ def test_path_append_refusals():
 def test_new_struct_mirrors_have_the_library_sizes():
     for which, mirror in ((7, _lib.PathLayer), (8, _lib.PathArgs), (9, _lib.TreeArgs)):
         assert _lib.lib().pkv_struct_bytes(which) == ctypes.sizeof(mirror) > 0
+
+
+def test_tokens_to_refresh():
+    from pariskv_amd.cache_hub.zones import LayerZones
+
+    for offload in (False, True):
+        for prompt in (0, 1, 5, 11, 12, 13, 40):
+            z = LayerZones(4, 8, 3, offload)
+            z.prefill(prompt)
+            for _ in range(30):
+                due, slot, steps = z.tokens_to_refresh(), z.append_slot(), 0
+                while True:
+                    assert z.append_slot() == slot + steps   # the rows of a run follow one another
+                    steps += 1
+                    if z.appended() is not None:
+                        break
+                assert steps == due

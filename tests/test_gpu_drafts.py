@@ -6,7 +6,9 @@ Tolerances, per element.  u = 2^-24 is half a step of fp32, h half a step of the
 Attention: with A = sum p |v| over the keys a row sees (p the exact weights), a score is off by at most 130 u S, S the largest sum of
 |q| |k| times the scale (128 exact or rounded products and their sum, the scale), which moves a weight by that much and the normaliser
 by as much again; the sum over n keys is off by (n + 200) u A (every key's addition, exponentials of 4 u, the merges), twice with the
-normaliser; bf16 rounds weights by h (A h).  Together: A (4 * 130 u S + 2 (n + 200) u + h [bf16]) + h |out|.
+normaliser.  bf16 weights are rounded to w (1 + d), |d| <= h, and summed up as they are: sum p (1 + d) v / sum p (1 + d) - sum p v
+= sum p (d - mean d) v (1 + O(h)), with mean d = sum p d, at most h A + h |out|.  Together: A (4 * 130 u S + 2 (n + 200) u + h [bf16]) + h |out|,
+and h |out| again for bf16.
 4-bit products: with B = sum |x| s (16 + q + 16 + z), every partial sum is at most B and a path through the sums of a column has
 at most 128 + K/128 + 20 additions: (148 + K/128) u B + h |y|.
 """
@@ -94,7 +96,7 @@ def exact_tree(c, scale=None):
                 o, a = p @ vv, p @ vv.abs()
                 s = (qq.abs() @ kk.abs().T).amax(-1, keepdim=True) * abs(scale)
                 out[b, u, j * group:(j + 1) * group] = o
-                tol[b, u, j * group:(j + 1) * group] = (a * (520 * U * s + 2 * (len(kk) + 200) * U + (half if half > U else 0)) + half * o.abs())
+                tol[b, u, j * group:(j + 1) * group] = (a * (520 * U * s + 2 * (len(kk) + 200) * U + (half if half > U else 0)) + half * (2 if half > U else 1) * o.abs())
     return out, tol
 
 
