@@ -43,10 +43,10 @@ struct TreePart {
   bool any;
 };
 __device__ __forceinline__ TreePart tree_part(const TreeCall &a) {
-  const int per = 8 * a.row_tiles, x = (int)blockIdx.x, in = x % per, pair = x / per * 8 + in % 8;
-  return {pair / a.n_splits, pair % a.n_splits, in / 8, pair < a.n_pairs};
+  const int pair = (int)blockIdx.y * 8 + (blockIdx.x & 7), bh = (unsigned)pair / (unsigned)a.n_splits;
+  return {bh, pair - bh * a.n_splits, (int)blockIdx.x >> 3, pair < a.n_pairs};
 }
-static unsigned tree_grid(const TreeCall &a) { return (unsigned)((a.n_pairs + 7) / 8 * 8 * a.row_tiles); }
+static dim3 tree_grid(const TreeCall &a) { return dim3(8u * a.row_tiles, (unsigned)((a.n_pairs + 7) / 8)); }
 
 template <bool BF16, int NT>
 struct TreeWave {
@@ -100,6 +100,12 @@ __device__ __forceinline__ void tree_scores(const TreeWave<BF16, NT> &w, const p
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = s0[e];
   }
+}
+
+// The larger of both halves each.
+__device__ __forceinline__ uint32_t tree_max_u16(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
 // Scores into weights 2^(scale s - use) of the keys in `bits` (MASKED; else of all), as the operand of the second product; the sum and
@@ -238,7 +244,29 @@ __device__ __forceinline__ void tree_masked_step(TreeWave<BF16, NT> &w, const Tr
   }
   // Keys that are not there were read again: zeros, so that nothing of them reaches the sums.  A drafted value that is not finite is for the
   // rows that see it and for no other, but in the product it would be 0 * inf for all: zero there, and added below.
-  uint32_t found = 0;
+  bool odd = false;
+  if (draft) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const pkv_u32x4 v = v_of(m);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        if constexpr (BF16) most = tree_max_u16(most, v[d] & 0x7fff7fffu);
+        else most = most > (v[d] & 0x7fffffffu) ? most : v[d] & 0x7fffffffu;
+      }
+    }
+    odd = __any(BF16 ? (most & 0xffffu) >= 0x7f80u || most >= 0x7f800000u : most >= 0x7f800000u);
+  }
+  if (!odd) {
+    tree_output(w, p, [&](int m) {
+      pkv_u32x4 v = v_of(m);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] &= keep[d];
+      return v;
+    });
+    return;
+  }
   tree_output(w, p, [&](int m) {
     pkv_u32x4 v = v_of(m);
 #pragma unroll
@@ -246,37 +274,35 @@ __device__ __forceinline__ void tree_masked_step(TreeWave<BF16, NT> &w, const Tr
       uint32_t x = v[d] & keep[d], bad;
       if constexpr (BF16) bad = ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
       else bad = (x & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
-      if (!draft) bad = 0;
-      found |= bad, v[d] = x & ~bad;
+      v[d] = x & ~bad;
     }
     return v;
   });
-  if (__any(found != 0)) {  // the whole wave: drafted values that are not finite, one key at a time
+  // the whole wave: one key at a time
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+  for (int t = 0; t < NT; ++t) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int e = 0; e < W::kE; ++e) {
-        const uint32_t d = BF16 ? p[t][e >> 1] : p[t][e & 3];
-        weight[n][tree_key(e, j)] = __uint_as_float(!BF16 ? d : e & 1 ? d & 0xffff0000u : d << 16);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      for (int key = 0; key < here; ++key) {
-        const char *vp = dv + (int64_t)(u0 + key) * a.dv_t;
-        float f[4];
+    for (int e = 0; e < W::kE; ++e) {
+      const uint32_t d = BF16 ? p[t][e >> 1] : p[t][e & 3];
+      weight[n][tree_key(e, j)] = __uint_as_float(!BF16 ? d : e & 1 ? d & 0xffff0000u : d << 16);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int key = 0; key < here; ++key) {
+      const char *vp = dv + (int64_t)(u0 + key) * a.dv_t;
+      float f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = weight[4 * j + i][key];
+      for (int i = 0; i < 4; ++i) f[i] = weight[4 * j + i][key];
 #pragma unroll
-        for (int m = 0; m < 8; ++m) {
-          const int d = tree_dim<BF16, TURNED>(n, m);
-          float x;
-          if constexpr (BF16) x = pkv_bf16_bits_to_f32(((const uint16_t *)vp)[d]);
-          else x = ((const float *)vp)[d];
+      for (int m = 0; m < 8; ++m) {
+        const int d = tree_dim<BF16, TURNED>(n, m);
+        float x;
+        if constexpr (BF16) x = pkv_bf16_bits_to_f32(((const uint16_t *)vp)[d]);
+        else x = ((const float *)vp)[d];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w.o[t][m][i] += f[i] != 0.f && !(fabsf(x) < INFINITY) ? f[i] * x : 0.f;
-        }
+        for (int i = 0; i < 4; ++i) w.o[t][m][i] += f[i] != 0.f && !(fabsf(x) < INFINITY) ? f[i] * x : 0.f;
       }
     }
   }
@@ -288,7 +314,7 @@ __device__ __forceinline__ void tree_finish(const TreeWave<BF16, NT> &w, const T
                                             float (&s_l)[WAVES][16], float (&s_o)[WAVES][16][132]) {
   constexpr int KW = WAVES / RW;
   const int tid = threadIdx.x, lane = pkv_lane(), wave = tid / PKV_WAVE, n = lane & 15, j = lane >> 4;
-  const int bh = part.bh, n_splits = a.n_splits, rows = a.n_draft * a.group, b = bh / a.n_kv_heads, h = bh % a.n_kv_heads;
+  const int bh = part.bh, n_splits = a.n_splits, rows = a.n_draft * a.group, b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     __syncthreads();
@@ -313,8 +339,9 @@ __device__ __forceinline__ void tree_finish(const TreeWave<BF16, NT> &w, const T
       }
     }
     __syncthreads();
-    for (int e = tid; e < RW * 16 * 32; e += WAVES * PKV_WAVE) {  // four dims at a time
-      const int rw = e >> 9, r = (e >> 5) & 15, d = 4 * (e & 31), row = (part.tile * RW + rw) * 16 * NT + 16 * t + r;
+#pragma unroll
+    for (int e0 = 0; e0 < RW * 16 * 32; e0 += WAVES * PKV_WAVE) {  // four dims at a time
+      const int e = e0 + tid, rw = e >> 9, r = (e >> 5) & 15, d = 4 * (e & 31), row = (part.tile * RW + rw) * 16 * NT + 16 * t + r;
       if (row >= rows) continue;
       float mx = s_m[rw][r];
 #pragma unroll
@@ -331,9 +358,11 @@ __device__ __forceinline__ void tree_finish(const TreeWave<BF16, NT> &w, const T
         for (int u = 0; u < 4; ++u) os[u] = fmaf(x[u], c, os[u]);
       }
       if (n_splits == 1) {
-        const int64_t to = (((int64_t)b * a.n_draft + row / a.group) * a.n_kv_heads * a.group + h * a.group + row % a.group) * 128 + d;
+        const int u = (unsigned)row / (unsigned)a.group;
+        const int64_t to = (((int64_t)b * a.n_draft + u) * a.n_kv_heads * a.group + h * a.group + (row - u * a.group)) * 128 + d;
+        const float share = ls == 0.f ? 0.f : 1.0f / ls;  // 0: nothing seen
 #pragma unroll
-        for (int u = 0; u < 4; ++u) os[u] = ls == 0.f ? 0.f : os[u] / ls;  // 0: nothing seen
+        for (int i = 0; i < 4; ++i) os[i] *= share;
         if constexpr (BF16) *(pkv_u32x2 *)((uint16_t *)a.out + to) = pkv_u32x2{tree_pack(os[0], os[1]), tree_pack(os[2], os[3])};
         else *(pkv_f32x4 *)((float *)a.out + to) = os;
       } else {
@@ -353,9 +382,9 @@ __device__ __forceinline__ void tree_begin(TreeWave<BF16, NT> &w, const TreeCall
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int r = r0 + 16 * t + n, rr = r < rows ? r : rows - 1;
-    token[t] = rr / a.group;
+    token[t] = (unsigned)rr / (unsigned)a.group;
     const char *qp = (const char *)a.q + ((int64_t)b * a.q_stride_b + (int64_t)token[t] * a.q_stride_t +
-                                          (int64_t)(h * a.group + rr % a.group) * 128) * es + 16 * j;
+                                          (int64_t)(h * a.group + rr - token[t] * a.group) * 128) * es + 16 * j;
 #pragma unroll
     for (int c = 0; c < TreeWave<BF16, NT>::kQ; ++c) w.q[t][c] = *(const pkv_u32x4 *)(qp + 64 * c);
     w.use[t] = 0.f, w.lim[t] = -INFINITY, w.l[t] = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -379,7 +408,9 @@ struct TreePlaces {
   const SEGS &segs;
   int bh, b, h;
   __device__ __forceinline__ TreePlaces(const SEGS &s, int bh_, int b_, int h_) : segs(s), bh(bh_), b(b_), h(h_) {}
-  __device__ __forceinline__ AttPlace<false> of(uint32_t at) const { return att_place<INDEXED, kRow>(segs, bh, b, h, at); }
+  using Found = AttPlace<false>;
+  __device__ __forceinline__ Found find(uint32_t at) const { return att_place<INDEXED, kRow>(segs, bh, b, h, at); }
+  __device__ __forceinline__ AttPlace<false> place(const Found &f) const { return f; }
 };
 template <bool BF16, bool INDEXED>
 struct TreePlaces<BF16, INDEXED, AttOne> {
@@ -399,13 +430,29 @@ struct TreePlaces<BF16, INDEXED, AttOne> {
     delta0 = d0, more1 = d1 - d0, more2 = d2 - d1, more3 = (uint32_t)att_field(s.delta[3]) - d2;
     if (INDEXED) idx = s.idx + (int64_t)bh * s.idx_stride, limit = s.idx_limit, lo = s.idx_lo, hi = s.idx_hi, row0 = s.idx_row0;
   }
-  __device__ __forceinline__ AttPlace<true> of(uint32_t at) const {
-    uint32_t r = at + delta0 + (at >= end0 ? more1 : 0u) + (at >= end1 ? more2 : 0u) + (at >= end2 ? more3 : 0u);
-    if (INDEXED && at >= lo && at < hi) {
-      const int64_t x = idx[at - lo];
-      r = row0 + (uint32_t)(x < 0 ? 0 : (x >= limit ? limit - 1 : x));
+  // A place in two steps, where the keys are selected: find() asks for the row's number, place() waits for it.  (In one, with a branch round the
+  // load, every search waited for all rows under way: 8 x 8 x 1617 selected keys, 256 rows 46 us, dense ones 37.)
+  struct Found {
+    uint32_t off;  // of a row that is not selected, else kSelected
+    int64_t x;
+  };
+  static constexpr uint32_t kSelected = 0xffffffffu;
+  __device__ __forceinline__ Found find(uint32_t at) const {
+    Found f;
+    f.off = (at + delta0 + (at >= end0 ? more1 : 0u) + (at >= end1 ? more2 : 0u) + (at >= end2 ? more3 : 0u)) * kRow;
+    if constexpr (INDEXED) {
+      const bool in = at >= lo && at < hi;
+      f.x = idx[in ? at - lo : 0u];
+      f.off = in ? kSelected : f.off;
     }
-    return {r * kRow};
+    return f;
+  }
+  __device__ __forceinline__ AttPlace<true> place(const Found &f) const {
+    if constexpr (INDEXED) {
+      const uint32_t r = row0 + (uint32_t)(f.x < 0 ? 0 : (f.x >= limit ? limit - 1 : f.x));
+      return {f.off == kSelected ? r * kRow : f.off};
+    }
+    return {f.off};
   }
 };
 
@@ -451,7 +498,7 @@ __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_ker
   const TreePart part = tree_part(a);
   if (!part.any) return;  // the whole workgroup
   const int split = part.split, n_splits = a.n_splits, bh = part.bh;
-  const int b = bh / a.n_kv_heads, h = bh % a.n_kv_heads;
+  const int b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
   const int lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PKV_WAVE);
 
   const uint32_t total = tree_total(a, bh);
@@ -463,7 +510,7 @@ __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_ker
   const TreePlaces<BF16, INDEXED, SEGS> places(segs, bh, b, h);
   auto find = [&](int first, int keys) {
     const int key = lane & (W::kKeys - 1);
-    return places.of((uint32_t)(first + (key < keys ? key : keys - 1)));
+    return places.find((uint32_t)(first + (key < keys ? key : keys - 1)));
   };
   auto k_at = [&](const AttPlace<ONE> &place) {
     return [&](int base, int key) -> const char * {
@@ -483,9 +530,10 @@ __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_ker
   int token[1];
   tree_begin<BF16, 1>(w, a, b, h, 0, token);
   // In the order of the loop, so that a wait there is for what it needs alone: K, the place of the next step, V.
-  AttPlace<ONE> mine, next;
+  AttPlace<ONE> mine;
+  typename TreePlaces<BF16, INDEXED, SEGS>::Found next;
   if (n_full > 0) {
-    mine = find(turn0 * W::kKeys, W::kKeys);
+    mine = places.place(find(turn0 * W::kKeys, W::kKeys));
     tree_load_k<BF16>(k, k_at(mine));
     next = find((n_full > 1 ? turn0 + turns : turn0) * W::kKeys, W::kKeys);
     tree_load_v<BF16>(v, v_at(mine));
@@ -494,7 +542,7 @@ __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_ker
   for (int i = 0; i < n_full; ++i) {
     float s[W::kE];
     tree_scores(w, k, 0, s);
-    mine = next;
+    mine = places.place(next);
     if (i + 1 < n_full) tree_load_k<BF16>(k, k_at(mine));
     if (i + 2 < n_full) next = find((turn0 + (i + 2) * turns) * W::kKeys, W::kKeys);
     const pkv_u32x4 p[1] = {tree_weights<false>(w, 0, s, 0u, a.scale_log2e)};
@@ -513,7 +561,7 @@ __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_ker
       tree_load_k<BF16>(k, [&](int base, int key) { return dk + (int64_t)(u0 + (base + key < here ? base + key : here - 1)) * a.dk_t; });
       tree_load_v<BF16>(v, [&](int base, int key) { return dv + (int64_t)(u0 + (base + key < here ? base + key : here - 1)) * a.dv_t; });
     } else {
-      mine = find(all_full * W::kKeys, rest);
+      mine = places.place(find(all_full * W::kKeys, rest));
       tree_load_k<BF16>(k, k_at(mine));
       tree_load_v<BF16>(v, v_at(mine));
     }
@@ -541,7 +589,7 @@ __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel
   const TreePart part = tree_part(a);
   if (!part.any) return;  // the whole workgroup
   const int split = part.split, n_splits = a.n_splits, bh = part.bh;
-  const int b = bh / a.n_kv_heads, h = bh % a.n_kv_heads;
+  const int b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
   const int tid = threadIdx.x, lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(tid / PKV_WAVE), n = lane & 15, j = lane >> 4;
   const int row_wave = wave % RW, key_wave = wave / RW, r0 = (part.tile * RW + row_wave) * 16 * NT;
   constexpr int kEnd = kWideWaves * (16 * 132 + 32) * 4, kLds = 4 * kTensor > kEnd ? 4 * kTensor : kEnd;
@@ -559,19 +607,21 @@ __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel
   struct Rows {
     pkv_u32x4 k[kLoads], v[kLoads];
   };
-  auto find = [&](int first, int count, AttPlace<ONE> (&at)[kLoads]) {
+  using Found = typename TreePlaces<BF16, INDEXED, SEGS>::Found;
+  auto find = [&](int first, int count, Found (&at)[kLoads]) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       const int r = my_row + kRowsAt * u;
-      at[u] = places.of((uint32_t)(first + (r < count ? r : count - 1)));
+      at[u] = places.find((uint32_t)(first + (r < count ? r : count - 1)));
     }
   };
-  auto fetch = [&](const AttPlace<ONE> (&at)[kLoads], Rows &r) {
+  auto fetch = [&](const Found (&found)[kLoads], Rows &r) {
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
+      const AttPlace<ONE> at = places.place(found[u]);
       const char *kp, *vp;
-      if constexpr (ONE) kp = places.k + (uint64_t)at[u].off, vp = places.v + (uint64_t)at[u].off;
-      else kp = (const char *)at[u].k, vp = (const char *)at[u].v;
+      if constexpr (ONE) kp = places.k + (uint64_t)at.off, vp = places.v + (uint64_t)at.off;
+      else kp = (const char *)at.k, vp = (const char *)at.v;
       r.k[u] = __builtin_nontemporal_load((const pkv_u32x4 *)kp + my_vec);
       r.v[u] = __builtin_nontemporal_load((const pkv_u32x4 *)vp + my_vec);
     }
@@ -618,28 +668,28 @@ __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel
 
   int token[NT];
   tree_begin<BF16, NT>(w, a, b, h, r0, token);
-  AttPlace<ONE> next[kLoads], later[kLoads];
+  Found places_of[2][kLoads];
   Rows ahead[2];
   auto first_of = [&](int i) { return (split + (i < n_full ? i : n_full - 1) * n_splits) * kTurnKeys; };  // past the last: read again, never used
   if (n_full > 0) {
-    find(first_of(0), kTurnKeys, next);
-    fetch(next, ahead[0]);
-    find(first_of(1), kTurnKeys, next);
-    fetch(next, ahead[1]);
-    find(first_of(2), kTurnKeys, later);
-    find(first_of(3), kTurnKeys, next);
+    Found first[2][kLoads];
+    find(first_of(0), kTurnKeys, first[0]);
+    find(first_of(1), kTurnKeys, first[1]);
+    find(first_of(2), kTurnKeys, places_of[1]);
+    find(first_of(3), kTurnKeys, places_of[0]);
+    fetch(first[0], ahead[0]);
+    fetch(first[1], ahead[1]);
     put(ahead[0], 0);
-    fetch(later, ahead[0]);
+    fetch(places_of[1], ahead[0]);
   }
   // Turn i is in LDS or on its way there, turn i + 1 in registers, turn i + 2 requested, the places of turn i + 3 known.  Places are asked
   // for before rows: a wait for them is then not for the rows as well.
-  auto turn = [&](int i, Rows &after) {
+  auto turn = [&](int i, Rows &after, const Found (&third)[kLoads], Found (&fourth)[kLoads]) {
     __syncthreads();  // turn i is there, and everybody is done with turn i - 1
     put(after, (i + 1) & 1);
-    find(first_of(i + 4), kTurnKeys, later);
-    fetch(next, after);
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u) next[u] = later[u];
+    find(first_of(i + 4), kTurnKeys, fourth);
+    fetch(third, after);
+    if (i >= n_full) return;  // the whole workgroup
     float s[NT][W::kE];
     get_k(i & 1);
 #pragma unroll
@@ -649,9 +699,9 @@ __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel
     for (int t = 0; t < NT; ++t) p[t] = tree_weights<false>(w, t, s[t], 0u, a.scale_log2e);
     tree_output(w, p, v_of(i & 1));
   };
-  for (int i = 0; i < n_full; i += 2) {
-    turn(i, ahead[1]);
-    if (i + 1 < n_full) turn(i + 1, ahead[0]);
+  for (int i = 0; i < n_full; i += 2) {  // no way round the second: waits count what was asked for since on every path
+    turn(i, ahead[1], places_of[0], places_of[1]);
+    turn(i + 1, ahead[0], places_of[1], places_of[0]);
   }
 
   // The cached keys behind the last full turn, and the drafted tokens, a turn of them at a time, dealt out behind the full ones.
@@ -668,8 +718,8 @@ __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel
         ahead[0].v[u] = ((const pkv_u32x4 *)(dv + (int64_t)at * a.dv_t))[my_vec];
       }
     } else {
-      find(first, count, next);
-      fetch(next, ahead[0]);
+      find(first, count, places_of[0]);
+      fetch(places_of[0], ahead[0]);
     }
     __syncthreads();
     put(ahead[0], 0);
@@ -806,7 +856,7 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
   const bool is_one = as_one_tensor(sg, (int)es, one);
   hipStream_t s = (hipStream_t)stream;
   c.n_splits = p.n_splits, c.row_tiles = p.row_tiles, c.n_pairs = a->bs * a->n_kv_heads * p.n_splits;
-  const dim3 grid(tree_grid(c));
+  const dim3 grid = tree_grid(c);
   const dim3 block((p.rw == 1 ? kTreeWaves : kWideWaves) * PKV_WAVE);
 #define PKV_TREE(IDX, S)                                                                                             \
   do {                                                                                                               \
