@@ -33,18 +33,49 @@ struct TreeCall {
   float *ws_o, *ws_ml;  // [row of (b, h)][split][query row][128], [..][2]
   void *out;
   int n_splits, row_tiles, n_pairs;  // (b, h) times splits
+  int n_bh, by_keys;                 // by_keys: splits in proportion to the rows' keys, 1 + log2 of the keys of a turn; else 0
 };
 
 // A workgroup's part: a split of the keys of one (b, h), and a tile of its query rows.  Workgroups go to the eight dies in turn, and the tiles of
-// one split read the same keys: they are eight numbers apart, so that a die's L2 reads the keys once for all.  us, 256 query rows (four tiles),
-// tiles side by side / on one die: see pkv_tree_wide_kernel.
+// one split read the same keys: they are eight numbers apart, so that a die's L2 reads the keys once for all.
 struct TreePart {
-  int bh, split, tile;
+  int bh, split, tile, n_splits, first;  // first: the partial result of the row's split 0
   bool any;
 };
+
+// Key counts that differ: the splits' slots go to the (at most 64) rows in proportion to their turns of keys, at least one each, so that all
+// workgroups have about as much to do.  Lane l finds the slots [first, end) of row l, of which it uses n: at most a turn each, at most
+// kTreeMaxSplits.  All lanes active.  3 x 4 x 9001 fp32 of which the rows see from none to all, 49 rows: 33 us; 46 with as many splits for every row.  (8 x 8 x 20000 bf16, 20 rows: 70, 79.)
+struct TreeShare {
+  int first, end, n;
+};
+__device__ __forceinline__ TreeShare tree_share(const int32_t *row_keys, uint32_t total, int n_bh, int slots, int by_keys) {
+  const int lane = pkv_lane(), rk = lane < n_bh ? row_keys[lane] : 0;
+  const uint32_t keys = rk <= 0 ? 0u : (uint32_t)rk < total ? (uint32_t)rk : total;
+  const int turns = keys == 0 ? 1 : (int)((keys - 1) >> (by_keys - 1)) + 1, mine = lane < n_bh ? turns : 0;
+  const int upto = pkv_wave_incl_scan(mine);
+  const float each = (float)(slots - n_bh) / (float)__builtin_amdgcn_readlane(upto, 63);
+  TreeShare t;
+  t.first = lane + (int)((float)(upto - mine) * each), t.end = lane + 1 + (int)((float)upto * each);
+  const int most = turns < kTreeMaxSplits ? turns : kTreeMaxSplits;
+  t.n = t.end - t.first < most ? t.end - t.first : most;
+  return t;
+}
+
+// SHARES: by_keys is set (of its own kernels: looked up at run time it costs every call 0.5 us).
+template <bool SHARES>
 __device__ __forceinline__ TreePart tree_part(const TreeCall &a) {
-  const int pair = (int)blockIdx.y * 8 + (blockIdx.x & 7), bh = (unsigned)pair / (unsigned)a.n_splits;
-  return {bh, pair - bh * a.n_splits, (int)blockIdx.x >> 3, pair < a.n_pairs};
+  const int pair = (int)blockIdx.y * 8 + (blockIdx.x & 7), tile = (int)blockIdx.x >> 3;
+  if constexpr (SHARES) {
+    const TreeShare t = tree_share(a.row_keys, a.total, a.n_bh, a.n_pairs, a.by_keys);
+    const int bh = __builtin_popcountll(__ballot(pkv_lane() < a.n_bh && t.first <= pair)) - 1;
+    const int first = __builtin_amdgcn_readlane(t.first, bh), n = __builtin_amdgcn_readlane(t.n, bh);
+    return {bh, pair - first, tile, n, first, pair - first < n};
+  }
+  if constexpr (!SHARES) {
+    const int bh = (unsigned)pair / (unsigned)a.n_splits;
+    return {bh, pair - bh * a.n_splits, tile, a.n_splits, bh * a.n_splits, pair < a.n_pairs};
+  }
 }
 static dim3 tree_grid(const TreeCall &a) { return dim3(8u * a.row_tiles, (unsigned)((a.n_pairs + 7) / 8)); }
 
@@ -314,7 +345,7 @@ __device__ __forceinline__ void tree_finish(const TreeWave<BF16, NT> &w, const T
                                             float (&s_l)[WAVES][16], float (&s_o)[WAVES][16][132]) {
   constexpr int KW = WAVES / RW;
   const int tid = threadIdx.x, lane = pkv_lane(), wave = tid / PKV_WAVE, n = lane & 15, j = lane >> 4;
-  const int bh = part.bh, n_splits = a.n_splits, rows = a.n_draft * a.group, b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
+  const int bh = part.bh, rows = a.n_draft * a.group, b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     __syncthreads();
@@ -357,7 +388,7 @@ __device__ __forceinline__ void tree_finish(const TreeWave<BF16, NT> &w, const T
 #pragma unroll
         for (int u = 0; u < 4; ++u) os[u] = fmaf(x[u], c, os[u]);
       }
-      if (n_splits == 1) {
+      if (a.n_splits == 1) {
         const int u = (unsigned)row / (unsigned)a.group;
         const int64_t to = (((int64_t)b * a.n_draft + u) * a.n_kv_heads * a.group + h * a.group + (row - u * a.group)) * 128 + d;
         const float share = ls == 0.f ? 0.f : 1.0f / ls;  // 0: nothing seen
@@ -366,7 +397,7 @@ __device__ __forceinline__ void tree_finish(const TreeWave<BF16, NT> &w, const T
         if constexpr (BF16) *(pkv_u32x2 *)((uint16_t *)a.out + to) = pkv_u32x2{tree_pack(os[0], os[1]), tree_pack(os[2], os[3])};
         else *(pkv_f32x4 *)((float *)a.out + to) = os;
       } else {
-        const int64_t at = ((int64_t)bh * n_splits + part.split) * rows + row;
+        const int64_t at = ((int64_t)part.first + part.split) * rows + row;
         *(pkv_f32x4 *)(a.ws_o + at * 128 + d) = os;
         if (d == 0) *(float2 *)(a.ws_ml + at * 2) = float2{mx, ls};
       }
@@ -491,13 +522,13 @@ __device__ __forceinline__ void tree_load_v(pkv_u32x4 (&v)[8], At at) {
 // Up to 16 query rows.  The four waves of a workgroup take steps of keys in turns, straight from memory into the operands' registers.
 // Full steps go round the waves of all splits, so that what the chip reads at one time lies side by side; the steps that not all rows see in
 // full, the cached keys behind the last full step and the drafted tokens, are dealt out behind them.
-template <bool BF16, bool INDEXED, typename SEGS>
+template <bool BF16, bool INDEXED, typename SEGS, bool SHARES>
 __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_kernel(TreeCall a, SEGS segs) {
   using W = TreeWave<BF16, 1>;
   constexpr bool ONE = __is_same(SEGS, AttOne);
-  const TreePart part = tree_part(a);
+  const TreePart part = tree_part<SHARES>(a);
   if (!part.any) return;  // the whole workgroup
-  const int split = part.split, n_splits = a.n_splits, bh = part.bh;
+  const int split = part.split, n_splits = part.n_splits, bh = part.bh;
   const int b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
   const int lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PKV_WAVE);
 
@@ -579,16 +610,16 @@ typedef __attribute__((address_space(3))) tree_s16x4 tree_lds_s16x4;
 // are requested two turns ahead into registers, written to one of two LDS buffers a turn ahead, and read from there as operands; one
 // barrier a turn.  us, straight from memory with each wave's own loads (two tiles a wave) / through LDS: 4 x 8 x 65536 keys, 64 rows 240 / 170;
 // 8 x 8 x 1617 selected keys, 256 rows 54 / 46.  A 16-byte vector c of a row r lies at c ^ (r mod 16), so that the 16 rows of an operand of K are on different banks.
-template <bool BF16, int NT, int RW, bool INDEXED, typename SEGS>
+template <bool BF16, int NT, int RW, bool INDEXED, typename SEGS, bool SHARES>
 __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel(TreeCall a, SEGS segs) {
   using W = TreeWave<BF16, NT>;
   constexpr bool ONE = __is_same(SEGS, AttOne);
   constexpr int KW = kWideWaves / RW, kTurnKeys = KW * W::kKeys, kRow = W::kRow, kVecs = kRow / 16;
   constexpr int kRowsAt = kWideWaves * PKV_WAVE / kVecs, kLoads = kTurnKeys / kRowsAt;  // rows a load of the workgroup covers; loads a turn
   constexpr int kTensor = kTurnKeys * kRow;
-  const TreePart part = tree_part(a);
+  const TreePart part = tree_part<SHARES>(a);
   if (!part.any) return;  // the whole workgroup
-  const int split = part.split, n_splits = a.n_splits, bh = part.bh;
+  const int split = part.split, n_splits = part.n_splits, bh = part.bh;
   const int b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
   const int tid = threadIdx.x, lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(tid / PKV_WAVE), n = lane & 15, j = lane >> 4;
   const int row_wave = wave % RW, key_wave = wave / RW, r0 = (part.tile * RW + row_wave) * 16 * NT;
@@ -738,15 +769,20 @@ __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel
 
 // One wave a query row: lane l weighs split l and holds dims 2 l, 2 l + 1 of the output.
 template <bool BF16>
-__global__ __launch_bounds__(256) void pkv_tree_merge_kernel(const float *__restrict__ ws_o, const float *__restrict__ ws_ml, int n_splits,
-                                                             int rows, int64_t n_rows, int n_draft, int group, int n_kv_heads,
-                                                             void *__restrict__ out) {
-  const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / PKV_WAVE;
+__global__ __launch_bounds__(256) void pkv_tree_merge_kernel(const float *__restrict__ ws_o, const float *__restrict__ ws_ml, void *__restrict__ out,
+                                                             const int32_t *__restrict__ row_keys, int n_splits, uint32_t rows, uint32_t n_rows,
+                                                             uint32_t n_draft, uint32_t group, uint32_t n_kv_heads, int by_keys, uint32_t total,
+                                                             int n_bh, int slots) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / PKV_WAVE);  // below 2^30: 65535 * 8192 rows
   const int lane = pkv_lane();
   if (at >= n_rows) return;
-  const int64_t bh = at / rows;
-  const int row = (int)(at % rows), b = (int)(bh / n_kv_heads), h = (int)(bh % n_kv_heads);
-  const int64_t first = bh * n_splits * rows + row;
+  const uint32_t bh = at / rows, row = at - bh * rows;
+  int first_split = bh * n_splits;
+  if (by_keys) {
+    const TreeShare t = tree_share(row_keys, total, n_bh, slots, by_keys);
+    n_splits = __builtin_amdgcn_readlane(t.n, bh), first_split = __builtin_amdgcn_readlane(t.first, bh);
+  }
+  const int64_t first = (int64_t)first_split * rows + row;
   float m = -INFINITY, l = 0.f;
   if (lane < n_splits) m = ws_ml[(first + (int64_t)lane * rows) * 2], l = ws_ml[(first + (int64_t)lane * rows) * 2 + 1];
   const float mx = pkv_wave_max(m), base = mx == -INFINITY ? 0.f : mx;
@@ -764,13 +800,14 @@ __global__ __launch_bounds__(256) void pkv_tree_merge_kernel(const float *__rest
       x = fmaf(o[i].x, f, x), y = fmaf(o[i].y, f, y);
     }
   }
-  const int64_t to = (((int64_t)b * n_draft + row / group) * n_kv_heads * group + h * group + row % group) * 128 + 2 * lane;
+  const uint32_t b = bh / n_kv_heads, h = bh - b * n_kv_heads, u = row / group;
+  const int64_t to = (((int64_t)b * n_draft + u) * n_kv_heads * group + h * group + (row - u * group)) * 128 + 2 * lane;
   if constexpr (BF16) *(uint32_t *)((uint16_t *)out + to) = tree_pack(x, y);
   else *(float2 *)((float *)out + to) = float2{x, y};
 }
 
 struct TreePlan {
-  int nt, rw, row_tiles, n_splits;
+  int nt, rw, row_tiles, n_splits, turn;
 };
 
 TreePlan tree_plan(int dtype, int bs, int n_kv_heads, int rows, int64_t total) {
@@ -780,9 +817,10 @@ TreePlan tree_plan(int dtype, int bs, int n_kv_heads, int rows, int64_t total) {
   const int64_t bh = (int64_t)bs * n_kv_heads;
   auto split = [&](int nt) {
     p.nt = nt;
-    const int per_wg = 16 * nt * p.rw, turn = (p.rw == 1 ? kTreeWaves : kWideWaves / p.rw) * (bf ? 32 : 16);  // keys a workgroup takes at a time
+    const int per_wg = 16 * nt * p.rw;
+    p.turn = (p.rw == 1 ? kTreeWaves : kWideWaves / p.rw) * (bf ? 32 : 16);  // keys a workgroup takes at a time
     p.row_tiles = (rows + per_wg - 1) / per_wg;
-    int64_t s = kTreeWorkgroups / (bh * p.row_tiles), most = (total + turn - 1) / turn;
+    int64_t s = kTreeWorkgroups / (bh * p.row_tiles), most = (total + p.turn - 1) / p.turn;
     if (s > most) s = most;
     if (s > kTreeMaxSplits) s = kTreeMaxSplits;
     p.n_splits = (int)(s < 1 ? 1 : s);
@@ -856,20 +894,23 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
   const bool is_one = as_one_tensor(sg, (int)es, one);
   hipStream_t s = (hipStream_t)stream;
   c.n_splits = p.n_splits, c.row_tiles = p.row_tiles, c.n_pairs = a->bs * a->n_kv_heads * p.n_splits;
+  c.n_bh = a->bs * a->n_kv_heads;
+  if (is_one && a->row_keys && p.n_splits > 1 && c.n_bh <= PKV_WAVE) c.by_keys = 1 + __builtin_ctz(p.turn);
   const dim3 grid = tree_grid(c);
   const dim3 block((p.rw == 1 ? kTreeWaves : kWideWaves) * PKV_WAVE);
-#define PKV_TREE(IDX, S)                                                                                             \
+#define PKV_TREE(IDX, S, SHARES)                                                                                     \
   do {                                                                                                               \
-    if (p.rw == 1) PKV_TREE_LAUNCH((pkv_tree_partial_kernel<BF, IDX, decltype(S)>), S);                              \
-    else if (p.rw == 2) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 2, IDX, decltype(S)>), S);                      \
-    else if (p.nt == 1) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 4, IDX, decltype(S)>), S);                      \
-    else PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 2, 4, IDX, decltype(S)>), S);                                     \
+    if (p.rw == 1) PKV_TREE_LAUNCH((pkv_tree_partial_kernel<BF, IDX, decltype(S), SHARES>), S);                      \
+    else if (p.rw == 2) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 2, IDX, decltype(S), SHARES>), S);              \
+    else if (p.nt == 1) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 4, IDX, decltype(S), SHARES>), S);              \
+    else PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 2, 4, IDX, decltype(S), SHARES>), S);                             \
   } while (0)
 #define PKV_TREE_LAUNCH(KERNEL, S) hipLaunchKernelGGL(KERNEL, grid, block, 0, s, c, S)
 #define PKV_TREE_S                                                              \
   do {                                                                          \
-    if (is_one) { if (indexed) PKV_TREE(true, one); else PKV_TREE(false, one); } \
-    else { if (indexed) PKV_TREE(true, sg); else PKV_TREE(false, sg); }          \
+    if (c.by_keys) { if (indexed) PKV_TREE(true, one, true); else PKV_TREE(false, one, true); } \
+    else if (is_one) { if (indexed) PKV_TREE(true, one, false); else PKV_TREE(false, one, false); } \
+    else { if (indexed) PKV_TREE(true, sg, false); else PKV_TREE(false, sg, false); }          \
   } while (0)
   if (bf) {
     constexpr bool BF = true;
@@ -885,11 +926,11 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
   if (p.n_splits == 1) return PKV_OK;
   const dim3 merge((unsigned)((n_rows + 3) / 4));
   if (bf)
-    hipLaunchKernelGGL(pkv_tree_merge_kernel<true>, merge, dim3(256), 0, s, (const float *)c.ws_o, (const float *)c.ws_ml, p.n_splits, rows,
-                       n_rows, a->n_draft, a->group, a->n_kv_heads, a->out);
+    hipLaunchKernelGGL(pkv_tree_merge_kernel<true>, merge, dim3(256), 0, s, c.ws_o, c.ws_ml, c.out, c.row_keys, c.n_splits, (uint32_t)rows,
+                       (uint32_t)n_rows, (uint32_t)c.n_draft, (uint32_t)c.group, (uint32_t)c.n_kv_heads, c.by_keys, c.total, c.n_bh, c.n_pairs);
   else
-    hipLaunchKernelGGL(pkv_tree_merge_kernel<false>, merge, dim3(256), 0, s, (const float *)c.ws_o, (const float *)c.ws_ml, p.n_splits, rows,
-                       n_rows, a->n_draft, a->group, a->n_kv_heads, a->out);
+    hipLaunchKernelGGL(pkv_tree_merge_kernel<false>, merge, dim3(256), 0, s, c.ws_o, c.ws_ml, c.out, c.row_keys, c.n_splits, (uint32_t)rows,
+                       (uint32_t)n_rows, (uint32_t)c.n_draft, (uint32_t)c.group, (uint32_t)c.n_kv_heads, c.by_keys, c.total, c.n_bh, c.n_pairs);
   PKV_LAUNCH_CHECK("pkv_tree_merge_kernel");
   return PKV_OK;
 }

@@ -297,6 +297,20 @@ def test_tree_attention_streams_and_graphs():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("bs,h,group,t,dtype", [(1, 1, 2, 3, BF), (2, 4, 4, 3, BF), (8, 8, 2, 6, BF), (5, 13, 1, 9, BF), (3, 4, 7, 7, F32), (1, 3, 8, 20, BF)])
+@pytest.mark.parametrize("counts", ["none", "all", "one", "ramp", "ones"])
+def test_tree_key_counts(bs, h, group, t, dtype, counts):
+    """Splits go to rows by their keys: all of them to one row, none, as many as there are turns, more rows than are dealt out that way."""
+    rows = 5000 if bs * h < 20 else 700
+    c = tree_case(9, bs, h, group, t, rows, dtype)
+    n = torch.arange(bs * h, dtype=torch.int32)
+    c["rk"] = {"none": -n, "all": n * 0 + rows + 5, "one": (n == bs * h // 2) * rows, "ramp": n * rows // (bs * h), "ones": n * 0 + 1}[counts].to(torch.int32).view(bs, h)
+    want, tol = exact_tree(c)
+    y = run_tree(c)
+    check(y, want, tol)
+    assert torch.equal(y, run_tree(c))
+
+
 # ------------------------------------------------------------- 4-bit weights
 
 
