@@ -306,9 +306,10 @@ def test_tree_key_counts(bs, h, group, t, dtype, counts):
     n = torch.arange(bs * h, dtype=torch.int32)
     c["rk"] = {"none": -n, "all": n * 0 + rows + 5, "one": (n == bs * h // 2) * rows, "ramp": n * rows // (bs * h), "ones": n * 0 + 1}[counts].to(torch.int32).view(bs, h)
     want, tol = exact_tree(c)
-    y = run_tree(c)
+    g = to_gpu(c)
+    y = run_tree(g)
     check(y, want, tol)
-    assert torch.equal(y, run_tree(c))
+    assert torch.equal(y, run_tree(g))
 
 
 # ------------------------------------------------------------- 4-bit weights
