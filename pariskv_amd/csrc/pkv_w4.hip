@@ -257,7 +257,7 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_w4_kernel(const uint
                                                                       int per_split, W4Out out, float *__restrict__ ws) {
   constexpr int kParts = 2, kGroup = GATED ? 4 : 8, kRowVecs = 32, kSlab = 16 * MT * kRowVecs * 16;
   static_assert(kSlab == MT * kWaves * PKV_WAVE * 16, "MT loads of the workgroup a round");
-  constexpr int kPart = kWaves * kParts * (MT > 1 ? MT / 2 : 1) * PKV_WAVE * 16, kLds = 2 * kSlab > kPart ? 2 * kSlab : kPart;
+  constexpr int kPart = kWaves * kParts * ((MT + 1) / 2) * PKV_WAVE * 16, kLds = 2 * kSlab > kPart ? 2 * kSlab : kPart;
   __shared__ alignas(16) char lds[kLds];
   const int tid = threadIdx.x, lane = tid & (PKV_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / PKV_WAVE), n = lane & 15, j = lane >> 4;
   const int kg = wave & 1, my_tile = wave >> 1;
@@ -323,14 +323,14 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_w4_kernel(const uint
     round(i + 1, ahead[0], ring[1]);
   }
   // Lane (n, j) has rows 4 j .. 4 j + 3 of its tiles for row n of x.  The two waves of a tile exchange halves of their shares: the one with the
-  // odd chunks finishes the upper half of the rows of x (of 16 rows: none).
-  constexpr int kHalf = MT > 1 ? MT / 2 : 1;
+  // odd chunks finishes the upper half of the rows of x (of 16 rows: none; of 48 both finish the middle).
+  constexpr int kHalf = (MT + 1) / 2;
   w4_f32x4(*const part)[kParts][kHalf][PKV_WAVE] = (w4_f32x4(*)[kParts][kHalf][PKV_WAVE])lds;
   __syncthreads();
 #pragma unroll
   for (int p = 0; p < kParts; ++p)
 #pragma unroll
-    for (int t = 0; t < kHalf; ++t)
+    for (int t = kHalf - 1; t >= 0; --t)
       if (kg) {
         part[wave][p][t][lane] = tot[p][t];
       } else {
@@ -506,7 +506,7 @@ W4Plan w4_plan(int64_t rows, int64_t n, int64_t k, bool gated) {
     p.xkb = x_bytes <= 16 * 1024 ? 16 : x_bytes <= 64 * 1024 ? 64 : 120;
     return p;
   }
-  p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.mt = rows >= 64 ? 4 : (int)(rows + 15) / 16;  // 48 rows as three tiles / as four: gated 12288 x 4096 24.8 / 28.9 us
   p.row_tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t groups = (gated ? (w4_tiles(n) + 3) / 4 : (w4_tiles(n) + 7) / 8) * p.row_tiles;
   int64_t s = 256 / groups, most = chunks / 8;  // at least four rounds each
@@ -570,6 +570,7 @@ int w4_launch(const void *x, int64_t x_stride, int64_t rows, W4Matrix a, W4Matri
   } while (0)
   if (p.mt == 1) PKV_W4_G(1);
   else if (p.mt == 2) PKV_W4_G(2);
+  else if (p.mt == 3) PKV_W4_G(3);
   else PKV_W4_G(4);
 #undef PKV_W4_G
 #undef PKV_W4
