@@ -825,6 +825,9 @@ TreePlan tree_plan(int dtype, int bs, int n_kv_heads, int rows, int64_t total) {
     if (s > kTreeMaxSplits) s = kTreeMaxSplits;
     p.n_splits = (int)(s < 1 ? 1 : s);
   };
+  // Two row tiles a wave read K and V from LDS once for both, but leave half the workgroups, which costs more where their share of keys is short:
+  // us, one / two: 8 x 8 x 1617 keys, 256 rows 38 / 50; 1 x 8 x 4096, 512 rows 30 / 35; 2 x 8 x 16384, 128 rows 44 / 42; 1 x 8 x 32768, 256 rows
+  // (two always) 62.  fp32 has no registers for two.
   split(1);
   if (bf && rows > 64) {
     split(2);

@@ -355,7 +355,7 @@ def test_w4_pack_and_unpack(group, n):
         assert torch.equal(handle(w).dequantize().double().cpu(), real.float().double())
 
 
-@pytest.mark.parametrize("m", [1, 2, 3, 8, 15, 16, 17, 31, 32, 33, 50, 64, 65, 130])
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 15, 16, 17, 31, 32, 33, 48, 50, 64, 65, 130])
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_w4_linear_rows(m, group):
     from pariskv_amd import ops
