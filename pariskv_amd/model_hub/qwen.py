@@ -312,6 +312,6 @@ class QwenModel:
                 before = t
         if len(path) != self.kv_cache.batch_size or any(len(row) != len(path[0]) for row in path):
             raise RuntimeError("path: as many tokens for every sequence")
-        self._draft = None
         if path[0]:
             self.kv_cache.commit_draft(ks, vs, path)
+        self._draft = None

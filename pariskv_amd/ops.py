@@ -669,6 +669,8 @@ class PathAppend:
         table = self._table.copy()
         table[:, 0], n_draft, k_layer, ks = self._rows_of(draft_k)
         table[:, 1], n_v, v_layer, vs = self._rows_of(draft_v)
+        if not isinstance(slots, int) and len(slots) != len(table):
+            raise RuntimeError("slots: one row, or one a layer")
         table[:, -1] = slots
         if n_v != n_draft:
             raise RuntimeError("drafted K and V rows differ in shape")
