@@ -669,8 +669,6 @@ class PathAppend:
         table = self._table.copy()
         table[:, 0], n_draft, k_layer, ks = self._rows_of(draft_k)
         table[:, 1], n_v, v_layer, vs = self._rows_of(draft_v)
-        if not isinstance(slots, int) and len(slots) != len(table):
-            raise RuntimeError("slots: one row, or one a layer")
         table[:, -1] = slots
         if n_v != n_draft:
             raise RuntimeError("drafted K and V rows differ in shape")
@@ -848,13 +846,13 @@ class TreeAttention:
         in their concatenated order, a row sees (0 or less: none).  Returns [bs,T,Hq,128]; a token that sees nothing gets zeros, and
         what a token does not see does not touch it, whatever it holds."""
         bs, H, G = self.bs, self.H, self.G
-        shape, dt, at = tuple(queries.shape), queries.dtype, queries.get_device()
+        shape, dt, at = queries.shape, queries.dtype, queries.get_device()
         T = shape[1] if len(shape) == 4 else 0
         if shape != (bs, T, H * G, HEAD_DIM) or not 1 <= T <= self.max_draft:
             raise RuntimeError("queries: [bs,T,Hq,128], 1 <= T <= max_draft")
-        code = _dt(dt)
+        code = _lib.DTYPE_BF16 if dt == torch.bfloat16 else _dt(dt)
         rows = (bs, T, H, HEAD_DIM)
-        if tuple(draft_k.shape) != rows or tuple(draft_v.shape) != rows or draft_k.dtype != dt or draft_v.dtype != dt:
+        if draft_k.shape != rows or draft_v.shape != rows or draft_k.dtype != dt or draft_v.dtype != dt:
             raise RuntimeError("draft_k, draft_v: [bs,T,Hkv,128] of the queries' type")
         if at < 0 or draft_k.get_device() != at or draft_v.get_device() != at:
             _cuda(queries, draft_k, draft_v)
@@ -874,9 +872,10 @@ class TreeAttention:
             dv = dv.clone(memory_format=torch.contiguous_format)
             vs = dv.stride()
         n_seg = len(segments)
-        _need(n_seg <= 4, "0..4 key segments")
+        if n_seg > 4:
+            raise RuntimeError("0..4 key segments")
         segs, total = [], 0
-        for i, seg in enumerate(segments):
+        for seg in segments:
             k, v, row0, n_rows = seg[:4]
             idx = seg[4] if len(seg) > 4 else None
             ss, kshape = k.stride(), k.shape
@@ -900,17 +899,21 @@ class TreeAttention:
                       0 <= n_rows <= idx.shape[2] and 0 <= row0 < kshape[2], "segment indices: contiguous int64 [bs,Hkv,>=n_rows]")
                 segs += (k.data_ptr(), v.data_ptr(), ss[0], ss[1], row0, n_rows, idx.data_ptr(), idx.shape[2], kshape[2] - row0)
         segs += _NO_SEGMENTS[9 * n_seg:]
-        _need(total <= self.max_keys, "more cached keys than max_keys")
+        if total > self.max_keys:
+            raise RuntimeError("more cached keys than max_keys")
         mask_at = mask_b = mask_t = keys_at = 0
         if mask is not None:
-            mshape = tuple(mask.shape)
-            _need(mask.dtype == torch.bool and mshape in ((bs, T, T), (T, T)), "mask: bool [T,T] or [bs,T,T]")
+            mshape = mask.shape
+            if mask.dtype != torch.bool or (mshape != (T, T) and mshape != (bs, T, T)):
+                raise RuntimeError("mask: bool [T,T] or [bs,T,T]")
             if mask.get_device() != at:
                 _cuda(mask)
                 _one_device(queries, mask)
-            if mask.stride(-1) != 1:
+            ms = mask.stride()
+            if ms[-1] != 1:
                 mask = mask.contiguous()
-            mask_at, mask_t, mask_b = mask.data_ptr(), mask.stride(-2), mask.stride(0) if len(mshape) == 3 else 0
+                ms = mask.stride()
+            mask_at, mask_t, mask_b = mask.data_ptr(), ms[-2], ms[0] if len(ms) == 3 else 0
         if row_keys is not None:
             _cuda(row_keys)
             _one_device(queries, row_keys)
@@ -921,7 +924,7 @@ class TreeAttention:
         else:
             _cuda(out)
             _one_device(queries, out)
-            _need(tuple(out.shape) == shape and out.dtype == dt and out.is_contiguous() and out.data_ptr() % 16 == 0, "out: contiguous, like queries")
+            _need(out.shape == shape and out.dtype == dt and out.is_contiguous() and out.data_ptr() % 16 == 0, "out: contiguous, like queries")
         lib = _lib.lib()
         need = lib.pkv_tree_attention_ws_bytes(code, bs, H, G, T, total)
         ws = queries.new_empty(need, dtype=torch.uint8) if need else None
@@ -1109,7 +1112,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
         _one_device(packed, bias)
         _need(bias.is_cuda and bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == n, "bias: contiguous bf16 [n]")
     code = _lib.DTYPE_BF16 if out_dtype is None else _dt(out_dtype)
-    y = x.new_empty((*shape[:-1], n)) if code == _lib.DTYPE_BF16 else x.new_empty((*shape[:-1], n), dtype=torch.float32)
+    to = (m, n) if len(shape) == 2 else (*shape[:-1], n)
+    y = x.new_empty(to) if code == _lib.DTYPE_BF16 else x.new_empty(to, dtype=torch.float32)
     if m > 0:
         need = weight.ws_bytes(m)
         ws = x.new_empty(need, dtype=torch.uint8) if need else None
