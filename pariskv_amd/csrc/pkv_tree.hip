@@ -789,15 +789,17 @@ __global__ __launch_bounds__(256) void pkv_tree_merge_kernel(const float *__rest
   const float c = __builtin_amdgcn_exp2f(m - base), all = pkv_wave_sum(l * c);
   const float weight = all == 0.f ? 0.f : c / all;
   float x = 0.f, y = 0.f;
+  const float *const parts = ws_o + first * 128;
   for (int s = 0; s < n_splits; s += 16) {
     float2 o[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      o[i] = s + i < n_splits ? *(const float2 *)(ws_o + (first + (int64_t)(s + i) * rows) * 128 + 2 * lane) : float2{0.f, 0.f};
+    for (int i = 0; i < 16; ++i)  // past the last split: the last again, as zeros
+      o[i] = *(const float2 *)(parts + (int64_t)(s + i < n_splits ? s + i : n_splits - 1) * rows * 128 + 2 * lane);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float f = s + i < n_splits ? __shfl(weight, s + i, PKV_WAVE) : 0.f;
-      x = fmaf(o[i].x, f, x), y = fmaf(o[i].y, f, y);
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), s + i));
+      const bool in = s + i < n_splits;
+      x = fmaf(in ? o[i].x : 0.f, f, x), y = fmaf(in ? o[i].y : 0.f, f, y);
     }
   }
   const uint32_t b = bh / n_kv_heads, h = bh - b * n_kv_heads, u = row / group;
