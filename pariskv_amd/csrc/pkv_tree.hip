@@ -431,18 +431,70 @@ __device__ __forceinline__ uint32_t tree_total(const TreeCall &a, int bh) {
   return rk <= 0 ? 0u : (uint32_t)rk < a.total ? (uint32_t)rk : a.total;
 }
 
-// Places of cached keys of one (b, h).  The fields of segments in one tensor are held in registers and added up: a field picked by a lane
-// would be loaded from memory, and the wait for it would be for all keys under way too.
+typedef const __attribute__((address_space(1))) char *tree_global;
+__device__ __forceinline__ pkv_u32x4 tree_read(const char *p) { return *(const pkv_u32x4 *)p; }
+__device__ __forceinline__ pkv_u32x4 tree_read(tree_global p) { return *(const __attribute__((address_space(1))) pkv_u32x4 *)p; }
+
+// Places of cached keys of one (b, h), found in two steps: find() asks for the row's number where the keys are selected, place() waits for it.  (In
+// one, with a branch round the load, every search waited for all rows under way: 8 x 8 x 1617 selected keys, 256 rows 46 us, dense ones 37.)
+// Fields of segments are held in registers and added up: a field picked by a lane would be loaded from memory, and the wait for it would be for
+// all keys under way too.
+//
+// Segments in any tensors: of each the addresses that key 0 would have if the segment were all there is.  Such addresses are plain numbers to
+// the compiler, which reads them with instructions that may go to LDS and are waited for with it, unless told that they are global.
+// us, two tensors, like this / with every field picked on its own and unmarked addresses: 2 x 8 x 20000 keys, 32 rows 40 / 68, fp32 81 / 148.
 template <bool BF16, bool INDEXED, typename SEGS>
 struct TreePlaces {
   static constexpr uint32_t kRow = BF16 ? 256 : 512;
-  const SEGS &segs;
-  int bh, b, h;
-  __device__ __forceinline__ TreePlaces(const SEGS &s, int bh_, int b_, int h_) : segs(s), bh(bh_), b(b_), h(h_) {}
-  using Found = AttPlace<false>;
-  __device__ __forceinline__ Found find(uint32_t at) const { return att_place<INDEXED, kRow>(segs, bh, b, h, at); }
-  __device__ __forceinline__ AttPlace<false> place(const Found &f) const { return f; }
+  static_assert(PKV_ATTN_MAX_SEGMENTS == 4, "segments one by one");
+  uint32_t end0, end1, end2;
+  uint64_t k0, k1, k2, k3, v0, v1, v2, v3, i0, i1, i2, i3;  // differences from the one before, after the first
+  uint32_t l0, l1, l2, l3;
+  struct Found {
+    uint32_t at, limit;  // limit: rows of a selected key's segment, 0 where it is not selected
+    int64_t x;
+  };
+  static __device__ __forceinline__ uint32_t end_of(const SEGS &s, int t) { return t < s.n ? (uint32_t)att_field(s.end[t]) : 0xffffffffu; }
+  static __device__ __forceinline__ void field(const SEGS &s, int t, int bh, int b, int h, uint64_t &k, uint64_t &v, uint64_t &i, uint32_t &l) {
+    const int64_t first = t > 0 ? att_field(s.end[t > 0 ? t - 1 : 0]) : 0;
+    const uint64_t ip = (uint64_t)att_field(s.idx[t]);
+    const bool selected = INDEXED && ip != 0;
+    const int64_t row0 = att_field(s.row0[t]) - (selected ? 0 : first);
+    const int64_t off = ((int64_t)b * att_field(s.stride_b[t]) + (int64_t)h * att_field(s.stride_h[t])) * (kRow / 128) + row0 * kRow;
+    k = (uint64_t)att_field(s.k[t]) + off, v = (uint64_t)att_field(s.v[t]) + off;
+    i = selected ? ip + ((int64_t)bh * att_field(s.idx_stride[t]) - first) * 8 : 0;
+    l = selected ? (uint32_t)att_field(s.idx_limit[t]) : 0;
+  }
+  __device__ __forceinline__ TreePlaces(const SEGS &s, int bh, int b, int h) {
+    end0 = end_of(s, 0), end1 = end_of(s, 1), end2 = end_of(s, 2);
+    field(s, 0, bh, b, h, k0, v0, i0, l0);
+    field(s, 1, bh, b, h, k1, v1, i1, l1);
+    field(s, 2, bh, b, h, k2, v2, i2, l2);
+    field(s, 3, bh, b, h, k3, v3, i3, l3);
+    k3 -= k2, v3 -= v2, i3 -= i2, l3 -= l2;
+    k2 -= k1, v2 -= v1, i2 -= i1, l2 -= l1;
+    k1 -= k0, v1 -= v0, i1 -= i0, l1 -= l0;
+  }
+  template <typename T>
+  __device__ __forceinline__ T pick(uint32_t at, T a, T b, T c, T d) const {
+    return a + (at >= end0 ? b : 0) + (at >= end1 ? c : 0) + (at >= end2 ? d : 0);
+  }
+  __device__ __forceinline__ Found find(uint32_t at) const {
+    Found f = {at, 0u, 0};
+    if constexpr (INDEXED) {
+      f.limit = pick(at, l0, l1, l2, l3);
+      if (f.limit) f.x = *(const __attribute__((address_space(1))) int64_t *)(pick(at, i0, i1, i2, i3) + (uint64_t)at * 8);
+    }
+    return f;
+  }
+  __device__ __forceinline__ AttPlace<false> place(const Found &f) const {
+    uint32_t r = f.at;
+    if constexpr (INDEXED) r = f.limit ? (uint32_t)(f.x < 0 ? 0 : (f.x >= (int64_t)f.limit ? f.limit - 1 : f.x)) : r;
+    const uint64_t off = (uint64_t)r * kRow;
+    return {pick(f.at, k0, k1, k2, k3) + off, pick(f.at, v0, v1, v2, v3) + off};
+  }
 };
+// Segments in one tensor: byte offsets in it.
 template <bool BF16, bool INDEXED>
 struct TreePlaces<BF16, INDEXED, AttOne> {
   static constexpr uint32_t kRow = BF16 ? 256 : 512;
@@ -461,8 +513,6 @@ struct TreePlaces<BF16, INDEXED, AttOne> {
     delta0 = d0, more1 = d1 - d0, more2 = d2 - d1, more3 = (uint32_t)att_field(s.delta[3]) - d2;
     if (INDEXED) idx = s.idx + (int64_t)bh * s.idx_stride, limit = s.idx_limit, lo = s.idx_lo, hi = s.idx_hi, row0 = s.idx_row0;
   }
-  // A place in two steps, where the keys are selected: find() asks for the row's number, place() waits for it.  (In one, with a branch round the
-  // load, every search waited for all rows under way: 8 x 8 x 1617 selected keys, 256 rows 46 us, dense ones 37.)
   struct Found {
     uint32_t off;  // of a row that is not selected, else kSelected
     int64_t x;
@@ -499,9 +549,9 @@ __device__ __forceinline__ void tree_load_k(pkv_u32x4 (&k)[8], At at) {
   constexpr int kTiles = BF16 ? 2 : 1, kVecs = BF16 ? 4 : 8;
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
-    const char *kp = at(n, 16 * t);
+    const auto kp = at(n, 16 * t);
 #pragma unroll
-    for (int c = 0; c < kVecs; ++c) k[kVecs * t + c] = *(const pkv_u32x4 *)(kp + 64 * c + 16 * j);
+    for (int c = 0; c < kVecs; ++c) k[kVecs * t + c] = tree_read(kp + 64 * c + 16 * j);
   }
 }
 template <bool BF16, typename At>
@@ -510,9 +560,9 @@ __device__ __forceinline__ void tree_load_v(pkv_u32x4 (&v)[8], At at) {
   constexpr int kE = BF16 ? 8 : 4, kVecs = BF16 ? 1 : 2;
 #pragma unroll
   for (int e = 0; e < kE; ++e) {
-    const char *vp = at(4 * j, tree_key(e, 0));
+    const auto vp = at(4 * j, tree_key(e, 0));
 #pragma unroll
-    for (int c = 0; c < kVecs; ++c) v[kVecs * e + c] = *(const pkv_u32x4 *)(vp + 16 * n + 256 * c);
+    for (int c = 0; c < kVecs; ++c) v[kVecs * e + c] = tree_read(vp + 16 * n + 256 * c);
   }
 }
 
@@ -544,15 +594,15 @@ __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_ker
     return places.find((uint32_t)(first + (key < keys ? key : keys - 1)));
   };
   auto k_at = [&](const AttPlace<ONE> &place) {
-    return [&](int base, int key) -> const char * {
+    return [&](int base, int key) {
       if constexpr (ONE) return places.k + (uint64_t)tree_from(place, 4 * base, key).off;
-      else return (const char *)place.pull(place.k, base + key);
+      else return (tree_global)place.pull(place.k, base + key);
     };
   };
   auto v_at = [&](const AttPlace<ONE> &place) {
-    return [&](int base, int key) -> const char * {
+    return [&](int base, int key) {
       if constexpr (ONE) return places.v + (uint64_t)tree_from(place, 4 * base, key).off;
-      else return (const char *)place.pull(place.v, base + key);
+      else return (tree_global)place.pull(place.v, base + key);
     };
   };
 
@@ -650,11 +700,13 @@ __global__ __launch_bounds__(kWideWaves * PKV_WAVE, 2) void pkv_tree_wide_kernel
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) {
       const AttPlace<ONE> at = places.place(found[u]);
-      const char *kp, *vp;
-      if constexpr (ONE) kp = places.k + (uint64_t)at.off, vp = places.v + (uint64_t)at.off;
-      else kp = (const char *)at.k, vp = (const char *)at.v;
-      r.k[u] = __builtin_nontemporal_load((const pkv_u32x4 *)kp + my_vec);
-      r.v[u] = __builtin_nontemporal_load((const pkv_u32x4 *)vp + my_vec);
+      if constexpr (ONE) {
+        r.k[u] = __builtin_nontemporal_load((const pkv_u32x4 *)(places.k + (uint64_t)at.off) + my_vec);
+        r.v[u] = __builtin_nontemporal_load((const pkv_u32x4 *)(places.v + (uint64_t)at.off) + my_vec);
+      } else {
+        r.k[u] = __builtin_nontemporal_load((const __attribute__((address_space(1))) pkv_u32x4 *)at.k + my_vec);
+        r.v[u] = __builtin_nontemporal_load((const __attribute__((address_space(1))) pkv_u32x4 *)at.v + my_vec);
+      }
     }
   };
   auto put = [&](const Rows &r, int buffer) {
@@ -900,7 +952,7 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
   hipStream_t s = (hipStream_t)stream;
   c.n_splits = p.n_splits, c.row_tiles = p.row_tiles, c.n_pairs = a->bs * a->n_kv_heads * p.n_splits;
   c.n_bh = a->bs * a->n_kv_heads;
-  if (is_one && a->row_keys && p.n_splits > 1 && c.n_bh <= PKV_WAVE) c.by_keys = 1 + __builtin_ctz(p.turn);
+  if (a->row_keys && p.n_splits > 1 && c.n_bh <= PKV_WAVE) c.by_keys = 1 + __builtin_ctz(p.turn);
   const dim3 grid = tree_grid(c);
   const dim3 block((p.rw == 1 ? kTreeWaves : kWideWaves) * PKV_WAVE);
 #define PKV_TREE(IDX, S, SHARES)                                                                                     \
@@ -908,14 +960,15 @@ extern "C" int pkv_tree_attention(const pkv_tree_args *a, void *stream) {
     if (p.rw == 1) PKV_TREE_LAUNCH((pkv_tree_partial_kernel<BF, IDX, decltype(S), SHARES>), S);                      \
     else if (p.rw == 2) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 2, IDX, decltype(S), SHARES>), S);              \
     else if (p.nt == 1) PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 1, 4, IDX, decltype(S), SHARES>), S);              \
-    else PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, 2, 4, IDX, decltype(S), SHARES>), S);                             \
+    else PKV_TREE_LAUNCH((pkv_tree_wide_kernel<BF, BF ? 2 : 1, 4, IDX, decltype(S), SHARES>), S);  /* two: bf16 */     \
   } while (0)
 #define PKV_TREE_LAUNCH(KERNEL, S) hipLaunchKernelGGL(KERNEL, grid, block, 0, s, c, S)
 #define PKV_TREE_S                                                              \
   do {                                                                          \
-    if (c.by_keys) { if (indexed) PKV_TREE(true, one, true); else PKV_TREE(false, one, true); } \
-    else if (is_one) { if (indexed) PKV_TREE(true, one, false); else PKV_TREE(false, one, false); } \
-    else { if (indexed) PKV_TREE(true, sg, false); else PKV_TREE(false, sg, false); }          \
+    if (c.by_keys && is_one) { if (indexed) PKV_TREE(true, one, true); else PKV_TREE(false, one, true); } \
+    else if (c.by_keys) { if (indexed) PKV_TREE(true, sg, true); else PKV_TREE(false, sg, true); }        \
+    else if (is_one) { if (indexed) PKV_TREE(true, one, false); else PKV_TREE(false, one, false); }       \
+    else { if (indexed) PKV_TREE(true, sg, false); else PKV_TREE(false, sg, false); }                     \
   } while (0)
   if (bf) {
     constexpr bool BF = true;

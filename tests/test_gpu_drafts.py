@@ -297,6 +297,25 @@ def test_tree_attention_streams_and_graphs():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("bs,h,group,t,dtype", [(2, 2, 2, 5, BF), (1, 3, 7, 7, BF), (2, 2, 4, 40, BF), (1, 2, 3, 9, F32), (2, 1, 2, 4, F32)])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("sizes", [(300, 1, 40, 700), (3, 64, 64, 0), (1, 2, 3, 4), (0, 500, 0, 33)])
+def test_tree_segments_in_any_tensors(bs, h, group, t, dtype, ragged, sizes):
+    """Four segments in four tensors, two of them selected (one with numbers out of range: the nearest row), short ones side by side in a turn."""
+    g = torch.Generator().manual_seed(sum(sizes) + t)
+    c = tree_case(3, bs, h, group, t, 0, dtype, mask="tree")
+    for i, n in enumerate(sizes):
+        k, v = _randn(g, bs, h, 900, D, dtype=dtype), _randn(g, bs, h, 900, D, dtype=dtype)
+        if i % 2:
+            idx = torch.randint(-5 if i == 3 else 0, 1000 if i == 3 else 890, (bs, h, n + 2), generator=g)
+            c["segs"].append((k, v, 7, n, idx))
+        else:
+            c["segs"].append((k, v, 11 * i, n))
+    if ragged:
+        c["rk"] = torch.randint(-1, sum(sizes) + 2, (bs, h), generator=g, dtype=torch.int32)
+    check(run_tree(to_gpu(c)), *exact_tree(c))
+
+
 @pytest.mark.parametrize("bs,h,group,t,dtype", [(1, 1, 2, 3, BF), (2, 4, 4, 3, BF), (8, 8, 2, 6, BF), (5, 13, 1, 9, BF), (3, 4, 7, 7, F32), (1, 3, 8, 20, BF)])
 @pytest.mark.parametrize("counts", ["none", "all", "one", "ramp", "ones"])
 def test_tree_key_counts(bs, h, group, t, dtype, counts):
