@@ -374,23 +374,23 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_w4_kernel(const uint
   }
 }
 
-// The splits' shares, added in their order; all of them are asked for at once, those that are not there as the last one again.
-constexpr int kMaxSplits = 8;
-template <bool GATED>
+// The splits' shares (at most MOST), added in their order; all of them are asked for at once, those that are not there as the last one again.
+constexpr int kMaxSplits = 16;
+template <bool GATED, int MOST>
 __global__ __launch_bounds__(256) void pkv_w4_sum_kernel(const float *__restrict__ ws, int splits, int64_t n_out, W4Out out) {
   constexpr int kParts = GATED ? 2 : 1;
   const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x, at = blockIdx.y * n_out + col, n_all = gridDim.y * n_out;
   if (col >= n_out) return;
-  float got[kParts][kMaxSplits], v[kParts];
+  float got[kParts][MOST], v[kParts];
 #pragma unroll
   for (int p = 0; p < kParts; ++p)
 #pragma unroll
-    for (int s = 0; s < kMaxSplits; ++s) got[p][s] = ws[((s < splits ? s : splits - 1) * (int64_t)kParts + p) * n_all + at];
+    for (int s = 0; s < MOST; ++s) got[p][s] = ws[((s < splits ? s : splits - 1) * (int64_t)kParts + p) * n_all + at];
 #pragma unroll
   for (int p = 0; p < kParts; ++p) {
     v[p] = got[p][0];
 #pragma unroll
-    for (int s = 1; s < kMaxSplits; ++s) v[p] = s < splits ? v[p] + got[p][s] : v[p];
+    for (int s = 1; s < MOST; ++s) v[p] = s < splits ? v[p] + got[p][s] : v[p];
   }
   w4_store<kParts>(out, at, col, v);
 }
@@ -509,7 +509,9 @@ W4Plan w4_plan(int64_t rows, int64_t n, int64_t k, bool gated) {
   p.mt = rows >= 64 ? 4 : (int)(rows + 15) / 16;  // 48 rows as three tiles / as four: gated 12288 x 4096 24.8 / 28.9 us
   p.row_tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t groups = (gated ? (w4_tiles(n) + 3) / 4 : (w4_tiles(n) + 7) / 8) * p.row_tiles;
-  int64_t s = 256 / groups, most = chunks / 8;  // at least four rounds each
+  // Columns are split where the tiles leave compute units idle and there are more than four rounds, into runs of at least two rounds.  us, runs of at
+  // least four rounds and at most 8 of them / these: 1077 x 1824, 43 rows 19.7 / 14.5; 374 x 12480, 44 rows 17.4 / 13.5; 4096 x 12288, 64 rows 22.5 both.
+  int64_t s = chunks > 8 ? 256 / groups : 1, most = chunks / 4;
   if (s > most) s = most;
   if (s > kMaxSplits) s = kMaxSplits;
   if (s < 1) s = 1;
@@ -576,8 +578,13 @@ int w4_launch(const void *x, int64_t x_stride, int64_t rows, W4Matrix a, W4Matri
 #undef PKV_W4
   PKV_LAUNCH_CHECK("pkv_w4_kernel");
   if (p.splits > 1) {
-    hipLaunchKernelGGL(pkv_w4_sum_kernel<GATED>, dim3((unsigned)((n + 255) / 256), (unsigned)rows), dim3(256), 0, s, (const float *)ws,
-                       p.splits, n, out);
+    const dim3 sum_grid((unsigned)((n + 255) / 256), (unsigned)rows);
+#define PKV_W4_SUM(MOST) hipLaunchKernelGGL((pkv_w4_sum_kernel<GATED, MOST>), sum_grid, dim3(256), 0, s, (const float *)ws, p.splits, n, out)
+    if (p.splits <= 2) PKV_W4_SUM(2);
+    else if (p.splits <= 4) PKV_W4_SUM(4);
+    else if (p.splits <= 8) PKV_W4_SUM(8);
+    else PKV_W4_SUM(kMaxSplits);
+#undef PKV_W4_SUM
     PKV_LAUNCH_CHECK("pkv_w4_sum_kernel");
   }
   return PKV_OK;
