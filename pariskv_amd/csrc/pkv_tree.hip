@@ -877,6 +877,9 @@ TreePlan tree_plan(int dtype, int bs, int n_kv_heads, int rows, int64_t total) {
     int64_t s = kTreeWorkgroups / (bh * p.row_tiles), most = (total + p.turn - 1) / p.turn;
     if (s > most) s = most;
     if (s > kTreeMaxSplits) s = kTreeMaxSplits;
+    // Few keys: no join, which is a launch (2.5 us of the host's time), rather than workgroups side by side.  us on the GPU, two launches / one, 8 KV heads:
+    // 180 keys, 12 rows 8.3 / 6.7, 160 rows 13.2 / 11.4; 380 keys, 12 rows 9.5 / 8.8, 20 rows 11.3 / 12.0; fp32, 120 keys, 12 rows 10.9 / 9.2, 160 rows 16.1 / 22.5.
+    if (total <= (bf ? 384 : p.rw == 1 ? 192 : 0)) s = 1;
     p.n_splits = (int)(s < 1 ? 1 : s);
   };
   // Two row tiles a wave read K and V from LDS once for both, but leave half the workgroups, which costs more where their share of keys is short:

@@ -297,6 +297,38 @@ def test_tree_attention_streams_and_graphs():
         assert torch.equal(a, b)
 
 
+def test_tree_counts_may_change_between_replays():
+    """A captured call deals its splits out by the counts of each replay, with a workspace of its own."""
+    from pariskv_amd import ops
+
+    c = tree_case(5, 3, 2, 4, 9, 4000, BF, mask="tree", ragged=True)
+    g = to_gpu(c)
+    att = ops.TreeAttention(3, 2, 4, 9, 4000, DEV)
+    run = lambda rk: att.run(g["q"], g["segs"], g["dk"], g["dv"], mask=g["mask"], row_keys=rk)
+    held = g["rk"].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(held)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(held)
+        graphs.append((graph, out))
+    for counts in ([4000] * 6, [0, 4000, 0, 0, 0, 7], [1, 2, 3, 4, 5, 6], [-3, 100, 3999, 4001, 64, 0]):
+        held.copy_(torch.tensor(counts, dtype=torch.int32).view(3, 2))
+        eager = run(held)
+        for graph, out in graphs:
+            out.fill_(7.0)
+            graph.replay()
+        torch.cuda.synchronize()
+        c["rk"] = held.cpu()
+        check(eager, *exact_tree(c))
+        assert all(torch.equal(out, eager) for _, out in graphs)
+
+
 @pytest.mark.parametrize("bs,h,group,t,dtype", [(2, 2, 2, 5, BF), (1, 3, 7, 7, BF), (2, 2, 4, 40, BF), (1, 2, 3, 9, F32), (2, 1, 2, 4, F32)])
 @pytest.mark.parametrize("ragged", [False, True])
 @pytest.mark.parametrize("sizes", [(300, 1, 40, 700), (3, 64, 64, 0), (1, 2, 3, 4), (0, 500, 0, 33)])
