@@ -115,22 +115,25 @@ __device__ __forceinline__ void w4_store(const W4Out &o, int64_t at, int64_t col
 // channels apart and came one after the other when they were read straight from there (4096 x 12288, 64 rows: 47 us, of them 12 of
 // instructions).  In LDS vector c (of 16) of a chunk of row r lies at c ^ (r mod 16): the 16 rows of an operand are on different banks.
 
-// Up to 16 rows whose x fits into XKB KB of LDS: it stays there while a workgroup goes through its row tiles.  1 << lg of its waves share a
+// 16 MT rows whose x fits into XKB KB of LDS: it stays there while a workgroup goes through its row tiles.  1 << lg of its waves share a
 // tile, chunk c going to wave c mod (1 << lg), and meet in LDS after it; U chunks ahead are under way, over the ends of tiles too.
 // A chunk costs a wave some 60 vector and 4 matrix instructions for its 1 KB.  151936 x 4096: 1 row 55 us (330 MB: 5.9 TB/s; a plain read
 // reaches 7.1), 8 rows 63 us; with a workgroup to each 16 rows of the matrix, which reads x again for each of them, 75 and 94 us.
-template <int G, bool GATED, int XKB, int U>
-__global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(const uint16_t *__restrict__ x, int64_t x_stride, int rows,
+template <int MT, int G, bool GATED, int XKB, int U>
+__global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(const uint16_t *__restrict__ x, int64_t x_stride, int64_t all_rows,
                                                                             W4Matrix wa, W4Matrix wb, int64_t n_out, int k, int chunks,
                                                                             int by_row_vecs, int lg, int each, int more,
                                                                             W4Out out) {
   constexpr int kParts = GATED ? 2 : 1, kFetch = XKB * 64 / (kWaves * PKV_WAVE) < 8 ? XKB * 64 / (kWaves * PKV_WAVE) : 8;
   __shared__ alignas(16) char lds[XKB * 1024];
-  constexpr int kHalves = XKB == 64 && !GATED ? 1 : 2;  // two workgroups a compute unit
+  constexpr int kHalves = MT > 1 || (XKB == 64 && !GATED) ? 1 : 2;  // what fits; XKB = 64: for two workgroups a compute unit
   __shared__ float s_sum[XKB * 512 / G];                // of x, by row and group
-  __shared__ w4_f32x4 s_part[kHalves][kWaves][kParts][PKV_WAVE];  // rows 4 j .. 4 j + 3 for row n of x at 16 j + (n ^ 4 j): no two on one bank
+  __shared__ w4_f32x4 s_part[kHalves][kWaves][kParts][MT][PKV_WAVE];  // rows 4 j .. 4 j + 3 for row n of x at 16 j + (n ^ 4 j): no two on one bank
   const int tid = threadIdx.x, lane = tid & (PKV_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / PKV_WAVE), n = lane & 15, j = lane >> 4;
   const int tiles = (int)((n_out + kTileRows - 1) / kTileRows), kg = wave & ((1 << lg) - 1), side = kWaves >> lg;
+  const int64_t m0 = (int64_t)blockIdx.y * 16 * MT;
+  const int rows = (int)(all_rows - m0 < 16 * MT ? all_rows - m0 : 16 * MT);
+  x += m0 * x_stride;
   const int per_wave = (chunks + (1 << lg) - 1) >> lg, row_vecs = chunks * (kTileCols / 8), x_vecs = rows * row_vecs;
   const W4Matrix m[2] = {wa, wb};
 
@@ -159,7 +162,7 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(cons
       const int row = in ? p_row : rows - 1, col = in ? p_col : row_vecs - 1, v = row * row_vecs + col;
       asm volatile("" : "+v"(got[u]));  // arrived on every path, or its register's next use would wait for all of the ring
       if (put_at < x_vecs) {            // the whole workgroup
-        *(pkv_u32x4 *)(lds + (v >> 4) * 256 + 16 * ((v & 15) ^ row)) = got[u];
+        *(pkv_u32x4 *)(lds + (v >> 4) * 256 + 16 * ((v ^ row) & 15)) = got[u];
         float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) sum += __uint_as_float(got[u][w] << 16) + __uint_as_float(got[u][w] & 0xffff0000u);
@@ -198,14 +201,14 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(cons
   if constexpr (XKB * 64 > kFetch * kWaves * PKV_WAVE)
     while (put_at < x_vecs) fetch(got), put(got);
   __syncthreads();
-  const int my = n < rows ? n : rows - 1;  // rows that are not there repeat the last; what is computed with them is not stored
-  const char *const x_row = lds + my * (row_vecs * 16);
-  auto x_of = [&](int c, int s) { return *(const pkv_u32x4 *)(x_row + c * 256 + 16 * ((4 * s + j) ^ my)); };
-  const float *const sums = s_sum + my * chunks * (kTileCols / G);
-
-  w4_f32x4 tot[kParts][1];
+  int my[MT];  // rows that are not there repeat the last; what is computed with them is not stored
 #pragma unroll
-  for (int p = 0; p < kParts; ++p) tot[p][0] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < MT; ++t) my[t] = 16 * t + n < rows ? 16 * t + n : rows - 1;
+  w4_f32x4 tot[kParts][MT];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) tot[p][t] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
   // One way through the loop, without a return inside: the waits for the ring count what came after on every path that might be.
   const int step = gridDim.x * side, steps = (each + ((int)blockIdx.x < more)) * per_wave;
   int tile = blockIdx.x * side, i = 0, half = 0;
@@ -214,27 +217,36 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(cons
     for (int u = 0; u < U; ++u) {
       const int c = (i << lg) + kg;
       if (c < chunks && at0 + u < steps)  // the whole wave
-        w4_chunk<1, G, kParts, true>(ring[u], [&](int, int s) { return x_of(c, s); }, [&](int, int g) { return sums[c * (kTileCols / G) + g]; }, tot);
+        w4_chunk<MT, G, kParts, true>(
+            ring[u],
+            [&](int t, int s) { return *(const pkv_u32x4 *)(lds + my[t] * (row_vecs * 16) + c * 256 + 16 * ((4 * s + j) ^ (my[t] & 15))); },
+            [&](int t, int g) { return s_sum[(my[t] * chunks + c) * (kTileCols / G) + g]; }, tot);
       ask(ring[u]);
       if (++i == per_wave && at0 + u < steps) {  // the whole workgroup
         // lane (n, j) has rows 4 j .. 4 j + 3 of the tile for row n of x; the waves' shares are added in their order
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-          s_part[half][wave][p][16 * j + (n ^ 4 * j)] = tot[p][0];
-          tot[p][0] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            s_part[half][wave][p][t][16 * j + (n ^ 4 * j)] = tot[p][t];
+            tot[p][t] = w4_f32x4{0.f, 0.f, 0.f, 0.f};
+          }
         __syncthreads();  // with two halves, one is enough: the other is written next, by waves that are past this
         for (int q = tid >> 8; q < side; q += 2) {
-          const int row = tid >> 4 & 15, at = ((tid & 12) << 4) + ((row ^ (tid & 12)) << 2) + (tid & 3);
+          const int row0 = tid >> 4 & 15, at = ((tid & 12) << 4) + ((row0 ^ (tid & 12)) << 2) + (tid & 3);
           const int64_t col = (int64_t)(tile + q) * kTileRows + (tid & 15);
-          if (row >= rows || col >= n_out) continue;
-          float v[kParts];
 #pragma unroll
-          for (int p = 0; p < kParts; ++p) {
-            v[p] = ((const float *)s_part[half][q << lg][p])[at];
-            for (int w = 1; w < 1 << lg; ++w) v[p] += ((const float *)s_part[half][(q << lg) + w][p])[at];
+          for (int t = 0; t < MT; ++t) {
+            const int row = 16 * t + row0;
+            if (row >= rows || col >= n_out) continue;
+            float v[kParts];
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+              v[p] = ((const float *)s_part[half][q << lg][p][t])[at];
+              for (int w = 1; w < 1 << lg; ++w) v[p] += ((const float *)s_part[half][(q << lg) + w][p][t])[at];
+            }
+            w4_store<kParts>(out, (m0 + row) * n_out + col, col, v);
           }
-          w4_store<kParts>(out, row * n_out + col, col, v);
         }
         tile += step, i = 0;
         if constexpr (kHalves == 2) half ^= 1;
@@ -493,17 +505,40 @@ W4Matrix w4_matrix(const void *packed, int64_t n, int64_t k) {
   PKV_REQUIRE(w4_shape_ok(n, k, group), what ": groups of 32, 64 or 128, k a multiple of them (got n=%lld k=%lld group=%d)", \
               (long long)n, (long long)k, group)
 
-// How a product is taken: rows of x up to 16 that fit into LDS stay there (xkb: how much of it); else 16 mt rows at a time, the columns in
-// `splits` runs of per_split chunks.
+// How a product is taken, 16 mt rows of x at a time: those that fit into LDS stay there (xkb: how much of it) while `workgroups` workgroups go through the
+// matrix, 1 << lg waves to a tile; else they are streamed, the columns in `splits` runs of per_split chunks.
 struct W4Plan {
-  int xkb, mt, splits, per_split;
-  int64_t row_tiles;
+  int xkb, mt, splits, per_split, lg;
+  int64_t row_tiles, workgroups;
 };
 W4Plan w4_plan(int64_t rows, int64_t n, int64_t k, bool gated) {
-  W4Plan p = {0, 1, 1, 0, 1};
-  const int64_t chunks = w4_chunks(k), x_bytes = rows * chunks * kTileCols * 2;
-  if (rows <= 16 && x_bytes <= 120 * 1024) {
-    p.xkb = x_bytes <= 16 * 1024 ? 16 : x_bytes <= 64 * 1024 ? 64 : 120;
+  W4Plan p = {0, 1, 1, 0, 0, 1, 0};
+  const int64_t chunks = w4_chunks(k), tiles = w4_tiles(n);
+  p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  p.row_tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
+  const int64_t x_bytes = (rows < 16 * p.mt ? rows : 16 * p.mt) * chunks * kTileCols * 2;
+  // More than 16 rows, streamed / kept in LDS, us: 96164 x 640, 87 rows 57 / 36; 38959 x 1152, 51 rows 28 / 22, 24 rows 18.5 / 15.0; 3000 x 896,
+  // 60 rows 11.4 / 8.8.  The gated block has to join two matrices' shares of more rows than there is room for: 12288 x 1536, 24 rows 9.6 / 12.6.
+  const int xkb = p.mt > 1 ? 120 : x_bytes <= 16 * 1024 ? 16 : x_bytes <= 64 * 1024 ? 64 : 120;
+  if (x_bytes <= xkb * 1024 && (p.mt == 1 || !gated)) {
+    p.xkb = xkb;
+    auto groups = [&](int lg) { return (tiles + (kWaves >> lg) - 1) / (kWaves >> lg); };
+    if (p.mt == 1) {
+      p.lg = chunks <= 1 ? 0 : chunks <= 2 ? 1 : chunks <= 4 ? 2 : 3;
+      // One workgroup a compute unit reads x once for it; two, where they fit, hide more of each other's waits, which pays from five tiles each.
+      // us with 256 / 512 of them: 6144 x 4096, 8 rows, 7.8 / 8.7; 16384 x 1024, 1 row, 6.0 / 6.3; 32768 x 4096, 1 row, 17.4 / 15.5;
+      // 151936 x 4096, 8 rows, 80 / 63; the gated block, 12288 x 4096, 1 row, 12.9 / 14.5, 65536 x 2048, 34.5 / 37.9
+      p.workgroups = !gated && p.xkb <= 64 && groups(p.lg) > 1024 ? 512 : 256;
+    } else {
+      // as many waves to a tile as leave the longest workgroup the fewest chunks, one of them for the tile's end
+      p.workgroups = 256 / p.row_tiles > 0 ? 256 / p.row_tiles : 1;
+      int64_t best = -1;
+      for (int lg = 3; lg >= 0; --lg) {
+        const int64_t per_wave = (chunks + (1 << lg) - 1) >> lg, cost = (groups(lg) + p.workgroups - 1) / p.workgroups * (per_wave + 1);
+        if (best < 0 || cost < best) best = cost, p.lg = lg;
+      }
+    }
+    if (p.workgroups > groups(p.lg)) p.workgroups = groups(p.lg);
     return p;
   }
   p.mt = rows >= 64 ? 4 : (int)(rows + 15) / 16;  // 48 rows as three tiles / as four: gated 12288 x 4096 24.8 / 28.9 us
@@ -535,22 +570,19 @@ int w4_launch(const void *x, int64_t x_stride, int64_t rows, W4Matrix a, W4Matri
   const W4Out out = {(const uint16_t *)bias, y, out_f32};
   const dim3 block(kWaves * PKV_WAVE);
   if (p.xkb) {
-    const int lg = chunks <= 1 ? 0 : chunks <= 2 ? 1 : chunks <= 4 ? 2 : 3;
-    const int64_t groups = (tiles + (kWaves >> lg) - 1) / (kWaves >> lg);
-    // One workgroup a compute unit reads x once for it; two, where they fit, hide more of each other's waits, which pays from five tiles each.
-    // us with 256 / 512 of them: 6144 x 4096, 8 rows, 7.8 / 8.7; 16384 x 1024, 1 row, 6.0 / 6.3; 32768 x 4096, 1 row, 17.4 / 15.5;
-    // 151936 x 4096, 8 rows, 80 / 63; the gated block, 12288 x 4096, 1 row, 12.9 / 14.5, 65536 x 2048, 34.5 / 37.9
-    const int64_t most = !GATED && p.xkb <= 64 && groups > 1024 ? 512 : 256;
-    const dim3 grid((unsigned)(groups < most ? groups : most));
+    const int64_t groups = (tiles + (kWaves >> p.lg) - 1) / (kWaves >> p.lg);
+    const dim3 grid((unsigned)p.workgroups, (unsigned)p.row_tiles);
     const int row_vecs = (int)chunks * (kTileCols / 8), by_row_vecs = ((1 << 24) + row_vecs - 1) / row_vecs;  // v / row_vecs = v by_row_vecs >> 24, v <= 512
-#define PKV_W4_X(G, XKB)                                                                                                       \
-  hipLaunchKernelGGL((pkv_w4_resident_kernel<G, GATED, XKB, (GATED && G == 32) ? 2 : 4>), grid, block, 0, s, (const uint16_t *)x, \
-                     x_stride, (int)rows, a, b, n, (int)k, (int)chunks, by_row_vecs, lg, (int)(groups / grid.x), (int)(groups % grid.x), out)
-#define PKV_W4_G(G)                        \
-  do {                                     \
-    if (p.xkb == 16) PKV_W4_X(G, 16);      \
-    else if (p.xkb == 64) PKV_W4_X(G, 64); \
-    else PKV_W4_X(G, 120);                 \
+#define PKV_W4_X(MT, G, XKB)                                                                                                       \
+  hipLaunchKernelGGL((pkv_w4_resident_kernel<MT, G, GATED, XKB, (GATED && G == 32) ? 2 : 4>), grid, block, 0, s, (const uint16_t *)x, \
+                     x_stride, rows, a, b, n, (int)k, (int)chunks, by_row_vecs, p.lg, (int)(groups / grid.x), (int)(groups % grid.x), out)
+#define PKV_W4_G(G)                                        \
+  do {                                                     \
+    if (p.mt == 4) PKV_W4_X(GATED ? 1 : 4, G, 120);        \
+    else if (p.mt == 2) PKV_W4_X(GATED ? 1 : 2, G, 120);   \
+    else if (p.xkb == 16) PKV_W4_X(1, G, 16);              \
+    else if (p.xkb == 64) PKV_W4_X(1, G, 64);              \
+    else PKV_W4_X(1, G, 120);                              \
   } while (0)
     if (group == 32) PKV_W4_G(32);
     else if (group == 64) PKV_W4_G(64);

@@ -437,9 +437,10 @@ def test_w4_linear_sizes(n, k, group, m):
 
 
 # a few rows that stay in LDS: all of it, more than a workgroup's share of row tiles, tiles shared by fewer waves; rows that do not fit; columns
-# split over workgroups, with an odd run of chunks at the end and with rows of the result that are not a multiple of four long
+# split over workgroups, with an odd run of chunks at the end and with rows of the result that are not a multiple of four long; more rows that fit
 @pytest.mark.parametrize("m,n,k,group", [(13, 50, 4096, 128), (3, 16500, 1024, 128), (2, 20011, 256, 32), (16, 5000, 640, 64), (5, 100, 16384, 128),
-                                         (40, 64, 4224, 128), (20, 131, 8192, 32), (64, 4096, 2048, 64)])
+                                         (40, 64, 4224, 128), (20, 131, 8192, 32), (64, 4096, 2048, 64),
+                                         (33, 5000, 896, 128), (100, 700, 160, 32), (64, 17000, 384, 64), (17, 90, 1920, 128), (32, 1003, 64, 32)])
 def test_w4_ways(m, n, k, group):
     from pariskv_amd import ops
 
@@ -455,6 +456,35 @@ def test_w4_ways(m, n, k, group):
     check(z, want, 1.1 * ta * (yb.abs() + tb) + ya.abs() * tb + 8 * U * want.abs() + HALF[BF] * want.abs() + 1e-37)
     for _ in range(2):
         assert torch.equal(y, ops.w4_linear(gx, ha, bias.to(DEV), F32)) and torch.equal(z, ops.w4_silu_mul(gx, ha, hb))
+
+
+@pytest.mark.parametrize("m,n,k,group", [(3, 500, 1024, 128), (48, 500, 4096, 64), (40, 700, 640, 32)])
+def test_w4_captured_calls_keep_their_own_shares(m, n, k, group):
+    """Two captured graphs and eager calls in turn, on rows that change: every replay is the eager result."""
+    from pariskv_amd import ops
+
+    ha, hb = handle(w4_case(1, n, k, group)), handle(w4_case(2, n, k, group))
+    g = torch.Generator().manual_seed(k)
+    held = _randn(g, m, k).to(DEV)
+    both = lambda: (ops.w4_linear(held, ha), ops.w4_silu_mul(held, ha, hb))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = both()
+        graphs.append((graph, outs))
+    for _ in range(4):
+        held.copy_(_randn(g, m, k))
+        want = both()
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for _, outs in graphs for x, y in zip(outs, want))
 
 
 def test_w4_linear_layouts_and_odd_values():
