@@ -541,7 +541,10 @@ W4Plan w4_plan(int64_t rows, int64_t n, int64_t k, bool gated) {
     if (p.workgroups > groups(p.lg)) p.workgroups = groups(p.lg);
     return p;
   }
-  p.mt = rows >= 64 ? 4 : (int)(rows + 15) / 16;  // 48 rows as three tiles / as four: gated 12288 x 4096 24.8 / 28.9 us
+  // Tiles of up to 64 rows, as even as they can be.  us, 48 rows as one tile of three times 16 / of four: gated 12288 x 4096 24.8 / 28.9;
+  // 76 rows as two of three / of four: 7159 x 9344 31.8 / 37.0.
+  const int64_t even = (rows + 63) / 64;
+  p.mt = (int)(((rows + even - 1) / even + 15) / 16);
   p.row_tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t groups = (gated ? (w4_tiles(n) + 3) / 4 : (w4_tiles(n) + 7) / 8) * p.row_tiles;
   // Columns are split where the tiles leave compute units idle and there are more than four rounds, into runs of at least two rounds.  us, runs of at
