@@ -297,9 +297,9 @@ int pkv_append_kv_run(const pkv_append_args *args, const void *k_new, int64_t k_
  * and likewise for V; t outside [0, n_draft): the row (and its norm) stays as it is, so that sequences that accepted fewer
  * tokens are padded with -1.  vnorm (all layers or none; rows of 128 bf16 or fp32 elements): the value norm as pkv_append_kv
  * writes it, at [b*vn_stride_b + h*vn_stride_h + slot + i].  Strides of rows in BYTES, multiples of 16; of norms in elements;
- * path int64 on the device; `layers` is host memory, read before the call returns; layer l's drafted rows are l*k_stride_l (v_) bytes
- * behind its draft_k (draft_v), so that layers of one tensor can all name its start.  Drafted rows must not overlap the
- * destination rows. */
+ * path int64 on the device; `layers` and `slots` (a slot for each layer, or NULL: the layers' own) are host memory, read before
+ * the call returns.  A layer without drafted rows of its own (NULL) has them l*k_stride_l (v_) bytes behind args' draft_k
+ * (draft_v): the layers of one tensor.  Drafted rows must not overlap the destination rows. */
 typedef struct pkv_path_layer {
   const void *draft_k, *draft_v;
   void *dst_k, *dst_v;
@@ -308,6 +308,7 @@ typedef struct pkv_path_layer {
 } pkv_path_layer;
 typedef struct pkv_path_args {
   const int64_t *path;
+  const void *draft_k, *draft_v;
   int64_t path_stride_b;
   int bs, n_kv_heads, n, n_draft, row_bytes;
   int64_t k_stride_l, v_stride_l;
@@ -315,7 +316,7 @@ typedef struct pkv_path_args {
   int64_t dst_stride_b, dst_stride_h, dst_len; /* bytes, bytes, rows */
   int64_t vn_stride_b, vn_stride_h;
 } pkv_path_args;
-int pkv_append_path(const pkv_path_args *args, const pkv_path_layer *layers, int n_layers, void *stream);
+int pkv_append_path(const pkv_path_args *args, const pkv_path_layer *layers, const int64_t *slots, int n_layers, void *stream);
 
 /* The oldest tokens of a layer leave the GPU: replaces the copy_() of staged
  * [bs][h][n][d] tensors into slices of the pinned host tensors on the side
@@ -505,7 +506,8 @@ int pkv_decode_attention(const void *q, int dtype, int bs, int n_kv_heads, int g
  * q [bs][n_draft][n_kv_heads*group][128], heads side by side, of `dtype`; out the same, contiguous; q_stride_* and the drafted
  * rows' strides in elements (rows 128 contiguous elements, 16-byte multiples); mask strides in bytes, 0 allowed.
  * 1 <= n_draft <= 1024, group >= 1 with n_draft * group <= 8192, fewer than 2^23 cached keys.
- * fp32 sums and statistics; bf16: probabilities are rounded to bf16 for the product with V.
+ * fp32 sums and statistics; bf16: probabilities are rounded to bf16 for the product with V, and the normaliser is the sum of the
+ * rounded ones.
  * ws: pkv_tree_attention_ws_bytes(dtype, bs, n_kv_heads, group, n_draft, cached keys) bytes for the partial results (0: none needed). */
 typedef struct pkv_tree_args {
   const void *q;
@@ -582,7 +584,8 @@ int pkv_w4_quantize(const void *w, int dtype, int64_t row_stride, int64_t n, int
 int pkv_w4_unpack(const void *packed, int64_t n, int64_t k, int group, float *w, void *stream);
 
 /* y[m][n] = sum_k x[m][k] weight[n][k] + bias[n] (no counterpart in the reference): x bf16 [rows][k] (row stride in elements, a
- * multiple of 8, 16-byte aligned), bias bf16 [n] or NULL, y [rows][n] contiguous of out_dtype.  Sums in fp32, one rounding.
+ * multiple of 8, 16-byte aligned), bias bf16 [n] or NULL, y [rows][n] contiguous of out_dtype.  Sums in fp32, one rounding; codes are
+ * summed up as 16 + code before their scale: a group's sum of |x| stays below 10^37.
  * ws: pkv_w4_ws_bytes(rows, n, k, group, 0) bytes for the shares of columns that several workgroups take (0: none needed). */
 size_t pkv_w4_ws_bytes(int64_t rows, int64_t n, int64_t k, int group, int gated);
 int pkv_w4_linear(const void *x, int64_t x_stride, int64_t rows, const void *packed, int64_t n, int64_t k, int group,

@@ -51,7 +51,7 @@ class PathLayer(C.Structure):
 class PathArgs(C.Structure):
     """Mirror of ``pkv_path_args``."""
 
-    _fields_ = [("path", _vp), ("path_stride_b", _i64), ("bs", _i), ("n_kv_heads", _i), ("n", _i), ("n_draft", _i), ("row_bytes", _i),
+    _fields_ = [("path", _vp), ("draft_k", _vp), ("draft_v", _vp), ("path_stride_b", _i64), ("bs", _i), ("n_kv_heads", _i), ("n", _i), ("n_draft", _i), ("row_bytes", _i),
                 ("k_stride_l", _i64), ("v_stride_l", _i64), ("k_stride_b", _i64), ("k_stride_h", _i64), ("k_stride_t", _i64), ("v_stride_b", _i64), ("v_stride_h", _i64),
                 ("v_stride_t", _i64), ("dst_stride_b", _i64), ("dst_stride_h", _i64), ("dst_len", _i64), ("vn_stride_b", _i64),
                 ("vn_stride_h", _i64)]
@@ -180,7 +180,7 @@ PROTOTYPES = {
     "pkv_decode_attention_run": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnArgs), _vp]),
     "pkv_decode_attention_counted": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnArgs), _vp, _i, _vp]),
     "pkv_append_kv_run": (_i, [C.POINTER(AppendArgs), _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp]),
-    "pkv_append_path": (_i, [_vp, _vp, _i, _vp]),
+    "pkv_append_path": (_i, [_vp, _vp, _vp, _i, _vp]),
     "pkv_tree_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i64]),
     "pkv_tree_attention": (_i, [_vp, _vp]),
     "pkv_w4_bytes": (_sz, [_i64, _i64, _i]),

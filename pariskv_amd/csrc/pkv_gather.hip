@@ -309,7 +309,7 @@ extern "C" int pkv_append_kv_run(const pkv_append_args *a, const void *k_new, in
                        a->vn_stride_h, stream);
 }
 
-extern "C" int pkv_append_path(const pkv_path_args *a, const pkv_path_layer *layers, int n_layers, void *stream) {
+extern "C" int pkv_append_path(const pkv_path_args *a, const pkv_path_layer *layers, const int64_t *slots, int n_layers, void *stream) {
   PKV_REQUIRE(a && layers && a->path, "append_path: null pointer");
   PKV_REQUIRE(n_layers > 0 && a->bs > 0 && a->n_kv_heads > 0 && a->n > 0 && a->n_draft > 0, "append_path: bad counts");
   PKV_REQUIRE(a->row_bytes > 0 && a->row_bytes % 16 == 0 && a->row_bytes <= 4096, "row_bytes must be a multiple of 16 (got %d)",
@@ -325,12 +325,14 @@ extern "C" int pkv_append_path(const pkv_path_args *a, const pkv_path_layer *lay
               "append_path: value norms need rows of 128 bf16 or fp32 elements");
   for (int i = 0; i < n_layers; ++i) {
     const pkv_path_layer &l = layers[i];
-    PKV_REQUIRE(l.draft_k && l.draft_v && l.dst_k && l.dst_v, "append_path: null pointer of layer %d", i);
-    PKV_REQUIRE(pkv_aligned(l.draft_k, 16) && pkv_aligned(l.draft_v, 16) && pkv_aligned(l.dst_k, 16) && pkv_aligned(l.dst_v, 16),
+    const int64_t slot = slots ? slots[i] : l.slot;
+    const void *const dk = l.draft_k ? l.draft_k : a->draft_k, *const dv = l.draft_v ? l.draft_v : a->draft_v;
+    PKV_REQUIRE(dk && dv && l.dst_k && l.dst_v, "append_path: null pointer of layer %d", i);
+    PKV_REQUIRE(pkv_aligned(dk, 16) && pkv_aligned(dv, 16) && pkv_aligned(l.dst_k, 16) && pkv_aligned(l.dst_v, 16),
                 "append_path: buffers must be 16-byte aligned");
     PKV_REQUIRE((l.vnorm != nullptr) == norms, "append_path: all layers keep value norms, or none");
-    PKV_REQUIRE(l.slot >= 0 && l.slot + a->n <= a->dst_len && (!norms || a->vn_stride_h >= l.slot + a->n),
-                "append_path: rows %lld .. of layer %d do not fit %lld", (long long)l.slot, i, (long long)a->dst_len);
+    PKV_REQUIRE(slot >= 0 && slot <= a->dst_len - a->n && (!norms || slot <= a->vn_stride_h - a->n),
+                "append_path: rows %lld .. of layer %d do not fit %lld", (long long)slot, i, (long long)a->dst_len);
   }
   const int vpr = a->row_bytes / 16, n_tasks = a->bs * a->n_kv_heads * a->n * 2;
   for (int at = 0; at < n_layers; at += kPathLayers) {
@@ -339,8 +341,10 @@ extern "C" int pkv_append_path(const pkv_path_args *a, const pkv_path_layer *lay
     memset(&part, 0, sizeof part);
     memcpy(part.layer, layers + at, (size_t)count * sizeof *layers);
     for (int i = 0; i < count; ++i) {
-      part.layer[i].draft_k = (const char *)part.layer[i].draft_k + (at + i) * a->k_stride_l;
-      part.layer[i].draft_v = (const char *)part.layer[i].draft_v + (at + i) * a->v_stride_l;
+      pkv_path_layer &l = part.layer[i];
+      if (!l.draft_k) l.draft_k = (const char *)a->draft_k + (at + i) * a->k_stride_l;
+      if (!l.draft_v) l.draft_v = (const char *)a->draft_v + (at + i) * a->v_stride_l;
+      if (slots) l.slot = slots[at + i];
     }
     const dim3 grid((unsigned)(((int64_t)n_tasks * vpr + kGatherThreads - 1) / kGatherThreads), (unsigned)count);
 #define PKV_PATH(VN)                                                                                                         \

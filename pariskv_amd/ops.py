@@ -624,21 +624,22 @@ class PathAppend:
                 _need(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.shape == vnorms[0].shape and
                       tuple(t.shape[:2]) == (bs, H), "vnorms: contiguous fp32 [bs,Hkv,rows] a layer")
             vn_strides = vnorms[0].stride()[:2]
-        # what a call adds to the layers' table are its first two columns and its last
+        # a call adds the drafted rows' addresses where they are not in one tensor
         fields = [f for f, _ in _lib.PathLayer._fields_]
         self._table = np.zeros((len(dst_k), len(fields)), dtype=np.int64)
         self._table[:, fields.index("dst_k")] = [t.data_ptr() for t in dst_k]
         self._table[:, fields.index("dst_v")] = [t.data_ptr() for t in dst_v]
         if vnorms is not None:
             self._table[:, fields.index("vnorm")] = [t.data_ptr() for t in vnorms]
+        self._table_bytes, self._slots = self._table.tobytes(), struct.Struct(f"@{len(dst_k)}q")
         self._shape, self._es = (bs, H, D), es
         self._tail = (k0.stride(0) * es, k0.stride(1) * es, rows, *vn_strides)
         self.keep = (dst_k, dst_v, vnorms)
         self._like = k0
 
     def _rows_of(self, draft):
-        """(address of the layers' drafted rows, or one a layer, T, strides in bytes: layer, batch, head, token) of a stacked tensor or
-        of one tensor a layer."""
+        """(address of the layers' drafted rows, T, strides in bytes: layer, batch, head, token) of a stacked tensor, or with a list of
+        addresses of one tensor a layer."""
         like, es = self._like, self._es
         if isinstance(draft, torch.Tensor):
             first, shape, strides, at = draft, draft.shape, draft.stride(), draft.data_ptr()
@@ -666,10 +667,20 @@ class PathAppend:
         """draft_k, draft_v: the drafted rows, [layers,bs,T,Hkv,D] or a sequence of [bs,T,Hkv,D]; path int64 [bs,n] on the GPU: the
         accepted tokens of each sequence in order, -1 where it accepted fewer (such a row stays as it is); slots: the cache row of the
         path's first token, one int or one a layer."""
-        table = self._table.copy()
-        table[:, 0], n_draft, k_layer, ks = self._rows_of(draft_k)
-        table[:, 1], n_v, v_layer, vs = self._rows_of(draft_v)
-        table[:, -1] = slots
+        at_k, n_draft, k_layer, ks = self._rows_of(draft_k)
+        at_v, n_v, v_layer, vs = self._rows_of(draft_v)
+        layers, n_layers = self._table_bytes, len(self._table)
+        if type(at_k) is list or type(at_v) is list:
+            table = self._table.copy()
+            if type(at_k) is list:
+                table[:, 0], at_k = at_k, 0
+            if type(at_v) is list:
+                table[:, 1], at_v = at_v, 0
+            layers = table.tobytes()
+        if not hasattr(slots, "__len__"):
+            slots = (slots,) * n_layers
+        if len(slots) != n_layers:
+            raise ValueError("slots: one row, or one a layer")
         if n_v != n_draft:
             raise RuntimeError("drafted K and V rows differ in shape")
         _cuda(path)
@@ -680,14 +691,15 @@ class PathAppend:
         n = path.shape[1]
         if n == 0 or bs == 0:
             return
-        block = _PATH_BLOCK.pack(path.data_ptr(), path.stride(0), bs, H, n, n_draft, D * self._es, k_layer, v_layer, *ks, *vs, *self._tail)
-        rc = _lib.lib().pkv_append_path(block, table.tobytes(), len(table), _stream(self._like))
+        block = _PATH_BLOCK.pack(path.data_ptr(), at_k, at_v, path.stride(0), bs, H, n, n_draft, D * self._es, k_layer, v_layer, *ks,
+                                 *vs, *self._tail)
+        rc = _lib.lib().pkv_append_path(block, layers, self._slots.pack(*slots), n_layers, _stream(self._like))
         if rc != 0:
             _lib.check(rc)
 
 
 # pkv_path_args as one packed block
-_PATH_BLOCK = struct.Struct("@Pq5i13q")
+_PATH_BLOCK = struct.Struct("@3Pq5i13q")
 assert _PATH_BLOCK.size == C.sizeof(_lib.PathArgs)
 
 
@@ -1076,14 +1088,14 @@ def w4_quantize(weight: torch.Tensor, group_size: int = 128):
     and hi = max(0, w): scale = bf16((hi - lo) / 15), zero = rint(-lo / scale), code = rint(w / scale) + zero within 0..15."""
     _cuda(weight)
     _need(weight.dim() == 2 and weight.numel() > 0, "weight: [n,k]")
-    n, k = weight.shape
+    (n, k), dtype = weight.shape, _dt(weight.dtype)
     _need(group_size in (32, 64, 128) and k % group_size == 0, "groups of 32, 64 or 128 columns that divide k")
     if weight.stride(1) != 1 or weight.stride(0) < k:
         weight = weight.contiguous()
     codes = torch.empty(n, k, dtype=torch.uint8, device=weight.device)
     scales = torch.empty(n, k // group_size, dtype=torch.bfloat16, device=weight.device)
     zeros = torch.empty(n, k // group_size, dtype=torch.uint8, device=weight.device)
-    _lib.check(_lib.lib().pkv_w4_quantize(_p(weight), _dt(weight.dtype), weight.stride(0), n, k, group_size, _p(codes), _p(scales),
+    _lib.check(_lib.lib().pkv_w4_quantize(_p(weight), dtype, weight.stride(0), n, k, group_size, _p(codes), _p(scales),
                                           _p(zeros), _stream(weight)))
     return codes, scales, zeros
 

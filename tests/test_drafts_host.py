@@ -1,5 +1,6 @@
 """What the operators of a step over several drafted tokens refuse, and their host-side rules: no GPU, nothing is launched (host
 tensors that say they are on a GPU stand in for device tensors; every call ends in the checks or at a null pointer)."""
+import contextlib
 import ctypes
 
 import pytest
@@ -8,6 +9,20 @@ import torch
 from pariskv_amd import _lib, ops
 
 BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def no_stream(monkeypatch):
+    """Calls reach the library's checks: looking up a stream raises without a GPU."""
+    monkeypatch.setattr(ops, "_stream", lambda t: None)
+
+
+@contextlib.contextmanager
+def refuses():
+    """A refusal by a check, and not the error of a launch, or of a stream's lookup, on a machine without a GPU."""
+    with pytest.raises(RuntimeError) as e:
+        yield
+    assert not any(words in str(e.value) for words in ("HIP error", "launch of", "No HIP")), str(e.value)
 
 
 class On:
@@ -148,7 +163,7 @@ def test_w4_refusals():
     c, s, z = _codes()
     for bad in ((c, s, On(z._t[:, :3])), (On(c._t[:19]), s, z), (On(c._t[:, :250]), s, z), (On(c._t.int()), s, z), (c, On(s._t.float()), z),
                 (On(torch.zeros(20, 64, dtype=torch.uint8)), s, z), (c, s, On(z._t, "cuda:1")), (c._t, s, z)):
-        with pytest.raises(RuntimeError):
+        with refuses():
             ops.W4Weight.from_codes(*bad)
     w = ops.W4Weight(On(torch.zeros(_lib.lib().pkv_w4_bytes(20, 256, 64), dtype=torch.uint8)), 20, 256, 64)
     other = ops.W4Weight(On(torch.zeros(_lib.lib().pkv_w4_bytes(20, 256, 32), dtype=torch.uint8)), 20, 256, 32)
@@ -156,18 +171,18 @@ def test_w4_refusals():
         ops.W4Weight(On(torch.zeros(100, dtype=torch.uint8)), 20, 256, 64)
     x = On(torch.zeros(3, 256, dtype=BF))
     for bad in (On(torch.zeros(3, 255, dtype=BF)), On(torch.zeros(3, 256)), torch.zeros(3, 256, dtype=BF), On(torch.zeros(3, 256, dtype=BF), "cuda:1")):
-        with pytest.raises(RuntimeError):
+        with refuses():
             ops.w4_linear(bad, w)
-        with pytest.raises(RuntimeError):
+        with refuses():
             ops.w4_silu_mul(bad, w, w)
     for bad in (On(torch.zeros(19, dtype=BF)), On(torch.zeros(20)), On(torch.zeros(40, dtype=BF)[::2]), On(torch.zeros(20, dtype=BF), "cuda:1")):
-        with pytest.raises(RuntimeError):
+        with refuses():
             ops.w4_linear(x, w, bad)
     with pytest.raises(RuntimeError, match="one shape"):
         ops.w4_silu_mul(x, w, other)
     for m, g in ((On(torch.zeros(4, 100)), 32), (On(torch.zeros(4, 128)), 16), (torch.zeros(4, 128), 32), (On(torch.zeros(4, 128, dtype=torch.float16)), 32),
                  (On(torch.zeros(128)), 32)):
-        with pytest.raises(RuntimeError):
+        with refuses():
             ops.w4_quantize(m, g)
     L = _lib.lib()
     A = 1 << 20
@@ -194,7 +209,7 @@ def test_path_append_refusals():
     k, v, dk, dv, vn = _path()
     for bad in ((k, v[:2]), ([], []), (k, v[:2] + [On(torch.zeros(2, 2, 21, 128, dtype=BF))]), (k, v[:2] + [On(v[2]._t, "cuda:1")]),
                 (k, v[:2] + [v[2]._t]), (k, v[:2] + [On(v[2]._t.float())]), (k, v, vn[:2]), (k, v, vn[:2] + [On(torch.zeros(2, 2, 20, dtype=BF))])):
-        with pytest.raises(RuntimeError):
+        with refuses():
             ops.PathAppend(*bad)
     plan = ops.PathAppend(k, v)
     path = On(torch.zeros(2, 3, dtype=torch.int64))
@@ -203,12 +218,15 @@ def test_path_append_refusals():
                            (dk, dv[:2] + [On(dv[2]._t, "cuda:1")], path, 0), (dk, dv[:2] + [On(torch.zeros(2, 6, 2, 128, dtype=BF))], path, 0),
                            (dk, [On(torch.zeros(2, 6, 2, 128, dtype=BF))] * 3, path, 0), ([On(x._t.float()) for x in dk], dv, path, 0),
                            (dk, dv, path, 18), (dk, dv, path, -1), (dk, dv, path, [0, 0, 18]), (dk, dv, path._t, 0)):
-        with pytest.raises(RuntimeError):
+        with refuses():
             plan.launch(a, b, p, slots)
+    for slot in (2**62, 2**63 - 1, 2**63 - 3):  # slot + rows passes 64 bits
+        with pytest.raises(RuntimeError, match="do not fit"):
+            plan.launch(dk, dv, path, slot)
     with pytest.raises(ValueError):
         plan.launch(dk, dv, path, [0, 1])
     L = _lib.lib()
-    assert L.pkv_append_path(None, None, 0, None) == _lib.EINVAL
+    assert L.pkv_append_path(None, None, None, 0, None) == _lib.EINVAL
 
 
 def test_new_struct_mirrors_have_the_library_sizes():
