@@ -31,6 +31,13 @@ __device__ __forceinline__ pkv_u32x4 w4_expand(uint32_t w) {
                    (__builtin_amdgcn_alignbit(w, w, 12) & keep) | sixteen};
 }
 
+// Columns past k of a chunk, whose scales are zero: a sum with them has to be finite for that to make them nothing, so x has zeros there.
+__device__ __forceinline__ pkv_u32x4 w4_columns(pkv_u32x4 x, int64_t col, int64_t k) {
+  uint32_t keep = col < k ? 0xffffffffu : 0u;
+  asm volatile("" : "+v"(keep));  // stays behind the caller's branch
+  return pkv_u32x4{x.x & keep, x.y & keep, x.z & keep, x.w & keep};
+}
+
 struct W4Matrix {
   const char *tiles;      // [row tile][chunk of 128 columns] of kTileBytes
   const uint32_t *words;  // [row tile][group][16]
@@ -137,9 +144,10 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(cons
   const int per_wave = (chunks + (1 << lg) - 1) >> lg, row_vecs = chunks * (kTileCols / 8), x_vecs = rows * row_vecs;
   const W4Matrix m[2] = {wa, wb};
 
-  // x is asked for first: vectors tid, tid + 512, .. of its rows one after the other; past the end the last one again, past the columns (whose
-  // scales are zero) the row's first.  Vector v goes to v, its
-  // last four bits changed by its row, and the 16 lanes of a chunk add its columns up.
+  // x is asked for first: vectors tid, tid + 512, .. of its rows one after the other; past the end the last one again, past the columns the row's
+  // first.  Vector v goes to v (as zeros where it is past the columns), its last four bits changed by its row, and the 16 lanes of a chunk add its
+  // columns up.
+  const bool ragged = G < kTileCols && k % kTileCols != 0;
   const int d_row = kWaves * PKV_WAVE * (unsigned)by_row_vecs >> 24, d_col = kWaves * PKV_WAVE - d_row * row_vecs;
   int f_row = (unsigned)tid * (unsigned)by_row_vecs >> 24, f_col = tid - f_row * row_vecs, p_row = f_row, p_col = f_col, put_at = 0;
   auto next = [&](int &row, int &col) {
@@ -162,6 +170,7 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(cons
       const int row = in ? p_row : rows - 1, col = in ? p_col : row_vecs - 1, v = row * row_vecs + col;
       asm volatile("" : "+v"(got[u]));  // arrived on every path, or its register's next use would wait for all of the ring
       if (put_at < x_vecs) {            // the whole workgroup
+        if (ragged) got[u] = w4_columns(got[u], col * 8, k);
         *(pkv_u32x4 *)(lds + (v >> 4) * 256 + 16 * ((v ^ row) & 15)) = got[u];
         float sum = 0.f;
 #pragma unroll
@@ -290,7 +299,8 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_w4_kernel(const uint
     const int at = chunk_of(i) + kg;
     c.load(w_at, s_at, at < last ? at : last - 1);
   };
-  // Vector my_vec of rows my_row + 16 u of the slab; rows past the last repeat it, columns past the last (whose scales are zero) the first.
+  // Vector my_vec of rows my_row + 16 u of the slab; rows past the last repeat it, columns past the last are read as the
+  // first and written as zeros: known for all of a round, so that the others do without (in every round it takes 1 to 3 %).
   const int my_row = tid / kRowVecs, my_vec = tid % kRowVecs;
   const uint16_t *x_at[MT];
 #pragma unroll
@@ -300,7 +310,12 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_w4_kernel(const uint
 #pragma unroll
     for (int u = 0; u < MT; ++u) r[u] = *(const pkv_u32x4 *)(x_at[u] + (col < k ? col : 0));
   };
-  auto put = [&](const pkv_u32x4 (&r)[MT], int buffer) {
+  auto put = [&](pkv_u32x4 (&r)[MT], int i) {
+    const int buffer = i & 1, chunk = chunk_of(i);
+    if (G < kTileCols && (chunk + 2) * kTileCols > k) {  // the whole workgroup
+#pragma unroll
+      for (int u = 0; u < MT; ++u) r[u] = w4_columns(r[u], chunk * kTileCols + my_vec * 8, k);
+    }
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
       const int row = my_row + 16 * u;
@@ -322,7 +337,7 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_w4_kernel(const uint
   fetch(2, ahead[0]);
   auto round = [&](int i, pkv_u32x4 (&after)[MT], W4Chunk<G, kParts> &now) {
     __syncthreads();  // round i is there, and everybody is done with round i - 1
-    put(after, (i + 1) & 1);
+    put(after, i + 1);
     fetch(i + 3, after);
     if (i < rounds && chunk_of(i) + kg < last)  // the whole wave
       w4_chunk<MT, G, kParts, false>(now, [&](int t, int s) {

@@ -624,3 +624,28 @@ def test_path_append(dtype, norms, layers, bs, h, t, n):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(gv[:, :, :, 2:2 + n], dv[:, :, p:p + 1].transpose(2, 3).expand(-1, -1, -1, n, -1))
+
+
+# ------------------------------------------------------------- 4-bit products at the ends of their range
+
+
+@pytest.mark.parametrize("m", [1, 5, 16, 20, 40, 70])
+@pytest.mark.parametrize("k,group", [(160, 32), (192, 64), (1056, 32), (16480, 32)])
+def test_w4_large_rows_in_front_of_padded_columns(m, k, group):
+    """A chunk that the columns do not fill is padded with nothing: x whose first columns add up to nearly the 10^37 that a group may have,
+    from rows that stay in LDS and rows that are streamed."""
+    from pariskv_amd import ops
+
+    n = 77
+    a, b = w4_case(k, n, k, group), w4_case(k + 1, n, k, group)
+    x = _randn(torch.Generator().manual_seed(m), m, k)
+    x[:, 8:group] = 0
+    x[0::2, :8], x[1::2, :8] = 1.15e36, -1.15e36
+    assert 8.9e36 < x[:, :group].double().abs().sum(1).max() < 1e37
+    check(ops.w4_linear(x.to(DEV), handle(a), out_dtype=F32), *exact_linear(x, a, None, F32))
+    small = lambda w: (w[0], (w[1].float() * 2.0 ** -110).to(BF), w[2])   # the product of both projections stays finite
+    a, b = small(a), small(b)
+    z = ops.w4_silu_mul(x.to(DEV), handle(a), handle(b))
+    (ya, ta), (yb, tb) = exact_linear(x, a, None, F32), exact_linear(x, b, None, F32)
+    want = ya * torch.sigmoid(ya) * yb
+    check(z, want, 1.1 * ta * (yb.abs() + tb) + ya.abs() * tb + 8 * U * want.abs() + HALF[BF] * want.abs() + 1e-37)
