@@ -700,7 +700,7 @@ class polar_cache(KV_Cache):
             pick = lambda ts, ls: [ts[l] for l in ls]
             self._path_plans = [(ls, ops.PathAppend(pick(self.unified_keys_gpu, ls), pick(self.unified_values_gpu, ls),
                                                     pick(norms, ls) if norms is not None else None)) for ls in alike.values()]
-        path = path.to(torch.int64).to(self.device)
+        path = path.to(torch.int64).clone(memory_format=torch.contiguous_format).to(self.device)  # any host layout: rows side by side
         done = 0
         while done < n:  # up to the next index refresh, which moves rows about
             run = min(n - done, min(z.tokens_to_refresh() for z in self._zones))

@@ -664,8 +664,8 @@ class PathAppend:
         return at, shape[2], strides[0] * es, (strides[1] * es, strides[3] * es, strides[2] * es)
 
     def launch(self, draft_k, draft_v, path: torch.Tensor, slots) -> None:
-        """draft_k, draft_v: the drafted rows, [layers,bs,T,Hkv,D] or a sequence of [bs,T,Hkv,D]; path int64 [bs,n] on the GPU: the
-        accepted tokens of each sequence in order, -1 where it accepted fewer (such a row stays as it is); slots: the cache row of the
+        """draft_k, draft_v: the drafted rows, [layers,bs,T,Hkv,D] or a sequence of [bs,T,Hkv,D]; path int64 [bs,n] on the GPU, a sequence's
+        numbers side by side: the accepted tokens of each sequence in order, -1 where it accepted fewer (such a row stays as it is); slots: the cache row of the
         path's first token, one int or one a layer."""
         at_k, n_draft, k_layer, ks = self._rows_of(draft_k)
         at_v, n_v, v_layer, vs = self._rows_of(draft_v)
@@ -687,7 +687,7 @@ class PathAppend:
         _one_device(self._like, path)
         bs, H, D = self._shape
         if path.dtype != torch.int64 or path.dim() != 2 or path.shape[0] != bs or (path.shape[1] > 0 and path.stride(1) != 1):
-            raise RuntimeError("path: int64 [bs,n]")
+            raise RuntimeError("path: int64 [bs,n], a sequence's numbers side by side")
         n = path.shape[1]
         if n == 0 or bs == 0:
             return

@@ -289,3 +289,25 @@ def test_model_refusals():
     assert model.kv_cache.context == 51
     with pytest.raises(RuntimeError, match="draft_forward first"):
         model.accept_draft([[0], [0]])
+
+
+@pytest.mark.parametrize("layout", ["transposed", "expanded", "strided", "int32"])
+def test_commit_takes_paths_of_any_layout(layout):
+    """A path as a host tensor, whatever its strides: what the same numbers as lists leave."""
+    bs, hkv, group, t, layers, n = 3, 2, 2, 12, 2, 5
+    a, b = (make_cache(False, bs, hkv, hkv * group, layers, 800, 4, 64, 8, 20) for _ in range(2))
+    prefill((a, b), 4, bs, 500, hkv, layers)
+    g = torch.Generator().manual_seed(9)
+    dk, dv = _randn(g, layers, bs, t, hkv, D).to(DEV), _randn(g, layers, bs, t, hkv, D).to(DEV)
+    path = torch.stack([torch.randperm(t, generator=g)[:n] for _ in range(bs)])
+    if layout == "expanded":
+        path = path[:1].expand(bs, n)
+    given = {"transposed": lambda: path.t().contiguous().t(), "expanded": lambda: path, "int32": lambda: path.t().contiguous().t().to(torch.int32),
+             "strided": lambda: path.repeat_interleave(2, 1)[:, ::2]}[layout]()
+    a.commit_draft(dk, dv, given)
+    b.commit_draft(dk, dv, path.tolist())
+    assert a._zones == b._zones and all(torch.equal(x, y) for x, y in zip(state(a), state(b)))
+    one = given[:, :1].t().contiguous().t()   # one token each: a column
+    a.commit_draft(dk, dv, one)
+    b.commit_draft(dk, dv, path[:, :1].tolist())
+    assert a._zones == b._zones and all(torch.equal(x, y) for x, y in zip(state(a), state(b)))
