@@ -691,8 +691,7 @@ class polar_cache(KV_Cache):
             raise RuntimeError("the accepted tokens do not fit into the cache")
         if self.enable_offload and (self._prefill_stage[0] is not None or self._prefill_stage[1] is not None):
             self.release_prefill_staging()  # as the first decoded token does
-        if not isinstance(draft_k, torch.Tensor):
-            draft_k, draft_v = ([t.to(self.dtype) for t in d] for d in (draft_k, draft_v))
+        draft_k, draft_v = (d.to(self.dtype) if isinstance(d, torch.Tensor) else [t.to(self.dtype) for t in d] for d in (draft_k, draft_v))
         if self._path_plans is None:  # a launch takes layers whose rows are laid out alike
             norms, alike = self._path_norms(), {}
             for l, t in enumerate(self.unified_keys_gpu):

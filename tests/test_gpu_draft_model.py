@@ -311,3 +311,17 @@ def test_commit_takes_paths_of_any_layout(layout):
     a.commit_draft(dk, dv, one)
     b.commit_draft(dk, dv, path[:, :1].tolist())
     assert a._zones == b._zones and all(torch.equal(x, y) for x, y in zip(state(a), state(b)))
+
+
+@pytest.mark.parametrize("kinds", [(torch.Tensor, torch.Tensor), (list, torch.Tensor), (torch.Tensor, list), (list, list)])
+def test_commit_converts_rows_of_another_type(kinds):
+    """Drafted rows of a model in another type enter the cache in its own, stacked or a layer at a time, as a decoded token's rows do."""
+    bs, hkv, group, t, layers = 2, 2, 2, 6, 2
+    a, b = (make_cache(False, bs, hkv, hkv * group, layers, 800, 4, 64, 8, 20) for _ in range(2))
+    prefill((a, b), 4, bs, 500, hkv, layers)
+    g = torch.Generator().manual_seed(9)
+    dk, dv = _randn(g, layers, bs, t, hkv, D, dtype=F32).to(DEV), _randn(g, layers, bs, t, hkv, D, dtype=F32).to(DEV)
+    path = [[0, 3, 5], [1, 2, 4]]
+    a.commit_draft(*(x if kind is torch.Tensor else list(x) for x, kind in zip((dk, dv), kinds)), path)
+    b.commit_draft(dk.to(BF), dv.to(BF), path)
+    assert a._zones == b._zones and all(torch.equal(x, y) for x, y in zip(state(a), state(b)))
