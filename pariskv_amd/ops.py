@@ -537,6 +537,11 @@ def gather_hbm(src_k, src_v, idx, dst_k, dst_v, idx_offset: int = 0, dst_row0: i
     _gather(_lib.lib().pkv_gather_hbm, src_k, src_v, idx, dst_k, dst_v, idx_offset, dst_row0)
 
 
+def _norm_rows(rows: torch.Tensor) -> bool:
+    """Whether the launches that append rows can leave their norms: they tell bf16 rows of 128 elements from fp32 ones by their bytes."""
+    return rows.shape[3] == HEAD_DIM and rows.dtype in (torch.bfloat16, torch.float32)
+
+
 class BoundAppend:
     """The destination of one layer's :func:`append_kv`, validated once: a token costs the checks of its own rows."""
 
@@ -548,7 +553,8 @@ class BoundAppend:
               dst_k.stride() == dst_v.stride() and dst_k.stride(3) == 1 and dst_k.stride(2) == D,
               "dst_k, dst_v: [bs,Hkv,rows,D] with contiguous rows")
         _need(vnorm is None or (vnorm.is_cuda and vnorm.dtype == torch.float32 and tuple(vnorm.shape[:2]) == (bs, H) and
-                                vnorm.is_contiguous()), "vnorm: contiguous fp32 [bs,Hkv,rows]")
+                                vnorm.is_contiguous() and _norm_rows(dst_k)),
+              "vnorm: contiguous fp32 [bs,Hkv,rows], of rows of 128 bf16 or fp32 elements")
         es = dst_k.element_size()
         self._a = _lib.AppendArgs(dst_k.data_ptr(), dst_v.data_ptr(), dst_k.stride(0) * es, dst_k.stride(1) * es, rows, bs, H,
                                   D * es, _p(vnorm), *(vnorm.stride()[:2] if vnorm is not None else (0, 0)))
@@ -589,7 +595,8 @@ def append_kv(key_states, value_states, dst_k, dst_v, slot: int, vnorm: Optional
     vn_b = vn_h = 0
     if vnorm is not None:
         _need(vnorm.is_cuda and vnorm.dtype == torch.float32 and tuple(vnorm.shape[:2]) == (bs, H) and
-              vnorm.stride(2) == 1 and vnorm.shape[2] > slot, "vnorm: fp32 [bs,Hkv,rows] with contiguous rows")
+              vnorm.stride(2) == 1 and vnorm.shape[2] > slot and _norm_rows(dst_k),
+              "vnorm: fp32 [bs,Hkv,rows] with contiguous rows, of rows of 128 bf16 or fp32 elements")
         vn_b, vn_h = vnorm.stride(0), vnorm.stride(1)
     _lib.check(_lib.lib().pkv_append_kv(
         key_states.data_ptr(), key_states.stride(0) * es, key_states.stride(2) * es,
@@ -601,7 +608,8 @@ def append_kv(key_states, value_states, dst_k, dst_v, slot: int, vnorm: Optional
 class PathAppend:
     """The accepted path of a tree of drafted tokens into the K/V rows of all layers, one launch for up to 48 of them: what a
     layer's :class:`BoundAppend` writes a token at a time.  ``dst_k`` / ``dst_v``: a layer's [bs,Hkv,rows,D] each, contiguous
-    rows, all of one shape and layout; ``vnorms``: each layer's fp32 [bs,Hkv,rows'] norms (contiguous), or None."""
+    rows, all of one shape and layout; ``vnorms``: each layer's fp32 [bs,Hkv,rows'] norms (contiguous; rows of 128 bf16 or fp32 elements),
+    or None."""
 
     def __init__(self, dst_k: Sequence[torch.Tensor], dst_v: Sequence[torch.Tensor], vnorms: Optional[Sequence[torch.Tensor]] = None):
         import numpy as np
@@ -620,6 +628,7 @@ class PathAppend:
         vn_strides = (0, 0)
         if vnorms is not None:
             vnorms = list(vnorms)
+            _need(_norm_rows(k0), "vnorms: of rows of 128 bf16 or fp32 elements")
             for t in vnorms:
                 _need(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.shape == vnorms[0].shape and
                       tuple(t.shape[:2]) == (bs, H), "vnorms: contiguous fp32 [bs,Hkv,rows] a layer")

@@ -249,3 +249,15 @@ def test_tokens_to_refresh():
                     if z.appended() is not None:
                         break
                 assert steps == due
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, F32), (128, torch.float16), (256, BF), (256, torch.float16)])
+def test_norms_of_other_rows_are_refused(dim, dtype):
+    """The launches tell bf16 rows of 128 elements from fp32 ones by their bytes: rows of as many bytes that are neither would get norms of
+    something else."""
+    rows = lambda *shape: On(torch.zeros(*shape, dim, dtype=dtype))
+    k, v, vn = rows(2, 2, 20), rows(2, 2, 20), On(torch.zeros(2, 2, 20))
+    for call in (lambda: ops.PathAppend([k], [v], [vn]), lambda: ops.BoundAppend(k, v, vn), lambda: ops.append_kv(rows(2, 1, 2), rows(2, 1, 2), k, v, 3, vn)):
+        with pytest.raises(RuntimeError, match="128 bf16 or fp32"):
+            call()
+    ops.PathAppend([k], [v]), ops.BoundAppend(k, v)   # without norms any rows are moved
