@@ -574,7 +574,8 @@ size_t pkv_w4_bytes(int64_t n, int64_t k, int group);
 int pkv_w4_pack(const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, int64_t n, int64_t k, int group, void *packed,
                 void *stream);
 
-/* Nearest codes of a matrix w [n][k] of `dtype` (row stride in elements; finite values; no counterpart in the reference).  Per
+/* Nearest codes of a matrix w [n][k] of `dtype` (row stride in elements; values of at most 10^38, so that what a code stands for
+ * stays below the largest fp32 number; no counterpart in the reference).  Per
  * group: lo = min(0, w), hi = max(0, w), scale = bf16((hi - lo) / 15), zero = rint(-lo / scale), code = rint(w / scale) + zero
  * clamped to 0..15 (a group of zeros, or one whose scale would be below the smallest normal number: scale, zero and codes 0). */
 int pkv_w4_quantize(const void *w, int dtype, int64_t row_stride, int64_t n, int64_t k, int group, uint8_t *codes, uint16_t *scales,

@@ -1082,7 +1082,7 @@ class W4Weight:
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, group_size: int = 128) -> "W4Weight":
-        """Nearest codes of a finite matrix [n,k] (bf16 or fp32), see :func:`w4_quantize`."""
+        """Nearest codes of a matrix [n,k] (bf16 or fp32), see :func:`w4_quantize`."""
         return cls.from_codes(*w4_quantize(weight, group_size))
 
     def dequantize(self) -> torch.Tensor:
@@ -1093,8 +1093,8 @@ class W4Weight:
 
 
 def w4_quantize(weight: torch.Tensor, group_size: int = 128):
-    """(codes u8 [n,k], scales bf16 [n,k/g], zeros u8 [n,k/g]) of a finite matrix [n,k], bf16 or fp32.  Per group, with lo = min(0, w)
-    and hi = max(0, w): scale = bf16((hi - lo) / 15), zero = rint(-lo / scale), code = rint(w / scale) + zero within 0..15."""
+    """(codes u8 [n,k], scales bf16 [n,k/g], zeros u8 [n,k/g]) of a matrix [n,k], bf16 or fp32, of values of at most 10^38.  Per group,
+    with lo = min(0, w) and hi = max(0, w): scale = bf16((hi - lo) / 15), zero = rint(-lo / scale), code = rint(w / scale) + zero within 0..15."""
     _cuda(weight)
     _need(weight.dim() == 2 and weight.numel() > 0, "weight: [n,k]")
     (n, k), dtype = weight.shape, _dt(weight.dtype)

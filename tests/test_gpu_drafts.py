@@ -649,3 +649,16 @@ def test_w4_large_rows_in_front_of_padded_columns(m, k, group):
     (ya, ta), (yb, tb) = exact_linear(x, a, None, F32), exact_linear(x, b, None, F32)
     want = ya * torch.sigmoid(ya) * yb
     check(z, want, 1.1 * ta * (yb.abs() + tb) + ya.abs() * tb + 8 * U * want.abs() + HALF[BF] * want.abs() + 1e-37)
+
+
+@pytest.mark.parametrize("group", [32, 128])
+def test_w4_quantize_of_the_largest_weights(group):
+    """Weights of up to 10^38: scales, codes and what comes back stay finite, within a step and what the scale's rounding clips."""
+    from pariskv_amd import ops
+
+    w = torch.randn(8, 256, generator=torch.Generator().manual_seed(3)).clamp(-3, 3) / 3 * 1e38
+    w[0, 0], w[0, 1], w[1], w[2] = 1e38, -1e38, w[1].abs(), -w[2].abs()
+    w[1, 0], w[2, 0] = 1e38, -1e38
+    real = ops.W4Weight.quantize(w.to(DEV), group).dequantize().cpu()
+    scale = ops.w4_quantize(w.to(DEV), group)[1].cpu().float().repeat_interleave(group, 1)
+    assert torch.isfinite(real).all() and ((real - w).abs() <= (1.0 + 15 * 2.0 ** -8) * scale).all()
