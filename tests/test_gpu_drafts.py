@@ -662,3 +662,112 @@ def test_w4_quantize_of_the_largest_weights(group):
     real = ops.W4Weight.quantize(w.to(DEV), group).dequantize().cpu()
     scale = ops.w4_quantize(w.to(DEV), group)[1].cpu().float().repeat_interleave(group, 1)
     assert torch.isfinite(real).all() and ((real - w).abs() <= (1.0 + 15 * 2.0 ** -8) * scale).all()
+
+
+# ------------------------------------------------------------- two row tiles a wave
+
+
+def one_head(c, b, j):
+    """The call of a case's (b, j) alone."""
+    bs, _, hq, _ = c["q"].shape
+    h = c["dk"].shape[2]
+    g = hq // h
+    at = lambda x: x[b:b + 1, j:j + 1]
+    return dict(q=c["q"][b:b + 1, :, j * g:(j + 1) * g], dk=c["dk"][b:b + 1, :, j:j + 1], dv=c["dv"][b:b + 1, :, j:j + 1],
+                segs=[(at(s[0]), at(s[1]), *s[2:4], *[at(i) for i in s[4:]]) for s in c["segs"]],
+                mask=c["mask"] if c["mask"] is None or c["mask"].dim() == 2 else c["mask"][b:b + 1], rk=None if c["rk"] is None else at(c["rk"]))
+
+
+def check_heads(c, got, heads, what=""):
+    h = c["dk"].shape[2]
+    g = c["q"].shape[2] // h
+    for b, j in heads:
+        want, tol = exact_tree(one_head(c, b, j))
+        check(got[b:b + 1, :, j * g:(j + 1) * g], want, tol, (what, b, j))
+
+
+# bf16, more than 64 query rows a KV head and at least 1024 keys to a split: a wave takes two tiles of 16 rows.  Row counts that leave the last of
+# 128 rows' workgroups nearly empty, part full and full; one split to a head (and no join), and 8 or 16.
+TWO_TILES = [(9, 15, 8, 9, 1130, 1), (2, 8, 8, 9, 16500, 16), (1, 8, 3, 43, 16500, 16), (1, 8, 7, 33, 17001, 16), (2, 4, 16, 25, 8300, 8), (1, 8, 16, 32, 8192, 8)]
+
+
+def two_tiles_case(shape, form, mask, ragged):
+    from pariskv_amd import _lib
+
+    bs, h, group, t, rows, splits = shape
+    n_rows = bs * h * group * t
+    assert _lib.lib().pkv_tree_attention_ws_bytes(_lib.DTYPE_BF16, bs, h, group, t, rows) == (0 if splits == 1 else n_rows * splits * 130 * 4)
+    return tree_case(rows + t, bs, h, group, t, rows, BF, form, mask, ragged)
+
+
+@pytest.mark.parametrize("shape", TWO_TILES)
+@pytest.mark.parametrize("form", ["dense", "two", "index", "index_two"])
+@pytest.mark.parametrize("mask,ragged", [("tree", False), ("holes", True)])
+def test_tree_two_row_tiles(shape, form, mask, ragged):
+    c = two_tiles_case(shape, form, mask, ragged)
+    g = to_gpu(c)
+    got = run_tree(g)
+    bs, h, group, t, _, _ = shape
+    check_heads(c, got, [(0, 0), (bs - 1, h - 1)], (shape, form))
+    assert torch.isfinite(got).all() and torch.equal(got, run_tree(g))
+    if ragged:  # the last row has nothing in the cache: tokens whose mask is empty see nothing at all
+        assert (got[-1, t // 2, -group:] == 0).all()
+
+
+@pytest.mark.parametrize("shape", [TWO_TILES[0], TWO_TILES[3], TWO_TILES[4]])
+def test_tree_two_row_tiles_of_values_nobody_sees(shape):
+    """Infinities and NaN behind row_keys, outside the segments and in drafted tokens that no or one other token sees."""
+    c = two_tiles_case(shape, "dense", "tree", True)
+    bs, h, group, t, rows, _ = shape
+    c["dk"], c["dv"] = c["dk"].clone(), c["dv"].clone()
+    odd = [2, t // 2, t - 2]
+    c["mask"][:, :, odd] = False
+    heads = [(0, 0), (bs - 1, h - 1)]
+    clean = dict(c, dk=c["dk"].clone(), dv=c["dv"].clone(), segs=[(s[0].clone(), s[1].clone(), *s[2:]) for s in c["segs"]])
+    for i, bad in zip(odd, (float("nan"), float("inf"), float("-inf"))):
+        c["dk"][:, i], c["dv"][:, i] = bad, bad
+    for k, v, row0, _ in c["segs"]:
+        for b in range(bs):
+            for j in range(h):
+                end = row0 + min(rows, max(0, int(c["rk"][b, j])))
+                for x in (k, v):
+                    x[b, j, :row0], x[b, j, end:] = float("nan"), float("inf")
+    check_heads(clean, run_tree(to_gpu(c)), heads)
+    c["dk"][:, odd] = 0.25
+    c["mask"][:, t - 1, odd[1]], c["mask"][:, 1, odd[2]] = True, True
+    got = run_tree(to_gpu(c)).cpu()
+    clean["mask"] = c["mask"].clone()
+    rest = [i for i in range(t) if i not in (1, t - 1)]
+    for b, j in heads:
+        want, tol = exact_tree(one_head(clean, b, j))
+        check(got[b:b + 1, rest, j * group:(j + 1) * group], want[:, rest], tol[:, rest])
+    assert (got[:, t - 1] == float("inf")).all() and (got[:, 1] == float("-inf")).all()
+
+
+def test_tree_scores_beyond_10_to_the_16_pick_a_key_of_the_largest():
+    """fp32 scores of some 10^16, apart by as much: the weight of one key is 1, or of those that lie closer to the largest than a score's rounding (twice
+    130 u S, S the largest sum of |q| |k|) some share it.  The output lies between their values, up to the rounding of a weighted mean of n
+    values, 2 (n + 200) u of the largest."""
+    for mask in ("tree", "holes"):
+        c = tree_case(6, 2, 2, 4, 6, 200, F32, "dense", mask)
+        c["q"] = c["q"] * 1e16
+        k, v, row0, n = c["segs"][0]
+        c["segs"] = [(k.sign(), v, row0, n)]
+        c["dk"] = c["dk"].sign()
+        got = run_tree(to_gpu(c)).double().cpu()
+        alone = 0
+        for b in range(2):
+            for j in range(2):
+                for t in range(6):
+                    see = c["mask"][b, t]
+                    kk = torch.cat([c["segs"][0][0][b, j, row0:row0 + n], c["dk"][b, see, j]]).double()
+                    vv = torch.cat([v[b, j, row0:row0 + n], c["dv"][b, see, j]]).double()
+                    for i in range(4):
+                        q = c["q"][b, t, 4 * j + i].double()
+                        s, size = kk @ q / math.sqrt(D), (kk.abs() @ q.abs()).max() / math.sqrt(D)
+                        top = vv[s >= s.max() - 2 * 130 * U * size]
+                        slack = 2 * (len(vv) + 200) * U * top.abs().amax()
+                        y = got[b, t, 4 * j + i]
+                        assert (y >= top.amin(0) - slack).all() and (y <= top.amax(0) + slack).all(), (mask, b, j, t, i)
+                        alone += len(top) == 1
+        assert alone > 90   # of 96: that is one value for most rows
