@@ -593,7 +593,8 @@ int pkv_w4_linear(const void *x, int64_t x_stride, int64_t rows, const void *pac
                   const void *bias, void *y, int out_dtype, void *ws, size_t ws_bytes, void *stream);
 
 /* y[m][j] = silu(x[m] . gate[j]) * (x[m] . up[j]), bf16 [rows][n] contiguous: both projections of the gated feed-forward block,
- * the activation and the product in one launch (model_hub/qwen.py:365-383 with 4-bit weights).  gate and up: two matrices
+ * the activation and the product in one call (model_hub/qwen.py:365-383 with 4-bit weights): one launch, and a second one where
+ * columns are split over workgroups (ws is not 0 bytes).  gate and up: two matrices
  * [n][k] as stored above, of one group size.  fp32 until the one rounding of y.  ws: pkv_w4_ws_bytes(rows, n, k, group, 1). */
 int pkv_w4_silu_mul(const void *x, int64_t x_stride, int64_t rows, const void *gate, const void *up, int64_t n, int64_t k, int group,
                     void *y, void *ws, size_t ws_bytes, void *stream);

@@ -652,6 +652,10 @@ __global__ __launch_bounds__(kTreeWaves * PKV_WAVE, 2) void pkv_tree_partial_ker
   tree_finish<BF16, false, 1, 1, kTreeWaves>(w, a, part, s_m, s_l, s_o);
 }
 
+// Registers: 256 a lane, for two waves a SIMD.  What does not fit into them (bytes of scratch a lane; without / with key counts of the rows): bf16
+// above, selected rows 8 / 8, in several tensors 20 / 20; below, 17 to 32 query rows with selected ones in several tensors 72 / 24 (fp32 108 / 24); two
+// row tiles a wave 36 / 36, several tensors 96 / 24, selected rows in them 244 / 100: two turns of rows under way and the sums of two tiles are more
+// than there is room for.  The other forms spill nothing.
 typedef short tree_s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) tree_s16x4 tree_lds_s16x4;
 
@@ -884,7 +888,7 @@ TreePlan tree_plan(int dtype, int bs, int n_kv_heads, int rows, int64_t total) {
   };
   // Two row tiles a wave read K and V from LDS once for both, but leave half the workgroups, which costs more where their share of keys is short:
   // us, one / two: 8 x 8 x 1617 keys, 256 rows 38 / 50; 1 x 8 x 4096, 512 rows 30 / 35; 2 x 8 x 16384, 128 rows 44 / 42; 1 x 8 x 32768, 256 rows
-  // (two always) 62.  fp32 has no registers for two.
+  // (two always) 62 to 65.  Measured as they are built: the kernel of two tiles spills.  fp32 has no registers for two.
   split(1);
   if (bf && rows > 64) {
     split(2);

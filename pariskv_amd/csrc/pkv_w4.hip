@@ -269,7 +269,7 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE) void pkv_w4_resident_kernel(cons
 // two a round.  A wave takes every other chunk of two tiles, which share what it reads of x from LDS and the sums of its columns (a tile a wave:
 // 24576 x 4096, 64 rows, 40 us instead of 30).  x is asked for three rounds ahead into registers and written to one of two LDS buffers a round
 // ahead, weights are asked for two rounds ahead.  Where that leaves some of the chip idle the columns are split over workgroups, and a
-// second launch adds the splits up.  4096 x 12288, 64 rows: 23 us, of them 6 rounds of 1.8 us: two waves' 250 vector and 48 matrix instructions each
+// second launch adds the splits up.  4096 x 12288, 64 rows: 21 us, of them 6 rounds of 1.8 us: two waves' 250 vector and 48 matrix instructions each
 // a SIMD, which take nearly the sum of their times.
 // grid (groups of tiles, tiles of 16 MT rows of x, splits)
 template <int MT, int G, bool GATED>
@@ -532,6 +532,8 @@ W4Plan w4_plan(int64_t rows, int64_t n, int64_t k, bool gated) {
   p.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   p.row_tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t x_bytes = (rows < 16 * p.mt ? rows : 16 * p.mt) * chunks * kTileCols * 2;
+  // 16 rows of more than 3840 columns do not fit.  us, 15 rows (kept) / 16 (streamed), groups of 32, 64, 128: 6144 x 4096 12.6 / 12.1, 11.1 / 10.1,
+  // 9.8 / 9.3; gated 12288 x 4096 21.3 / 24.5, 18.9 / 17.9, 16.4 / 15.2.
   // More than 16 rows, streamed / kept in LDS, us: 96164 x 640, 87 rows 57 / 36; 38959 x 1152, 51 rows 28 / 22, 24 rows 18.5 / 15.0; 3000 x 896,
   // 60 rows 11.4 / 8.8.  The gated block has to join two matrices' shares of more rows than there is room for: 12288 x 1536, 24 rows 9.6 / 12.6.
   const int xkb = p.mt > 1 ? 120 : x_bytes <= 16 * 1024 ? 16 : x_bytes <= 64 * 1024 ? 64 : 120;

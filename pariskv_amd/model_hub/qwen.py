@@ -54,7 +54,7 @@ class QwenLayer:
         self.wo = pack(w(h, q))
         gate_up = w(2 * inter, h)
         packed = pack(gate_up[:inter])
-        if isinstance(packed, ops.W4Weight):  # two matrices to one launch
+        if isinstance(packed, ops.W4Weight):  # two matrices to one call
             self.gate_up_proj, self.gate_proj, self.up_proj = None, packed, pack(gate_up[inter:])
         else:
             self.gate_up_proj = gate_up

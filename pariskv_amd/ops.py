@@ -1146,8 +1146,9 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
 
 
 def w4_silu_mul(x: torch.Tensor, gate: W4Weight, up: W4Weight) -> torch.Tensor:
-    """silu(x gate^T) * (x up^T), bf16 [..., n]: both projections of the gated feed-forward block, the activation and the product in one
-    launch (model_hub/qwen.py:365-383 with 4-bit weights); nothing is rounded in between, unlike :func:`silu_mul` of a bf16 product."""
+    """silu(x gate^T) * (x up^T), bf16 [..., n]: both projections of the gated feed-forward block, the activation and the product
+    (model_hub/qwen.py:365-383 with 4-bit weights), in one launch, or two for rows that need a workspace; nothing is rounded in between, unlike
+    :func:`silu_mul` of a bf16 product."""
     packed = gate.packed
     rows, m, step, shape = _w4_rows(x, gate.k, packed.get_device())
     if gate.n != up.n or gate.k != up.k or gate.group_size != up.group_size:
