@@ -325,3 +325,25 @@ def test_commit_converts_rows_of_another_type(kinds):
     a.commit_draft(*(x if kind is torch.Tensor else list(x) for x, kind in zip((dk, dv), kinds)), path)
     b.commit_draft(dk.to(BF), dv.to(BF), path)
     assert a._zones == b._zones and all(torch.equal(x, y) for x, y in zip(state(a), state(b)))
+
+
+@pytest.mark.parametrize("kind,offload", [("polar_cache_adaptivek_varlen", True), ("polar_cache_atten_value_indices_adaptive_k", False)])
+@pytest.mark.parametrize("s", [40, 300])
+def test_draft_attend_to_everything_in_adaptive_caches(kind, offload, s):
+    """Below the length at which they retrieve these caches take drafts as the other does, and a committed path is attended to afterwards."""
+    bs, hkv, group, t, layers = 2, 2, 4, 5, 2
+    cache = make_cache(offload, bs, hkv, hkv * group, layers, 1000, 4, 64, 32, 50, thr=600, kind=kind, collision_ratio=0.3, candidate_ratio=0.05)
+    k, v = prefill((cache,), s, bs, s, hkv, layers)
+    g = torch.Generator().manual_seed(3)
+    path = torch.tensor([[0, 3], [1, 4]])
+    for step in range(2):
+        drafts = []
+        for l in range(layers):
+            q, dk, dv = (_randn(g, bs, t, h, D) for h in (hkv * group, hkv, hkv))
+            drafts.append((dk, dv))
+            out = cache.draft_attend(q.to(DEV), dk.to(DEV), dv.to(DEV), l)
+            rows = [x[l].transpose(1, 2).contiguous() for x in (k, v)]
+            check(out, *exact_tree(dict(q=q, segs=[(*rows, 0, s + 2 * step)], dk=dk, dv=dv, mask=None, rk=None)))
+        cache.commit_draft([d[0].to(DEV) for d in drafts], [d[1].to(DEV) for d in drafts], path)
+        kept = lambda x: torch.stack([x[b, path[b]] for b in range(bs)])
+        k, v = (torch.cat([x, torch.stack([kept(d[i]) for d in drafts])], 2) for i, x in enumerate((k, v)))
