@@ -51,7 +51,7 @@ const char *pkv_last_error(void);
 /* sizeof of the argument structs as this library was compiled, for a binding to
  * compare with its own mirror: 0 pkv_attn_segment, 1 pkv_attn_args,
  * 2 pkv_retrieve_args, 3 pkv_adaptive_args, 5 pkv_prefill_args, 6 pkv_append_args, 7 pkv_path_layer, 8 pkv_path_args,
- * 9 pkv_tree_args (0 for any other number).
+ * 9 pkv_tree_args, 10 pkv_fp8_kv, 11 pkv_fp8_attn_args (0 for any other number).
  * No counterpart in the reference. */
 size_t pkv_struct_bytes(int which);
 
@@ -598,6 +598,102 @@ int pkv_w4_linear(const void *x, int64_t x_stride, int64_t rows, const void *pac
  * [n][k] as stored above, of one group size.  fp32 until the one rounding of y.  ws: pkv_w4_ws_bytes(rows, n, k, group, 1). */
 int pkv_w4_silu_mul(const void *x, int64_t x_stride, int64_t rows, const void *gate, const void *up, int64_t n, int64_t k, int group,
                     void *y, void *ws, size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------- eight bits */
+
+/* Values in eight bits, no counterpart in the reference (bf16 caches, activations and weights): e4m3 codes (OCP: sign, 4 exponent bits, 3
+ * mantissa bits; largest 448) times a scale 2^e that a group of values shares, e the least whole number from -100 on with
+ * |x| <= 448 2^e for every finite x of the group.  A code is the nearest one to x / 2^e (ties to even), of an infinity 448 with its sign, of a NaN
+ * the NaN 0x7f.  Values of at most 10^38.
+ *
+ * A K/V cache in that form: k, v uint8 [bs][n_kv_heads][capacity][128], 16-byte aligned; k_scale, v_scale fp32
+ * [bs][n_kv_heads][capacity / block], one for the rows block*i .. block*(i+1)-1 of a head; block 16, 32, 64 or 128, capacity a multiple of it and at
+ * most PKV_FP8_MAX_ROWS.  A scale of 0 (a block never written): its rows are zeros.  The kernels that read a cache take any finite scales. */
+#define PKV_FP8_MAX_ROWS ((int64_t)1 << 24)
+typedef struct pkv_fp8_kv {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;
+  int bs, n_kv_heads;
+  int64_t capacity;
+  int block;
+} pkv_fp8_kv;
+
+/* Rows into a cache in eight bits (no counterpart in the reference; what pkv_append_kv and a prompt's copy are for bf16 caches).  Token t of
+ * sequence b, heads h of k and v [bs][n_tokens][n_kv_heads][128] of `dtype` (strides in elements, 16-byte multiples; rows
+ * contiguous), becomes row starts[b] + t (`start` + t where starts is NULL) for t < lengths[b] (NULL: all).  A block whose
+ * first rows are there already, before starts[b], keeps them: its scale becomes the larger of the one it has and the one that the new rows
+ * need, and where it grows the older codes are rounded again.  Rows behind the written ones stay as they are, but where they share a
+ * block with written ones they hold nothing that counts.  A sequence whose start is not a row of the cache, or whose length is <= 0, stores
+ * nothing; rows past the capacity are left out. */
+int pkv_fp8_store(const pkv_fp8_kv *cache, const void *k, const void *v, int dtype, int64_t n_tokens, int64_t k_stride_b,
+                  int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_b, int64_t v_stride_t, int64_t v_stride_h, int64_t start,
+                  const int32_t *starts, const int32_t *lengths, void *stream);
+
+/* Rows of a cache in eight bits as values of `dtype` (no counterpart in the reference; pkv_gather_hbm and pkv_gather_uva for such a cache, whose codes may lie
+ * in mapped host memory): out[b][h][i] = row row0 + i, or row row0 + idx[(b*n_kv_heads + h)*idx_stride + i] where idx is
+ * not NULL (a row that is not there: zeros), i < n_rows.  Output strides in elements, 16-byte multiples; rows contiguous. */
+int pkv_fp8_read(const pkv_fp8_kv *cache, int64_t row0, int64_t n_rows, const int64_t *idx, int64_t idx_stride, int dtype, void *out_k,
+                 void *out_v, int64_t ok_stride_b, int64_t ok_stride_h, int64_t ok_stride_row, int64_t ov_stride_b, int64_t ov_stride_h,
+                 int64_t ov_stride_row, void *stream);
+
+/* Attention over a cache in eight bits (no counterpart in the reference; pkv_decode_attention over such a cache, for one query token a
+ * sequence or several).  The keys of a row (b, h) are the concatenation of the segments, rows row0 .. row0 + n_rows - 1 of the cache or
+ * row0 + idx[(b*n_kv_heads + h)*idx_stride + j] (values outside the cache are clamped), of them the first
+ * L = min(row_keys[b*n_kv_heads + h], all) (NULL: all; none where it is <= 0).  Token t sees the keys j < L - (n_tokens - 1 - t): the
+ * last key is the last token's own.
+ *   out[b][t][hq] = sum_j softmax_j(scale q[b][t][hq] . k_j) v_j
+ * A token that sees nothing gets zeros; what a token does not see does not touch it, NaN included.
+ * q [bs][n_tokens][n_kv_heads*group][128], heads side by side, of `dtype` (strides in elements, 16-byte multiples); out the same,
+ * contiguous.  1 <= n_tokens <= 1024, n_tokens * group <= 8192, at most PKV_FP8_MAX_ROWS keys.  fp32 sums and statistics; bf16: weights are
+ * rounded to bf16 for the product with V, and the normaliser is the sum of the rounded ones; fp32: no rounding but that of fp32.
+ * ws: pkv_fp8_attention_ws_bytes(bs, n_kv_heads, group, n_tokens, keys) bytes for the partial results (0: none needed). */
+typedef struct pkv_fp8_segment {
+  int64_t row0, n_rows;
+  const int64_t *idx;  /* or NULL */
+  int64_t idx_stride;
+} pkv_fp8_segment;
+typedef struct pkv_fp8_attn_args {
+  const void *q;
+  int dtype, group, n_tokens, n_segments;
+  int64_t q_stride_b, q_stride_t;
+  pkv_fp8_kv cache;
+  pkv_fp8_segment segments[PKV_ATTN_MAX_SEGMENTS];
+  const int32_t *row_keys;  /* or NULL */
+  float scale;
+  void *out, *ws;
+  size_t ws_bytes;
+} pkv_fp8_attn_args;
+size_t pkv_fp8_attention_ws_bytes(int bs, int n_kv_heads, int group, int n_tokens, int64_t total_keys);
+int pkv_fp8_attention(const pkv_fp8_attn_args *args, void *stream);
+
+/* pkv_add_rmsnorm with the norm's rows in eight bits, a scale each (no counterpart in the reference, model_hub/qwen.py:395-407 in bf16): t = bf16(x + residual), or x where
+ * residual is NULL; y = t / sqrt(mean t^2 + eps) * weight in fp32, the mean and its root in 64 bits.  x, residual and out_sum (or NULL: t) bf16
+ * [rows][width] contiguous, weight bf16 [width]; codes uint8 [rows][width rounded up to 128], 128-byte aligned, zeros past width;
+ * scales fp32 [rows].  width up to 16384. */
+int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const void *weight, double eps, int64_t rows, int64_t width, void *out_sum,
+                        uint8_t *codes, float *scales, void *stream);
+
+/* Rows in eight bits as they are (no counterpart in the reference): x [rows][width] of `dtype`, row stride in elements; the rest as
+ * pkv_add_rmsnorm_fp8 leaves it. */
+int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t *codes, float *scales, void *stream);
+
+/* Matrices in eight bits, a scale for each row (no counterpart in the reference, whose projections are bf16 GEMMs,
+ * model_hub/qwen.py:327-383), stored for the matrix instructions that read them (pkv_fp8_bytes bytes, 16-byte aligned): tiles of 16 rows x 128
+ * columns, padded with zeros, 2048 bytes each, [n/16][k/128]; of a tile's 128 16-byte vectors vector 64 h + 16 j + r (h < 2, j < 4) holds
+ * columns 64 h + 16 j .. +15 of row r.  Behind all tiles the rows' scales, fp32 [n rounded up to 16]. */
+size_t pkv_fp8_bytes(int64_t n, int64_t k);
+
+/* Codes u8 [n][k] (row stride in bytes) and scales fp32 [n], any finite ones, into that form (no counterpart in the reference). */
+int pkv_fp8_pack(const uint8_t *codes, int64_t row_stride, const float *scales, int64_t n, int64_t k, void *packed, void *stream);
+
+/* The matrix back from its stored form, fp32 [n][k] contiguous (no counterpart in the reference). */
+int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w, void *stream);
+
+/* y[m][n] = x_scales[m] scale[n] sum_k x[m][k] code[n][k] + bias[n] (no counterpart in the reference): x codes [rows][k rounded up to 128],
+ * zeros past k, as pkv_fp8_rows leaves them, 16-byte aligned; bias bf16 [n] or NULL; y [rows][n] contiguous of out_dtype.  Sums of codes in
+ * fp32, then the scales; at most 2^22 rows. */
+int pkv_fp8_linear(const uint8_t *x, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,
+                   void *y, int out_dtype, void *stream);
 
 /* ------------------------------------------------------- fused decode step */
 

@@ -67,6 +67,26 @@ class TreeArgs(C.Structure):
                 ("scale", C.c_float), ("out", _vp), ("ws", _vp), ("ws_bytes", _sz)]
 
 
+class Fp8Kv(C.Structure):
+    """Mirror of ``pkv_fp8_kv``."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("bs", _i), ("n_kv_heads", _i), ("capacity", _i64), ("block", _i)]
+
+
+class Fp8Segment(C.Structure):
+    """Mirror of ``pkv_fp8_segment``."""
+
+    _fields_ = [("row0", _i64), ("n_rows", _i64), ("idx", _vp), ("idx_stride", _i64)]
+
+
+class Fp8AttnArgs(C.Structure):
+    """Mirror of ``pkv_fp8_attn_args``."""
+
+    _fields_ = [("q", _vp), ("dtype", _i), ("group", _i), ("n_tokens", _i), ("n_segments", _i), ("q_stride_b", _i64), ("q_stride_t", _i64),
+                ("cache", Fp8Kv), ("segments", Fp8Segment * 4), ("row_keys", _vp), ("scale", C.c_float), ("out", _vp), ("ws", _vp),
+                ("ws_bytes", _sz)]
+
+
 class KvAppend(C.Structure):
     """Mirror of ``pkv_kv_append``."""
 
@@ -189,6 +209,16 @@ PROTOTYPES = {
     "pkv_w4_unpack": (_i, [_vp, _i64, _i64, _i, _vp, _vp]),
     "pkv_w4_ws_bytes": (_sz, [_i64, _i64, _i64, _i, _i]),
     "pkv_w4_linear": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i, _vp, _sz, _vp]),
+    "pkv_fp8_store": (_i, [_vp, _vp, _vp, _i] + [_i64] * 8 + [_vp, _vp, _vp]),
+    "pkv_fp8_read": (_i, [_vp, _i64, _i64, _vp, _i64, _i, _vp, _vp] + [_i64] * 6 + [_vp]),
+    "pkv_fp8_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i64]),
+    "pkv_fp8_attention": (_i, [_vp, _vp]),
+    "pkv_add_rmsnorm_fp8": (_i, [_vp, _vp, _vp, C.c_double, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "pkv_fp8_rows": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "pkv_fp8_bytes": (_sz, [_i64, _i64]),
+    "pkv_fp8_pack": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _vp]),
+    "pkv_fp8_unpack": (_i, [_vp, _i64, _i64, _vp, _vp]),
+    "pkv_fp8_linear": (_i, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i, _vp]),
     "pkv_w4_silu_mul": (_i, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i, _vp, _vp, _sz, _vp]),
     "pkv_decode_attention": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnSegment), _i, _vp, C.c_float, _vp, _vp, _sz, _vp]),
     "pkv_qk_norm_rope": (_i, [_vp, _i64, _i, _i, _i, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp]),
@@ -238,7 +268,7 @@ def lib():
             fn.restype = res
             fn.argtypes = args
         for which, mirror in ((0, AttnSegment), (1, AttnArgs), (2, RetrieveArgs), (3, AdaptiveArgs), (5, PrefillArgs),
-                              (6, AppendArgs), (7, PathLayer), (8, PathArgs), (9, TreeArgs)):
+                              (6, AppendArgs), (7, PathLayer), (8, PathArgs), (9, TreeArgs), (10, Fp8Kv), (11, Fp8AttnArgs)):
             if os.environ.get("PARISKV_HIP_SO") and handle.pkv_struct_bytes(which) == 0:
                 continue
             if handle.pkv_struct_bytes(which) != C.sizeof(mirror):

@@ -1,0 +1,163 @@
+// Rows in eight bits, each with a scale of its own (pkv_fp8.h), as the products with eight-bit matrices take them: the
+// root-mean-square norm with the residual's addition in front (pkv_add_rmsnorm with eight-bit rows for its norm), or rows as they are.
+// (No counterpart in the reference, whose activations stay bf16.)
+//
+// A row is read once and held in registers; the sum of its squares is a sum of 64-bit numbers, where those of bf16 numbers are exact
+// (16 bits of mantissa each): what a code rounds to does not depend on the order.
+#include "pkv_fp8.h"
+
+namespace {
+
+constexpr int kMaxWidth = 16384;
+constexpr int row_threads(int e) { return e == 8 ? 256 : 1024; }
+
+__device__ __forceinline__ double fp8_wave_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < PKV_WAVE; m <<= 1) v += __shfl_xor(v, m, PKV_WAVE);
+  return v;
+}
+
+struct RowsArgs {
+  const char *x;
+  const uint16_t *residual, *weight;
+  int64_t x_stride;  // bytes
+  double eps;
+  int width, padded;
+  uint16_t *out_sum;
+  uint8_t *codes;
+  float *scales;
+};
+
+// E: neighbouring elements a thread takes at a time: 8 (16-byte vectors of bf16), or 1 where width, stride or alignment do not allow it.
+template <bool NORM, bool BF16, int E>
+__global__ __launch_bounds__(row_threads(E)) void pkv_fp8_rows_kernel(RowsArgs a) {
+  constexpr int kRowThreads = row_threads(E), kRowWaves = kRowThreads / PKV_WAVE, kReps = kMaxWidth / (kRowThreads * E);
+  __shared__ double s_sum[kRowWaves];
+  __shared__ uint32_t s_top[kRowWaves];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const char *const x = a.x + row * a.x_stride;
+  float v[kReps][E], w[NORM ? kReps : 1][E];
+  double sum = 0.0;
+  uint32_t top = 0;
+#pragma unroll
+  for (int r = 0; r < kReps; ++r) {
+    const int at = (r * kRowThreads + tid) * E;
+    if (at >= a.width) continue;
+    if constexpr (E == 8) {
+      fp8_load8<BF16>(x + (int64_t)at * (BF16 ? 2 : 4), v[r]);
+    } else {
+      v[r][0] = BF16 ? pkv_bf16_bits_to_f32(((const uint16_t *)x)[at]) : ((const float *)x)[at];
+    }
+    if constexpr (NORM) {
+      if constexpr (E == 8) fp8_load8<true>((const char *)(a.weight + at), w[r]);
+      else w[r][0] = pkv_bf16_bits_to_f32(a.weight[at]);
+      if (a.residual) {
+        const uint16_t *const res = a.residual + row * a.width + at;
+        float add[E];
+        if constexpr (E == 8) fp8_load8<true>((const char *)res, add);
+        else add[0] = pkv_bf16_bits_to_f32(*res);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[r][e] = pkv_bf16_round(v[r][e] + add[e]);
+        if (a.out_sum) {
+          uint16_t *const to = a.out_sum + row * a.width + at;
+          if constexpr (E == 8) {
+            pkv_u32x4 o;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) o[p] = (__float_as_uint(v[r][2 * p]) >> 16) | (__float_as_uint(v[r][2 * p + 1]) & 0xffff0000u);
+            *(pkv_u32x4 *)to = o;
+          } else {
+            *to = (uint16_t)(__float_as_uint(v[r][0]) >> 16);
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += (double)v[r][e] * (double)v[r][e];
+    }
+  }
+  if constexpr (NORM) {
+    sum = fp8_wave_sum(sum);
+    if (pkv_lane() == 0) s_sum[tid / PKV_WAVE] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kRowWaves; ++i) sum += s_sum[i];
+    const float inv = (float)(1.0 / sqrt(sum / (double)a.width + a.eps));
+#pragma unroll
+    for (int r = 0; r < kReps; ++r) {
+      if ((r * kRowThreads + tid) * E >= a.width) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[r][e] = v[r][e] * inv * w[r][e];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kReps; ++r) {
+    if ((r * kRowThreads + tid) * E >= a.width) continue;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t m = fp8_magnitude(v[r][e]);
+      top = m > top ? m : top;
+    }
+  }
+  top = pkv_wave_max(top);
+  if (pkv_lane() == 0) s_top[tid / PKV_WAVE] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRowWaves; ++i) top = s_top[i] > top ? s_top[i] : top;
+  const int e2 = fp8_exponent(top);
+  const float shrink = fp8_pow2(-e2);
+  uint8_t *const codes = a.codes + row * a.padded;
+#pragma unroll
+  for (int r = 0; r < kReps; ++r) {
+    const int at = (r * kRowThreads + tid) * E;
+    if (at >= a.width) continue;
+    if constexpr (E == 8) *(pkv_u32x2 *)(codes + at) = fp8_codes8(v[r], shrink);
+    else codes[at] = (uint8_t)fp8_codes4(v[r][0], 0.f, 0.f, 0.f, shrink);
+  }
+  if (a.width + tid < a.padded) codes[a.width + tid] = 0;  // fewer than 128
+  if (tid == 0) a.scales[row] = fp8_pow2(e2);
+}
+
+template <bool NORM, bool BF16>
+int launch(const RowsArgs &a, int64_t rows, bool whole, hipStream_t s) {
+  if (whole) hipLaunchKernelGGL((pkv_fp8_rows_kernel<NORM, BF16, 8>), dim3((unsigned)rows), dim3(row_threads(8)), 0, s, a);
+  else hipLaunchKernelGGL((pkv_fp8_rows_kernel<NORM, BF16, 1>), dim3((unsigned)rows), dim3(row_threads(1)), 0, s, a);
+  PKV_LAUNCH_CHECK("pkv_fp8_rows_kernel");
+  return PKV_OK;
+}
+
+int shape_ok(const char *who, int64_t rows, int64_t width, const void *codes, const void *scales) {
+  PKV_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && width > 0 && width <= kMaxWidth, "%s: 1..%d columns, at least one row (got %lld x %lld)", who,
+              kMaxWidth, (long long)rows, (long long)width);
+  PKV_REQUIRE(pkv_aligned(codes, 128) && pkv_aligned(scales, 4), "%s: codes must be 128-byte aligned", who);
+  return PKV_OK;
+}
+
+}  // namespace
+
+extern "C" int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const void *weight, double eps, int64_t rows, int64_t width,
+                                   void *out_sum, uint8_t *codes, float *scales, void *stream) {
+  PKV_REQUIRE(x && weight && codes && scales, "pkv_add_rmsnorm_fp8: null pointer");
+  if (const int rc = shape_ok("pkv_add_rmsnorm_fp8", rows, width, codes, scales)) return rc;
+  PKV_REQUIRE(pkv_aligned(x, 2) && pkv_aligned(residual, 2) && pkv_aligned(weight, 2) && pkv_aligned(out_sum, 2), "pkv_add_rmsnorm_fp8: bf16 operands");
+  RowsArgs a;
+  a.x = (const char *)x, a.residual = (const uint16_t *)residual, a.weight = (const uint16_t *)weight, a.x_stride = width * 2, a.eps = eps;
+  a.width = (int)width, a.padded = (int)pkv_align_up((size_t)width, 128), a.out_sum = (uint16_t *)out_sum, a.codes = codes, a.scales = scales;
+  const bool whole = width % 8 == 0 && pkv_aligned(x, 16) && pkv_aligned(residual, 16) && pkv_aligned(weight, 16) && pkv_aligned(out_sum, 16);
+  return launch<true, true>(a, rows, whole, (hipStream_t)stream);
+}
+
+extern "C" int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t *codes, float *scales, void *stream) {
+  PKV_REQUIRE(x && codes && scales, "pkv_fp8_rows: null pointer");
+  PKV_REQUIRE(dtype == PKV_DTYPE_F32 || dtype == PKV_DTYPE_BF16, "unknown dtype %d", dtype);
+  if (const int rc = shape_ok("pkv_fp8_rows", rows, width, codes, scales)) return rc;
+  const int64_t es = dtype == PKV_DTYPE_BF16 ? 2 : 4;
+  PKV_REQUIRE(pkv_aligned(x, es) && x_stride >= 0, "pkv_fp8_rows: rows of whole elements");
+  RowsArgs a;
+  memset(&a, 0, sizeof a);
+  a.x = (const char *)x, a.x_stride = x_stride * es, a.width = (int)width, a.padded = (int)pkv_align_up((size_t)width, 128);
+  a.codes = codes, a.scales = scales;
+  const bool whole = width % 8 == 0 && x_stride * es % 16 == 0 && pkv_aligned(x, 16);
+  if (dtype == PKV_DTYPE_BF16) return launch<false, true>(a, rows, whole, (hipStream_t)stream);
+  return launch<false, false>(a, rows, whole, (hipStream_t)stream);
+}

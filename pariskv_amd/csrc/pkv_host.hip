@@ -35,6 +35,8 @@ extern "C" size_t pkv_struct_bytes(int which) {
     case 7: return sizeof(pkv_path_layer);
     case 8: return sizeof(pkv_path_args);
     case 9: return sizeof(pkv_tree_args);
+    case 10: return sizeof(pkv_fp8_kv);
+    case 11: return sizeof(pkv_fp8_attn_args);
     default: return 0;
   }
 }

@@ -1165,6 +1165,356 @@ def w4_silu_mul(x: torch.Tensor, gate: W4Weight, up: W4Weight) -> torch.Tensor:
     return y
 
 
+FP8 = torch.float8_e4m3fn
+
+
+def _fp8_bytes(t: torch.Tensor, what: str) -> torch.Tensor:
+    _need(t.dtype in (FP8, torch.uint8), f"{what}: e4m3 codes, float8_e4m3fn or their bytes")
+    return t.view(torch.uint8)
+
+
+class Fp8KVCache:
+    """K and V rows of one layer in eight bits: e4m3 codes ``k``, ``v`` [bs,Hkv,capacity,128] and power-of-two scales ``k_scale``,
+    ``v_scale`` fp32 [bs,Hkv,capacity/block], one for each block of 16, 32, 64 or 128 rows of a head.  A row is its code times its block's scale.
+    ``capacity`` is rounded up to whole blocks.  ``host``: the codes live in pinned host memory (half the bytes over PCIe of a bf16
+    store; :meth:`store` and :meth:`read` only), the scales on the GPU."""
+
+    def __init__(self, bs: int, n_kv_heads: int, capacity: int, device, block: int = 64, host: bool = False):
+        _need(bs > 0 and n_kv_heads > 0 and capacity > 0 and block in (16, 32, 64, 128), "blocks of 16, 32, 64 or 128 rows, at least one row")
+        capacity = -(-capacity // block) * block
+        shape, scales = (bs, n_kv_heads, capacity, HEAD_DIM), (bs, n_kv_heads, capacity // block)
+        if host:
+            k, v = (alloc_pinned(shape, torch.uint8, zero=True) for _ in range(2))
+        else:
+            k, v = (torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
+        self._set(k, torch.zeros(scales, dtype=torch.float32, device=device), v, torch.zeros(scales, dtype=torch.float32, device=device), block)
+
+    @classmethod
+    def from_codes(cls, k: torch.Tensor, k_scale: torch.Tensor, v: torch.Tensor, v_scale: torch.Tensor, block: int) -> "Fp8KVCache":
+        """A cache out of tensors in its own layout, which it keeps; any finite scales."""
+        self = cls.__new__(cls)
+        self._set(_fp8_bytes(k, "k"), k_scale, _fp8_bytes(v, "v"), v_scale, block)
+        return self
+
+    def _set(self, k, k_scale, v, v_scale, block):
+        _need(k.dim() == 4 and k.shape == v.shape and k.shape[3] == HEAD_DIM and k.is_contiguous() and v.is_contiguous() and
+              k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0, "k, v: contiguous [bs,Hkv,capacity,128], 16-byte aligned")
+        bs, H, capacity, _ = k.shape
+        _need(block in (16, 32, 64, 128) and capacity % block == 0 and 0 < capacity <= 1 << 24, "blocks of 16, 32, 64 or 128 rows that divide the capacity (at most 2^24)")
+        for t in (k_scale, v_scale):
+            _need(t.dtype == torch.float32 and tuple(t.shape) == (bs, H, capacity // block) and t.is_contiguous(),
+                  "scales: contiguous fp32 [bs,Hkv,capacity/block]")
+        _cuda(k_scale, v_scale)
+        self.host = not k.is_cuda
+        if self.host:
+            _need(k.is_pinned() and v.is_pinned(), "codes on the GPU, or in pinned host memory")
+            _one_device(k_scale, v_scale)
+        else:
+            _one_device(k, v, k_scale, v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k.view(FP8), v.view(FP8), k_scale, v_scale
+        self.bs, self.n_kv_heads, self.capacity, self.block, self.device = bs, H, capacity, block, k_scale.device
+        self._kv = _lib.Fp8Kv(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bs, H, capacity, block)
+        self._ref = C.byref(self._kv)
+        self._fields = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bs, H, capacity, block)
+        self._at = k_scale.get_device()
+
+    def store(self, k: torch.Tensor, v: torch.Tensor, start=0, lengths: Optional[torch.Tensor] = None) -> None:
+        """Rows k, v [bs,S,Hkv,128] (bf16 or fp32, of at most 10^38; any strides) quantised into rows start .. of every sequence.  start: an integer, or
+        int32 [bs] on the GPU (a sequence whose start is no row of the cache stores nothing, rows past the capacity are left out);
+        lengths: int32 [bs] on the GPU, how many of its S rows a sequence has (None: all).  Rows that a block holds
+        already, before the start, stay: its scale only grows, and their codes are rounded again when it does."""
+        shape, dt = k.shape, k.dtype
+        if len(shape) != 4 or v.shape != shape or v.dtype != dt or shape[0] != self.bs or shape[2] != self.n_kv_heads or shape[3] != HEAD_DIM:
+            raise RuntimeError("k, v: [bs,S,Hkv,128] of one type")
+        code, S, at = _dt(dt), shape[1], self._at
+        if k.get_device() != at or v.get_device() != at:
+            _cuda(k, v)
+            _one_device(self.k_scale, k, v)
+        if S == 0:
+            return
+        odd = 7 if code == _lib.DTYPE_BF16 else 3  # strides that are not multiples of 16 bytes
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1 or (ks[0] | ks[1] | ks[2]) & odd or k.data_ptr() & 15:
+            k = k.clone(memory_format=torch.contiguous_format)
+            ks = k.stride()
+        if vs[3] != 1 or (vs[0] | vs[1] | vs[2]) & odd or v.data_ptr() & 15:
+            v = v.clone(memory_format=torch.contiguous_format)
+            vs = v.stride()
+        starts = 0
+        if isinstance(start, torch.Tensor):
+            self._counts(start, "start")
+            start, starts = 0, start.data_ptr()
+        if lengths is not None:
+            self._counts(lengths, "lengths")
+        rc = _lib.lib().pkv_fp8_store(self._ref, k.data_ptr(), v.data_ptr(), code, S, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], start, starts,
+                                      None if lengths is None else lengths.data_ptr(), _stream(self.k_scale))
+        if rc != 0:
+            _lib.check(rc)
+
+    def _counts(self, t, what):
+        if t.dtype != torch.int32 or t.get_device() != self._at or t.shape != (self.bs,) or not t.is_contiguous():
+            raise RuntimeError(f"{what}: contiguous int32 [bs] on the cache's GPU")
+
+    def read(self, row0: int = 0, n: Optional[int] = None, idx: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16, out=None):
+        """Rows as values: (K, V) [bs,Hkv,n,128] in ``dtype`` (bf16 or fp32).  Rows row0 .. row0+n-1 (n None: to the end), or rows
+        row0 + idx[b,h,:n] with idx int64 [bs,Hkv,>=n] on the GPU (n None: all of it; a row that is not there: zeros).  ``out``: two tensors of that
+        shape and type with contiguous rows to write to, for instance the rows behind a dense prefix."""
+        bs, H, code = self.bs, self.n_kv_heads, _dt(dtype)
+        idx_at, idx_stride = None, 0
+        if idx is not None:
+            if idx.dtype != torch.int64 or idx.get_device() != self._at or idx.dim() != 3 or idx.shape[:2] != (bs, H) or not idx.is_contiguous():
+                raise RuntimeError("idx: contiguous int64 [bs,Hkv,n] on the cache's GPU")
+            n = idx.shape[2] if n is None else n
+            if not 0 <= n <= idx.shape[2] or not 0 <= row0 < self.capacity:
+                raise RuntimeError("idx: as many as rows are asked for, from a row of the cache on")
+            idx_at, idx_stride = idx.data_ptr(), idx.shape[2]
+        else:
+            n = self.capacity - row0 if n is None else n
+            if row0 < 0 or n < 0 or row0 + n > self.capacity:
+                raise RuntimeError("rows out of range")
+        if out is None:
+            ok, ov = (torch.empty((bs, H, n, HEAD_DIM), dtype=dtype, device=self.device) for _ in range(2))
+        else:
+            ok, ov = out
+            for t in (ok, ov):
+                if (t.shape != (bs, H, n, HEAD_DIM) or t.dtype != dtype or t.get_device() != self._at or t.stride(3) != 1 or t.data_ptr() & 15 or
+                        any(s & (7 if code == _lib.DTYPE_BF16 else 3) for s in t.stride()[:3])):
+                    raise RuntimeError("out: [bs,Hkv,n,128] of dtype on the cache's GPU, rows contiguous and 16-byte aligned")
+        if n > 0:
+            so, sv = ok.stride(), ov.stride()
+            rc = _lib.lib().pkv_fp8_read(self._ref, row0, n, idx_at, idx_stride, code, ok.data_ptr(), ov.data_ptr(), so[0], so[1], so[2], sv[0], sv[1],
+                                         sv[2], _stream(self.k_scale))
+            if rc != 0:
+                _lib.check(rc)
+        return ok, ov
+
+
+class Fp8Attention:
+    """:class:`DecodeAttention` over a cache in eight bits (:class:`Fp8KVCache`), for one query token a sequence or several.  Partial results are
+    allocated with every call, so that calls on several streams, or of several captured graphs, do not share any."""
+
+    def __init__(self, bs: int, n_kv_heads: int, group: int, max_tokens: int, max_keys: int, device):
+        _need(bs > 0 and n_kv_heads > 0 and group > 0 and 1 <= max_tokens <= 1024 and max_tokens * group <= 8192,
+              "1..1024 query tokens, at most 8192 query rows a KV head")
+        self.bs, self.H, self.G, self.max_tokens, self.max_keys = bs, n_kv_heads, group, max_tokens, max_keys
+        self.device = torch.device(device)
+
+    def run(self, queries: torch.Tensor, cache: Fp8KVCache, segments, row_keys: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """queries [bs,T,Hq,128] (bf16 or fp32); segments: at most four (row0, n_rows) or (row0, n_rows, idx) of the cache, its keys in that order: rows
+        row0 .. row0+n_rows-1, or rows row0 + idx[b,h,:n_rows] with idx int64 [bs,Hkv,>=n_rows] on the GPU (values outside the cache are clamped);
+        row_keys int32 [bs,Hkv]: how many of these keys a row has (None: all; 0 or less: none).  The last key is the last token's
+        own: token t sees all but the last T-1-t.  Returns [bs,T,Hq,128]; a token that sees nothing gets zeros, and what a token does not see does not touch it."""
+        bs, H, G = self.bs, self.H, self.G
+        shape, dt, at = queries.shape, queries.dtype, queries.get_device()
+        T = shape[1] if len(shape) == 4 else 0
+        if shape != (bs, T, H * G, HEAD_DIM) or not 1 <= T <= self.max_tokens:
+            raise RuntimeError("queries: [bs,T,Hq,128], 1 <= T <= max_tokens")
+        code = _dt(dt)
+        if cache.bs != bs or cache.n_kv_heads != H or cache.host:
+            raise RuntimeError("cache: of this batch and these KV heads, its codes on the GPU")
+        if at < 0 or cache._at != at:
+            _cuda(queries)
+            _one_device(queries, cache.k)
+        odd = 7 if code == _lib.DTYPE_BF16 else 3
+        q, qs = queries, queries.stride()
+        if qs[3] != 1 or qs[2] != HEAD_DIM or (qs[0] | qs[1]) & odd or q.data_ptr() & 15:
+            q = q.clone(memory_format=torch.contiguous_format)
+            qs = q.stride()
+        n_seg = len(segments)
+        if n_seg > 4:
+            raise RuntimeError("0..4 key segments")
+        segs, total = [], 0
+        for seg in segments:
+            row0, n_rows = seg[:2]
+            idx = seg[2] if len(seg) > 2 else None
+            total += n_rows
+            if row0 < 0 or n_rows < 0:
+                raise RuntimeError("segment rows out of range")
+            if idx is None:
+                if row0 + n_rows > cache.capacity:
+                    raise RuntimeError("segment rows out of range")
+                segs += (row0, n_rows, 0, 0)
+            else:
+                if (idx.dtype != torch.int64 or idx.get_device() != at or not idx.is_contiguous() or idx.dim() != 3 or idx.shape[:2] != (bs, H) or
+                        n_rows > idx.shape[2] or row0 >= cache.capacity):
+                    raise RuntimeError("segment indices: contiguous int64 [bs,Hkv,>=n_rows] on the GPU of the queries")
+                segs += (row0, n_rows, idx.data_ptr(), idx.shape[2])
+        segs += (0,) * (16 - 4 * n_seg)
+        if total > self.max_keys:
+            raise RuntimeError("more keys than max_keys")
+        keys_at = 0
+        if row_keys is not None:
+            if row_keys.dtype != torch.int32 or row_keys.get_device() != at or not row_keys.is_contiguous() or row_keys.numel() != bs * H:
+                raise RuntimeError("row_keys: contiguous int32 [bs,Hkv] on the GPU of the queries")
+            keys_at = row_keys.data_ptr()
+        if out is None:
+            out = queries.new_empty(shape)
+        elif out.shape != shape or out.dtype != dt or out.get_device() != at or not out.is_contiguous() or out.data_ptr() & 15:
+            raise RuntimeError("out: contiguous, like queries")
+        lib = _lib.lib()
+        need = lib.pkv_fp8_attention_ws_bytes(bs, H, G, T, total)
+        ws = queries.new_empty(need, dtype=torch.uint8) if need else None
+        block = _FP8_ATTN_BLOCK.pack(q.data_ptr(), code, G, T, n_seg, qs[0], qs[1], *cache._fields, *segs, keys_at, _SCALE if scale is None else scale,
+                                     out.data_ptr(), ws.data_ptr() if need else 0, need)
+        rc = lib.pkv_fp8_attention(block, _stream(queries))
+        if rc != 0:
+            _lib.check(rc)
+        return out
+
+
+# pkv_fp8_attn_args as one packed block
+_FP8_ATTN_BLOCK = struct.Struct("@P4i2q4P2iqi" + "qqPq" * 4 + "PfPPN")
+assert _FP8_ATTN_BLOCK.size == C.sizeof(_lib.Fp8AttnArgs)
+
+
+class Fp8Rows:
+    """Rows [..., k] in eight bits: e4m3 ``codes`` and a power-of-two scale each, ``scales`` fp32 [...].  A row is its codes times its scale."""
+
+    __slots__ = ("padded", "scales", "shape", "k")
+
+    def __init__(self, padded: torch.Tensor, scales: torch.Tensor, shape):
+        # padded: uint8 [rows, k rounded up to 128], zeros past k
+        self.padded, self.scales, self.shape, self.k = padded, scales, shape, shape[-1]
+
+    @property
+    def codes(self) -> torch.Tensor:
+        rows = self.padded if self.padded.shape[1] == self.k else self.padded[:, :self.k]
+        return rows.view(FP8).view(self.shape)
+
+    @property
+    def device(self):
+        return self.padded.device
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Fp8Rows":
+        """codes [..., k] (float8_e4m3fn or their bytes), scales fp32 [...], any finite ones."""
+        _need(codes.dim() >= 1 and codes.shape[-1] > 0 and scales.dtype == torch.float32 and scales.shape == codes.shape[:-1], "codes [..., k], scales fp32 [...]")
+        _cuda(codes, scales)
+        _one_device(codes, scales)
+        k, rows = codes.shape[-1], _fp8_bytes(codes, "codes").reshape(-1, codes.shape[-1])
+        if k % 128 or not rows.is_contiguous() or rows.data_ptr() % 16:
+            padded = torch.zeros(rows.shape[0], -(-k // 128) * 128, dtype=torch.uint8, device=codes.device)
+            padded[:, :k] = rows
+            rows = padded
+        return cls(rows, scales.contiguous(), tuple(codes.shape))
+
+
+def fp8_rows(x: torch.Tensor) -> Fp8Rows:
+    """Rows x [..., k] (bf16 or fp32, of at most 10^38; k up to 16384) in eight bits, in one launch."""
+    shape, code, k = x.shape, _dt(x.dtype), x.shape[-1] if x.dim() else 0
+    if not x.is_cuda or k == 0:
+        raise RuntimeError("x: [..., k] on the GPU")
+    rows = x if len(shape) == 2 else x.reshape(-1, k)
+    step, unit = rows.stride()
+    if unit != 1 and k > 1 or step < 0:
+        rows = rows.contiguous()
+        step = k
+    n = rows.shape[0]
+    codes = x.new_empty((n, -(-k // 128) * 128), dtype=torch.uint8)
+    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    if n > 0:
+        rc = _lib.lib().pkv_fp8_rows(rows.data_ptr(), code, step, n, k, codes.data_ptr(), scales.data_ptr(), _stream(x))
+        if rc != 0:
+            _lib.check(rc)
+    return Fp8Rows(codes, scales, shape)
+
+
+def add_rmsnorm_fp8(x: torch.Tensor, residual, weight: torch.Tensor, eps: float, want_sum: bool = True):
+    """:func:`add_rmsnorm` with the norm as :class:`Fp8Rows`, in one launch: (x + residual, eight-bit rows of RMSNorm(x + residual) * weight);
+    ``residual`` may be None.  bf16, contiguous, any width up to 16384.  The norm is not rounded before its codes are."""
+    shape = x.shape
+    width = shape[-1]
+    if not x.is_cuda or x.dtype != torch.bfloat16 or not x.is_contiguous() or width == 0:
+        raise RuntimeError("x: contiguous bf16 [..., width] on the GPU")
+    at = x.get_device()
+    if weight.dtype != torch.bfloat16 or weight.numel() != width or not weight.is_contiguous() or weight.get_device() != at:
+        raise RuntimeError("weight: contiguous bf16 [width] on the GPU of x")
+    if residual is not None and (residual.shape != shape or residual.dtype != torch.bfloat16 or not residual.is_contiguous() or residual.get_device() != at):
+        raise RuntimeError("residual must match x")
+    rows = x.numel() // width
+    out_sum = torch.empty_like(x) if (want_sum and residual is not None) else None
+    codes = x.new_empty((rows, -(-width // 128) * 128), dtype=torch.uint8)
+    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    if rows > 0:
+        rc = _lib.lib().pkv_add_rmsnorm_fp8(x.data_ptr(), _p(residual), weight.data_ptr(), eps, rows, width, _p(out_sum), codes.data_ptr(),
+                                            scales.data_ptr(), _stream(x))
+        if rc != 0:
+            _lib.check(rc)
+    return (out_sum if out_sum is not None else x), Fp8Rows(codes, scales, shape)
+
+
+class Fp8Weight:
+    """A matrix [n,k] in eight bits, a scale for each of its rows, laid out once for the kernels that read it: weight = scale * code."""
+
+    __slots__ = ("packed", "n", "k")
+
+    def __init__(self, packed: torch.Tensor, n: int, k: int):
+        _need(packed.dtype == torch.uint8 and packed.is_cuda and packed.is_contiguous() and packed.data_ptr() % 16 == 0 and
+              packed.numel() == _lib.lib().pkv_fp8_bytes(n, k) > 0, "packed: what from_codes or quantize laid out")
+        self.packed, self.n, self.k = packed, int(n), int(k)
+
+    @property
+    def shape(self):
+        return (self.n, self.k)
+
+    @property
+    def device(self):
+        return self.packed.device
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Fp8Weight":
+        """codes [n,k] (float8_e4m3fn or their bytes), scales fp32 [n], any finite ones: a quantized checkpoint's."""
+        _need(codes.dim() == 2 and scales.dtype == torch.float32 and scales.shape == codes.shape[:1], "codes [n,k], scales fp32 [n]")
+        _cuda(codes, scales)
+        _one_device(codes, scales)
+        n, k = codes.shape
+        nbytes = _lib.lib().pkv_fp8_bytes(n, k)
+        _need(nbytes > 0, f"n and k of at least 1, k up to 2^20 (got n={n} k={k})")
+        packed = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+        codes, scales = _fp8_bytes(codes, "codes"), scales.contiguous()
+        if codes.stride(1) != 1 and k > 1 or codes.stride(0) < k:
+            codes = codes.contiguous()
+        _lib.check(_lib.lib().pkv_fp8_pack(_p(codes), codes.stride(0), _p(scales), n, k, _p(packed), _stream(codes)))
+        return cls(packed, n, k)
+
+    @classmethod
+    def quantize(cls, weight: torch.Tensor) -> "Fp8Weight":
+        """Nearest codes of a matrix [n,k], bf16 or fp32 (k up to 16384)."""
+        _need(weight.dim() == 2 and weight.numel() > 0, "weight: [n,k]")
+        rows = fp8_rows(weight)
+        return cls.from_codes(rows.codes, rows.scales)
+
+    def dequantize(self) -> torch.Tensor:
+        """fp32 [n,k]."""
+        w = torch.empty(self.n, self.k, dtype=torch.float32, device=self.device)
+        _lib.check(_lib.lib().pkv_fp8_unpack(_p(self.packed), self.n, self.k, _p(w), _stream(w)))
+        return w
+
+
+def fp8_linear(x, weight: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x [..., k] times the transpose of an eight-bit matrix, plus ``bias`` (bf16 [n]): [..., n] in ``out_dtype`` (bf16, the default, or
+    fp32).  x: :class:`Fp8Rows`, or bf16 or fp32 rows, which :func:`fp8_rows` quantises first.  Sums in fp32, one rounding."""
+    if not isinstance(x, Fp8Rows):
+        x = fp8_rows(x)
+    padded, packed, n = x.padded, weight.packed, weight.n
+    if x.k != weight.k:
+        raise RuntimeError(f"x: [..., {weight.k}]")
+    if padded.get_device() != packed.get_device():
+        _one_device(packed, padded)
+    if bias is not None:
+        _one_device(packed, bias)
+        _need(bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == n, "bias: contiguous bf16 [n]")
+    code = _lib.DTYPE_BF16 if out_dtype is None else _dt(out_dtype)
+    m = padded.shape[0]
+    y = padded.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
+    if m > 0:
+        rc = _lib.lib().pkv_fp8_linear(padded.data_ptr(), x.scales.data_ptr(), m, packed.data_ptr(), n, weight.k, _p(bias), y.data_ptr(), code, _stream(packed))
+        if rc != 0:
+            _lib.check(rc)
+    return y
+
+
 def alloc_pinned(shape, dtype: torch.dtype, zero: bool = False) -> torch.Tensor:
     """Pinned, device-mapped host tensor of exactly the requested size, optionally zero-filled (``pkv_host_alloc_mapped`` =
     hipHostMalloc).  torch's own pinned allocator rounds every block up to a power of two, which nearly doubles the
