@@ -668,14 +668,15 @@ int pkv_fp8_attention(const pkv_fp8_attn_args *args, void *stream);
 
 /* pkv_add_rmsnorm with the norm's rows in eight bits, a scale each (no counterpart in the reference, model_hub/qwen.py:395-407 in bf16): t = bf16(x + residual), or x where
  * residual is NULL; y = t / sqrt(mean t^2 + eps) * weight in fp32, the mean and its root in 64 bits.  x, residual and out_sum (or NULL: t) bf16
- * [rows][width] contiguous, weight bf16 [width]; codes uint8 [rows][width rounded up to 128], 128-byte aligned, zeros past width;
- * scales fp32 [rows].  width up to 16384. */
+ * [rows][width] contiguous, weight bf16 [width]; codes uint8 [rows], rows code_stride bytes apart (16-byte multiples, 16-byte aligned, at least width
+ * rounded up to 128, where zeros follow the row); scales fp32 [rows].  width up to 16384. */
 int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const void *weight, double eps, int64_t rows, int64_t width, void *out_sum,
-                        uint8_t *codes, float *scales, void *stream);
+                        uint8_t *codes, int64_t code_stride, float *scales, void *stream);
 
 /* Rows in eight bits as they are (no counterpart in the reference): x [rows][width] of `dtype`, row stride in elements; the rest as
  * pkv_add_rmsnorm_fp8 leaves it. */
-int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t *codes, float *scales, void *stream);
+int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t *codes, int64_t code_stride, float *scales,
+                 void *stream);
 
 /* Matrices in eight bits, a scale for each row (no counterpart in the reference, whose projections are bf16 GEMMs,
  * model_hub/qwen.py:327-383), stored for the matrix instructions that read them (pkv_fp8_bytes bytes, 16-byte aligned): tiles of 16 rows x 128
@@ -689,10 +690,10 @@ int pkv_fp8_pack(const uint8_t *codes, int64_t row_stride, const float *scales, 
 /* The matrix back from its stored form, fp32 [n][k] contiguous (no counterpart in the reference). */
 int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w, void *stream);
 
-/* y[m][n] = x_scales[m] scale[n] sum_k x[m][k] code[n][k] + bias[n] (no counterpart in the reference): x codes [rows][k rounded up to 128],
- * zeros past k, as pkv_fp8_rows leaves them, 16-byte aligned; bias bf16 [n] or NULL; y [rows][n] contiguous of out_dtype.  Sums of codes in
+/* y[m][n] = x_scales[m] scale[n] sum_k x[m][k] code[n][k] + bias[n] (no counterpart in the reference): x codes [rows], x_stride bytes apart
+ * (16-byte multiples, 16-byte aligned), zeros past k up to the next multiple of 128, as pkv_fp8_rows leaves them; bias bf16 [n] or NULL; y [rows][n] contiguous of out_dtype.  Sums of codes in
  * fp32, then the scales; at most 2^22 rows. */
-int pkv_fp8_linear(const uint8_t *x, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,
+int pkv_fp8_linear(const uint8_t *x, int64_t x_stride, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,
                    void *y, int out_dtype, void *stream);
 
 /* ------------------------------------------------------- fused decode step */

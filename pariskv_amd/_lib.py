@@ -213,12 +213,12 @@ PROTOTYPES = {
     "pkv_fp8_read": (_i, [_vp, _i64, _i64, _vp, _i64, _i, _vp, _vp] + [_i64] * 6 + [_vp]),
     "pkv_fp8_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i64]),
     "pkv_fp8_attention": (_i, [_vp, _vp]),
-    "pkv_add_rmsnorm_fp8": (_i, [_vp, _vp, _vp, C.c_double, _i64, _i64, _vp, _vp, _vp, _vp]),
-    "pkv_fp8_rows": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "pkv_add_rmsnorm_fp8": (_i, [_vp, _vp, _vp, C.c_double, _i64, _i64, _vp, _vp, _i64, _vp, _vp]),
+    "pkv_fp8_rows": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "pkv_fp8_bytes": (_sz, [_i64, _i64]),
     "pkv_fp8_pack": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _vp]),
     "pkv_fp8_unpack": (_i, [_vp, _i64, _i64, _vp, _vp]),
-    "pkv_fp8_linear": (_i, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i, _vp]),
+    "pkv_fp8_linear": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i, _vp]),
     "pkv_w4_silu_mul": (_i, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i, _vp, _vp, _sz, _vp]),
     "pkv_decode_attention": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnSegment), _i, _vp, C.c_float, _vp, _vp, _sz, _vp]),
     "pkv_qk_norm_rope": (_i, [_vp, _i64, _i, _i, _i, _vp, _vp, C.c_float, _vp, _vp, _vp, _vp, _vp]),

@@ -1,9 +1,11 @@
 // Products of eight-bit rows with eight-bit matrices, a scale for each row of both: y[m][n] = sx[m] sw[n] sum_k xc[m][k] wc[n][k] + bias[n],
 // codes e4m3.  (No counterpart in the reference, whose projections are bf16 GEMMs, model_hub/qwen.py:327-383.)
 //
-// Codes become bf16 numbers in registers, exactly (two to an instruction), and go to v_mfma_f32_16x16x32_bf16, whose products of them
+// Codes become bf16 numbers in registers, exactly (two to an instruction), and go to bf16 matrix instructions, whose products of them
 // are exact and whose sums are fp32.  The instructions that take e4m3 codes themselves have twice the rate, but add eight neighbouring products
-// up with nothing below 2^-13 of the largest of them: 2^16 + 4 is 2^16, and rows of normal numbers come out 1.5e-5 off.
+// up with nothing below 2^-13 of the largest of them (2^16 + 4 is 2^16); the sums of eight are added in fp32.  Rows of normal numbers come out 1.5e-5 of
+// their norm off, a hundredth of what rounding to bf16 does.  So they are used where the results are bf16 and the matrix rate counts, many
+// rows, and nowhere else: 4096 rows x (6144 x 4096) 108 us, 193 with bf16 instructions.
 // Which columns a lane has is free as long as both operands agree: lane (r, j) takes columns 16 j .. 16 j + 15 and 64 + 16 j .. of a chunk of 128,
 // so that the rows of x are read 64 bytes side by side.  The matrix is laid out once in tiles of 16 rows x 128 columns in the order of the lanes.
 #include "pkv_fp8.h"
@@ -12,33 +14,56 @@ namespace {
 
 typedef __bf16 fp8_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float fp8_f32x4 __attribute__((ext_vector_type(4)));
+typedef float fp8_f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTileRows = 16, kTileCols = 128, kTileBytes = kTileRows * kTileCols;
 
+typedef int fp8_i32x8 __attribute__((ext_vector_type(8)));
 struct Codes {  // 32 codes of a lane
   pkv_u32x4 half[2];
-};
-struct Operand {  // ... as bf16 numbers
-  pkv_u32x4 part[4];
-  __device__ __forceinline__ Operand(const Codes &c) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-#pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        const uint32_t w = c.half[p >> 1][2 * (p & 1) + d];
-        part[p][2 * d] = fp8_bf16x2<false>(w), part[p][2 * d + 1] = fp8_bf16x2<true>(w);
-      }
+  // a quarter of them as bf16 numbers
+  __device__ __forceinline__ pkv_u32x4 part(int p) const {
+    const uint32_t a = half[p >> 1][2 * (p & 1)], b = half[p >> 1][2 * (p & 1) + 1];
+    return pkv_u32x4{fp8_bf16x2<false>(a), fp8_bf16x2<true>(a), fp8_bf16x2<false>(b), fp8_bf16x2<true>(b)};
   }
 };
-__device__ __forceinline__ fp8_f32x4 fp8_mfma(const Operand &a, const Operand &b, fp8_f32x4 c) {
+__device__ __forceinline__ fp8_f32x4 fp8_mfma_part(pkv_u32x4 a, pkv_u32x4 b, fp8_f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fp8_bf16x8, a), __builtin_bit_cast(fp8_bf16x8, b), c, 0, 0, 0);
+}
+// 32 x 32 x 64 codes, and 32 x 32 x 16 of them as bf16 numbers
+__device__ __forceinline__ fp8_f32x16 fp8_mfma32_codes(const Codes &a, const Codes &b, fp8_f32x16 c) {
+  const fp8_i32x8 x = {(int)a.half[0].x, (int)a.half[0].y, (int)a.half[0].z, (int)a.half[0].w,
+                       (int)a.half[1].x, (int)a.half[1].y, (int)a.half[1].z, (int)a.half[1].w};
+  const fp8_i32x8 y = {(int)b.half[0].x, (int)b.half[0].y, (int)b.half[0].z, (int)b.half[0].w,
+                       (int)b.half[1].x, (int)b.half[1].y, (int)b.half[1].z, (int)b.half[1].w};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ fp8_f32x16 fp8_mfma32_part(pkv_u32x4 a, pkv_u32x4 b, fp8_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(fp8_bf16x8, a), __builtin_bit_cast(fp8_bf16x8, b), c, 0, 0, 0);
+}
+// Until at most LEFT of this wave's loads are on their way, and none of its reads of LDS; the instructions before stay before.
+template <int LEFT>
+__device__ __forceinline__ void fp8_wait() {
+  static_assert(LEFT >= 0 && LEFT < 64, "six bits");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+}
+
+// Order of the instructions since the last barrier: between the matrix instructions the reads of LDS first, then the loads, evenly.
+template <int MFMA, int READS, int LOADS>
+__device__ __forceinline__ void fp8_mix() {
+  constexpr int kHalf = MFMA > 1 ? MFMA / 2 : 1, kReads = (READS + kHalf - 1) / kHalf, kLoads = (LOADS + kHalf - 1) / kHalf;
 #pragma unroll
-  for (int p = 0; p < 4; ++p)
-    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fp8_bf16x8, a.part[p]), __builtin_bit_cast(fp8_bf16x8, b.part[p]), c, 0, 0, 0);
-  return c;
+  for (int i = 0; i < MFMA; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if (i * kReads < READS) __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    else if (kLoads > 0) __builtin_amdgcn_sched_group_barrier(0x010, kLoads, 0);
+  }
 }
 
 struct LinearArgs {
-  const uint8_t *x;     // [m][chunks * 128]
+  const uint8_t *x;     // [m], rows x_stride bytes apart, chunks * 128 of them read
+  int64_t x_stride;
   const float *sx;
   const uint8_t *tiles; // [row tile][chunk][half][lane] of 16 bytes
   const float *sw;      // [row tiles * 16]
@@ -48,11 +73,53 @@ struct LinearArgs {
   int chunks, f32;
 };
 
-__device__ __forceinline__ void put(const LinearArgs &a, int64_t row, int64_t col, float sum, float sx) {
-  float v = sum * sx * a.sw[col];
-  if (a.bias) v += pkv_bf16_bits_to_f32(a.bias[col]);
-  if (a.f32) ((float *)a.y)[row * a.n + col] = v;
-  else ((uint16_t *)a.y)[row * a.n + col] = pkv_f32_to_bf16_bits(v);
+// Columns col .. col + 3 of a row of y, col a multiple of four.  WHOLE: rows of y are whole vectors.  The flags are chosen once for all of a
+// workgroup's results: asked for at each of the 64 a lane may have, they take longer than eight chunks of columns (20 us of 256 x 256).
+template <bool F32, bool BIAS, bool WHOLE>
+__device__ __forceinline__ void put4(const LinearArgs &a, int64_t row, int64_t col, fp8_f32x4 sum, float sx) {
+  if (row >= a.m || col >= a.n) return;
+  const fp8_f32x4 sw = *(const fp8_f32x4 *)(a.sw + col);  // there are scales up to the next multiple of 16
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = sum[i] * sx * sw[i];
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += pkv_bf16_bits_to_f32(a.bias[WHOLE || col + i < a.n ? col + i : col]);
+  }
+  const int64_t at = row * a.n + col;
+  if constexpr (WHOLE) {
+    if constexpr (F32) *(fp8_f32x4 *)((float *)a.y + at) = fp8_f32x4{v[0], v[1], v[2], v[3]};
+    else
+      *(pkv_u32x2 *)((uint16_t *)a.y + at) = pkv_u32x2{(uint32_t)pkv_f32_to_bf16_bits(v[0]) | ((uint32_t)pkv_f32_to_bf16_bits(v[1]) << 16),
+                                                       (uint32_t)pkv_f32_to_bf16_bits(v[2]) | ((uint32_t)pkv_f32_to_bf16_bits(v[3]) << 16)};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (col + i >= a.n) break;
+      if constexpr (F32) ((float *)a.y)[at + i] = v[i];
+      else ((uint16_t *)a.y)[at + i] = pkv_f32_to_bf16_bits(v[i]);
+    }
+  }
+}
+// f(put4 of this call)
+template <typename F>
+__device__ __forceinline__ void with_put4(const LinearArgs &a, F f) {
+  const bool whole = (a.n & 3) == 0;
+#define PKV_PUT(F32, BIAS, WHOLE) f([&](int64_t row, int64_t col, fp8_f32x4 sum, float sx) { put4<F32, BIAS, WHOLE>(a, row, col, sum, sx); })
+  if (whole && !a.bias) {
+    if (a.f32) PKV_PUT(true, false, true);
+    else PKV_PUT(false, false, true);
+  } else if (whole) {
+    if (a.f32) PKV_PUT(true, true, true);
+    else PKV_PUT(false, true, true);
+  } else if (a.bias) {
+    if (a.f32) PKV_PUT(true, true, false);
+    else PKV_PUT(false, true, false);
+  } else {
+    if (a.f32) PKV_PUT(true, false, false);
+    else PKV_PUT(false, false, false);
+  }
+#undef PKV_PUT
 }
 
 // Few rows: the matrix is read once and the bytes bound it.  A workgroup takes 16 RT rows of the matrix and 16 MT of x, its waves every
@@ -60,7 +127,7 @@ __device__ __forceinline__ void put(const LinearArgs &a, int64_t row, int64_t co
 constexpr int kStreamWaves = 8;
 template <int MT, int RT>
 __global__ __launch_bounds__(kStreamWaves * PKV_WAVE) void pkv_fp8_stream_kernel(LinearArgs a) {
-  constexpr int kAhead = MT * RT > 4 ? 1 : MT + RT > 3 ? 2 : 4;  // chunks under way
+  constexpr int kAhead = MT + RT > 4 ? 1 : MT + RT > 3 ? 2 : 4;  // chunks under way
   __shared__ fp8_f32x4 s_part[kStreamWaves][RT][MT][PKV_WAVE];
   const int tid = threadIdx.x, lane = pkv_lane(), wave = tid / PKV_WAVE, n = lane & 15, j = lane >> 4;
   const int64_t tiles = (a.n + kTileRows - 1) / kTileRows, m0 = (int64_t)blockIdx.y * 16 * MT, t0 = (int64_t)blockIdx.x * RT;
@@ -68,7 +135,7 @@ __global__ __launch_bounds__(kStreamWaves * PKV_WAVE) void pkv_fp8_stream_kernel
 #pragma unroll
   for (int r = 0; r < RT; ++r) w_at[r] = a.tiles + (t0 + r < tiles ? t0 + r : tiles - 1) * a.chunks * kTileBytes + lane * 16;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) x_at[t] = a.x + (m0 + 16 * t + n < a.m ? m0 + 16 * t + n : a.m - 1) * a.chunks * kTileCols + 16 * j;
+  for (int t = 0; t < MT; ++t) x_at[t] = a.x + (m0 + 16 * t + n < a.m ? m0 + 16 * t + n : a.m - 1) * a.x_stride + 16 * j;
   fp8_f32x4 acc[RT][MT];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
@@ -94,9 +161,12 @@ __global__ __launch_bounds__(kStreamWaves * PKV_WAVE) void pkv_fp8_stream_kernel
       if (c0 + u * kStreamWaves >= a.chunks) break;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        const Operand wo(w[u][r]);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[r][t] = fp8_mfma(wo, Operand(x[u][t]), acc[r][t]);
+        for (int p = 0; p < 4; ++p) {
+          const pkv_u32x4 wo = w[u][r].part(p);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) acc[r][t] = fp8_mfma_part(wo, x[u][t].part(p), acc[r][t]);
+        }
       }
     }
   }
@@ -105,78 +175,233 @@ __global__ __launch_bounds__(kStreamWaves * PKV_WAVE) void pkv_fp8_stream_kernel
 #pragma unroll
     for (int t = 0; t < MT; ++t) s_part[wave][r][t][lane] = acc[r][t];
   __syncthreads();
-  // number e of the workgroup's: column e mod 16 RT of the matrix' rows, row e / (16 RT) of x
-  for (int e = tid; e < 256 * RT * MT; e += kStreamWaves * PKV_WAVE) {
-    const int col = e % (16 * RT), row = e / (16 * RT), r = col / 16, t = row / 16;
-    const int at = (((col & 15) >> 2) * 16 + (row & 15)) * 4 + (col & 3);  // lane (row, col / 4), its element col mod 4
-    float sum = ((const float *)s_part[0][r][t])[at];
+  with_put4(a, [&](auto put) {
+    for (int e = tid; e < RT * MT * PKV_WAVE; e += kStreamWaves * PKV_WAVE) {  // a lane's four columns of a tile at a time
+      const int r = e / (MT * PKV_WAVE), t = e / PKV_WAVE % MT, l = e % PKV_WAVE;
+      fp8_f32x4 sum = s_part[0][r][t][l];
 #pragma unroll
-    for (int w = 1; w < kStreamWaves; ++w) sum += ((const float *)s_part[w][r][t])[at];
-    if (m0 + row < a.m && t0 * 16 + col < a.n) put(a, m0 + row, t0 * 16 + col, sum, a.sx[m0 + row]);
+      for (int w = 1; w < kStreamWaves; ++w) sum += s_part[w][r][t][l];
+      const int64_t row = m0 + 16 * t + (l & 15);
+      put(row, (t0 + r) * 16 + 4 * (l >> 4), sum, a.sx[row < a.m ? row : a.m - 1]);
+    }
+  });
+}
+
+// Many rows: 64 TM rows of x by 64 TN of the matrix a workgroup, a quarter of them a wave, a chunk of columns at a time, straight from memory to
+// LDS.  Of x a load takes 8 rows x 128 columns, whole lines: 64 bytes of each of 16 rows, all in the same half of their lines, come at half the rate
+// (16 KB 0.7 us a compute unit; 0.4).  Vector v of row r lies at v ^ (r mod 8) of the row, so that rows of an operand are on different banks.
+typedef const __attribute__((address_space(1))) void *fp8_global;
+typedef __attribute__((address_space(3))) void *fp8_lds;
+// A wave's results, rows m0 .., columns n0 .. of y, 32 rows at a time through a part of LDS of its own and out as whole rows of it: 16 bytes of each of
+// 32 rows, as they lie in the registers, would take 20 us of 256 x 256 where rows of y are a multiple of 4096 bytes.
+template <int TM, int TN, bool F32>
+__device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x16 (&acc)[TN][TM], uint8_t *lds, int64_t m0, int64_t n0) {
+  constexpr int kEs = F32 ? 4 : 2, kRow = 32 * TN * kEs, kStep = kRow + 16, kVecs = kRow / 16, kRows = PKV_WAVE / kVecs;
+  static_assert(4 * 32 * kStep <= 2 * 4 * (TM + TN) * kTileBytes, "room for it");
+  const int lane = pkv_lane(), wave = threadIdx.x / PKV_WAVE, row = lane & 31;
+  uint8_t *const mine = lds + wave * (32 * kStep);
+  const int64_t left = a.n - n0;
+  const bool whole = a.n % (16 / kEs) == 0;
+  const int vec = lane % kVecs, col = vec * (16 / kEs);
+#pragma unroll
+  for (int t = 0; t < TM; ++t) {
+    const float sx = a.sx[m0 + 32 * t + row < a.m ? m0 + 32 * t + row : a.m - 1];
+#pragma unroll
+    for (int r = 0; r < TN; ++r)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * r + 8 * q + 4 * (lane >> 5);
+        const bool in = c < left;
+        const fp8_f32x4 sw = *(const fp8_f32x4 *)(a.sw + (in ? n0 + c : 0));  // there are scales up to the next multiple of 16
+        fp8_f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = acc[r][t][4 * q + i] * sx * sw[i];
+        if (a.bias) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] += pkv_bf16_bits_to_f32(a.bias[c + i < left ? n0 + c + i : 0]);
+        }
+        if constexpr (F32) *(fp8_f32x4 *)(mine + row * kStep + c * 4) = v;
+        else
+          *(pkv_u32x2 *)(mine + row * kStep + c * 2) = pkv_u32x2{(uint32_t)pkv_f32_to_bf16_bits(v[0]) | ((uint32_t)pkv_f32_to_bf16_bits(v[1]) << 16),
+                                                                 (uint32_t)pkv_f32_to_bf16_bits(v[2]) | ((uint32_t)pkv_f32_to_bf16_bits(v[3]) << 16)};
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    for (int r0 = lane / kVecs; r0 < 32; r0 += kRows) {
+      const int64_t at = m0 + 32 * t + r0;
+      const pkv_u32x4 v = *(const pkv_u32x4 *)(mine + r0 * kStep + vec * 16);
+      if (at >= a.m || col >= left) continue;
+      char *const to = (char *)a.y + (at * a.n + n0 + col) * kEs;
+      if (whole) *(pkv_u32x4 *)to = v;
+      else
+#pragma unroll
+        for (int i = 0; i < 16 / kEs; ++i) {
+          if (col + i >= left) break;
+          if constexpr (F32) ((uint32_t *)to)[i] = v[i];
+          else ((uint16_t *)to)[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// Many rows: 128 x 128 of y a workgroup, 64 x 64 a wave.  A chunk of both operands goes straight from memory to LDS in the order of the lanes.
-constexpr int kBlock = 128, kBlockTiles = kBlock / 16;
-typedef const __attribute__((address_space(1))) void *fp8_global;
-typedef __attribute__((address_space(3))) void *fp8_lds;
-__global__ __launch_bounds__(256) void pkv_fp8_block_kernel(LinearArgs a) {
-  __shared__ alignas(16) uint8_t lds[2][kBlockTiles * kTileBytes];  // x, matrix
-  const int tid = threadIdx.x, lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(tid / PKV_WAVE), n = lane & 15, j = lane >> 4;
-  const int64_t tiles = (a.n + kTileRows - 1) / kTileRows, m0 = (int64_t)blockIdx.y * kBlock, t0 = (int64_t)blockIdx.x * kBlockTiles;
+template <int TM, int TN, int DEPTH, bool E4M3>
+__global__ __launch_bounds__(256, TM * TN > 4 ? 1 : 2) void pkv_fp8_block_kernel(LinearArgs a, int m_blocks, int n_blocks) {
+  constexpr int kEach = TM + TN, kX = 4 * TM * kTileBytes, kBuffer = kX + 4 * TN * kTileBytes;  // pieces of 1 KB that a wave brings in, of x and of the matrix
+  extern __shared__ uint8_t lds[];
+  const int lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PKV_WAVE);
+  // Workgroups go to the eight dies in turn: each die takes a run of blocks that share rows.
+  const int blocks = m_blocks * n_blocks, per = (blocks + 7) / 8, id = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || id >= blocks) return;  // the whole workgroup
+  constexpr int kGroup = 4;  // blocks of x rows side by side
+  const int group = id / (kGroup * n_blocks), in = id - group * kGroup * n_blocks, here = m_blocks - group * kGroup < kGroup ? m_blocks - group * kGroup : kGroup;
+  const int mb = group * kGroup + in % here, nb = in / here;
+  const int64_t tiles = (a.n + kTileRows - 1) / kTileRows, m0 = (int64_t)mb * (64 * TM), t0 = (int64_t)nb * (4 * TN);
   const int wm = wave & 1, wn = wave >> 1;
-  // what this wave brings in: two tiles of each
-  const uint8_t *x_at[2], *w_at[2];
+  // what this wave brings in: 8 rows each of x, half tiles of the matrix
+  const uint8_t *x_from[2 * TM], *w_from[TN];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int64_t row = m0 + (2 * wave + u) * 16 + n, tile = t0 + 2 * wave + u;
-    x_at[u] = a.x + (row < a.m ? row : a.m - 1) * a.chunks * kTileCols + 16 * j;
-    w_at[u] = a.tiles + (tile < tiles ? tile : tiles - 1) * a.chunks * kTileBytes + lane * 16;
+  for (int u = 0; u < 2 * TM; ++u) {
+    const int64_t row = m0 + (wave * 2 * TM + u) * 8 + (lane >> 3);
+    x_from[u] = a.x + (row < a.m ? row : a.m - 1) * a.x_stride + 16 * ((lane & 7) ^ (lane >> 3));
   }
-  fp8_f32x4 acc[4][4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int u = 0; u < TN; ++u) {
+    const int64_t tile = t0 + wave * TN + u;
+    w_from[u] = a.tiles + (tile < tiles ? tile : tiles - 1) * a.chunks * kTileBytes + lane * 16;
+  }
+  auto fetch = [&](int c, int buffer) {
+    uint8_t *const to = lds + buffer * kBuffer;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[r][t] = fp8_f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int c = 0; c < a.chunks; ++c) {
+    for (int u = 0; u < 2 * TM; ++u)
+      __builtin_amdgcn_global_load_lds((fp8_global)(x_from[u] + c * kTileCols), (fp8_lds)(to + (wave * 2 * TM + u) * 1024), 16, 0, 0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < TN; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        __builtin_amdgcn_global_load_lds((fp8_global)(x_at[u] + c * kTileCols + h * 64), (fp8_lds)(lds[0] + (2 * wave + u) * kTileBytes + h * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((fp8_global)(w_at[u] + (int64_t)c * kTileBytes + h * 1024), (fp8_lds)(lds[1] + (2 * wave + u) * kTileBytes + h * 1024), 16, 0, 0);
+      for (int h = 0; h < 2; ++h)
+        __builtin_amdgcn_global_load_lds((fp8_global)(w_from[u] + (int64_t)c * kTileBytes + h * 1024), (fp8_lds)(to + kX + (wave * TN + u) * kTileBytes + h * 1024),
+                                         16, 0, 0);
+  };
+  // operands: row lane mod 32 of a pair of tiles, vectors 4 half + 2 (lane / 32) + e of its chunk
+  const int row = lane & 31, x_row = wm * TM * 4096 + (row >> 3) * 1024 + (row & 7) * 128, w_row = kX + wn * TN * 4096 + (row >> 4) * 2048 + (row & 15) * 16;
+  int x_vec[2][2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) x_vec[half][e] = x_row + 16 * ((4 * half + 2 * (lane >> 5) + e) ^ (row & 7));
+  const int w_vec = w_row + (lane >> 5) * 512;
+  auto read = [&](int buffer, int half, Codes (&x)[TM], Codes (&w)[TN]) {
+    const uint8_t *const p = lds + buffer * kBuffer;
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) x[t].half[e] = *(const pkv_u32x4 *)(p + x_vec[half][e] + t * 4096);
+#pragma unroll
+    for (int r = 0; r < TN; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) w[r].half[e] = *(const pkv_u32x4 *)(p + w_vec + half * 1024 + e * 256 + r * 4096);
+  };
+  fp8_f32x16 acc[TN][TM];
+#pragma unroll
+  for (int r = 0; r < TN; ++r)
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[r][t][i] = 0.f;
+  auto product = [&](const Codes (&x)[TM], const Codes (&w)[TN]) {
+    if constexpr (E4M3) {
+#pragma unroll
+      for (int r = 0; r < TN; ++r)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[r][t] = fp8_mfma32_codes(w[r], x[t], acc[r][t]);
+    } else {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        pkv_u32x4 xo[TM];
+#pragma unroll
+        for (int t = 0; t < TM; ++t) xo[t] = x[t].part(p);
+#pragma unroll
+        for (int r = 0; r < TN; ++r) {
+          const pkv_u32x4 wo = w[r].part(p);
+#pragma unroll
+          for (int t = 0; t < TM; ++t) acc[r][t] = fp8_mfma32_part(wo, xo[t], acc[r][t]);
+        }
       }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    Codes x[4], w[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        x[t].half[h] = *(const pkv_u32x4 *)(lds[0] + (4 * wm + t) * kTileBytes + h * 1024 + lane * 16);
-        w[t].half[h] = *(const pkv_u32x4 *)(lds[1] + (4 * wn + t) * kTileBytes + h * 1024 + lane * 16);
-      }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const Operand wo(w[r]);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[r][t] = fp8_mfma(wo, Operand(x[t]), acc[r][t]);
     }
-    __syncthreads();
+  };
+  // Operands of the next half chunk are read while this one's are multiplied; a chunk is asked for when the one DEPTH before it has been
+  // read, half a chunk before its end.
+  const int last = a.chunks - 1;
+  Codes x[2][TM], w[2][TN];
+#pragma unroll
+  for (int c = 0; c < DEPTH; ++c) fetch(c < last ? c : last, c);  // past the last: read again, not used
+  fp8_wait<(DEPTH - 1) * 2 * kEach>();
+  __builtin_amdgcn_s_barrier();
+  read(0, 0, x[0], w[0]);
+  int now = 0;
+  for (int c = 0; c <= last; ++c) {
+    const int next = now + 1 == DEPTH ? 0 : now + 1;
+    read(now, 1, x[1], w[1]);
+    product(x[0], w[0]);
+    fp8_mix<E4M3 ? TM * TN : 4 * TM * TN, 2 * (TM + TN), 0>();
+    fp8_wait<(DEPTH - 2) * 2 * kEach>();  // chunk c + 1 is there, for this wave, and its reads of chunk c are done
+    __builtin_amdgcn_s_barrier();         // ... for all
+    fetch(c + DEPTH < last ? c + DEPTH : last, now);
+    read(next, 0, x[0], w[0]);
+    product(x[1], w[1]);
+    fp8_mix<E4M3 ? TM * TN : 4 * TM * TN, 2 * (TM + TN), 2 * kEach>();
+    __builtin_amdgcn_sched_barrier(0);
+    now = next;
   }
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t row = m0 + (4 * wm + t) * 16 + n;
-    if (row >= a.m) continue;
-    const float sx = a.sx[row];
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t col = (t0 + 4 * wn + r) * 16 + 4 * j + i;
-        if (col < a.n) put(a, row, col, acc[r][t][i], sx);
-      }
+  fp8_wait<0>();  // nothing may be on its way to LDS that another workgroup gets
+  __builtin_amdgcn_s_barrier();
+  if (a.f32) block_store<TM, TN, true>(a, acc, lds, m0 + TM * wm * 32, t0 * 16 + TN * wn * 32);
+  else block_store<TM, TN, false>(a, acc, lds, m0 + TM * wm * 32, t0 * 16 + TN * wn * 32);
+}
+
+template <int MT, int RT>
+void launch_stream(const LinearArgs &a, hipStream_t s) {
+  const unsigned tiles = (unsigned)((a.n + kTileRows - 1) / kTileRows);
+  hipLaunchKernelGGL((pkv_fp8_stream_kernel<MT, RT>), dim3((tiles + RT - 1) / RT, (unsigned)((a.m + 16 * MT - 1) / (16 * MT))), dim3(kStreamWaves * PKV_WAVE), 0, s, a);
+}
+
+template <int TM, int TN, int DEPTH, bool E4M3>
+int launch_block_as(const LinearArgs &a, hipStream_t s) {
+  const int mb = (int)((a.m + 64 * TM - 1) / (64 * TM)), nb = (int)((a.n + 64 * TN - 1) / (64 * TN));
+  const int lds = DEPTH * 4 * (TM + TN) * kTileBytes;
+  PKV_HIP(hipFuncSetAttribute((const void *)pkv_fp8_block_kernel<TM, TN, DEPTH, E4M3>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL((pkv_fp8_block_kernel<TM, TN, DEPTH, E4M3>), dim3((unsigned)((mb * (int64_t)nb + 7) / 8 * 8)), dim3(256), lds, s, a, mb, nb);
+  PKV_LAUNCH_CHECK("pkv_fp8_block_kernel");
+  return PKV_OK;
+}
+template <int TM, int TN, int DEPTH>
+int launch_block(const LinearArgs &a, hipStream_t s) {
+  return a.f32 ? launch_block_as<TM, TN, DEPTH, false>(a, s) : launch_block_as<TM, TN, DEPTH, true>(a, s);
+}
+
+// What a workgroup takes: 16 MT rows of x by 16 RT of the matrix (stream), 64 TM by 64 TN (block).
+enum Shape { kStream11, kStream12, kStream14, kStream22, kStream24, kBlock11, kBlock12, kBlock21, kBlock22, kBlock22Two };
+
+// A compute unit takes about 50 KB a microsecond of what its workgroups read, whatever the shape, so a shape costs the rows of x and of the matrix
+// that a workgroup reads, times the workgroups a compute unit gets, at least one; blocks 0.85 of that (their loads of x are whole lines).  us,
+// rows x (n x k), 32x64 stream / 64x64 stream / 64x64 block / 128x128 block: 128 x (4096 x 4096) 10.5 / 17.7 / 12.1 / 22; 256 x same 18.6 / 17.7 /
+// 12.3 / 22; 64 x (28672 x 4096) 42 / 37 / 26.5 / 27, 64x128 block 25; 256 x same 152 / 129 / 61 / 44; 1 x (4096 x 4096), 16x16 / 16x64
+// stream: 5.3 / 8.7, 16 x (28672 x 4096) 28 / 21.
+Shape linear_shape(int64_t m, int64_t n) {
+  static const int kRows[][2] = {{16, 16}, {16, 32}, {16, 64}, {32, 32}, {32, 64}, {64, 64}, {64, 128}, {128, 64}, {128, 128}};
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 9; ++i) {
+    const int bm = kRows[i][0], bn = kRows[i][1];
+    const double groups = (double)((m + bm - 1) / bm) * (double)((n + bn - 1) / bn);
+    const double cost = (groups > 256 ? groups / 256 : 1.0) * (bm + bn) * (i >= kBlock11 ? 0.85 : 1.0);
+    if (i == 0 || cost < least) best = i, least = cost;
+    // two to a compute unit, with two buffers each, where there are so many: 4096 x (6144 x 4096) 105 us, with four buffers 137; 1024 x (4096 x 4096)
+    // (256 of them) 28.7 and 22.6
+    if (best == kBlock22 && i == kBlock22 && groups > 256) return kBlock22Two;
   }
+  return (Shape)best;
 }
 
 // Codes [n][k] into tiles and back: one 16-byte vector of a tile a thread.
@@ -240,21 +465,29 @@ extern "C" int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w
   return PKV_OK;
 }
 
-extern "C" int pkv_fp8_linear(const uint8_t *x, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,
+extern "C" int pkv_fp8_linear(const uint8_t *x, int64_t x_stride, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,
                               void *y, int out_dtype, void *stream) {
   PKV_REQUIRE(x && x_scales && packed && y, "pkv_fp8_linear: null pointer");
   PKV_REQUIRE(out_dtype == PKV_DTYPE_F32 || out_dtype == PKV_DTYPE_BF16, "unknown dtype %d", out_dtype);
   PKV_REQUIRE(matrix_ok(n, k) && rows > 0 && rows <= ((int64_t)1 << 22), "pkv_fp8_linear: bad shape %lld rows, %lld x %lld", (long long)rows, (long long)n, (long long)k);
-  PKV_REQUIRE(pkv_aligned(x, 16) && pkv_aligned(packed, 16) && pkv_aligned(x_scales, 4) && pkv_aligned(bias, 2) && pkv_aligned(y, 4), "pkv_fp8_linear: 16-byte aligned operands required");
+  PKV_REQUIRE(x_stride % 16 == 0 && x_stride >= (int64_t)chunks_of(k) * kTileCols, "pkv_fp8_linear: rows of x must be 16-byte multiples apart and hold whole chunks of 128");
+  PKV_REQUIRE(pkv_aligned(x, 16) && pkv_aligned(packed, 16) && pkv_aligned(x_scales, 4) && pkv_aligned(bias, 2) && pkv_aligned(y, 16), "pkv_fp8_linear: 16-byte aligned operands required");
   LinearArgs a;
-  a.x = x, a.sx = x_scales, a.tiles = (const uint8_t *)packed, a.sw = (const float *)((const uint8_t *)packed + tile_bytes(n, k));
+  a.x = x, a.x_stride = x_stride, a.sx = x_scales, a.tiles = (const uint8_t *)packed, a.sw = (const float *)((const uint8_t *)packed + tile_bytes(n, k));
   a.bias = (const uint16_t *)bias, a.y = y, a.m = rows, a.n = n, a.chunks = chunks_of(k), a.f32 = out_dtype == PKV_DTYPE_F32;
   hipStream_t s = (hipStream_t)stream;
-  const unsigned tiles = (unsigned)row_tiles(n);
-  if (rows <= 16) hipLaunchKernelGGL((pkv_fp8_stream_kernel<1, 1>), dim3(tiles), dim3(kStreamWaves * PKV_WAVE), 0, s, a);
-  else if (rows <= 32) hipLaunchKernelGGL((pkv_fp8_stream_kernel<2, 1>), dim3(tiles), dim3(kStreamWaves * PKV_WAVE), 0, s, a);
-  else if (rows <= 128) hipLaunchKernelGGL((pkv_fp8_stream_kernel<4, 1>), dim3(tiles, (unsigned)((rows + 63) / 64)), dim3(kStreamWaves * PKV_WAVE), 0, s, a);
-  else hipLaunchKernelGGL(pkv_fp8_block_kernel, dim3((tiles + kBlockTiles - 1) / kBlockTiles, (unsigned)((rows + kBlock - 1) / kBlock)), dim3(256), 0, s, a);
+  switch (linear_shape(rows, n)) {
+    case kStream11: launch_stream<1, 1>(a, s); break;
+    case kStream12: launch_stream<1, 2>(a, s); break;
+    case kStream14: launch_stream<1, 4>(a, s); break;
+    case kStream22: launch_stream<2, 2>(a, s); break;
+    case kStream24: launch_stream<2, 4>(a, s); break;
+    case kBlock11: return launch_block<1, 1, 4>(a, s);
+    case kBlock12: return launch_block<1, 2, 3>(a, s);
+    case kBlock21: return launch_block<2, 1, 3>(a, s);
+    case kBlock22: return launch_block<2, 2, 4>(a, s);
+    default: return launch_block<2, 2, 2>(a, s);
+  }
   PKV_LAUNCH_CHECK("pkv_fp8_linear");
   return PKV_OK;
 }

@@ -20,7 +20,7 @@ __device__ __forceinline__ double fp8_wave_sum(double v) {
 struct RowsArgs {
   const char *x;
   const uint16_t *residual, *weight;
-  int64_t x_stride;  // bytes
+  int64_t x_stride, code_stride;  // bytes
   double eps;
   int width, padded;
   uint16_t *out_sum;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(row_threads(E)) void pkv_fp8_rows_kernel(RowsArgs a
   for (int i = 0; i < kRowWaves; ++i) top = s_top[i] > top ? s_top[i] : top;
   const int e2 = fp8_exponent(top);
   const float shrink = fp8_pow2(-e2);
-  uint8_t *const codes = a.codes + row * a.padded;
+  uint8_t *const codes = a.codes + row * a.code_stride;
 #pragma unroll
   for (int r = 0; r < kReps; ++r) {
     const int at = (r * kRowThreads + tid) * E;
@@ -126,37 +126,39 @@ int launch(const RowsArgs &a, int64_t rows, bool whole, hipStream_t s) {
   return PKV_OK;
 }
 
-int shape_ok(const char *who, int64_t rows, int64_t width, const void *codes, const void *scales) {
+int shape_ok(const char *who, int64_t rows, int64_t width, const void *codes, int64_t code_stride, const void *scales) {
   PKV_REQUIRE(rows > 0 && rows < ((int64_t)1 << 31) && width > 0 && width <= kMaxWidth, "%s: 1..%d columns, at least one row (got %lld x %lld)", who,
               kMaxWidth, (long long)rows, (long long)width);
-  PKV_REQUIRE(pkv_aligned(codes, 128) && pkv_aligned(scales, 4), "%s: codes must be 128-byte aligned", who);
+  PKV_REQUIRE(pkv_aligned(codes, 16) && code_stride % 16 == 0 && code_stride >= (int64_t)pkv_align_up((size_t)width, 128) && pkv_aligned(scales, 4),
+              "%s: rows of codes must be 16-byte aligned and hold whole chunks of 128", who);
   return PKV_OK;
 }
 
 }  // namespace
 
 extern "C" int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const void *weight, double eps, int64_t rows, int64_t width,
-                                   void *out_sum, uint8_t *codes, float *scales, void *stream) {
+                                   void *out_sum, uint8_t *codes, int64_t code_stride, float *scales, void *stream) {
   PKV_REQUIRE(x && weight && codes && scales, "pkv_add_rmsnorm_fp8: null pointer");
-  if (const int rc = shape_ok("pkv_add_rmsnorm_fp8", rows, width, codes, scales)) return rc;
+  if (const int rc = shape_ok("pkv_add_rmsnorm_fp8", rows, width, codes, code_stride, scales)) return rc;
   PKV_REQUIRE(pkv_aligned(x, 2) && pkv_aligned(residual, 2) && pkv_aligned(weight, 2) && pkv_aligned(out_sum, 2), "pkv_add_rmsnorm_fp8: bf16 operands");
   RowsArgs a;
   a.x = (const char *)x, a.residual = (const uint16_t *)residual, a.weight = (const uint16_t *)weight, a.x_stride = width * 2, a.eps = eps;
-  a.width = (int)width, a.padded = (int)pkv_align_up((size_t)width, 128), a.out_sum = (uint16_t *)out_sum, a.codes = codes, a.scales = scales;
+  a.width = (int)width, a.padded = (int)pkv_align_up((size_t)width, 128), a.out_sum = (uint16_t *)out_sum, a.codes = codes, a.code_stride = code_stride, a.scales = scales;
   const bool whole = width % 8 == 0 && pkv_aligned(x, 16) && pkv_aligned(residual, 16) && pkv_aligned(weight, 16) && pkv_aligned(out_sum, 16);
   return launch<true, true>(a, rows, whole, (hipStream_t)stream);
 }
 
-extern "C" int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t *codes, float *scales, void *stream) {
+extern "C" int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t *codes, int64_t code_stride, float *scales,
+                            void *stream) {
   PKV_REQUIRE(x && codes && scales, "pkv_fp8_rows: null pointer");
   PKV_REQUIRE(dtype == PKV_DTYPE_F32 || dtype == PKV_DTYPE_BF16, "unknown dtype %d", dtype);
-  if (const int rc = shape_ok("pkv_fp8_rows", rows, width, codes, scales)) return rc;
+  if (const int rc = shape_ok("pkv_fp8_rows", rows, width, codes, code_stride, scales)) return rc;
   const int64_t es = dtype == PKV_DTYPE_BF16 ? 2 : 4;
   PKV_REQUIRE(pkv_aligned(x, es) && x_stride >= 0, "pkv_fp8_rows: rows of whole elements");
   RowsArgs a;
   memset(&a, 0, sizeof a);
   a.x = (const char *)x, a.x_stride = x_stride * es, a.width = (int)width, a.padded = (int)pkv_align_up((size_t)width, 128);
-  a.codes = codes, a.scales = scales;
+  a.codes = codes, a.code_stride = code_stride, a.scales = scales;
   const bool whole = width % 8 == 0 && x_stride * es % 16 == 0 && pkv_aligned(x, 16);
   if (dtype == PKV_DTYPE_BF16) return launch<false, true>(a, rows, whole, (hipStream_t)stream);
   return launch<false, false>(a, rows, whole, (hipStream_t)stream);

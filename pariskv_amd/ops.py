@@ -1369,18 +1369,18 @@ assert _FP8_ATTN_BLOCK.size == C.sizeof(_lib.Fp8AttnArgs)
 
 
 class Fp8Rows:
-    """Rows [..., k] in eight bits: e4m3 ``codes`` and a power-of-two scale each, ``scales`` fp32 [...].  A row is its codes times its scale."""
+    """Rows [..., k] in eight bits: e4m3 ``codes`` [..., k] and a power-of-two scale each, ``scales`` fp32 [...].  A row is its codes times its scale."""
 
     __slots__ = ("padded", "scales", "shape", "k")
 
     def __init__(self, padded: torch.Tensor, scales: torch.Tensor, shape):
-        # padded: uint8 [rows, k rounded up to 128], zeros past k
+        # padded: float8 [rows, k rounded up to 128], zeros past k
         self.padded, self.scales, self.shape, self.k = padded, scales, shape, shape[-1]
 
     @property
     def codes(self) -> torch.Tensor:
         rows = self.padded if self.padded.shape[1] == self.k else self.padded[:, :self.k]
-        return rows.view(FP8).view(self.shape)
+        return rows if len(self.shape) == 2 else rows.view(self.shape)
 
     @property
     def device(self):
@@ -1394,10 +1394,15 @@ class Fp8Rows:
         _one_device(codes, scales)
         k, rows = codes.shape[-1], _fp8_bytes(codes, "codes").reshape(-1, codes.shape[-1])
         if k % 128 or not rows.is_contiguous() or rows.data_ptr() % 16:
-            padded = torch.zeros(rows.shape[0], -(-k // 128) * 128, dtype=torch.uint8, device=codes.device)
+            padded = torch.zeros(rows.shape[0], _fp8_step(k), dtype=torch.uint8, device=codes.device)
             padded[:, :k] = rows
             rows = padded
-        return cls(rows, scales.contiguous(), tuple(codes.shape))
+        return cls(rows.view(FP8), scales.contiguous(), tuple(codes.shape))
+
+
+def _fp8_step(k: int) -> int:
+    """Bytes from one row of codes to the next: whole chunks of 128."""
+    return (k + 127) & -128
 
 
 def fp8_rows(x: torch.Tensor) -> Fp8Rows:
@@ -1410,11 +1415,11 @@ def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     if unit != 1 and k > 1 or step < 0:
         rows = rows.contiguous()
         step = k
-    n = rows.shape[0]
-    codes = x.new_empty((n, -(-k // 128) * 128), dtype=torch.uint8)
+    n, wide = rows.shape[0], _fp8_step(k)
+    codes = x.new_empty((n, wide), dtype=FP8)
     scales = x.new_empty(shape[:-1], dtype=torch.float32)
     if n > 0:
-        rc = _lib.lib().pkv_fp8_rows(rows.data_ptr(), code, step, n, k, codes.data_ptr(), scales.data_ptr(), _stream(x))
+        rc = _lib.lib().pkv_fp8_rows(rows.data_ptr(), code, step, n, k, codes.data_ptr(), wide, scales.data_ptr(), _stream(x))
         if rc != 0:
             _lib.check(rc)
     return Fp8Rows(codes, scales, shape)
@@ -1430,18 +1435,23 @@ def add_rmsnorm_fp8(x: torch.Tensor, residual, weight: torch.Tensor, eps: float,
     at = x.get_device()
     if weight.dtype != torch.bfloat16 or weight.numel() != width or not weight.is_contiguous() or weight.get_device() != at:
         raise RuntimeError("weight: contiguous bf16 [width] on the GPU of x")
-    if residual is not None and (residual.shape != shape or residual.dtype != torch.bfloat16 or not residual.is_contiguous() or residual.get_device() != at):
-        raise RuntimeError("residual must match x")
-    rows = x.numel() // width
-    out_sum = torch.empty_like(x) if (want_sum and residual is not None) else None
-    codes = x.new_empty((rows, -(-width // 128) * 128), dtype=torch.uint8)
+    rows, wide = x.numel() // width, _fp8_step(width)
+    codes = x.new_empty((rows, wide), dtype=FP8)
     scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    total, res_at, sum_at = x, None, None
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != torch.bfloat16 or not residual.is_contiguous() or residual.get_device() != at:
+            raise RuntimeError("residual must match x")
+        res_at = residual.data_ptr()
+        if want_sum:
+            total = torch.empty_like(x)
+            sum_at = total.data_ptr()
     if rows > 0:
-        rc = _lib.lib().pkv_add_rmsnorm_fp8(x.data_ptr(), _p(residual), weight.data_ptr(), eps, rows, width, _p(out_sum), codes.data_ptr(),
+        rc = _lib.lib().pkv_add_rmsnorm_fp8(x.data_ptr(), res_at, weight.data_ptr(), eps, rows, width, sum_at, codes.data_ptr(), wide,
                                             scales.data_ptr(), _stream(x))
         if rc != 0:
             _lib.check(rc)
-    return (out_sum if out_sum is not None else x), Fp8Rows(codes, scales, shape)
+    return total, Fp8Rows(codes, scales, shape)
 
 
 class Fp8Weight:
@@ -1509,7 +1519,7 @@ def fp8_linear(x, weight: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dt
     m = padded.shape[0]
     y = padded.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
     if m > 0:
-        rc = _lib.lib().pkv_fp8_linear(padded.data_ptr(), x.scales.data_ptr(), m, packed.data_ptr(), n, weight.k, _p(bias), y.data_ptr(), code, _stream(packed))
+        rc = _lib.lib().pkv_fp8_linear(padded.data_ptr(), padded.shape[1], x.scales.data_ptr(), m, packed.data_ptr(), n, weight.k, _p(bias), y.data_ptr(), code, _stream(packed))
         if rc != 0:
             _lib.check(rc)
     return y

@@ -6,7 +6,7 @@ Tolerances.  u = 2^-24 is half a step of fp32, h half a step of the output's typ
 Written and read rows: none.  Dividing by a power of two is exact, a code is rounded once, and code times scale has four bits.
 Norm: y = t inv w with inv = fp32(1 / sqrt(mean t^2 + eps)) out of 64 bits and two more roundings: off by at most 3 u |y|, so the code lies between
 those of y (1 - 4 u) and y (1 + 4 u), and the scale is one of theirs.
-Products: with B = sum |x| |w| a path through the sums of k exact products has at most 128 + k/128 + 20 additions, each off by at most a step
+Products (of few rows, or with fp32 results; see test_linear_blocks_rounded for the others): with B = sum |x| |w| a path through the sums of k exact products has at most 128 + k/128 + 20 additions, each off by at most a step
 (2 u) of B, should an instruction cut off rather than round: 2 (148 + k/128) u B; two scales, 2 u |y|; the bias u (|y| + |bias|); h |y|.
 Attention: with A = sum p |v| over the keys a row sees (p the exact weights) and S the largest sum of |q| |k| times the scale: a score is off by at
 most 2 * 130 u S (128 exact products, their sum, two scales), which moves a weight by that much and the normaliser by as much again; the sum
@@ -493,7 +493,7 @@ def test_rows(rows, width, dtype):
     e = _exponent(_top(x).amax(1)) if rows else x[:, 0]
     assert tuple(r.shape) == (rows, width) and r.codes.dtype == F8 and tuple(r.codes.shape) == (rows, width)
     assert same(r.scales, torch.exp2(e)) and same(r.codes.float(), _round(x / torch.exp2(e).unsqueeze(1)))
-    assert r.padded.shape[1] % 128 == 0 and not bool(r.padded[:, width:].any())
+    assert not bool(r.padded.view(U8)[:, width:-(-width // 128) * 128].any())
 
 
 def test_rows_layouts():
@@ -525,7 +525,7 @@ def test_add_rmsnorm_fp8(rows, width, residual):
     assert bool(((s == torch.exp2(e0)) | (s == torch.exp2(e1))).all())
     code = q.codes.float().cpu().to(F64)
     assert bool((code >= _round(lo / s.unsqueeze(1))).all()) and bool((code <= _round(hi / s.unsqueeze(1))).all())
-    assert not bool(q.padded[:, width:].any())
+    assert not bool(q.padded.view(U8)[:, width:-(-width // 128) * 128].any())
 
 
 def test_add_rmsnorm_fp8_special():
@@ -583,6 +583,44 @@ def test_linear_large():
         wd = weight.dequantize().cpu().to(F64)
         y = ops.fp8_linear(rows, weight, out_dtype=F32)
         check_linear(y, rows.codes.float().cpu().to(F64), rows.scales.cpu().to(F64), wd, torch.ones(n, dtype=F64), None, F32)
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 8192, 256), (65, 33000, 130), (130, 20000, 384), (300, 5000, 128), (520, 9001, 1000), (700, 12288, 640)])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+def test_linear_blocks(m, n, k, out_dtype):
+    """Shapes that go through LDS.  Codes whose products are multiples of 2^-6 up to 2^2: nothing is below 2^-13 of the largest of eight, so the sums are
+    exact in fp32 whatever instruction adds them up."""
+    ops, g = _ops(), _gen(m + n)
+    codes, wcodes = ((torch.randint(0x38, 0x48, (r, k), generator=g) + 128 * torch.randint(0, 2, (r, k), generator=g)).to(U8).to(DEV) for r in (m, n))
+    sx, sw = (torch.rand(m, generator=g) + 0.1).to(DEV), (torch.rand(n, generator=g) - 0.5).to(DEV)
+    bias = torch.randn(n, generator=g).to(BF).to(DEV) if m % 2 == 0 else None
+    y = ops.fp8_linear(ops.Fp8Rows.from_codes(codes, sx), ops.Fp8Weight.from_codes(wcodes, sw), bias=bias, out_dtype=out_dtype)
+    ref = codes.view(F8).to(F64) @ wcodes.view(F8).to(F64).t() * sx.to(F64).unsqueeze(1) * sw.to(F64)
+    tol = 2 * U * ref.abs()
+    if bias is not None:
+        ref = ref + bias.to(F64)
+        tol = tol + U * (ref.abs() + bias.to(F64).abs())
+    err = (y.to(F64) - ref).abs()
+    assert bool((err <= tol + HALF[out_dtype] * ref.abs() + 1e-30).all())
+
+
+def test_linear_blocks_rounded():
+    """bf16 results of many rows: the instructions for e4m3 codes cut each of eight neighbouring products off below 2^-13 of the largest of
+    them, so every group of eight loses at most 7 * 2^-13 of its largest."""
+    ops, g = _ops(), _gen(33)
+    m, n, k = 130, 20000, 512
+    x, w = _rows(g, m, k, dtype=F32), _rows(g, n, k, spread=2.0)
+    rows, weight = ops.fp8_rows(x.to(DEV)), ops.Fp8Weight.quantize(w.to(DEV))
+    xv, wv = rows.codes.to(F64) * rows.scales.to(F64).unsqueeze(1), weight.dequantize().to(F64)
+    ref, B = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    lost = torch.zeros_like(ref)
+    for i in range(0, k, 8):
+        top = torch.zeros_like(ref)
+        for e in range(i, i + 8):
+            top = torch.maximum(top, (xv[:, e].unsqueeze(1) * wv[:, e]).abs())
+        lost += 7 * 2.0 ** -13 * top
+    err = (ops.fp8_linear(rows, weight).to(F64) - ref).abs()
+    assert bool((err <= lost * (1 + 2.0 ** -7) + 2 * (148 + k / 128) * U * B + (2 * U + 2.0 ** -8) * ref.abs()).all())
 
 
 def test_linear_codes_and_shapes():
