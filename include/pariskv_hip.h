@@ -646,7 +646,7 @@ int pkv_fp8_read(const pkv_fp8_kv *cache, int64_t row0, int64_t n_rows, const in
  * q [bs][n_tokens][n_kv_heads*group][128], heads side by side, of `dtype` (strides in elements, 16-byte multiples); out the same,
  * contiguous.  1 <= n_tokens <= 1024, n_tokens * group <= 8192, at most PKV_FP8_MAX_ROWS keys.  fp32 sums and statistics; bf16: weights are
  * rounded to bf16 for the product with V, and the normaliser is the sum of the rounded ones; fp32: no rounding but that of fp32.
- * ws: pkv_fp8_attention_ws_bytes(bs, n_kv_heads, group, n_tokens, keys) bytes for the partial results (0: none needed). */
+ * ws: pkv_fp8_attention_ws_bytes(dtype, bs, n_kv_heads, group, n_tokens, keys) bytes for the partial results (0: none needed). */
 typedef struct pkv_fp8_segment {
   int64_t row0, n_rows;
   const int64_t *idx;  /* or NULL */
@@ -663,7 +663,7 @@ typedef struct pkv_fp8_attn_args {
   void *out, *ws;
   size_t ws_bytes;
 } pkv_fp8_attn_args;
-size_t pkv_fp8_attention_ws_bytes(int bs, int n_kv_heads, int group, int n_tokens, int64_t total_keys);
+size_t pkv_fp8_attention_ws_bytes(int dtype, int bs, int n_kv_heads, int group, int n_tokens, int64_t total_keys);
 int pkv_fp8_attention(const pkv_fp8_attn_args *args, void *stream);
 
 /* pkv_add_rmsnorm with the norm's rows in eight bits, a scale each (no counterpart in the reference, model_hub/qwen.py:395-407 in bf16): t = bf16(x + residual), or x where

@@ -211,7 +211,7 @@ PROTOTYPES = {
     "pkv_w4_linear": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i, _vp, _sz, _vp]),
     "pkv_fp8_store": (_i, [_vp, _vp, _vp, _i] + [_i64] * 8 + [_vp, _vp, _vp]),
     "pkv_fp8_read": (_i, [_vp, _i64, _i64, _vp, _i64, _i, _vp, _vp] + [_i64] * 6 + [_vp]),
-    "pkv_fp8_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i64]),
+    "pkv_fp8_attention_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i64]),
     "pkv_fp8_attention": (_i, [_vp, _vp]),
     "pkv_add_rmsnorm_fp8": (_i, [_vp, _vp, _vp, C.c_double, _i64, _i64, _vp, _vp, _i64, _vp, _vp]),
     "pkv_fp8_rows": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),

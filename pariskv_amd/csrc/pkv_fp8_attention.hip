@@ -38,6 +38,7 @@ struct Call {
   float *ws_o, *ws_ml;  // [row of (b, h)][split][query row][128], [..][2]
   void *out;
   int n_kv_heads, group, n_tokens, lg_block, n_segments, n_splits, n_pairs;
+  bool once;  // a key is read by one workgroup only
   uint32_t total;
   Seg seg[PKV_ATTN_MAX_SEGMENTS];
 };
@@ -49,9 +50,9 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
 // Key of a half step (32 keys) that element e of lane (., j) belongs to.
 __device__ __forceinline__ int key_of(int e, int j) { return 16 * (e >> 2) + 4 * j + (e & 3); }
 
-// PARTS: bf16 numbers that make up a number of q and of the weights.
+// PARTS: bf16 numbers that make up a number of q and of the weights.  One tile of 16 query rows.
 template <int PARTS>
-struct Wave {
+struct Tile {
   pkv_u32x4 q[PARTS][4];
   // Weights are 2^(score - use).  use moves, and the sums with it, when a score is above it by more than lim = 8, so that most steps neither
   // look for the row's maximum across lanes nor touch the sums; lim = -inf: the row has seen nothing yet.
@@ -71,7 +72,7 @@ __device__ __forceinline__ void split_off(float (&x)[8], pkv_u32x4 &part) {
 
 // Scores (times log2 e) into weights of the keys in `bits` (MASKED; else of all); p stays as numbers, for bf16 rounded.
 template <bool MASKED, int PARTS>
-__device__ __forceinline__ void weights(Wave<PARTS> &w, const float (&s)[8], uint32_t bits, float (&p)[8]) {
+__device__ __forceinline__ void weights(Tile<PARTS> &w, const float (&s)[8], uint32_t bits, float (&p)[8]) {
   const int j = pkv_lane() >> 4;
   float x[8], top = -INFINITY;
 #pragma unroll
@@ -126,12 +127,32 @@ __device__ __forceinline__ void turn_v(const pkv_u32x2 (&v)[8], int half, pkv_u3
   }
 }
 
-// Half a step: 32 keys.  k: two tiles of 16; kx, vx: the scales of the lane's keys (K's with scale log2 e); first: of the 32, in the key order.
-template <bool MASKED, int PARTS>
-__device__ __forceinline__ void half_step(Wave<PARTS> &w, const pkv_u32x4 (&k)[2][2], pkv_u32x2 (&v)[8], const float (&kx)[8], const float (&vx)[8],
-                                          int first, int n_here, int limit) {
+// The codes of half a step, 32 keys, that a lane multiplies: of two tiles of keys, and eight dims of its eight keys' values.
+struct Half {
+  pkv_u32x4 k[2][2];
+  pkv_u32x2 v[8];
+  // in LDS: row i of K at 128 i, of V 4096 further, 16-byte vector v of it at v ^ (i mod 8), so that rows of an operand are on different banks
+  __device__ __forceinline__ void from_lds(const uint8_t *at) {
+    const int lane = pkv_lane(), n = lane & 15, j = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) k[t][i] = *(const pkv_u32x4 *)(at + (16 * t + n) * 128 + 16 * ((4 * i + j) ^ (n & 7)));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = *(const pkv_u32x2 *)(at + 4096 + key_of(e, j) * 128 + 16 * ((n >> 1) ^ (key_of(e, j) & 7)) + 8 * (n & 1));
+  }
+};
+
+// Half a step.  kx, vx: the scales of the lane's keys (K's with scale log2 e); first: of the 32, in the key order.
+template <bool MASKED, int PARTS, int NT>
+__device__ __forceinline__ void half_step(Tile<PARTS> (&w)[NT], Half &x, const float (&kx)[8], const float (&vx)[8], int first, int n_here,
+                                          const int (&limit)[NT]) {
   const int j = pkv_lane() >> 4;
-  pkv_f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+  pkv_f32x4 s0[NT], s1[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) s0[t] = s1[t] = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
+  const pkv_u32x4(&k)[2][2] = x.k;
+  pkv_u32x2(&v)[8] = x.v;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     pkv_u32x4 a, b;
@@ -141,30 +162,38 @@ __device__ __forceinline__ void half_step(Wave<PARTS> &w, const pkv_u32x4 (&k)[2
       b[2 * d] = fp8_bf16x2<false>(k[1][c >> 1][2 * (c & 1) + d]), b[2 * d + 1] = fp8_bf16x2<true>(k[1][c >> 1][2 * (c & 1) + d]);
     }
 #pragma unroll
-    for (int p = PARTS - 1; p >= 0; --p) s0 = mfma_bf16(a, w.q[p][c], s0), s1 = mfma_bf16(b, w.q[p][c], s1);
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int p = PARTS - 1; p >= 0; --p) s0[t] = mfma_bf16(a, w[t].q[p][c], s0[t]), s1[t] = mfma_bf16(b, w[t].q[p][c], s1[t]);
   }
-  float s[8], p[8];
-  uint32_t bits = 0xffu, there = 0xffu;
+  uint32_t bits[NT], there = 0xffu;
+  pkv_u32x4 a[NT][PARTS];
   if constexpr (MASKED) {
-    bits = there = 0;
+    there = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int key = first + key_of(e, j);
-      bits |= key < limit ? 1u << e : 0u, there |= key < n_here ? 1u << e : 0u;
-    }
+    for (int e = 0; e < 8; ++e) there |= first + key_of(e, j) < n_here ? 1u << e : 0u;
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) s[e] = (e < 4 ? s0[e & 3] : s1[e & 3]) * kx[e];
-  weights<MASKED, PARTS>(w, s, bits, p);
+  for (int t = 0; t < NT; ++t) {
+    bits[t] = 0xffu;
+    if constexpr (MASKED) {
+      bits[t] = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) p[e] *= MASKED && !((bits >> e) & 1u) ? 0.f : vx[e];
-  pkv_u32x4 a[PARTS];
-  if constexpr (PARTS == 1) {
+      for (int e = 0; e < 8; ++e) bits[t] |= first + key_of(e, j) < limit[t] ? 1u << e : 0u;
+    }
+    float s[8], p[8];
 #pragma unroll
-    for (int d = 0; d < 4; ++d) a[0][d] = bf16x2(p[2 * d], p[2 * d + 1]);
-  } else {
+    for (int e = 0; e < 8; ++e) s[e] = (e < 4 ? s0[t][e & 3] : s1[t][e & 3]) * kx[e];
+    weights<MASKED, PARTS>(w[t], s, bits[t], p);
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) split_off(p, a[i]);
+    for (int e = 0; e < 8; ++e) p[e] *= MASKED && !((bits[t] >> e) & 1u) ? 0.f : vx[e];
+    if constexpr (PARTS == 1) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) a[t][0][d] = bf16x2(p[2 * d], p[2 * d + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) split_off(p, a[t][i]);
+    }
   }
   bool odd = false;
   if constexpr (MASKED) {
@@ -186,35 +215,60 @@ __device__ __forceinline__ void half_step(Wave<PARTS> &w, const pkv_u32x4 (&k)[2
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       if (MASKED && odd) {
-        pkv_u32x4 is_nan, seen;
+        pkv_u32x4 is_nan;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           const uint32_t lo = (b[m][d] & 0x7fffu) > 0x7f80u ? 0xffffu : 0u, hi = (b[m][d] & 0x7fff0000u) > 0x7f800000u ? 0xffff0000u : 0u;
           is_nan[d] = (lo | hi) & 0x3f803f80u, b[m][d] &= ~(lo | hi);
-          seen[d] = ((bits >> (2 * d)) & 1u ? 0x3f80u : 0u) | ((bits >> (2 * d + 1)) & 1u ? 0x3f800000u : 0u);
         }
-        const pkv_f32x4 hits = mfma_bf16(seen, is_nan, pkv_f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (hits[i] > 0.f) w.o[4 * h + m][i] = NAN;
+        for (int t = 0; t < NT; ++t) {
+          pkv_u32x4 seen;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) seen[d] = ((bits[t] >> (2 * d)) & 1u ? 0x3f80u : 0u) | ((bits[t] >> (2 * d + 1)) & 1u ? 0x3f800000u : 0u);
+          const pkv_f32x4 hits = mfma_bf16(seen, is_nan, pkv_f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hits[i] > 0.f) w[t].o[4 * h + m][i] = NAN;
+        }
       }
 #pragma unroll
-      for (int i = PARTS - 1; i >= 0; --i) w.o[4 * h + m] = mfma_bf16(a[i], b[m], w.o[4 * h + m]);
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = PARTS - 1; i >= 0; --i) w[t].o[4 * h + m] = mfma_bf16(a[t][i], b[m], w[t].o[4 * h + m]);
     }
   }
 }
 
-// Row of concatenated key jj.
-template <bool INDEXED>
-__device__ __forceinline__ uint32_t row_of(const Call &a, int bh, uint32_t jj) {
-  uint32_t r = jj + (uint32_t)a.seg[0].delta;
+// The kStep rows of keys jj .. lie one behind the other in a segment, at a distance of a multiple of four from their numbers.  (Fields of segments as
+// values in scalar registers: picked by a lane they would be loaded from memory, and waited for with all that is under way.)
+__device__ __forceinline__ bool is_plain(const Call &a, uint32_t jj) {
+  bool plain = false;
+  uint32_t lo = 0;
 #pragma unroll
-  for (int t = 1; t < PKV_ATTN_MAX_SEGMENTS; ++t) r = jj >= a.seg[t - 1].end ? jj + (uint32_t)a.seg[t].delta : r;
-  if constexpr (INDEXED) {
+  for (int t = 0; t < PKV_ATTN_MAX_SEGMENTS; ++t) {
+    const uint32_t end = att_field(a.seg[t].end), off = (uint32_t)att_field(a.seg[t].delta) | (a.seg[t].idx ? 1u : 0u);
+    plain |= jj >= lo && jj + kStep <= end && (off & 3u) == 0;
+    lo = end;
+  }
+  return plain && jj + kStep <= a.total;  // the last segment's end is open
+}
+
+// Row of concatenated key jj (plain: of a step for which is_plain says so).
+template <bool INDEXED>
+__device__ __forceinline__ uint32_t row_of(const Call &a, int bh, uint32_t jj, bool plain) {
+  int32_t d = att_field(a.seg[0].delta);
+#pragma unroll
+  for (int t = 1; t < PKV_ATTN_MAX_SEGMENTS; ++t) {
+    const int32_t next = att_field(a.seg[t].delta);
+    d = jj >= att_field(a.seg[t - 1].end) ? next : d;
+  }
+  uint32_t r = jj + (uint32_t)d;
+  if (INDEXED && !plain) {
     uint32_t lo = 0;
 #pragma unroll
     for (int t = 0; t < PKV_ATTN_MAX_SEGMENTS; ++t) {
-      const uint32_t hi = a.seg[t].end;
+      const uint32_t hi = att_field(a.seg[t].end);
       if (t < a.n_segments && a.seg[t].idx && jj >= lo && jj < hi) {
         const int64_t x = a.seg[t].idx[(int64_t)bh * a.seg[t].idx_stride + (jj - lo)];
         r = lo + (uint32_t)a.seg[t].delta + (uint32_t)(x < 0 ? 0 : x >= a.seg[t].limit ? a.seg[t].limit - 1 : x);
@@ -225,116 +279,209 @@ __device__ __forceinline__ uint32_t row_of(const Call &a, int bh, uint32_t jj) {
   return r;
 }
 
-template <bool BF16, bool INDEXED>
+// Until at most LEFT of this wave's loads are on their way, and none of its reads of LDS.
+template <int LEFT>
+__device__ __forceinline__ void wait_for() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+}
+typedef const __attribute__((address_space(1))) void *global_at;
+typedef __attribute__((address_space(3))) void *lds_at;
+
+// A wave takes steps of 64 keys, dealt round the waves of all splits.  Rows go straight from memory to LDS, half a step at a time into a part of the
+// wave's own: a half is asked for as soon as the one before in its place has been used, and no registers wait for it.  4 x 8 heads x 65536 keys (541 MB): 106 us
+// with the join, of them 101 without any arithmetic and 51 without the loads (a plain read of as many bytes takes 77); rows kept by the caches 120;
+// straight to registers, half a step ahead, 115 to 125.  More than 16 query rows: two tiles of them a wave, which share the codes' conversion: 1 x 8 x 32768
+// keys, 256 rows 65 us, one tile 105.  Where several workgroups read a key, for their tiles of rows, the caches keep it: 65 and 74 us.
+template <bool BF16, int NT, bool INDEXED>
 __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_fp8_attention_kernel(Call a) {
-  constexpr int PARTS = BF16 ? 1 : 3;
+  constexpr int PARTS = BF16 ? 1 : 3, kHalf = 8192;
+  __shared__ alignas(16) uint8_t lds[kWaves * 2 * kHalf];
   // Workgroups go to the eight dies in turn, and the row tiles of one split read the same keys: they are eight numbers apart.
   const int pair = (int)blockIdx.y * 8 + (blockIdx.x & 7), tile = (int)blockIdx.x >> 3;
   if (pair >= a.n_pairs) return;  // the whole workgroup
   const int bh = (unsigned)pair / (unsigned)a.n_splits, split = pair - bh * a.n_splits;
   const int b = (unsigned)bh / (unsigned)a.n_kv_heads, h = bh - b * a.n_kv_heads;
   const int tid = threadIdx.x, lane = pkv_lane(), wave = __builtin_amdgcn_readfirstlane(tid / PKV_WAVE), n = lane & 15, j = lane >> 4;
-  const int rows = a.n_tokens * a.group, my_row = tile * 16 + n < rows ? tile * 16 + n : rows - 1, token = (unsigned)my_row / (unsigned)a.group;
+  const int rows = a.n_tokens * a.group;
   int total = (int)a.total;
   if (a.row_keys) total = a.row_keys[bh] < total ? a.row_keys[bh] : total;
-  const int limit = total - (a.n_tokens - 1 - token), full = total - (a.n_tokens - 1);
+  const int full = total - (a.n_tokens - 1);
 
-  Wave<PARTS> w;
-  const char *const qp = a.q + b * a.q_stride_b + token * a.q_stride_t + (int64_t)(h * a.group + my_row - token * a.group) * (BF16 ? 256 : 512);
+  Tile<PARTS> w[NT];
+  int limit[NT];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int dim = 64 * (c >> 1) + 16 * j + 8 * (c & 1);  // of the eight of bytes 16 j + 64 (c / 2) + 8 (c % 2) ..
-    if constexpr (BF16) {
-      w.q[0][c] = *(const pkv_u32x4 *)(qp + dim * 2);
-    } else {
-      float x[8];
-      fp8_load8<false>(qp + dim * 4, x);
+  for (int t = 0; t < NT; ++t) {
+    const int r = (tile * NT + t) * 16 + n, my_row = r < rows ? r : rows - 1, token = (unsigned)my_row / (unsigned)a.group;  // past the last: not stored
+    limit[t] = total - (a.n_tokens - 1 - token);
+    const char *const qp = a.q + b * a.q_stride_b + token * a.q_stride_t + (int64_t)(h * a.group + my_row - token * a.group) * (BF16 ? 256 : 512);
 #pragma unroll
-      for (int i = 0; i < PARTS; ++i) split_off(x, w.q[i][c]);
-    }
-  }
-  w.use = 0.f, w.lim = -INFINITY, w.l = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < 4; ++c) {
+      const int dim = 64 * (c >> 1) + 16 * j + 8 * (c & 1);  // of the eight of bytes 16 j + 64 (c / 2) + 8 (c % 2) ..
+      if constexpr (BF16) {
+        w[t].q[0][c] = *(const pkv_u32x4 *)(qp + dim * 2);
+      } else {
+        float x[8];
+        fp8_load8<false>(qp + dim * 4, x);
 #pragma unroll
-  for (int m = 0; m < 8; ++m) w.o[m] = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const uint8_t *const kb = a.k + (int64_t)bh * a.capacity * 128, *const vb = a.v + (int64_t)bh * a.capacity * 128;
-  const float *const ks = a.k_scale + (int64_t)bh * a.n_blocks, *const vs = a.v_scale + (int64_t)bh * a.n_blocks;
-  const int turns = kWaves * a.n_splits;
-  for (int first = (split * kWaves + wave) * kStep; first < total; first += turns * kStep) {
-    const uint32_t my_key = (uint32_t)(first + lane < total ? first + lane : total - 1), row = row_of<INDEXED>(a, bh, my_key);
-    const float my_k = ks[row >> a.lg_block] * a.scale_log2e, my_v = vs[row >> a.lg_block];
-    pkv_u32x4 k[2][2][2];
-    pkv_u32x2 v[2][8];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint8_t *const p = kb + (uint64_t)(uint32_t)__shfl((int)row, 32 * s + 16 * t + n, PKV_WAVE) * 128 + 16 * j;
-        k[s][t][0] = *(const pkv_u32x4 *)p, k[s][t][1] = *(const pkv_u32x4 *)(p + 64);
+        for (int i = 0; i < PARTS; ++i) split_off(x, w[t].q[i][c]);
       }
     }
+    w[t].use = 0.f, w[t].lim = -INFINITY, w[t].l = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int m = 0; m < 8; ++m) w[t].o[m] = pkv_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const uint8_t *const kb = a.k + (int64_t)bh * a.capacity * 128, *const vb = a.v + (int64_t)bh * a.capacity * 128;  // below 2^31 bytes each
+  const float *const ks = a.k_scale + (int64_t)bh * a.n_blocks, *const vs = a.v_scale + (int64_t)bh * a.n_blocks;
+  uint8_t *const mine = lds + wave * 2 * kHalf;
+  // Lane l of a step knows the place and the scales of its key l.  plain: the step's rows lie one behind the other, and four keys from a multiple of
+  // four on are in one block: addresses are sums and a lane's eight keys of half a step have two scales.  Else both come from the lanes that know
+  // them, by exchanges through LDS, which take it 16 cycles each.
+  struct Place {
+    uint32_t row;
+    float k, v;
+    bool plain;
+  };
+  auto place = [&](int first) {
+    Place p;
+    p.plain = is_plain(a, (uint32_t)first);
+    p.row = row_of<INDEXED>(a, bh, (uint32_t)(first + lane < total ? first + lane : total - 1), p.plain);
+    p.k = ks[p.row >> a.lg_block] * a.scale_log2e, p.v = vs[p.row >> a.lg_block];
+    return p;
+  };
+  auto fetch = [&](const Place &p, int s) {  // eight loads
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t row[4];
+    if (p.plain) {  // the whole wave
+      const uint32_t row0 = __builtin_amdgcn_readfirstlane(p.row) + 32 * s + (lane >> 3);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v[s][e] = *(const pkv_u32x2 *)(vb + (uint64_t)(uint32_t)__shfl((int)row, 32 * s + key_of(e, j), PKV_WAVE) * 128 + 8 * n);
+      for (int u = 0; u < 4; ++u) row[u] = row0 + 8 * u;
+    } else {
 #pragma unroll
+      for (int u = 0; u < 4; ++u) row[u] = (uint32_t)__shfl((int)p.row, 32 * s + 8 * u + (lane >> 3), PKV_WAVE);
+    }
+#define PKV_FETCH(POLICY)                                                                                                                     \
+  _Pragma("unroll") for (int u = 0; u < 4; ++u) {                                                                                             \
+    const uint32_t at = row[u] * 128u + 16u * ((lane & 7) ^ (lane >> 3));                                                                     \
+    __builtin_amdgcn_global_load_lds((global_at)(kb + at), (lds_at)(mine + s * kHalf + u * 1024), 16, 0, POLICY);                             \
+    __builtin_amdgcn_global_load_lds((global_at)(vb + at), (lds_at)(mine + s * kHalf + 4096 + u * 1024), 16, 0, POLICY);                      \
+  }
+    if (a.once) PKV_FETCH(2) else PKV_FETCH(0)  // 2: streaming
+#undef PKV_FETCH
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto scales = [&](const Place &p, int s, float (&kx)[8], float (&vx)[8]) {
+    if (p.plain) {  // the whole wave
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const float k = __shfl(p.k, 32 * s + 16 * t + 4 * j, PKV_WAVE), v = __shfl(p.v, 32 * s + 16 * t + 4 * j, PKV_WAVE);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kx[4 * t + e] = k, vx[4 * t + e] = v;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kx[e] = __shfl(p.k, 32 * s + key_of(e, j), PKV_WAVE), vx[e] = __shfl(p.v, 32 * s + key_of(e, j), PKV_WAVE);
+    }
+  };
+  auto compute = [&](const Place &p, int s) {
+    float kx[8], vx[8];
+    Half x;
+    x.from_lds(mine + s * kHalf);
+    scales(p, s, kx, vx);
+    half_step<false, PARTS, NT>(w, x, kx, vx, 0, 0, limit);
+  };
+  const int turn = kWaves * a.n_splits * kStep;
+  int first = (split * kWaves + wave) * kStep;
+  if (first + kStep <= full) {  // the whole wave; steps that all rows see in full
+    Place here = place(first), next = here;
+    fetch(here, 0);
+    fetch(here, 1);
+    for (;;) {
+      const bool more = first + turn + kStep <= full;
+      wait_for<8>();  // the first half is there
+      if (more) next = place(first + turn);
+      compute(here, 0);
+      if (more) {
+        fetch(next, 0);
+        wait_for<8>();  // the second half is there
+      } else {
+        wait_for<0>();
+      }
+      compute(here, 1);
+      first += turn;
+      if (!more) break;
+      fetch(next, 1);
+      here = next;
+    }
+  }
+  for (; first < total; first += turn) {
+    const Place here = place(first);
+    wait_for<63>();  // its reads of the last step are done; loads need not be
+    fetch(here, 0);
+    fetch(here, 1);
+    wait_for<0>();
+#pragma unroll 1
     for (int s = 0; s < 2; ++s) {
       float kx[8], vx[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) kx[e] = __shfl(my_k, 32 * s + key_of(e, j), PKV_WAVE), vx[e] = __shfl(my_v, 32 * s + key_of(e, j), PKV_WAVE);
-      if (first + kStep <= full) half_step<false, PARTS>(w, k[s], v[s], kx, vx, first + 32 * s, total, limit);
-      else half_step<true, PARTS>(w, k[s], v[s], kx, vx, first + 32 * s, total, limit);
+      Half x;
+      x.from_lds(mine + s * kHalf);
+      scales(here, s, kx, vx);
+      half_step<true, PARTS, NT>(w, x, kx, vx, first + 32 * s, total, limit);
     }
   }
 
-  // The waves meet and leave their result, or the split's part of it.
-  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-  __shared__ alignas(16) float s_o[kWaves][16][132];
-  if (j == 0) s_m[wave][n] = w.lim < 0.f ? -INFINITY : w.use;
-  if constexpr (PARTS == 1) {
+  // The waves meet, a tile of 16 rows at a time, and leave their result, or the split's part of it.
+  float(*const s_m)[16] = (float(*)[16])lds, (*const s_l)[16] = (float(*)[16])(lds + 64 * kWaves), (*const s_o)[16][132] = (float(*)[16][132])(lds + 128 * kWaves);
+  static_assert(128 * kWaves + kWaves * 16 * 132 * 4 <= (int)sizeof lds, "room for it");
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n == 0) s_l[wave][4 * j + i] = w.l[i];
-  } else {
-    const float l = pkv_pair_add<32>(pkv_pair_add<16>(w.l[0]));
-    if (j == 0) s_l[wave][n] = l;
-  }
+  for (int t = 0; t < NT; ++t) {
+    __syncthreads();
+    if (j == 0) s_m[wave][n] = w[t].lim < 0.f ? -INFINITY : w[t].use;
+    if constexpr (PARTS == 1) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    *(float4 *)&s_o[wave][4 * j + i][8 * n] = float4{w.o[0][i], w.o[1][i], w.o[2][i], w.o[3][i]};
-    *(float4 *)&s_o[wave][4 * j + i][8 * n + 4] = float4{w.o[4][i], w.o[5][i], w.o[6][i], w.o[7][i]};
-  }
-  __syncthreads();
-  for (int e = tid; e < 16 * 32; e += kWaves * PKV_WAVE) {  // four dims at a time
-    const int r = e >> 5, d = 4 * (e & 31), row = tile * 16 + r;
-    if (row >= rows) continue;
-    float mx = s_m[0][r];
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) mx = fmaxf(mx, s_m[i][r]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float ls = 0.f;
-    pkv_f32x4 os = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const float c = __builtin_amdgcn_exp2f(s_m[i][r] - base);
-      const pkv_f32x4 x = *(const pkv_f32x4 *)&s_o[i][r][d];
-      ls = fmaf(s_l[i][r], c, ls);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) os[u] = fmaf(x[u], c, os[u]);
-    }
-    if (a.n_splits == 1) {
-      const int u = (unsigned)row / (unsigned)a.group;
-      const int64_t to = (((int64_t)b * a.n_tokens + u) * a.n_kv_heads * a.group + h * a.group + (row - u * a.group)) * 128 + d;
-      const float share = ls == 0.f ? 0.f : 1.0f / ls;  // 0: nothing seen
-#pragma unroll
-      for (int i = 0; i < 4; ++i) os[i] *= share;
-      if constexpr (BF16) *(pkv_u32x2 *)((uint16_t *)a.out + to) = pkv_u32x2{bf16x2(os[0], os[1]), bf16x2(os[2], os[3])};
-      else *(pkv_f32x4 *)((float *)a.out + to) = os;
+      for (int i = 0; i < 4; ++i)
+        if (n == 0) s_l[wave][4 * j + i] = w[t].l[i];
     } else {
-      const int64_t at = (int64_t)pair * rows + row;
-      *(pkv_f32x4 *)(a.ws_o + at * 128 + d) = os;
-      if (d == 0) *(float2 *)(a.ws_ml + at * 2) = float2{mx, ls};
+      const float l = pkv_pair_add<32>(pkv_pair_add<16>(w[t].l[0]));
+      if (j == 0) s_l[wave][n] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *(float4 *)&s_o[wave][4 * j + i][8 * n] = float4{w[t].o[0][i], w[t].o[1][i], w[t].o[2][i], w[t].o[3][i]};
+      *(float4 *)&s_o[wave][4 * j + i][8 * n + 4] = float4{w[t].o[4][i], w[t].o[5][i], w[t].o[6][i], w[t].o[7][i]};
+    }
+    __syncthreads();
+    for (int e = tid; e < 16 * 32; e += kWaves * PKV_WAVE) {  // four dims at a time
+      const int r = e >> 5, d = 4 * (e & 31), row = (tile * NT + t) * 16 + r;
+      if (row >= rows) continue;
+      float mx = s_m[0][r];
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) mx = fmaxf(mx, s_m[i][r]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float ls = 0.f;
+      pkv_f32x4 os = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const float c = __builtin_amdgcn_exp2f(s_m[i][r] - base);
+        const pkv_f32x4 x = *(const pkv_f32x4 *)&s_o[i][r][d];
+        ls = fmaf(s_l[i][r], c, ls);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) os[u] = fmaf(x[u], c, os[u]);
+      }
+      if (a.n_splits == 1) {
+        const int u = (unsigned)row / (unsigned)a.group;
+        const int64_t to = (((int64_t)b * a.n_tokens + u) * a.n_kv_heads * a.group + h * a.group + (row - u * a.group)) * 128 + d;
+        const float share = ls == 0.f ? 0.f : 1.0f / ls;  // 0: nothing seen
+#pragma unroll
+        for (int i = 0; i < 4; ++i) os[i] *= share;
+        if constexpr (BF16) *(pkv_u32x2 *)((uint16_t *)a.out + to) = pkv_u32x2{bf16x2(os[0], os[1]), bf16x2(os[2], os[3])};
+        else *(pkv_f32x4 *)((float *)a.out + to) = os;
+      } else {
+        const int64_t at = (int64_t)pair * rows + row;
+        *(pkv_f32x4 *)(a.ws_o + at * 128 + d) = os;
+        if (d == 0) *(float2 *)(a.ws_ml + at * 2) = float2{mx, ls};
+      }
     }
   }
 }
@@ -374,9 +521,15 @@ __global__ __launch_bounds__(256) void pkv_fp8_join_kernel(const float *__restri
   else *(float2 *)((float *)out + to) = float2{x, y};
 }
 
+// Row tiles of 16 a wave.
+int tiles_a_wave(int dtype, int rows) { return dtype == PKV_DTYPE_BF16 && rows > 16 ? 2 : 1; }
+
+// Workgroups: four to a compute unit, two where there is more than one tile of rows (two fit there at a time, and each leaves a result a row that is read
+// again).  us, 256 / 512 / 1024: 4 x 8 x 65536 keys, 4 rows 112 / 111 / 106; 1 x 8 x 16384, 64 rows 21 / 22 / 28; 1 x 8 x 32768, 256 rows 83 / 65 / 71;
+// 3 x 4 x 9001, 35 fp32 rows 20 / 18 / 22.
 int splits_of(int64_t bh, int row_tiles, int64_t total) {
-  const int64_t turn = kWaves * kStep, most = (total + turn - 1) / turn;
-  int64_t s = (1024 + bh * row_tiles - 1) / (bh * row_tiles);
+  const int64_t turn = kWaves * kStep, most = (total + turn - 1) / turn, groups = row_tiles > 1 ? 512 : 1024;
+  int64_t s = (groups + bh * row_tiles - 1) / (bh * row_tiles);
   if (s > most) s = most;
   if (s > kMaxSplits) s = kMaxSplits;
   return (int)(s < 1 ? 1 : s);
@@ -388,9 +541,9 @@ bool shape_ok(int bs, int n_kv_heads, int group, int n_tokens) {
 
 }  // namespace
 
-extern "C" size_t pkv_fp8_attention_ws_bytes(int bs, int n_kv_heads, int group, int n_tokens, int64_t total_keys) {
+extern "C" size_t pkv_fp8_attention_ws_bytes(int dtype, int bs, int n_kv_heads, int group, int n_tokens, int64_t total_keys) {
   if (!shape_ok(bs, n_kv_heads, group, n_tokens) || total_keys < 0) return 0;
-  const int rows = n_tokens * group, s = splits_of((int64_t)bs * n_kv_heads, (rows + 15) / 16, total_keys);
+  const int rows = n_tokens * group, per = 16 * tiles_a_wave(dtype, rows), s = splits_of((int64_t)bs * n_kv_heads, (rows + per - 1) / per, total_keys);
   return s == 1 ? 0 : (size_t)bs * n_kv_heads * s * rows * 130 * sizeof(float);
 }
 
@@ -429,7 +582,7 @@ extern "C" int pkv_fp8_attention(const pkv_fp8_attn_args *a, void *stream) {
   }
   for (int i = c.n_segments; i < PKV_ATTN_MAX_SEGMENTS; ++i) c.seg[i].end = 0xffffffffu;
   if (c.n_segments) c.seg[c.n_segments - 1].end = 0xffffffffu;
-  const int rows = a->n_tokens * a->group, row_tiles = (rows + 15) / 16;
+  const int rows = a->n_tokens * a->group, nt = tiles_a_wave(a->dtype, rows), row_tiles = (rows + 16 * nt - 1) / (16 * nt);
   const int64_t bh = (int64_t)bs * H, n_rows = bh * rows;
   c.n_splits = splits_of(bh, row_tiles, total), c.n_pairs = (int)(bh * c.n_splits);
   const size_t need = c.n_splits == 1 ? 0 : (size_t)n_rows * c.n_splits * 130 * sizeof(float);
@@ -442,14 +595,19 @@ extern "C" int pkv_fp8_attention(const pkv_fp8_attn_args *a, void *stream) {
   c.capacity = a->cache.capacity, c.n_blocks = a->cache.capacity / a->cache.block, c.lg_block = __builtin_ctz(a->cache.block);
   c.row_keys = a->row_keys, c.scale_log2e = a->scale * 1.4426950408889634f, c.total = (uint32_t)total;
   c.ws_o = (float *)a->ws, c.ws_ml = need ? c.ws_o + (size_t)n_rows * c.n_splits * 128 : nullptr, c.out = a->out;
-  c.n_kv_heads = H, c.group = a->group, c.n_tokens = a->n_tokens;
+  c.n_kv_heads = H, c.group = a->group, c.n_tokens = a->n_tokens, c.once = row_tiles == 1;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid(8u * row_tiles, (unsigned)((c.n_pairs + 7) / 8)), block(kWaves * PKV_WAVE);
   const bool bf = a->dtype == PKV_DTYPE_BF16;
-  if (bf && indexed) hipLaunchKernelGGL((pkv_fp8_attention_kernel<true, true>), grid, block, 0, s, c);
-  else if (bf) hipLaunchKernelGGL((pkv_fp8_attention_kernel<true, false>), grid, block, 0, s, c);
-  else if (indexed) hipLaunchKernelGGL((pkv_fp8_attention_kernel<false, true>), grid, block, 0, s, c);
-  else hipLaunchKernelGGL((pkv_fp8_attention_kernel<false, false>), grid, block, 0, s, c);
+#define PKV_FP8_ATTENTION(BF16, NT)                                                                                 \
+  do {                                                                                                              \
+    if (indexed) hipLaunchKernelGGL((pkv_fp8_attention_kernel<BF16, NT, true>), grid, block, 0, s, c);              \
+    else hipLaunchKernelGGL((pkv_fp8_attention_kernel<BF16, NT, false>), grid, block, 0, s, c);                     \
+  } while (0)
+  if (bf && nt == 2) PKV_FP8_ATTENTION(true, 2);
+  else if (bf) PKV_FP8_ATTENTION(true, 1);
+  else PKV_FP8_ATTENTION(false, 1);
+#undef PKV_FP8_ATTENTION
   PKV_LAUNCH_CHECK("pkv_fp8_attention_kernel");
   if (c.n_splits == 1) return PKV_OK;
   const dim3 join((unsigned)((n_rows + 3) / 4));

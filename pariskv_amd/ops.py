@@ -1353,7 +1353,7 @@ class Fp8Attention:
         elif out.shape != shape or out.dtype != dt or out.get_device() != at or not out.is_contiguous() or out.data_ptr() & 15:
             raise RuntimeError("out: contiguous, like queries")
         lib = _lib.lib()
-        need = lib.pkv_fp8_attention_ws_bytes(bs, H, G, T, total)
+        need = lib.pkv_fp8_attention_ws_bytes(code, bs, H, G, T, total)
         ws = queries.new_empty(need, dtype=torch.uint8) if need else None
         block = _FP8_ATTN_BLOCK.pack(q.data_ptr(), code, G, T, n_seg, qs[0], qs[1], *cache._fields, *segs, keys_at, _SCALE if scale is None else scale,
                                      out.data_ptr(), ws.data_ptr() if need else 0, need)
