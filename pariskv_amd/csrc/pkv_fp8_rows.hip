@@ -8,8 +8,7 @@
 
 namespace {
 
-constexpr int kMaxWidth = 16384;
-constexpr int row_threads(int e) { return e == 8 ? 256 : 1024; }
+constexpr int kMaxWidth = 16384, kRowThreads = 256, kRowWaves = kRowThreads / PKV_WAVE, E = 8;  // E: neighbouring elements a thread takes at a time
 
 __device__ __forceinline__ double fp8_wave_sum(double v) {
 #pragma unroll
@@ -28,46 +27,67 @@ struct RowsArgs {
   float *scales;
 };
 
-// E: neighbouring elements a thread takes at a time: 8 (16-byte vectors of bf16), or 1 where width, stride or alignment do not allow it.
-template <bool NORM, bool BF16, int E>
-__global__ __launch_bounds__(row_threads(E)) void pkv_fp8_rows_kernel(RowsArgs a) {
-  constexpr int kRowThreads = row_threads(E), kRowWaves = kRowThreads / PKV_WAVE, kReps = kMaxWidth / (kRowThreads * E);
+// Eight elements at any address of whole elements, or the `left` of them that the row still has with zeros behind them.  The memory takes 16-byte
+// accesses at any alignment: 4096 rows of 4095 with the residual take 28.6 us (element by element: 52.2), of 4096 23.4.
+template <bool BF16>
+__device__ __forceinline__ void load_any(const char *p, int left, float (&v)[E]) {
+  if (left >= E) {
+    struct __attribute__((packed)) Raw {
+      uint32_t w[BF16 ? 4 : 8];
+    } raw;
+    __builtin_memcpy(&raw, p, sizeof raw);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      v[e] = __uint_as_float(!BF16 ? raw.w[BF16 ? 0 : e] : e & 1 ? raw.w[e / 2] & 0xffff0000u : raw.w[e / 2] << 16);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = e >= left ? 0.f : BF16 ? pkv_bf16_bits_to_f32(((const uint16_t *)p)[e]) : ((const float *)p)[e];
+}
+
+// ALIGNED: whole 16-byte vectors everywhere.  REPS: how often a thread takes eight elements at most: registers for the longest rows (8) leave three
+// waves a SIMD.  4096 rows of 4096 with the residual, us: REPS 2 23.4 (5.0 TB/s, what a copy reaches), 8 27.5; 16384 x 1024: 30.0 and 59.1.
+template <bool NORM, bool BF16, bool ALIGNED, int REPS>
+__global__ __launch_bounds__(kRowThreads) void pkv_fp8_rows_kernel(RowsArgs a) {
+  static_assert(REPS * kRowThreads * E <= kMaxWidth, "longer than any row");
   __shared__ double s_sum[kRowWaves];
   __shared__ uint32_t s_top[kRowWaves];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const char *const x = a.x + row * a.x_stride;
-  float v[kReps][E], w[NORM ? kReps : 1][E];
+  float v[REPS][E], w[NORM ? REPS : 1][E];
   double sum = 0.0;
   uint32_t top = 0;
 #pragma unroll
-  for (int r = 0; r < kReps; ++r) {
-    const int at = (r * kRowThreads + tid) * E;
-    if (at >= a.width) continue;
-    if constexpr (E == 8) {
-      fp8_load8<BF16>(x + (int64_t)at * (BF16 ? 2 : 4), v[r]);
-    } else {
-      v[r][0] = BF16 ? pkv_bf16_bits_to_f32(((const uint16_t *)x)[at]) : ((const float *)x)[at];
-    }
+  for (int r = 0; r < REPS; ++r) {
+    const int at = (r * kRowThreads + tid) * E, left = a.width - at;
+    if (left <= 0) continue;
+    const char *const from = x + (int64_t)at * (BF16 ? 2 : 4);
+    if constexpr (ALIGNED) fp8_load8<BF16>(from, v[r]);
+    else load_any<BF16>(from, left, v[r]);
     if constexpr (NORM) {
-      if constexpr (E == 8) fp8_load8<true>((const char *)(a.weight + at), w[r]);
-      else w[r][0] = pkv_bf16_bits_to_f32(a.weight[at]);
+      if constexpr (ALIGNED) fp8_load8<true>((const char *)(a.weight + at), w[r]);
+      else load_any<true>((const char *)(a.weight + at), left, w[r]);
       if (a.residual) {
-        const uint16_t *const res = a.residual + row * a.width + at;
+        const char *const res = (const char *)(a.residual + row * a.width + at);
         float add[E];
-        if constexpr (E == 8) fp8_load8<true>((const char *)res, add);
-        else add[0] = pkv_bf16_bits_to_f32(*res);
+        if constexpr (ALIGNED) fp8_load8<true>(res, add);
+        else load_any<true>(res, left, add);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[r][e] = pkv_bf16_round(v[r][e] + add[e]);
         if (a.out_sum) {
           uint16_t *const to = a.out_sum + row * a.width + at;
-          if constexpr (E == 8) {
-            pkv_u32x4 o;
+          pkv_u32x4 o;
 #pragma unroll
-            for (int p = 0; p < 4; ++p) o[p] = (__float_as_uint(v[r][2 * p]) >> 16) | (__float_as_uint(v[r][2 * p + 1]) & 0xffff0000u);
+          for (int p = 0; p < 4; ++p) o[p] = (__float_as_uint(v[r][2 * p]) >> 16) | (__float_as_uint(v[r][2 * p + 1]) & 0xffff0000u);
+          if constexpr (ALIGNED) {
             *(pkv_u32x4 *)to = o;
+          } else if (left >= E) {
+            __builtin_memcpy(to, &o, sizeof o);
           } else {
-            *to = (uint16_t)(__float_as_uint(v[r][0]) >> 16);
+#pragma unroll
+            for (int e = 0; e < E - 1; ++e)
+              if (e < left) to[e] = (uint16_t)(__float_as_uint(v[r][e]) >> 16);
           }
         }
       }
@@ -84,14 +104,14 @@ __global__ __launch_bounds__(row_threads(E)) void pkv_fp8_rows_kernel(RowsArgs a
     for (int i = 0; i < kRowWaves; ++i) sum += s_sum[i];
     const float inv = (float)(1.0 / sqrt(sum / (double)a.width + a.eps));
 #pragma unroll
-    for (int r = 0; r < kReps; ++r) {
+    for (int r = 0; r < REPS; ++r) {
       if ((r * kRowThreads + tid) * E >= a.width) continue;
 #pragma unroll
       for (int e = 0; e < E; ++e) v[r][e] = v[r][e] * inv * w[r][e];
     }
   }
 #pragma unroll
-  for (int r = 0; r < kReps; ++r) {
+  for (int r = 0; r < REPS; ++r) {
     if ((r * kRowThreads + tid) * E >= a.width) continue;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -108,20 +128,29 @@ __global__ __launch_bounds__(row_threads(E)) void pkv_fp8_rows_kernel(RowsArgs a
   const float shrink = fp8_pow2(-e2);
   uint8_t *const codes = a.codes + row * a.code_stride;
 #pragma unroll
-  for (int r = 0; r < kReps; ++r) {
+  for (int r = 0; r < REPS; ++r) {
     const int at = (r * kRowThreads + tid) * E;
     if (at >= a.width) continue;
-    if constexpr (E == 8) *(pkv_u32x2 *)(codes + at) = fp8_codes8(v[r], shrink);
-    else codes[at] = (uint8_t)fp8_codes4(v[r][0], 0.f, 0.f, 0.f, shrink);
+    *(pkv_u32x2 *)(codes + at) = fp8_codes8(v[r], shrink);  // zeros behind the row's last element: a row holds whole chunks of 128
   }
-  if (a.width + tid < a.padded) codes[a.width + tid] = 0;  // fewer than 128
+  const int pad = (a.width + E - 1) / E * E + tid * E;
+  if (pad < a.padded) *(pkv_u32x2 *)(codes + pad) = pkv_u32x2{0, 0};
   if (tid == 0) a.scales[row] = fp8_pow2(e2);
 }
 
 template <bool NORM, bool BF16>
-int launch(const RowsArgs &a, int64_t rows, bool whole, hipStream_t s) {
-  if (whole) hipLaunchKernelGGL((pkv_fp8_rows_kernel<NORM, BF16, 8>), dim3((unsigned)rows), dim3(row_threads(8)), 0, s, a);
-  else hipLaunchKernelGGL((pkv_fp8_rows_kernel<NORM, BF16, 1>), dim3((unsigned)rows), dim3(row_threads(1)), 0, s, a);
+int launch(const RowsArgs &a, int64_t rows, bool aligned, hipStream_t s) {
+#define PKV_ROWS(ALIGNED, REPS) \
+  hipLaunchKernelGGL((pkv_fp8_rows_kernel<NORM, BF16, ALIGNED, REPS>), dim3((unsigned)rows), dim3(kRowThreads), 0, s, a)
+  const bool shorter = a.width <= 2 * kRowThreads * E;
+  if (aligned) {
+    if (shorter) PKV_ROWS(true, 2);
+    else PKV_ROWS(true, 8);
+  } else {
+    if (shorter) PKV_ROWS(false, 2);
+    else PKV_ROWS(false, 8);
+  }
+#undef PKV_ROWS
   PKV_LAUNCH_CHECK("pkv_fp8_rows_kernel");
   return PKV_OK;
 }
@@ -144,8 +173,8 @@ extern "C" int pkv_add_rmsnorm_fp8(const void *x, const void *residual, const vo
   RowsArgs a;
   a.x = (const char *)x, a.residual = (const uint16_t *)residual, a.weight = (const uint16_t *)weight, a.x_stride = width * 2, a.eps = eps;
   a.width = (int)width, a.padded = (int)pkv_align_up((size_t)width, 128), a.out_sum = (uint16_t *)out_sum, a.codes = codes, a.code_stride = code_stride, a.scales = scales;
-  const bool whole = width % 8 == 0 && pkv_aligned(x, 16) && pkv_aligned(residual, 16) && pkv_aligned(weight, 16) && pkv_aligned(out_sum, 16);
-  return launch<true, true>(a, rows, whole, (hipStream_t)stream);
+  const bool aligned = width % 8 == 0 && pkv_aligned(x, 16) && pkv_aligned(residual, 16) && pkv_aligned(weight, 16) && pkv_aligned(out_sum, 16);
+  return launch<true, true>(a, rows, aligned, (hipStream_t)stream);
 }
 
 extern "C" int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t rows, int64_t width, uint8_t *codes, int64_t code_stride, float *scales,
@@ -159,7 +188,7 @@ extern "C" int pkv_fp8_rows(const void *x, int dtype, int64_t x_stride, int64_t 
   memset(&a, 0, sizeof a);
   a.x = (const char *)x, a.x_stride = x_stride * es, a.width = (int)width, a.padded = (int)pkv_align_up((size_t)width, 128);
   a.codes = codes, a.code_stride = code_stride, a.scales = scales;
-  const bool whole = width % 8 == 0 && x_stride * es % 16 == 0 && pkv_aligned(x, 16);
-  if (dtype == PKV_DTYPE_BF16) return launch<false, true>(a, rows, whole, (hipStream_t)stream);
-  return launch<false, false>(a, rows, whole, (hipStream_t)stream);
+  const bool aligned = width % 8 == 0 && x_stride * es % 16 == 0 && pkv_aligned(x, 16);
+  if (dtype == PKV_DTYPE_BF16) return launch<false, true>(a, rows, aligned, (hipStream_t)stream);
+  return launch<false, false>(a, rows, aligned, (hipStream_t)stream);
 }
