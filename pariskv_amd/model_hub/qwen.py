@@ -5,7 +5,8 @@ random-initialised Qwen3-shaped model needs, and nothing else: no checkpoint loa
 model or sampling beyond arg-max.
 
 The dense projections are plain library GEMMs (``F.linear``), or, with ``weight_bits=4``, products with 4-bit weights
-(``ops.w4_linear``, and ``ops.w4_silu_mul`` for the gated half of the feed-forward block; no counterpart in the reference, nor has
+(``ops.w4_linear``, and ``ops.w4_silu_mul`` for the gated half of the feed-forward block), or, with ``fp8=True``, with eight-bit
+weights and rows (``ops.fp8_linear``; no counterpart in the reference, nor has
 :meth:`QwenModel.draft_forward`, a step over several drafted tokens); the layer norms and the SiLU gate are torch ops; the
 per-head q/k norms and the rotary embedding of a decode token are one HIP launch (``ops.qk_norm_rope``; the torch
 forms below remain for other shapes and as the checked restatement); the attention of a decode step is
@@ -42,7 +43,7 @@ class QwenConfig:
 class QwenLayer:
     """Weights of one decoder layer (reference ``QwenLayer``, qwen.py:14-70), random-initialised."""
 
-    def __init__(self, cfg: QwenConfig, device, dtype, gen: torch.Generator, pack=None):
+    def __init__(self, cfg: QwenConfig, device, dtype, gen: torch.Generator, pack=None, gate_apart: bool = False):
         h, q, kv, inter = cfg.hidden_size, cfg.num_heads * cfg.head_dim, cfg.num_key_value_heads * cfg.head_dim, cfg.intermediate_size
 
         def w(rows, cols):  # ~ N(0, 1/cols): activations keep unit scale through the layer
@@ -53,11 +54,10 @@ class QwenLayer:
         self.bqkv = None
         self.wo = pack(w(h, q))
         gate_up = w(2 * inter, h)
-        packed = pack(gate_up[:inter])
-        if isinstance(packed, ops.W4Weight):  # two matrices to one call
-            self.gate_up_proj, self.gate_proj, self.up_proj = None, packed, pack(gate_up[inter:])
+        if gate_apart:  # two matrices to one call
+            self.gate_up_proj, self.gate_proj, self.up_proj = None, pack(gate_up[:inter]), pack(gate_up[inter:])
         else:
-            self.gate_up_proj = gate_up
+            self.gate_up_proj = pack(gate_up)
         self.down_proj = pack(w(h, inter))
         ones = lambda n: torch.ones(n, device=device, dtype=dtype)
         self.input_layernorm_weight = ones(h)
@@ -71,20 +71,24 @@ class QwenLayer:
 
 class QwenModel:
     """Random-initialised decoder with the reference's decode call structure.  ``kv_cache`` is a ``polar_cache``
-    (either variant) that already holds the prompt; :meth:`decode_forward` runs one token per sequence, :meth:`draft_forward` a tree of
+    (either variant) or an ``fp8_cache`` that already holds the prompt; :meth:`decode_forward` runs one token per sequence, :meth:`draft_forward` a tree of
     drafted ones, of which :meth:`accept_draft` keeps a path.  ``weight_bits=4``: the projections and the logits' matrix in 4-bit codes
-    with a scale and a zero to every ``weight_group`` columns (bf16 models)."""
+    with a scale and a zero to every ``weight_group`` columns; ``fp8``: in eight-bit ones with a scale a row, and so are the rows they multiply, which the
+    norms of a decoded token write as such (both for bf16 models)."""
 
     def __init__(self, cfg: QwenConfig, kv_cache, device="cuda:0", dtype=torch.bfloat16, max_positions: int = 1 << 20,
-                 seed: int = 0, weight_bits: int = 16, weight_group: int = 128):
+                 seed: int = 0, weight_bits: int = 16, weight_group: int = 128, fp8: bool = False):
         if weight_bits not in (4, 16) or (weight_bits == 4 and dtype != torch.bfloat16):
             raise ValueError("weight_bits: 16, or 4 in a bfloat16 model")
+        if fp8 and (weight_bits != 16 or dtype != torch.bfloat16):
+            raise ValueError("fp8: instead of weight_bits=4, in a bfloat16 model")
         self.cfg, self.kv_cache, self.device, self.dtype = cfg, kv_cache, torch.device(device), dtype
         self.num_layers, self.hidden_size = cfg.num_layers, cfg.hidden_size
         self.num_heads, self.num_key_value_heads, self.head_dim = cfg.num_heads, cfg.num_key_value_heads, cfg.head_dim
         gen = torch.Generator(device=self.device).manual_seed(seed)
-        pack = (lambda weight: ops.W4Weight.quantize(weight, weight_group)) if weight_bits == 4 else None
-        self.layers = [QwenLayer(cfg, self.device, dtype, gen, pack) for _ in range(cfg.num_layers)]
+        pack = ops.Fp8Weight.quantize if fp8 else (lambda weight: ops.W4Weight.quantize(weight, weight_group)) if weight_bits == 4 else None
+        self.fp8 = fp8
+        self.layers = [QwenLayer(cfg, self.device, dtype, gen, pack, gate_apart=weight_bits == 4) for _ in range(cfg.num_layers)]
         self.embed_tokens = (torch.randn(cfg.vocab_size, cfg.hidden_size, generator=gen, device=self.device,
                                          dtype=torch.float32)).to(dtype)
         self.lm_head = (torch.randn(cfg.vocab_size, cfg.hidden_size, generator=gen, device=self.device, dtype=torch.float32)
@@ -108,11 +112,15 @@ class QwenModel:
     def linear(hidden_states, weight, bias=None):
         if isinstance(weight, ops.W4Weight):
             return ops.w4_linear(hidden_states, weight, bias)
+        if isinstance(weight, ops.Fp8Weight):
+            return ops.fp8_linear(hidden_states, weight, bias)
         return F.linear(hidden_states, weight, bias)
 
     def lm(self, hidden_states):
         if isinstance(self.lm_head, ops.W4Weight):
             return ops.w4_linear(hidden_states, self.lm_head, out_dtype=torch.float32)
+        if isinstance(self.lm_head, ops.Fp8Weight):
+            return ops.fp8_linear(hidden_states, self.lm_head, out_dtype=torch.float32)
         return F.linear(hidden_states, self.lm_head).float()
 
     def layernorm(self, hidden_states, epsilon, weight):
@@ -154,9 +162,9 @@ class QwenModel:
     def mlp(self, hidden_states, layer):
         if layer.gate_up_proj is None:
             return ops.w4_linear(ops.w4_silu_mul(hidden_states, layer.gate_proj, layer.up_proj), layer.down_proj)
-        gu = F.linear(hidden_states, layer.gate_up_proj)
+        gu = self.linear(hidden_states, layer.gate_up_proj)
         inter = gu.shape[-1] // 2
-        return F.linear(F.silu(gu[..., :inter]) * gu[..., inter:], layer.down_proj)
+        return self.linear(F.silu(gu[..., :inter]) * gu[..., inter:], layer.down_proj)
 
     def decode_attention(self, query_states, key_states, value_states, layer_idx):
         return polar_decode_attn(query_states, key_states, value_states, layer_idx, self.kv_cache)
@@ -223,7 +231,7 @@ class QwenModel:
     def _fused_mlp(self, normed, layer):
         if layer.gate_up_proj is None:
             return self.mlp(normed, layer)
-        return F.linear(ops.silu_mul(F.linear(normed, layer.gate_up_proj)), layer.down_proj)
+        return self.linear(ops.silu_mul(self.linear(normed, layer.gate_up_proj)), layer.down_proj)
 
     def _fusable(self):
         return (self.dtype == torch.bfloat16 and self.head_dim == 128 and self.hidden_size % 8 == 0 and self.hidden_size <= 16384 and
@@ -241,14 +249,15 @@ class QwenModel:
             return self.lm(hidden_states)
         # One token per sequence in bf16: the same arithmetic with each residual add folded into the norm that follows
         # it (also across the layer boundary) and the MLP gate in one launch.
+        norm = ops.add_rmsnorm_fp8 if self.fp8 else ops.add_rmsnorm
         x, pending = hidden_states.contiguous(), None   # residual stream, and what is still to be added to it
         for ldx, layer in enumerate(self.layers):
-            x, normed = ops.add_rmsnorm(pending if pending is not None else x, x if pending is not None else None,
-                                        layer.input_layernorm_weight, layer.input_layernorm_variance_epsilon)
-            x, normed = ops.add_rmsnorm(self._attention_block(ldx, normed), x, layer.post_attention_layernorm_weight,
-                                        layer.post_attention_layernorm_variance_epsilon)
+            x, normed = norm(pending if pending is not None else x, x if pending is not None else None,
+                             layer.input_layernorm_weight, layer.input_layernorm_variance_epsilon)
+            x, normed = norm(self._attention_block(ldx, normed), x, layer.post_attention_layernorm_weight,
+                             layer.post_attention_layernorm_variance_epsilon)
             pending = self._fused_mlp(normed, layer)
-        _, normed = ops.add_rmsnorm(pending, x, self.norm_weight, self.norm_variance_epsilon, want_sum=False)
+        _, normed = norm(pending, x, self.norm_weight, self.norm_variance_epsilon, want_sum=False)
         return self.lm(normed)
 
     # ------------------------------------------------------------------ drafted tokens (no counterpart in the reference)
