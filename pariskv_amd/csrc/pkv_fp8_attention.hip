@@ -565,7 +565,7 @@ extern "C" int pkv_fp8_attention(const pkv_fp8_attn_args *a, void *stream) {
   bool indexed = false;
   for (int i = 0; i < a->n_segments; ++i) {
     const pkv_fp8_segment &g = a->segments[i];
-    PKV_REQUIRE(g.n_rows >= 0 && g.row0 >= 0 && g.row0 <= a->cache.capacity, "segment %d: rows out of range", i);
+    PKV_REQUIRE(g.n_rows >= 0 && g.n_rows <= PKV_FP8_MAX_ROWS && g.row0 >= 0 && g.row0 <= a->cache.capacity, "segment %d: rows out of range", i);
     if (g.n_rows == 0) continue;
     Seg &to = c.seg[c.n_segments++];
     if (g.idx) {

@@ -147,8 +147,8 @@ extern "C" int pkv_fp8_store(const pkv_fp8_kv *cache, const void *k, const void 
   PKV_REQUIRE(k && v, "pkv_fp8_store: null pointer");
   PKV_REQUIRE(dtype == PKV_DTYPE_F32 || dtype == PKV_DTYPE_BF16, "unknown dtype %d", dtype);
   PKV_REQUIRE(n_tokens > 0 && n_tokens <= cache->capacity, "pkv_fp8_store: 1..capacity tokens (got %lld)", (long long)n_tokens);
-  PKV_REQUIRE(starts || (start >= 0 && start + n_tokens <= cache->capacity), "pkv_fp8_store: rows %lld..%lld of %lld", (long long)start,
-              (long long)(start + n_tokens - 1), (long long)cache->capacity);
+  PKV_REQUIRE(starts || (start >= 0 && start <= cache->capacity - n_tokens), "pkv_fp8_store: rows %lld.. (%lld of them) of %lld",
+              (long long)start, (long long)n_tokens, (long long)cache->capacity);
   PKV_REQUIRE(pkv_aligned(k, 16) && pkv_aligned(v, 16) && pkv_aligned(starts, 4) && pkv_aligned(lengths, 4), "pkv_fp8_store: 16-byte aligned rows required");
   const int64_t es = dtype == PKV_DTYPE_BF16 ? 2 : 4;
   const int64_t strides[] = {k_stride_b, k_stride_t, k_stride_h, v_stride_b, v_stride_t, v_stride_h};

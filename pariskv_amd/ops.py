@@ -1167,6 +1167,19 @@ def w4_silu_mul(x: torch.Tensor, gate: W4Weight, up: W4Weight) -> torch.Tensor:
 
 FP8 = torch.float8_e4m3fn
 
+_this_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def _launch(at: int, entry, *args) -> None:
+    """An entry point on GPU ``at``, whose stream is among its arguments: a launch goes to the calling thread's current device."""
+    if _this_device() == at:
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(at):
+            rc = entry(*args)
+    if rc != 0:
+        _lib.check(rc)
+
 
 def _fp8_bytes(t: torch.Tensor, what: str) -> torch.Tensor:
     _need(t.dtype in (FP8, torch.uint8), f"{what}: e4m3 codes, float8_e4m3fn or their bytes")
@@ -1241,15 +1254,13 @@ class Fp8KVCache:
             v = v.clone(memory_format=torch.contiguous_format)
             vs = v.stride()
         starts = 0
-        if isinstance(start, torch.Tensor):
+        if hasattr(start, "data_ptr"):
             self._counts(start, "start")
             start, starts = 0, start.data_ptr()
         if lengths is not None:
             self._counts(lengths, "lengths")
-        rc = _lib.lib().pkv_fp8_store(self._ref, k.data_ptr(), v.data_ptr(), code, S, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], start, starts,
-                                      None if lengths is None else lengths.data_ptr(), _stream(self.k_scale))
-        if rc != 0:
-            _lib.check(rc)
+        _launch(at, _lib.lib().pkv_fp8_store, self._ref, k.data_ptr(), v.data_ptr(), code, S, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], start, starts,
+                None if lengths is None else lengths.data_ptr(), _stream(self.k_scale))
 
     def _counts(self, t, what):
         if t.dtype != torch.int32 or t.get_device() != self._at or t.shape != (self.bs,) or not t.is_contiguous():
@@ -1273,7 +1284,8 @@ class Fp8KVCache:
             if row0 < 0 or n < 0 or row0 + n > self.capacity:
                 raise RuntimeError("rows out of range")
         if out is None:
-            ok, ov = (torch.empty((bs, H, n, HEAD_DIM), dtype=dtype, device=self.device) for _ in range(2))
+            like = self.k_scale
+            ok, ov = like.new_empty((bs, H, n, HEAD_DIM), dtype=dtype), like.new_empty((bs, H, n, HEAD_DIM), dtype=dtype)
         else:
             ok, ov = out
             for t in (ok, ov):
@@ -1282,10 +1294,8 @@ class Fp8KVCache:
                     raise RuntimeError("out: [bs,Hkv,n,128] of dtype on the cache's GPU, rows contiguous and 16-byte aligned")
         if n > 0:
             so, sv = ok.stride(), ov.stride()
-            rc = _lib.lib().pkv_fp8_read(self._ref, row0, n, idx_at, idx_stride, code, ok.data_ptr(), ov.data_ptr(), so[0], so[1], so[2], sv[0], sv[1],
-                                         sv[2], _stream(self.k_scale))
-            if rc != 0:
-                _lib.check(rc)
+            _launch(self._at, _lib.lib().pkv_fp8_read, self._ref, row0, n, idx_at, idx_stride, code, ok.data_ptr(), ov.data_ptr(), so[0], so[1], so[2],
+                    sv[0], sv[1], sv[2], _stream(self.k_scale))
         return ok, ov
 
 
@@ -1357,9 +1367,7 @@ class Fp8Attention:
         ws = queries.new_empty(need, dtype=torch.uint8) if need else None
         block = _FP8_ATTN_BLOCK.pack(q.data_ptr(), code, G, T, n_seg, qs[0], qs[1], *cache._fields, *segs, keys_at, _SCALE if scale is None else scale,
                                      out.data_ptr(), ws.data_ptr() if need else 0, need)
-        rc = lib.pkv_fp8_attention(block, _stream(queries))
-        if rc != 0:
-            _lib.check(rc)
+        _launch(at, lib.pkv_fp8_attention, block, _stream(queries))
         return out
 
 
@@ -1419,9 +1427,7 @@ def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     codes = x.new_empty((n, wide), dtype=FP8)
     scales = x.new_empty(shape[:-1], dtype=torch.float32)
     if n > 0:
-        rc = _lib.lib().pkv_fp8_rows(rows.data_ptr(), code, step, n, k, codes.data_ptr(), wide, scales.data_ptr(), _stream(x))
-        if rc != 0:
-            _lib.check(rc)
+        _launch(x.get_device(), _lib.lib().pkv_fp8_rows, rows.data_ptr(), code, step, n, k, codes.data_ptr(), wide, scales.data_ptr(), _stream(x))
     return Fp8Rows(codes, scales, shape)
 
 
@@ -1447,10 +1453,8 @@ def add_rmsnorm_fp8(x: torch.Tensor, residual, weight: torch.Tensor, eps: float,
             total = torch.empty_like(x)
             sum_at = total.data_ptr()
     if rows > 0:
-        rc = _lib.lib().pkv_add_rmsnorm_fp8(x.data_ptr(), res_at, weight.data_ptr(), eps, rows, width, sum_at, codes.data_ptr(), wide,
-                                            scales.data_ptr(), _stream(x))
-        if rc != 0:
-            _lib.check(rc)
+        _launch(at, _lib.lib().pkv_add_rmsnorm_fp8, x.data_ptr(), res_at, weight.data_ptr(), eps, rows, width, sum_at, codes.data_ptr(), wide,
+                scales.data_ptr(), _stream(x))
     return total, Fp8Rows(codes, scales, shape)
 
 
@@ -1485,7 +1489,7 @@ class Fp8Weight:
         codes, scales = _fp8_bytes(codes, "codes"), scales.contiguous()
         if codes.stride(1) != 1 and k > 1 or codes.stride(0) < k:
             codes = codes.contiguous()
-        _lib.check(_lib.lib().pkv_fp8_pack(_p(codes), codes.stride(0), _p(scales), n, k, _p(packed), _stream(codes)))
+        _launch(packed.get_device(), _lib.lib().pkv_fp8_pack, _p(codes), codes.stride(0), _p(scales), n, k, _p(packed), _stream(codes))
         return cls(packed, n, k)
 
     @classmethod
@@ -1498,7 +1502,7 @@ class Fp8Weight:
     def dequantize(self) -> torch.Tensor:
         """fp32 [n,k]."""
         w = torch.empty(self.n, self.k, dtype=torch.float32, device=self.device)
-        _lib.check(_lib.lib().pkv_fp8_unpack(_p(self.packed), self.n, self.k, _p(w), _stream(w)))
+        _launch(w.get_device(), _lib.lib().pkv_fp8_unpack, _p(self.packed), self.n, self.k, _p(w), _stream(w))
         return w
 
 
@@ -1519,9 +1523,8 @@ def fp8_linear(x, weight: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dt
     m = padded.shape[0]
     y = padded.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
     if m > 0:
-        rc = _lib.lib().pkv_fp8_linear(padded.data_ptr(), padded.shape[1], x.scales.data_ptr(), m, packed.data_ptr(), n, weight.k, _p(bias), y.data_ptr(), code, _stream(packed))
-        if rc != 0:
-            _lib.check(rc)
+        _launch(packed.get_device(), _lib.lib().pkv_fp8_linear, padded.data_ptr(), padded.shape[1], x.scales.data_ptr(), m, packed.data_ptr(), n, weight.k,
+                _p(bias), y.data_ptr(), code, _stream(packed))
     return y
 
 
