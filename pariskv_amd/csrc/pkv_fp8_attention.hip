@@ -526,10 +526,11 @@ int tiles_a_wave(int dtype, int rows) { return dtype == PKV_DTYPE_BF16 && rows >
 
 // Workgroups: four to a compute unit, two where there is more than one tile of rows (two fit there at a time, and each leaves a result a row that is read
 // again).  us, 256 / 512 / 1024: 4 x 8 x 65536 keys, 4 rows 112 / 111 / 106; 1 x 8 x 16384, 64 rows 21 / 22 / 28; 1 x 8 x 32768, 256 rows 83 / 65 / 71;
-// 3 x 4 x 9001, 35 fp32 rows 20 / 18 / 22.
+// 3 x 4 x 9001, 35 fp32 rows 20 / 18 / 22.  Up to 512 keys are two steps a wave of one workgroup, which saves the join: 1 x 8 x 300 keys 7.5 us, split in
+// two 8.3 and a launch more; 600 keys 9.7 and 8.4.
 int splits_of(int64_t bh, int row_tiles, int64_t total) {
   const int64_t turn = kWaves * kStep, most = (total + turn - 1) / turn, groups = row_tiles > 1 ? 512 : 1024;
-  int64_t s = (groups + bh * row_tiles - 1) / (bh * row_tiles);
+  int64_t s = most <= 2 ? 1 : (groups + bh * row_tiles - 1) / (bh * row_tiles);
   if (s > most) s = most;
   if (s > kMaxSplits) s = kMaxSplits;
   return (int)(s < 1 ? 1 : s);

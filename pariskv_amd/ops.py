@@ -1413,9 +1413,10 @@ def _fp8_step(k: int) -> int:
     return (k + 127) & -128
 
 
-def fp8_rows(x: torch.Tensor) -> Fp8Rows:
-    """Rows x [..., k] (bf16 or fp32, of at most 10^38; k up to 16384) in eight bits, in one launch."""
-    shape, code, k = x.shape, _dt(x.dtype), x.shape[-1] if x.dim() else 0
+def _fp8_source(x: torch.Tensor):
+    """x [..., k] as (rows [n,k] whose elements lie side by side, row stride, n, k, type)."""
+    shape, code = x.shape, _dt(x.dtype)
+    k = shape[-1] if len(shape) else 0
     if not x.is_cuda or k == 0:
         raise RuntimeError("x: [..., k] on the GPU")
     rows = x if len(shape) == 2 else x.reshape(-1, k)
@@ -1423,12 +1424,18 @@ def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     if unit != 1 and k > 1 or step < 0:
         rows = rows.contiguous()
         step = k
-    n, wide = rows.shape[0], _fp8_step(k)
+    return rows, step, rows.shape[0], k, code
+
+
+def fp8_rows(x: torch.Tensor) -> Fp8Rows:
+    """Rows x [..., k] (bf16 or fp32, of at most 10^38; k up to 16384) in eight bits, in one launch."""
+    rows, step, n, k, code = _fp8_source(x)
+    wide = _fp8_step(k)
     codes = x.new_empty((n, wide), dtype=FP8)
-    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
     if n > 0:
         _launch(x.get_device(), _lib.lib().pkv_fp8_rows, rows.data_ptr(), code, step, n, k, codes.data_ptr(), wide, scales.data_ptr(), _stream(x))
-    return Fp8Rows(codes, scales, shape)
+    return Fp8Rows(codes, scales, x.shape)
 
 
 def add_rmsnorm_fp8(x: torch.Tensor, residual, weight: torch.Tensor, eps: float, want_sum: bool = True):
@@ -1509,22 +1516,31 @@ class Fp8Weight:
 def fp8_linear(x, weight: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., k] times the transpose of an eight-bit matrix, plus ``bias`` (bf16 [n]): [..., n] in ``out_dtype`` (bf16, the default, or
     fp32).  x: :class:`Fp8Rows`, or bf16 or fp32 rows, which :func:`fp8_rows` quantises first.  Sums in fp32, one rounding."""
-    if not isinstance(x, Fp8Rows):
-        x = fp8_rows(x)
-    padded, packed, n = x.padded, weight.packed, weight.n
-    if x.k != weight.k:
+    packed, n = weight.packed, weight.n
+    at = packed.get_device()
+    if isinstance(x, Fp8Rows):
+        like, m, k, step = x.padded, x.padded.shape[0], x.k, None
+        codes, wide, scales = like.data_ptr(), like.shape[1], x.scales.data_ptr()
+    else:
+        like, step, m, k, kind = _fp8_source(x)
+        wide = _fp8_step(k)
+    if k != weight.k:
         raise RuntimeError(f"x: [..., {weight.k}]")
-    if padded.get_device() != packed.get_device():
-        _one_device(packed, padded)
+    if like.get_device() != at:
+        _one_device(packed, like)
     if bias is not None:
         _one_device(packed, bias)
         _need(bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == n, "bias: contiguous bf16 [n]")
     code = _lib.DTYPE_BF16 if out_dtype is None else _dt(out_dtype)
-    m = padded.shape[0]
-    y = padded.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
+    y = like.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
     if m > 0:
-        _launch(packed.get_device(), _lib.lib().pkv_fp8_linear, padded.data_ptr(), padded.shape[1], x.scales.data_ptr(), m, packed.data_ptr(), n, weight.k,
-                _p(bias), y.data_ptr(), code, _stream(packed))
+        lib, stream = _lib.lib(), _stream(packed)
+        if step is not None:  # codes and scales, for this call alone
+            ws = like.new_empty(m * (wide + 4), dtype=torch.uint8)
+            codes = ws.data_ptr()
+            scales = codes + m * wide
+            _launch(at, lib.pkv_fp8_rows, like.data_ptr(), kind, step, m, k, codes, wide, scales, stream)
+        _launch(at, lib.pkv_fp8_linear, codes, wide, scales, m, packed.data_ptr(), n, k, _p(bias), y.data_ptr(), code, stream)
     return y
 
 
