@@ -469,7 +469,7 @@ extern "C" int pkv_fp8_linear(const uint8_t *x, int64_t x_stride, const float *x
                               void *y, int out_dtype, void *stream) {
   PKV_REQUIRE(x && x_scales && packed && y, "pkv_fp8_linear: null pointer");
   PKV_REQUIRE(out_dtype == PKV_DTYPE_F32 || out_dtype == PKV_DTYPE_BF16, "unknown dtype %d", out_dtype);
-  PKV_REQUIRE(matrix_ok(n, k) && rows > 0 && rows <= ((int64_t)1 << 22), "pkv_fp8_linear: bad shape %lld rows, %lld x %lld", (long long)rows, (long long)n, (long long)k);
+  PKV_REQUIRE(matrix_ok(n, k) && rows > 0 && rows <= ((int64_t)1 << 22) && rows * n <= ((int64_t)1 << 40), "pkv_fp8_linear: bad shape %lld rows, %lld x %lld", (long long)rows, (long long)n, (long long)k);
   PKV_REQUIRE(x_stride % 16 == 0 && x_stride >= (int64_t)chunks_of(k) * kTileCols, "pkv_fp8_linear: rows of x must be 16-byte multiples apart and hold whole chunks of 128");
   PKV_REQUIRE(pkv_aligned(x, 16) && pkv_aligned(packed, 16) && pkv_aligned(x_scales, 4) && pkv_aligned(bias, 2) && pkv_aligned(y, 16), "pkv_fp8_linear: 16-byte aligned operands required");
   LinearArgs a;

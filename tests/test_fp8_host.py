@@ -281,7 +281,7 @@ def test_rows_and_product_entry_points():
     assert rows(dtype=7) == _lib.EINVAL and rows(step=-1) == _lib.EINVAL and rows(x=B + 2, dtype=_lib.DTYPE_F32) == _lib.EINVAL
     assert norm(weight=None) == _lib.EINVAL and norm(res=B + 1) == _lib.EINVAL and norm(total=B + 1) == _lib.EINVAL and norm(weight=B + 1) == _lib.EINVAL
     linear = lambda x=B, step=256, xs=2 * B, m=3, packed=3 * B, n=20, k=200, bias=None, y=4 * B, out=_lib.DTYPE_F32: L.pkv_fp8_linear(x, step, xs, m, packed, n, k, bias, y, out, None)
-    for bad in (dict(x=None), dict(xs=None), dict(packed=None), dict(y=None), dict(out=7), dict(m=0), dict(m=(1 << 22) + 1), dict(n=0), dict(k=0), dict(k=(1 << 20) + 1, step=1 << 21), dict(n=1 << 31),
+    for bad in (dict(x=None), dict(xs=None), dict(packed=None), dict(y=None), dict(out=7), dict(m=0), dict(m=(1 << 22) + 1), dict(n=0), dict(k=0), dict(k=(1 << 20) + 1, step=1 << 21), dict(n=1 << 31), dict(m=1 << 22, n=(1 << 18) + 1),
                 dict(step=128), dict(step=264), dict(x=B + 8), dict(xs=2 * B + 2), dict(packed=3 * B + 8), dict(bias=B + 1), dict(y=4 * B + 8)):
         assert linear(**bad) == _lib.EINVAL, bad
     assert L.pkv_fp8_pack(None, 200, B, 20, 200, B, None) == _lib.EINVAL and L.pkv_fp8_pack(B, 199, B, 20, 200, B, None) == _lib.EINVAL
