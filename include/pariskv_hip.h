@@ -646,6 +646,7 @@ int pkv_fp8_read(const pkv_fp8_kv *cache, int64_t row0, int64_t n_rows, const in
  * q [bs][n_tokens][n_kv_heads*group][128], heads side by side, of `dtype` (strides in elements, 16-byte multiples); out the same,
  * contiguous.  1 <= n_tokens <= 1024, n_tokens * group <= 8192, at most PKV_FP8_MAX_ROWS keys.  fp32 sums and statistics; bf16: weights are
  * rounded to bf16 for the product with V, and the normaliser is the sum of the rounded ones; fp32: no rounding but that of fp32.
+ * Weights are kept relative to a score up to 8 (log2) below the row's largest: values times keys below 10^35.
  * ws: pkv_fp8_attention_ws_bytes(dtype, bs, n_kv_heads, group, n_tokens, keys) bytes for the partial results (0: none needed). */
 typedef struct pkv_fp8_segment {
   int64_t row0, n_rows;

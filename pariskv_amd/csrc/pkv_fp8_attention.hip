@@ -8,7 +8,8 @@
 //   scores   S^T[key][row] = K[key][dim] . Q^T[dim][row], v_mfma_f32_16x16x32_bf16: lane (n, j) has bytes 16 j .. and 64 + 16 j .. of key n of a tile
 //            of 16, and receives the scores of row n for keys 4 j .. 4 j + 3 ...
 //   output   O[row][dim] += P[row][key] . V[key][dim]: ... which is where this product wants the weights: nothing is moved.
-// bf16 queries: weights are rounded to bf16 (half a step of 2^-8 each) and the normaliser is the sum of the rounded ones.
+// bf16 queries: weights are rounded to bf16 (half a step of 2^-8 each) and the normaliser is the sum of the rounded ones; a value's scale that is no power of
+// two rounds its weight once more.
 // fp32 queries: q and the weights as sums of three bf16 numbers each, which hold their 24 bits; products with codes are exact.
 // Softmax over all keys a row sees in one pass, with a running base and sum in fp32.
 #include "pkv_attn.h"

@@ -1224,7 +1224,7 @@ class Fp8KVCache:
             _one_device(k_scale, v_scale)
         else:
             _one_device(k, v, k_scale, v_scale)
-        self.k, self.v, self.k_scale, self.v_scale = k.view(FP8), v.view(FP8), k_scale, v_scale
+        self.k, self.v, self.k_scale, self.v_scale = self._keep = k.view(FP8), v.view(FP8), k_scale, v_scale  # _keep: what the addresses below belong to
         self.bs, self.n_kv_heads, self.capacity, self.block, self.device = bs, H, capacity, block, k_scale.device
         self._kv = _lib.Fp8Kv(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), bs, H, capacity, block)
         self._ref = C.byref(self._kv)
