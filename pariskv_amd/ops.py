@@ -1285,7 +1285,7 @@ class Fp8KVCache:
                 raise RuntimeError("rows out of range")
         if out is None:
             like = self.k_scale
-            ok, ov = like.new_empty((bs, H, n, HEAD_DIM), dtype=dtype), like.new_empty((bs, H, n, HEAD_DIM), dtype=dtype)
+            ok, ov = like.new_empty(bs, H, n, HEAD_DIM, dtype=dtype), like.new_empty(bs, H, n, HEAD_DIM, dtype=dtype)
         else:
             ok, ov = out
             for t in (ok, ov):
@@ -1359,7 +1359,7 @@ class Fp8Attention:
                 raise RuntimeError("row_keys: contiguous int32 [bs,Hkv] on the GPU of the queries")
             keys_at = row_keys.data_ptr()
         if out is None:
-            out = queries.new_empty(shape)
+            out = queries.new_empty(*shape)
         elif out.shape != shape or out.dtype != dt or out.get_device() != at or not out.is_contiguous() or out.data_ptr() & 15:
             raise RuntimeError("out: contiguous, like queries")
         lib = _lib.lib()
@@ -1431,8 +1431,8 @@ def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     """Rows x [..., k] (bf16 or fp32, of at most 10^38; k up to 16384) in eight bits, in one launch."""
     rows, step, n, k, code = _fp8_source(x)
     wide = _fp8_step(k)
-    codes = x.new_empty((n, wide), dtype=FP8)
-    scales = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    codes = x.new_empty(n, wide, dtype=FP8)
+    scales = x.new_empty(*x.shape[:-1], dtype=torch.float32) if x.dim() > 1 else x.new_empty((), dtype=torch.float32)
     if n > 0:
         _launch(x.get_device(), _lib.lib().pkv_fp8_rows, rows.data_ptr(), code, step, n, k, codes.data_ptr(), wide, scales.data_ptr(), _stream(x))
     return Fp8Rows(codes, scales, x.shape)
@@ -1449,8 +1449,8 @@ def add_rmsnorm_fp8(x: torch.Tensor, residual, weight: torch.Tensor, eps: float,
     if weight.dtype != torch.bfloat16 or weight.numel() != width or not weight.is_contiguous() or weight.get_device() != at:
         raise RuntimeError("weight: contiguous bf16 [width] on the GPU of x")
     rows, wide = x.numel() // width, _fp8_step(width)
-    codes = x.new_empty((rows, wide), dtype=FP8)
-    scales = x.new_empty(shape[:-1], dtype=torch.float32)
+    codes = x.new_empty(rows, wide, dtype=FP8)
+    scales = x.new_empty(*shape[:-1], dtype=torch.float32) if len(shape) > 1 else x.new_empty((), dtype=torch.float32)
     total, res_at, sum_at = x, None, None
     if residual is not None:
         if residual.shape != shape or residual.dtype != torch.bfloat16 or not residual.is_contiguous() or residual.get_device() != at:
@@ -1532,7 +1532,7 @@ def fp8_linear(x, weight: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dt
         _one_device(packed, bias)
         _need(bias.dtype == torch.bfloat16 and bias.is_contiguous() and bias.numel() == n, "bias: contiguous bf16 [n]")
     code = _lib.DTYPE_BF16 if out_dtype is None else _dt(out_dtype)
-    y = like.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
+    y = like.new_empty(*x.shape[:-1], n, dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
     if m > 0:
         lib, stream = _lib.lib(), _stream(packed)
         if step is not None:  # codes and scales, for this call alone
