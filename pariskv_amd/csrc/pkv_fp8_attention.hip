@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr int kWaves = 4, kStep = 64, kMaxSplits = 64;
+constexpr int kWaves = 4, kStep = 64, kJoinSplits = 16, kMaxSplits = 16 * kJoinSplits;
 
 struct Seg {
   int64_t idx_stride;
@@ -487,35 +487,56 @@ __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_fp8_attention_kernel
   }
 }
 
-// One wave a query row: lane l weighs split l and holds dims 2 l, 2 l + 1 of the output.
-template <bool BF16>
-__global__ __launch_bounds__(256) void pkv_fp8_join_kernel(const float *__restrict__ ws_o, const float *__restrict__ ws_ml, void *__restrict__ out,
-                                                           int n_splits, uint32_t rows, uint32_t n_rows, uint32_t n_tokens, uint32_t group,
-                                                           uint32_t n_kv_heads) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / PKV_WAVE);
-  const int lane = pkv_lane();
-  if (at >= n_rows) return;
+// 16 splits of a query row a wave, so that all partial results are one memory round trip: WAVES of them a row, or four rows a workgroup.  Lane l weighs split l of
+// the wave and holds dims 2 l, 2 l + 1.  us with the join, 64 splits, one wave a row in four rounds / four waves: 1 x 8 x 32768 keys 19.5 / 17.5,
+// 1 x 8 x 8000 10.3 / 9.3.
+template <bool BF16, int WAVES>
+__global__ __launch_bounds__(WAVES > 4 ? WAVES * PKV_WAVE : 256) void pkv_fp8_join_kernel(const float *__restrict__ ws_o, const float *__restrict__ ws_ml,
+                                                                                          void *__restrict__ out, int n_splits, uint32_t rows, uint32_t n_rows,
+                                                                                          uint32_t n_tokens, uint32_t group, uint32_t n_kv_heads) {
+  __shared__ float s_m[WAVES], s_l[WAVES];
+  __shared__ float2 s_o[WAVES][PKV_WAVE];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / PKV_WAVE), lane = pkv_lane(), s0 = WAVES > 1 ? wave * kJoinSplits : 0;
+  const uint32_t at = WAVES > 1 ? blockIdx.x : blockIdx.x * 4 + wave;
+  if (at >= n_rows) return;  // WAVES > 1: no such workgroup
   const uint32_t bh = at / rows, row = at - bh * rows;
   const int64_t first = (int64_t)bh * n_splits * rows + row;
-  float m = -INFINITY, l = 0.f;
-  if (lane < n_splits) m = ws_ml[(first + (int64_t)lane * rows) * 2], l = ws_ml[(first + (int64_t)lane * rows) * 2 + 1];
-  const float mx = pkv_wave_max(m), base = mx == -INFINITY ? 0.f : mx;
-  const float c = __builtin_amdgcn_exp2f(m - base), all = pkv_wave_sum(l * c);
-  const float weight = all == 0.f ? 0.f : c / all;
-  float x = 0.f, y = 0.f;
   const float *const parts = ws_o + first * 128;
-  for (int s = 0; s < n_splits; s += 16) {
-    float2 o[16];
+  float2 o[kJoinSplits];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)  // past the last split: the last again, as zeros
-      o[i] = *(const float2 *)(parts + (int64_t)(s + i < n_splits ? s + i : n_splits - 1) * rows * 128 + 2 * lane);
+  for (int i = 0; i < kJoinSplits; ++i)  // past the last split: the last again, as zeros
+    o[i] = *(const float2 *)(parts + (int64_t)(s0 + i < n_splits ? s0 + i : n_splits - 1) * rows * 128 + 2 * lane);
+  float m = -INFINITY, l = 0.f;
+  if (lane < kJoinSplits && s0 + lane < n_splits) {
+    const float2 ml = *(const float2 *)(ws_ml + (first + (int64_t)(s0 + lane) * rows) * 2);
+    m = ml.x, l = ml.y;
+  }
+  float mx = pkv_wave_max(m);
+  const float c = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.f : mx));
+  float all = pkv_wave_sum(l * c), x = 0.f, y = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), s + i));
-      const bool in = s + i < n_splits;
-      x = fmaf(in ? o[i].x : 0.f, f, x), y = fmaf(in ? o[i].y : 0.f, f, y);
+  for (int i = 0; i < kJoinSplits; ++i) {
+    const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), i));
+    const bool in = s0 + i < n_splits;
+    x = fmaf(in ? o[i].x : 0.f, f, x), y = fmaf(in ? o[i].y : 0.f, f, y);
+  }
+  if constexpr (WAVES > 1) {
+    s_o[wave][lane] = float2{x, y};
+    if (lane == 0) s_m[wave] = mx, s_l[wave] = all;
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) mx = fmaxf(mx, s_m[w]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    all = x = y = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const float f = __builtin_amdgcn_exp2f(s_m[w] - base);
+      all = fmaf(s_l[w], f, all), x = fmaf(s_o[w][lane].x, f, x), y = fmaf(s_o[w][lane].y, f, y);
     }
   }
+  const float share = all == 0.f ? 0.f : 1.0f / all;  // 0: nothing seen
+  x *= share, y *= share;
   const uint32_t b = bh / n_kv_heads, h = bh - b * n_kv_heads, u = row / group;
   const int64_t to = (((int64_t)b * n_tokens + u) * n_kv_heads * group + h * group + (row - u * group)) * 128 + 2 * lane;
   if constexpr (BF16) *(uint32_t *)((uint16_t *)out + to) = bf16x2(x, y);
@@ -528,12 +549,15 @@ int tiles_a_wave(int dtype, int rows) { return dtype == PKV_DTYPE_BF16 && rows >
 // Workgroups: four to a compute unit, two where there is more than one tile of rows (two fit there at a time, and each leaves a result a row that is read
 // again).  us, 256 / 512 / 1024: 4 x 8 x 65536 keys, 4 rows 112 / 111 / 106; 1 x 8 x 16384, 64 rows 21 / 22 / 28; 1 x 8 x 32768, 256 rows 83 / 65 / 71;
 // 3 x 4 x 9001, 35 fp32 rows 20 / 18 / 22.  Up to 512 keys are two steps a wave of one workgroup, which saves the join: 1 x 8 x 300 keys 7.5 us, split in
-// two 8.3 and a launch more; 600 keys 9.7 and 8.4.
+// two 8.3 and a launch more; 600 keys 9.7 and 8.4.  At most 64 a row tile, or a workgroup to a compute unit if that is more: 1 x 8 x 32768 keys, 64 splits
+// 17.3, 128 21.9; 1 x 1 x 65536 keys 14.8, 256 splits 11.8.
 int splits_of(int64_t bh, int row_tiles, int64_t total) {
   const int64_t turn = kWaves * kStep, most = (total + turn - 1) / turn, groups = row_tiles > 1 ? 512 : 1024;
   int64_t s = most <= 2 ? 1 : (groups + bh * row_tiles - 1) / (bh * row_tiles);
   if (s > most) s = most;
-  if (s > kMaxSplits) s = kMaxSplits;
+  int64_t cap = kMaxSplits / (bh * row_tiles);  // kMaxSplits: a workgroup to each compute unit
+  if (cap < 64) cap = 64;
+  if (s > cap) s = cap;
   return (int)(s < 1 ? 1 : s);
 }
 
@@ -612,11 +636,19 @@ extern "C" int pkv_fp8_attention(const pkv_fp8_attn_args *a, void *stream) {
 #undef PKV_FP8_ATTENTION
   PKV_LAUNCH_CHECK("pkv_fp8_attention_kernel");
   if (c.n_splits == 1) return PKV_OK;
-  const dim3 join((unsigned)((n_rows + 3) / 4));
-  if (bf) hipLaunchKernelGGL(pkv_fp8_join_kernel<true>, join, dim3(256), 0, s, c.ws_o, c.ws_ml, c.out, c.n_splits, (uint32_t)rows, (uint32_t)n_rows,
-                             (uint32_t)c.n_tokens, (uint32_t)c.group, (uint32_t)H);
-  else hipLaunchKernelGGL(pkv_fp8_join_kernel<false>, join, dim3(256), 0, s, c.ws_o, c.ws_ml, c.out, c.n_splits, (uint32_t)rows, (uint32_t)n_rows,
-                          (uint32_t)c.n_tokens, (uint32_t)c.group, (uint32_t)H);
+#define PKV_FP8_JOIN(BF16, WAVES)                                                                                                                    \
+  hipLaunchKernelGGL((pkv_fp8_join_kernel<BF16, WAVES>), dim3((unsigned)(WAVES > 1 ? n_rows : (n_rows + 3) / 4)), dim3(WAVES > 4 ? WAVES * PKV_WAVE : 256), 0, s, \
+                     c.ws_o, c.ws_ml, c.out, c.n_splits, (uint32_t)rows, (uint32_t)n_rows, (uint32_t)c.n_tokens, (uint32_t)c.group, (uint32_t)H)
+  if (bf) {
+    if (c.n_splits <= kJoinSplits) PKV_FP8_JOIN(true, 1);
+    else if (c.n_splits <= 4 * kJoinSplits) PKV_FP8_JOIN(true, 4);
+    else PKV_FP8_JOIN(true, 16);
+  } else {
+    if (c.n_splits <= kJoinSplits) PKV_FP8_JOIN(false, 1);
+    else if (c.n_splits <= 4 * kJoinSplits) PKV_FP8_JOIN(false, 4);
+    else PKV_FP8_JOIN(false, 16);
+  }
+#undef PKV_FP8_JOIN
   PKV_LAUNCH_CHECK("pkv_fp8_join_kernel");
   return PKV_OK;
 }

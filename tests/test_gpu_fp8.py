@@ -457,6 +457,20 @@ def test_attention_layouts_streams_graph():
         check_attention(graphs[0][1][0], q1, want, [(0, cap)], keys.cpu())
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,H", [(4300, 1), (17000, 1), (33000, 2), (66000, 1)])
+def test_attention_many_splits(rows, H, dtype):
+    """Few heads and long rows: results joined from up to 256 parts, of which those past the row's last key have seen nothing."""
+    ops, g = _ops(), _gen(rows)
+    cache, want = _filled(ops, g, 1, H, -(-rows // 128) * 128, 128, spread=0.3)
+    q = torch.randn(1, 2, H * 3, D, generator=g).to(dtype)
+    check_attention(run_attention(ops, q, cache, [(0, rows)]), q, want, [(0, rows)])
+    for n in (0, 1, 700, rows // 2):
+        rk = torch.full((1, H), n, dtype=torch.int32)
+        rk[0, -1] -= n % 2
+        check_attention(run_attention(ops, q, cache, [(0, rows)], row_keys=rk), q, want, [(0, rows)], row_keys=rk)
+
+
 def test_attention_far_rows():
     """Offsets past 2^32 bytes: a head's rows take 2 GiB."""
     ops, g = _ops(), _gen(12)
