@@ -8,8 +8,8 @@
 //   scores   S^T[key][row] = K[key][dim] . Q^T[dim][row], v_mfma_f32_16x16x32_bf16: lane (n, j) has bytes 16 j .. and 64 + 16 j .. of key n of a tile
 //            of 16, and receives the scores of row n for keys 4 j .. 4 j + 3 ...
 //   output   O[row][dim] += P[row][key] . V[key][dim]: ... which is where this product wants the weights: nothing is moved.
-// bf16 queries: weights are rounded to bf16 (half a step of 2^-8 each) and the normaliser is the sum of the rounded ones; a value's scale that is no power of
-// two rounds its weight once more.
+// bf16 queries: weights are rounded to bf16 (half a step, 2^-8 of themselves), times their values' scales for the product and as they are for the normaliser: the same
+// ones where scales are powers of two.
 // fp32 queries: q and the weights as sums of three bf16 numbers each, which hold their 24 bits; products with codes are exact.
 // Softmax over all keys a row sees in one pass, with a running base and sum in fp32.
 #include "pkv_attn.h"
@@ -71,21 +71,24 @@ __device__ __forceinline__ void split_off(float (&x)[8], pkv_u32x4 &part) {
   }
 }
 
-// Scores (times log2 e) into weights of the keys in `bits` (MASKED; else of all); p stays as numbers, for bf16 rounded.
+// Products of q and codes, times kx (a key's scale, and scale log2 e), into weights of the keys in `bits` (MASKED; else of all).
 template <bool MASKED, int PARTS>
-__device__ __forceinline__ void weights(Tile<PARTS> &w, const float (&s)[8], uint32_t bits, float (&p)[8]) {
+__device__ __forceinline__ void weights(Tile<PARTS> &w, const float (&s)[8], const float (&kx)[8], uint32_t bits, float (&p)[8]) {
   const int j = pkv_lane() >> 4;
-  float x[8], top = -INFINITY;
+  float x[8], top = -INFINITY;  // scores above use
+  auto above = [&] {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    x[e] = !MASKED || ((bits >> e) & 1u) ? s[e] : -INFINITY;
-    top = fmaxf(top, x[e]);
-  }
-  if (__any(top - w.use > w.lim)) {
+    for (int e = 0; e < 8; ++e) x[e] = !MASKED || ((bits >> e) & 1u) ? fmaf(s[e], kx[e], -w.use) : -INFINITY;
+  };
+  above();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+  if (__any(top > w.lim)) {
     top = pkv_pair_max<32>(pkv_pair_max<16>(top));
-    const bool fresh = w.lim < 0.f, moves = top > -INFINITY && (fresh || top > w.use);
-    const float next = moves ? top : w.use, corr = fresh ? 0.f : __builtin_amdgcn_exp2f(w.use - next);
+    const bool fresh = w.lim < 0.f, moves = top > -INFINITY && (fresh || top > 0.f);
+    const float next = moves ? w.use + top : w.use, corr = fresh ? 0.f : __builtin_amdgcn_exp2f(w.use - next);
     w.use = next, w.lim = moves ? 8.f : w.lim;
+    above();
     float cr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) cr[i] = __shfl(corr, 4 * j + i, PKV_WAVE);
@@ -101,15 +104,12 @@ __device__ __forceinline__ void weights(Tile<PARTS> &w, const float (&s)[8], uin
     }
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - w.use);
+  for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e]);
   if constexpr (PARTS == 1) {
     const pkv_u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
     pkv_u32x4 a;
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      a[d] = bf16x2(p[2 * d], p[2 * d + 1]);
-      p[2 * d] = __uint_as_float(a[d] << 16), p[2 * d + 1] = __uint_as_float(a[d] & 0xffff0000u);
-    }
+    for (int d = 0; d < 4; ++d) a[d] = bf16x2(p[2 * d], p[2 * d + 1]);
     w.l = mfma_bf16(a, ones, w.l);
   } else {
 #pragma unroll
@@ -184,8 +184,8 @@ __device__ __forceinline__ void half_step(Tile<PARTS> (&w)[NT], Half &x, const f
     }
     float s[8], p[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[e] = (e < 4 ? s0[t][e & 3] : s1[t][e & 3]) * kx[e];
-    weights<MASKED, PARTS>(w[t], s, bits[t], p);
+    for (int e = 0; e < 8; ++e) s[e] = e < 4 ? s0[t][e & 3] : s1[t][e & 3];
+    weights<MASKED, PARTS>(w[t], s, kx, bits[t], p);
 #pragma unroll
     for (int e = 0; e < 8; ++e) p[e] *= MASKED && !((bits[t] >> e) & 1u) ? 0.f : vx[e];
     if constexpr (PARTS == 1) {
@@ -546,16 +546,22 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * PKV_WAVE : 256) void pkv_fp8_jo
 // Row tiles of 16 a wave.
 int tiles_a_wave(int dtype, int rows) { return dtype == PKV_DTYPE_BF16 && rows > 16 ? 2 : 1; }
 
-// Workgroups: four to a compute unit, two where there is more than one tile of rows (two fit there at a time, and each leaves a result a row that is read
-// again).  us, 256 / 512 / 1024: 4 x 8 x 65536 keys, 4 rows 112 / 111 / 106; 1 x 8 x 16384, 64 rows 21 / 22 / 28; 1 x 8 x 32768, 256 rows 83 / 65 / 71;
-// 3 x 4 x 9001, 35 fp32 rows 20 / 18 / 22.  Up to 512 keys are two steps a wave of one workgroup, which saves the join: 1 x 8 x 300 keys 7.5 us, split in
-// two 8.3 and a launch more; 600 keys 9.7 and 8.4.  At most 64 a row tile, or a workgroup to a compute unit if that is more: 1 x 8 x 32768 keys, 64 splits
-// 17.3, 128 21.9; 1 x 1 x 65536 keys 14.8, 256 splits 11.8.
-int splits_of(int64_t bh, int row_tiles, int64_t total) {
-  const int64_t turn = kWaves * kStep, most = (total + turn - 1) / turn, groups = row_tiles > 1 ? 512 : 1024;
-  int64_t s = most <= 2 ? 1 : (groups + bh * row_tiles - 1) / (bh * row_tiles);
+// Workgroups: two to a compute unit, as many as fit there at a time, for bf16 and not one more: a second round starts anew for what is left.  us, up to 512 of
+// them / rounded up / up to 1024: 3 x 8 x 20000 keys, 32 rows 35.2 / 42.7 / 42.2; 3 x 7 x 9000, 20 rows 20.4 / 22.6 / 23.6; 1 x 8 x 32768, 256 rows 65 / 65 / 71.
+// Four where a wave of one row tile has sixteen steps or more, and the rounds even out what memory does: 4 x 8 x 65536 keys, 4 rows 110 / 110 / 105;
+// 7 x 8 x 30000 (fewer) 84.4 / 90 / 84.6.  fp32, whose steps are longer, rounds up: 3 x 4 x 9001, 35 rows 17.5, not so 19.1 (but 3 x 3 x 20000, 24 rows 23.2 and 21.3);
+// one row tile up to 1024, 4 x 2 x 20000 19.1.
+// Up to 512 keys are two steps a wave of one workgroup, which saves the join: 1 x 8 x 300 keys 7.5 us, split in two 8.3 and a launch more; 600 keys 9.7 and
+// 8.4.  At most 64 a row tile, or a workgroup to a compute unit if that is more: 1 x 8 x 32768 keys, 64 splits 17.3, 128 21.9; 1 x 1 x 65536 keys 14.8,
+// 256 splits 11.8.
+int splits_of(int dtype, int64_t bh, int row_tiles, int64_t total) {
+  const int64_t turn = kWaves * kStep, most = (total + turn - 1) / turn, tiles = bh * row_tiles;
+  int64_t s;
+  if (most <= 2) s = 1;
+  else if (dtype == PKV_DTYPE_BF16) s = row_tiles == 1 && tiles <= 512 && most >= 16 * (512 / tiles) ? 1024 / tiles : 512 / tiles;
+  else s = ((row_tiles > 1 ? 512 : 1024) + tiles - 1) / tiles;
   if (s > most) s = most;
-  int64_t cap = kMaxSplits / (bh * row_tiles);  // kMaxSplits: a workgroup to each compute unit
+  int64_t cap = kMaxSplits / tiles;  // kMaxSplits: a workgroup to each compute unit
   if (cap < 64) cap = 64;
   if (s > cap) s = cap;
   return (int)(s < 1 ? 1 : s);
@@ -569,7 +575,7 @@ bool shape_ok(int bs, int n_kv_heads, int group, int n_tokens) {
 
 extern "C" size_t pkv_fp8_attention_ws_bytes(int dtype, int bs, int n_kv_heads, int group, int n_tokens, int64_t total_keys) {
   if (!shape_ok(bs, n_kv_heads, group, n_tokens) || total_keys < 0) return 0;
-  const int rows = n_tokens * group, per = 16 * tiles_a_wave(dtype, rows), s = splits_of((int64_t)bs * n_kv_heads, (rows + per - 1) / per, total_keys);
+  const int rows = n_tokens * group, per = 16 * tiles_a_wave(dtype, rows), s = splits_of(dtype, (int64_t)bs * n_kv_heads, (rows + per - 1) / per, total_keys);
   return s == 1 ? 0 : (size_t)bs * n_kv_heads * s * rows * 130 * sizeof(float);
 }
 
@@ -610,7 +616,7 @@ extern "C" int pkv_fp8_attention(const pkv_fp8_attn_args *a, void *stream) {
   if (c.n_segments) c.seg[c.n_segments - 1].end = 0xffffffffu;
   const int rows = a->n_tokens * a->group, nt = tiles_a_wave(a->dtype, rows), row_tiles = (rows + 16 * nt - 1) / (16 * nt);
   const int64_t bh = (int64_t)bs * H, n_rows = bh * rows;
-  c.n_splits = splits_of(bh, row_tiles, total), c.n_pairs = (int)(bh * c.n_splits);
+  c.n_splits = splits_of(a->dtype, bh, row_tiles, total), c.n_pairs = (int)(bh * c.n_splits);
   const size_t need = c.n_splits == 1 ? 0 : (size_t)n_rows * c.n_splits * 130 * sizeof(float);
   if (need && (!a->ws || a->ws_bytes < need || !pkv_aligned(a->ws, 16))) {
     pkv_set_error("pkv_fp8_attention: workspace of %zu bytes required, got %zu", need, a->ws ? a->ws_bytes : (size_t)0);
