@@ -551,16 +551,21 @@ int tiles_a_wave(int dtype, int rows) { return dtype == PKV_DTYPE_BF16 && rows >
 // Four where a wave of one row tile has sixteen steps or more, and the rounds even out what memory does: 4 x 8 x 65536 keys, 4 rows 110 / 110 / 105;
 // 7 x 8 x 30000 (fewer) 84.4 / 90 / 84.6.  fp32, whose steps are longer, rounds up: 3 x 4 x 9001, 35 rows 17.5, not so 19.1 (but 3 x 3 x 20000, 24 rows 23.2 and 21.3);
 // one row tile up to 1024, 4 x 2 x 20000 19.1.
+// Two row tiles a wave: two steps at least where that leaves each compute unit a workgroup, since a workgroup's 32 rows of results cost as much as a step:
+// 4 x 8 x 4096 keys, 32 rows 17.6, one step 20.3; 4 x 8 x 1000 (128 of them) 14.3 and 12.0.
 // Up to 512 keys are two steps a wave of one workgroup, which saves the join: 1 x 8 x 300 keys 7.5 us, split in two 8.3 and a launch more; 600 keys 9.7 and
 // 8.4.  At most 64 a row tile, or a workgroup to a compute unit if that is more: 1 x 8 x 32768 keys, 64 splits 17.3, 128 21.9; 1 x 1 x 65536 keys 14.8,
 // 256 splits 11.8.
-int splits_of(int dtype, int64_t bh, int row_tiles, int64_t total) {
+int splits_of(int dtype, int64_t bh, int rows, int64_t total) {
+  const int nt = tiles_a_wave(dtype, rows), row_tiles = (rows + 16 * nt - 1) / (16 * nt);
   const int64_t turn = kWaves * kStep, most = (total + turn - 1) / turn, tiles = bh * row_tiles;
   int64_t s;
   if (most <= 2) s = 1;
   else if (dtype == PKV_DTYPE_BF16) s = row_tiles == 1 && tiles <= 512 && most >= 16 * (512 / tiles) ? 1024 / tiles : 512 / tiles;
   else s = ((row_tiles > 1 ? 512 : 1024) + tiles - 1) / tiles;
   if (s > most) s = most;
+  const int64_t two = (most + 1) / 2 > 256 / tiles ? (most + 1) / 2 : 256 / tiles;
+  if (nt > 1 && s > two) s = two;
   int64_t cap = kMaxSplits / tiles;  // kMaxSplits: a workgroup to each compute unit
   if (cap < 64) cap = 64;
   if (s > cap) s = cap;
@@ -575,7 +580,7 @@ bool shape_ok(int bs, int n_kv_heads, int group, int n_tokens) {
 
 extern "C" size_t pkv_fp8_attention_ws_bytes(int dtype, int bs, int n_kv_heads, int group, int n_tokens, int64_t total_keys) {
   if (!shape_ok(bs, n_kv_heads, group, n_tokens) || total_keys < 0) return 0;
-  const int rows = n_tokens * group, per = 16 * tiles_a_wave(dtype, rows), s = splits_of(dtype, (int64_t)bs * n_kv_heads, (rows + per - 1) / per, total_keys);
+  const int rows = n_tokens * group, s = splits_of(dtype, (int64_t)bs * n_kv_heads, rows, total_keys);
   return s == 1 ? 0 : (size_t)bs * n_kv_heads * s * rows * 130 * sizeof(float);
 }
 
@@ -616,7 +621,7 @@ extern "C" int pkv_fp8_attention(const pkv_fp8_attn_args *a, void *stream) {
   if (c.n_segments) c.seg[c.n_segments - 1].end = 0xffffffffu;
   const int rows = a->n_tokens * a->group, nt = tiles_a_wave(a->dtype, rows), row_tiles = (rows + 16 * nt - 1) / (16 * nt);
   const int64_t bh = (int64_t)bs * H, n_rows = bh * rows;
-  c.n_splits = splits_of(a->dtype, bh, row_tiles, total), c.n_pairs = (int)(bh * c.n_splits);
+  c.n_splits = splits_of(a->dtype, bh, rows, total), c.n_pairs = (int)(bh * c.n_splits);
   const size_t need = c.n_splits == 1 ? 0 : (size_t)n_rows * c.n_splits * 130 * sizeof(float);
   if (need && (!a->ws || a->ws_bytes < need || !pkv_aligned(a->ws, 16))) {
     pkv_set_error("pkv_fp8_attention: workspace of %zu bytes required, got %zu", need, a->ws ? a->ws_bytes : (size_t)0);
