@@ -71,6 +71,9 @@ struct LinearArgs {
   void *y;
   int64_t m, n;
   int chunks, f32;
+  float *part;         // splits > 1: sums of each split's columns, [split][m][part_n], part_n = n rounded up to 4
+  int64_t part_n;
+  int splits;
 };
 
 // Columns col .. col + 3 of a row of y, col a multiple of four.  WHOLE: rows of y are whole vectors.  The flags are chosen once for all of a
@@ -187,21 +190,24 @@ __global__ __launch_bounds__(kStreamWaves * PKV_WAVE) void pkv_fp8_stream_kernel
   });
 }
 
-// Many rows: 64 TM rows of x by 64 TN of the matrix a workgroup, a quarter of them a wave, a chunk of columns at a time, straight from memory to
+// Many rows: 64 TM rows of x by 64 TN of the matrix a workgroup, a quarter of them a wave, a chunk of columns at a time (of its split's), straight from memory to
 // LDS.  Of x a load takes 8 rows x 128 columns, whole lines: 64 bytes of each of 16 rows, all in the same half of their lines, come at half the rate
 // (16 KB 0.7 us a compute unit; 0.4).  Vector v of row r lies at v ^ (r mod 8) of the row, so that rows of an operand are on different banks.
 typedef const __attribute__((address_space(1))) void *fp8_global;
 typedef __attribute__((address_space(3))) void *fp8_lds;
 // A wave's results, rows m0 .., columns n0 .. of y, 32 rows at a time through a part of LDS of its own and out as whole rows of it: 16 bytes of each of
 // 32 rows, as they lie in the registers, would take 20 us of 256 x 256 where rows of y are a multiple of 4096 bytes.
-template <int TM, int TN, bool F32>
+// RAW: as sums, to a split's part.
+template <int TM, int TN, bool F32, bool RAW>
 __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x16 (&acc)[TN][TM], uint8_t *lds, int64_t m0, int64_t n0) {
   constexpr int kEs = F32 ? 4 : 2, kRow = 32 * TN * kEs, kStep = kRow + 16, kVecs = kRow / 16, kRows = PKV_WAVE / kVecs;
   static_assert(4 * 32 * kStep <= 2 * 4 * (TM + TN) * kTileBytes, "room for it");
   const int lane = pkv_lane(), wave = threadIdx.x / PKV_WAVE, row = lane & 31;
   uint8_t *const mine = lds + wave * (32 * kStep);
-  const int64_t left = a.n - n0;
-  const bool whole = a.n % (16 / kEs) == 0;
+  static_assert(F32 || !RAW, "sums are fp32");
+  const int64_t n = RAW ? a.part_n : a.n, left = n - n0;  // RAW: past the matrix's last row its last tile has zeros
+  const bool whole = n % (16 / kEs) == 0;
+  char *const y = RAW ? (char *)(a.part + blockIdx.y * a.m * n) : (char *)a.y;
   const int vec = lane % kVecs, col = vec * (16 / kEs);
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
@@ -215,8 +221,8 @@ __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x1
         const fp8_f32x4 sw = *(const fp8_f32x4 *)(a.sw + (in ? n0 + c : 0));  // there are scales up to the next multiple of 16
         fp8_f32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = acc[r][t][4 * q + i] * sx * sw[i];
-        if (a.bias) {
+        for (int i = 0; i < 4; ++i) v[i] = RAW ? acc[r][t][4 * q + i] : acc[r][t][4 * q + i] * sx * sw[i];
+        if (!RAW && a.bias) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] += pkv_bf16_bits_to_f32(a.bias[c + i < left ? n0 + c + i : 0]);
         }
@@ -231,7 +237,7 @@ __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x1
       const int64_t at = m0 + 32 * t + r0;
       const pkv_u32x4 v = *(const pkv_u32x4 *)(mine + r0 * kStep + vec * 16);
       if (at >= a.m || col >= left) continue;
-      char *const to = (char *)a.y + (at * a.n + n0 + col) * kEs;
+      char *const to = y + (at * n + n0 + col) * kEs;
       if (whole) *(pkv_u32x4 *)to = v;
       else
 #pragma unroll
@@ -258,18 +264,18 @@ __global__ __launch_bounds__(256, TM * TN > 4 ? 1 : 2) void pkv_fp8_block_kernel
   const int group = id / (kGroup * n_blocks), in = id - group * kGroup * n_blocks, here = m_blocks - group * kGroup < kGroup ? m_blocks - group * kGroup : kGroup;
   const int mb = group * kGroup + in % here, nb = in / here;
   const int64_t tiles = (a.n + kTileRows - 1) / kTileRows, m0 = (int64_t)mb * (64 * TM), t0 = (int64_t)nb * (4 * TN);
-  const int wm = wave & 1, wn = wave >> 1;
+  const int wm = wave & 1, wn = wave >> 1, c0 = (int)blockIdx.y * a.chunks / a.splits, last = ((int)blockIdx.y + 1) * a.chunks / a.splits - c0 - 1;
   // what this wave brings in: 8 rows each of x, half tiles of the matrix
   const uint8_t *x_from[2 * TM], *w_from[TN];
 #pragma unroll
   for (int u = 0; u < 2 * TM; ++u) {
     const int64_t row = m0 + (wave * 2 * TM + u) * 8 + (lane >> 3);
-    x_from[u] = a.x + (row < a.m ? row : a.m - 1) * a.x_stride + 16 * ((lane & 7) ^ (lane >> 3));
+    x_from[u] = a.x + (row < a.m ? row : a.m - 1) * a.x_stride + c0 * kTileCols + 16 * ((lane & 7) ^ (lane >> 3));
   }
 #pragma unroll
   for (int u = 0; u < TN; ++u) {
     const int64_t tile = t0 + wave * TN + u;
-    w_from[u] = a.tiles + (tile < tiles ? tile : tiles - 1) * a.chunks * kTileBytes + lane * 16;
+    w_from[u] = a.tiles + ((tile < tiles ? tile : tiles - 1) * a.chunks + c0) * kTileBytes + lane * 16;
   }
   auto fetch = [&](int c, int buffer) {
     uint8_t *const to = lds + buffer * kBuffer;
@@ -332,7 +338,6 @@ __global__ __launch_bounds__(256, TM * TN > 4 ? 1 : 2) void pkv_fp8_block_kernel
   };
   // Operands of the next half chunk are read while this one's are multiplied; a chunk is asked for when the one DEPTH before it has been
   // read, half a chunk before its end.
-  const int last = a.chunks - 1;
   Codes x[2][TM], w[2][TN];
 #pragma unroll
   for (int c = 0; c < DEPTH; ++c) fetch(c < last ? c : last, c);  // past the last: read again, not used
@@ -356,8 +361,20 @@ __global__ __launch_bounds__(256, TM * TN > 4 ? 1 : 2) void pkv_fp8_block_kernel
   }
   fp8_wait<0>();  // nothing may be on its way to LDS that another workgroup gets
   __builtin_amdgcn_s_barrier();
-  if (a.f32) block_store<TM, TN, true>(a, acc, lds, m0 + TM * wm * 32, t0 * 16 + TN * wn * 32);
-  else block_store<TM, TN, false>(a, acc, lds, m0 + TM * wm * 32, t0 * 16 + TN * wn * 32);
+  if (a.splits > 1) block_store<TM, TN, true, true>(a, acc, lds, m0 + TM * wm * 32, t0 * 16 + TN * wn * 32);
+  else if (a.f32) block_store<TM, TN, true, false>(a, acc, lds, m0 + TM * wm * 32, t0 * 16 + TN * wn * 32);
+  else block_store<TM, TN, false, false>(a, acc, lds, m0 + TM * wm * 32, t0 * 16 + TN * wn * 32);
+}
+
+// The splits' sums, in their order: four columns a thread.
+__global__ __launch_bounds__(256) void pkv_fp8_sum_kernel(LinearArgs a) {
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x, across = (uint32_t)a.part_n / 4, row = at / across, col = 4 * (at - row * across);
+  if (row >= a.m) return;
+  const float *const from = a.part + (int64_t)row * a.part_n + col;
+  fp8_f32x4 sum = *(const fp8_f32x4 *)from;
+#pragma unroll 4
+  for (int i = 1; i < a.splits; ++i) sum += *(const fp8_f32x4 *)(from + i * a.m * a.part_n);
+  with_put4(a, [&](auto put) { put(row, col, sum, a.sx[row]); });
 }
 
 template <int MT, int RT>
@@ -371,8 +388,12 @@ int launch_block_as(const LinearArgs &a, hipStream_t s) {
   const int mb = (int)((a.m + 64 * TM - 1) / (64 * TM)), nb = (int)((a.n + 64 * TN - 1) / (64 * TN));
   const int lds = DEPTH * 4 * (TM + TN) * kTileBytes;
   PKV_HIP(hipFuncSetAttribute((const void *)pkv_fp8_block_kernel<TM, TN, DEPTH, E4M3>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  hipLaunchKernelGGL((pkv_fp8_block_kernel<TM, TN, DEPTH, E4M3>), dim3((unsigned)((mb * (int64_t)nb + 7) / 8 * 8)), dim3(256), lds, s, a, mb, nb);
+  hipLaunchKernelGGL((pkv_fp8_block_kernel<TM, TN, DEPTH, E4M3>), dim3((unsigned)((mb * (int64_t)nb + 7) / 8 * 8), (unsigned)a.splits), dim3(256), lds, s, a, mb, nb);
   PKV_LAUNCH_CHECK("pkv_fp8_block_kernel");
+  if (a.splits > 1) {
+    hipLaunchKernelGGL(pkv_fp8_sum_kernel, dim3((unsigned)((a.m * (a.part_n / 4) + 255) / 256)), dim3(256), 0, s, a);
+    PKV_LAUNCH_CHECK("pkv_fp8_sum_kernel");
+  }
   return PKV_OK;
 }
 template <int TM, int TN, int DEPTH>
@@ -380,28 +401,53 @@ int launch_block(const LinearArgs &a, hipStream_t s) {
   return a.f32 ? launch_block_as<TM, TN, DEPTH, false>(a, s) : launch_block_as<TM, TN, DEPTH, true>(a, s);
 }
 
+int64_t row_tiles(int64_t n) { return (n + kTileRows - 1) / kTileRows; }
+int chunks_of(int64_t k) { return (int)((k + kTileCols - 1) / kTileCols); }
+size_t tile_bytes(int64_t n, int64_t k) { return (size_t)row_tiles(n) * chunks_of(k) * kTileBytes; }
+
 // What a workgroup takes: 16 MT rows of x by 16 RT of the matrix (stream), 64 TM by 64 TN (block).
 enum Shape { kStream11, kStream12, kStream14, kStream22, kStream24, kBlock11, kBlock12, kBlock21, kBlock22, kBlock22Two };
 
-// A compute unit takes about 50 KB a microsecond of what its workgroups read, whatever the shape, so a shape costs the rows of x and of the matrix
-// that a workgroup reads, times the workgroups a compute unit gets, at least one; blocks 0.85 of that (their loads of x are whole lines).  us,
-// rows x (n x k), 32x64 stream / 64x64 stream / 64x64 block / 128x128 block: 128 x (4096 x 4096) 10.5 / 17.7 / 12.1 / 22; 256 x same 18.6 / 17.7 /
-// 12.3 / 22; 64 x (28672 x 4096) 42 / 37 / 26.5 / 27, 64x128 block 25; 256 x same 152 / 129 / 61 / 44; 1 x (4096 x 4096), 16x16 / 16x64
-// stream: 5.3 / 8.7, 16 x (28672 x 4096) 28 / 21.
-Shape linear_shape(int64_t m, int64_t n) {
-  static const int kRows[][2] = {{16, 16}, {16, 32}, {16, 64}, {32, 32}, {32, 64}, {64, 64}, {64, 128}, {128, 64}, {128, 128}};
-  int best = 0;
+struct Plan {
+  Shape shape;
+  int splits;
+};
+
+// The shape and number of splits of the least estimate, in us: a start, and for each round of workgroups (one to a compute unit; of kBlock22Two two)
+// another one and what they read at what a compute unit takes in with that shape, or the matrix at what memory gives, whichever is longer and a tenth of the other; splits write their sums, read again by a
+// second launch.  Over 240 products of 1 .. 4096 rows with matrices of 64 .. 150 000 rows and 100 .. 16 384 columns its choice takes 3 % more than the best of
+// all shapes and splits (up to 16, of four chunks at least), 1.3 times at the worst.  us: 1 x (4096 x 4096), 16x16 / 16x64 stream 5.3 / 8.7; 22 x (9637 x 4096)
+// 19.5 / 20.0, 32x64 11.5; 294 x (1840 x 4096), 32x64 stream 21.9, 64x64 block 9.9; 256 x (28672 x 4096) 152 and 61, 128x128 44; 145 x (955 x 12288),
+// 64x64 block in 1 / 4 / 8 splits 24.1 / 12.3 / 14.2; 4096 x (6144 x 4096), 128x128 blocks, one to a compute unit with four buffers 137, two with two 105;
+// 1024 x (4096 x 4096) 22.6 and 28.7.
+Plan linear_plan(int64_t m, int64_t n, int64_t k, bool f32) {
+  struct Kind {
+    int bm, bn, at_once;
+    double start, each, rate[2];  // KB a us of a compute unit: codes to the matrix instructions, and as bf16 numbers
+  };
+  static const Kind kKinds[] = {{16, 16, 1, 2.4, 0.85, {43, 43}},  {16, 32, 1, 2.4, 0.85, {43, 43}}, {16, 64, 1, 2.4, 0.85, {43, 43}}, {32, 32, 1, 2.4, 0.85, {43, 43}},
+                                {32, 64, 1, 2.4, 0.85, {43, 43}},  {64, 64, 1, 4.5, 2.5, {100, 58}}, {64, 128, 1, 4.5, 3.5, {100, 57}}, {128, 64, 1, 4.5, 3.5, {92, 53}},
+                                {128, 128, 1, 4.5, 5.0, {75, 36}}, {128, 128, 2, 4.5, 5.0, {80, 44}}};
+  static_assert(sizeof kKinds / sizeof kKinds[0] == kBlock22Two + 1, "a row a shape");
+  const int chunks = chunks_of(k);
+  Plan best = {kStream11, 1};
   double least = 0;
-  for (int i = 0; i < 9; ++i) {
-    const int bm = kRows[i][0], bn = kRows[i][1];
-    const double groups = (double)((m + bm - 1) / bm) * (double)((n + bn - 1) / bn);
-    const double cost = (groups > 256 ? groups / 256 : 1.0) * (bm + bn) * (i >= kBlock11 ? 0.85 : 1.0);
-    if (i == 0 || cost < least) best = i, least = cost;
-    // two to a compute unit, with two buffers each, where there are so many: 4096 x (6144 x 4096) 105 us, with four buffers 137; 1024 x (4096 x 4096)
-    // (256 of them) 28.7 and 22.6
-    if (best == kBlock22 && i == kBlock22 && groups > 256) return kBlock22Two;
+  for (int i = 0; i <= kBlock22Two; ++i) {
+    const Kind &q = kKinds[i];
+    const int64_t groups = (m + q.bm - 1) / q.bm * ((n + q.bn - 1) / q.bn);
+    if (q.at_once > 1 && groups <= 256) continue;
+    const int most = i < kBlock11 || q.at_once > 1 || chunks < 8 ? 1 : chunks < 64 ? chunks / 4 : 16;
+    for (int s = 1; s <= most && (s == 1 || groups * s <= 512); ++s) {
+      const int64_t round = 256 * q.at_once, whole = (groups * s + round - 1) / round;
+      // workgroups that the vector instructions bound, which make bf16 numbers of codes, end less in step
+      const double rounds = !f32 || whole == 1 ? (double)whole : 0.6 * (double)whole + 0.4 * (double)(groups * s) / (double)round;
+      const double reads = 0.128 * ((chunks + s - 1) / s) * ((m < q.bm ? m : q.bm) + q.bn) * q.at_once;
+      const double units = rounds * (reads / q.rate[f32] + q.each), memory = (double)n * (double)k / 6e6;
+      const double us = q.start + (units > memory ? units + 0.1 * memory : memory + 0.1 * units) + (s > 1 ? 1.25e-6 * s * (double)m * (double)n : 0.0);
+      if ((i == 0 && s == 1) || us < least) best = {(Shape)i, s}, least = us;
+    }
   }
-  return (Shape)best;
+  return best;
 }
 
 // Codes [n][k] into tiles and back: one 16-byte vector of a tile a thread.
@@ -432,10 +478,8 @@ __global__ __launch_bounds__(256) void pkv_fp8_unpack_kernel(const uint8_t *__re
   w[e] = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false)[0] * sw[row];
 }
 
-int64_t row_tiles(int64_t n) { return (n + kTileRows - 1) / kTileRows; }
-int chunks_of(int64_t k) { return (int)((k + kTileCols - 1) / kTileCols); }
-size_t tile_bytes(int64_t n, int64_t k) { return (size_t)row_tiles(n) * chunks_of(k) * kTileBytes; }
 bool matrix_ok(int64_t n, int64_t k) { return n > 0 && n < ((int64_t)1 << 31) - 16 && k > 0 && k <= ((int64_t)1 << 20); }
+bool rows_ok(int64_t rows, int64_t n, int64_t k) { return matrix_ok(n, k) && rows > 0 && rows <= ((int64_t)1 << 22) && rows * n <= ((int64_t)1 << 40); }
 
 }  // namespace
 
@@ -465,18 +509,31 @@ extern "C" int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w
   return PKV_OK;
 }
 
+extern "C" size_t pkv_fp8_linear_ws_bytes(int64_t rows, int64_t n, int64_t k, int out_dtype) {
+  if (!rows_ok(rows, n, k)) return 0;
+  const int splits = linear_plan(rows, n, k, out_dtype == PKV_DTYPE_F32).splits;
+  return splits == 1 ? 0 : (size_t)splits * rows * ((n + 3) / 4 * 4) * sizeof(float);
+}
+
 extern "C" int pkv_fp8_linear(const uint8_t *x, int64_t x_stride, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,
-                              void *y, int out_dtype, void *stream) {
+                              void *y, int out_dtype, void *ws, size_t ws_bytes, void *stream) {
   PKV_REQUIRE(x && x_scales && packed && y, "pkv_fp8_linear: null pointer");
   PKV_REQUIRE(out_dtype == PKV_DTYPE_F32 || out_dtype == PKV_DTYPE_BF16, "unknown dtype %d", out_dtype);
-  PKV_REQUIRE(matrix_ok(n, k) && rows > 0 && rows <= ((int64_t)1 << 22) && rows * n <= ((int64_t)1 << 40), "pkv_fp8_linear: bad shape %lld rows, %lld x %lld", (long long)rows, (long long)n, (long long)k);
+  PKV_REQUIRE(rows_ok(rows, n, k), "pkv_fp8_linear: bad shape %lld rows, %lld x %lld", (long long)rows, (long long)n, (long long)k);
   PKV_REQUIRE(x_stride % 16 == 0 && x_stride >= (int64_t)chunks_of(k) * kTileCols, "pkv_fp8_linear: rows of x must be 16-byte multiples apart and hold whole chunks of 128");
   PKV_REQUIRE(pkv_aligned(x, 16) && pkv_aligned(packed, 16) && pkv_aligned(x_scales, 4) && pkv_aligned(bias, 2) && pkv_aligned(y, 16), "pkv_fp8_linear: 16-byte aligned operands required");
   LinearArgs a;
   a.x = x, a.x_stride = x_stride, a.sx = x_scales, a.tiles = (const uint8_t *)packed, a.sw = (const float *)((const uint8_t *)packed + tile_bytes(n, k));
   a.bias = (const uint16_t *)bias, a.y = y, a.m = rows, a.n = n, a.chunks = chunks_of(k), a.f32 = out_dtype == PKV_DTYPE_F32;
   hipStream_t s = (hipStream_t)stream;
-  switch (linear_shape(rows, n)) {
+  const Plan plan = linear_plan(rows, n, k, a.f32);
+  a.splits = plan.splits, a.part_n = (n + 3) / 4 * 4, a.part = (float *)ws;
+  const size_t need = a.splits == 1 ? 0 : (size_t)a.splits * rows * a.part_n * sizeof(float);
+  if (need && (!ws || ws_bytes < need || !pkv_aligned(ws, 16))) {
+    pkv_set_error("pkv_fp8_linear: workspace of %zu bytes required, got %zu", need, ws ? ws_bytes : (size_t)0);
+    return PKV_ENOMEM;
+  }
+  switch (plan.shape) {
     case kStream11: launch_stream<1, 1>(a, s); break;
     case kStream12: launch_stream<1, 2>(a, s); break;
     case kStream14: launch_stream<1, 4>(a, s); break;

@@ -1468,12 +1468,24 @@ def add_rmsnorm_fp8(x: torch.Tensor, residual, weight: torch.Tensor, eps: float,
 class Fp8Weight:
     """A matrix [n,k] in eight bits, a scale for each of its rows, laid out once for the kernels that read it: weight = scale * code."""
 
-    __slots__ = ("packed", "n", "k")
+    __slots__ = ("packed", "n", "k", "_ws")
 
     def __init__(self, packed: torch.Tensor, n: int, k: int):
         _need(packed.dtype == torch.uint8 and packed.is_cuda and packed.is_contiguous() and packed.data_ptr() % 16 == 0 and
               packed.numel() == _lib.lib().pkv_fp8_bytes(n, k) > 0, "packed: what from_codes or quantize laid out")
-        self.packed, self.n, self.k = packed, int(n), int(k)
+        self.packed, self.n, self.k, self._ws = packed, int(n), int(k), {}
+
+    def ws_bytes(self, rows: int, out_dtype: torch.dtype = torch.bfloat16) -> int:
+        """Bytes of workspace that a product of ``rows`` rows takes."""
+        return self._ws_bytes(rows, _dt(out_dtype))
+
+    def _ws_bytes(self, rows, code):
+        need = self._ws.get((rows, code))
+        if need is None:
+            if len(self._ws) >= 1024:
+                self._ws.clear()
+            need = self._ws[rows, code] = _lib.lib().pkv_fp8_linear_ws_bytes(rows, self.n, self.k, code)
+        return need
 
     @property
     def shape(self):
@@ -1535,12 +1547,17 @@ def fp8_linear(x, weight: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dt
     y = like.new_empty(*x.shape[:-1], n, dtype=torch.bfloat16 if code == _lib.DTYPE_BF16 else torch.float32)
     if m > 0:
         lib, stream = _lib.lib(), _stream(packed)
-        if step is not None:  # codes and scales, for this call alone
-            ws = like.new_empty(m * (wide + 4), dtype=torch.uint8)
+        need, room = weight._ws_bytes(m, code), 0 if step is None else -(-m * (wide + 4) // 16) * 16  # sums; codes and scales of x
+        if need + room:  # for this call alone
+            ws = like.new_empty(need + room, dtype=torch.uint8)
+            sums = ws.data_ptr() + room
+        else:
+            sums = None
+        if step is not None:
             codes = ws.data_ptr()
             scales = codes + m * wide
             _launch(at, lib.pkv_fp8_rows, like.data_ptr(), kind, step, m, k, codes, wide, scales, stream)
-        _launch(at, lib.pkv_fp8_linear, codes, wide, scales, m, packed.data_ptr(), n, k, _p(bias), y.data_ptr(), code, stream)
+        _launch(at, lib.pkv_fp8_linear, codes, wide, scales, m, packed.data_ptr(), n, k, _p(bias), y.data_ptr(), code, sums, need, stream)
     return y
 
 

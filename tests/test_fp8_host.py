@@ -280,10 +280,17 @@ def test_rows_and_product_entry_points():
         assert rows(**bad) == _lib.EINVAL and norm(**bad) == _lib.EINVAL, bad
     assert rows(dtype=7) == _lib.EINVAL and rows(step=-1) == _lib.EINVAL and rows(x=B + 2, dtype=_lib.DTYPE_F32) == _lib.EINVAL
     assert norm(weight=None) == _lib.EINVAL and norm(res=B + 1) == _lib.EINVAL and norm(total=B + 1) == _lib.EINVAL and norm(weight=B + 1) == _lib.EINVAL
-    linear = lambda x=B, step=256, xs=2 * B, m=3, packed=3 * B, n=20, k=200, bias=None, y=4 * B, out=_lib.DTYPE_F32: L.pkv_fp8_linear(x, step, xs, m, packed, n, k, bias, y, out, None)
+    linear = lambda x=B, step=256, xs=2 * B, m=3, packed=3 * B, n=20, k=200, bias=None, y=4 * B, out=_lib.DTYPE_F32: L.pkv_fp8_linear(
+        x, step, xs, m, packed, n, k, bias, y, out, None, 0, None)
     for bad in (dict(x=None), dict(xs=None), dict(packed=None), dict(y=None), dict(out=7), dict(m=0), dict(m=(1 << 22) + 1), dict(n=0), dict(k=0), dict(k=(1 << 20) + 1, step=1 << 21), dict(n=1 << 31), dict(m=1 << 22, n=(1 << 18) + 1),
                 dict(step=128), dict(step=264), dict(x=B + 8), dict(xs=2 * B + 2), dict(packed=3 * B + 8), dict(bias=B + 1), dict(y=4 * B + 8)):
         assert linear(**bad) == _lib.EINVAL, bad
+    need = L.pkv_fp8_linear_ws_bytes(145, 955, 12288, _lib.DTYPE_F32)
+    assert need > 0 and need % (145 * 956 * 4) == 0 and L.pkv_fp8_linear_ws_bytes(3, 20, 200, _lib.DTYPE_BF16) == 0
+    for ws, size in ((None, 0), (None, need), (5 * B, need - 1), (5 * B + 8, need)):
+        assert L.pkv_fp8_linear(B, 12288, 2 * B, 145, 3 * B, 955, 12288, None, 4 * B, _lib.DTYPE_F32, ws, size, None) == _lib.ENOMEM and b"workspace" in L.pkv_last_error()
+    for bad in ((0, 955, 12288), (145, 0, 12288), (145, 955, 0), ((1 << 22) + 1, 955, 12288)):
+        assert L.pkv_fp8_linear_ws_bytes(*bad, _lib.DTYPE_BF16) == 0, bad
     assert L.pkv_fp8_pack(None, 200, B, 20, 200, B, None) == _lib.EINVAL and L.pkv_fp8_pack(B, 199, B, 20, 200, B, None) == _lib.EINVAL
     assert L.pkv_fp8_pack(B, 200, B, 20, 200, B + 8, None) == _lib.EINVAL and L.pkv_fp8_pack(B, 200, B + 2, 20, 200, B, None) == _lib.EINVAL
     assert L.pkv_fp8_unpack(None, 20, 200, B, None) == _lib.EINVAL and L.pkv_fp8_unpack(B + 8, 20, 200, B, None) == _lib.EINVAL

@@ -618,6 +618,27 @@ def test_linear_blocks(m, n, k, out_dtype):
     assert bool((err <= tol + HALF[out_dtype] * ref.abs() + 1e-30).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(145, 955, 12288), (40, 300, 8000), (300, 130, 9001), (78, 2452, 12288), (1000, 70, 12300), (65, 17, 16384), (129, 257, 8097)])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+def test_linear_splits(m, n, k, out_dtype):
+    """Long rows and few results: sums in parts, joined by a second launch.  The codes of test_linear_blocks: sums of 16384 products of at most 2^4 are below 2^18,
+    multiples of 2^-6, and exact in fp32 however they are parted."""
+    ops, g = _ops(), _gen(m + n)
+    codes, wcodes = ((torch.randint(0x38, 0x48, (r, k), generator=g) + 128 * torch.randint(0, 2, (r, k), generator=g)).to(U8).to(DEV) for r in (m, n))
+    sx, sw = (torch.rand(m, generator=g) + 0.1).to(DEV), (torch.rand(n, generator=g) - 0.5).to(DEV)
+    bias = torch.randn(n, generator=g).to(BF).to(DEV) if m % 2 == 0 else None
+    weight = ops.Fp8Weight.from_codes(wcodes, sw)
+    assert weight.ws_bytes(m, out_dtype) > 0
+    y = ops.fp8_linear(ops.Fp8Rows.from_codes(codes, sx), weight, bias=bias, out_dtype=out_dtype)
+    ref = codes.view(F8).to(F64) @ wcodes.view(F8).to(F64).t() * sx.to(F64).unsqueeze(1) * sw.to(F64)
+    tol = 2 * U * ref.abs()
+    if bias is not None:
+        ref = ref + bias.to(F64)
+        tol = tol + U * (ref.abs() + bias.to(F64).abs())
+    err = (y.to(F64) - ref).abs()
+    assert bool((err <= tol + HALF[out_dtype] * ref.abs() + 1e-30).all())
+
+
 def test_linear_blocks_rounded():
     """bf16 results of many rows: the instructions for e4m3 codes cut each of eight neighbouring products off below 2^-13 of the largest of
     them, so every group of eight loses at most 7 * 2^-13 of its largest."""
