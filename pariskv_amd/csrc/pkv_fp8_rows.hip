@@ -8,7 +8,7 @@
 
 namespace {
 
-constexpr int kMaxWidth = 16384, kRowThreads = 256, kRowWaves = kRowThreads / PKV_WAVE, E = 8;  // E: neighbouring elements a thread takes at a time
+constexpr int kMaxWidth = 16384, kReps = 2, E = 8;  // E: neighbouring elements a thread takes at a time
 
 __device__ __forceinline__ double fp8_wave_sum(double v) {
 #pragma unroll
@@ -45,21 +45,21 @@ __device__ __forceinline__ void load_any(const char *p, int left, float (&v)[E])
   for (int e = 0; e < E; ++e) v[e] = e >= left ? 0.f : BF16 ? pkv_bf16_bits_to_f32(((const uint16_t *)p)[e]) : ((const float *)p)[e];
 }
 
-// ALIGNED: whole 16-byte vectors everywhere.  REPS: how often a thread takes eight elements at most: registers for the longest rows (8) leave three
-// waves a SIMD.  4096 rows of 4096 with the residual, us: REPS 2 23.4 (5.0 TB/s, what a copy reaches), 8 27.5; 16384 x 1024: 30.0 and 59.1.
-template <bool NORM, bool BF16, bool ALIGNED, int REPS>
-__global__ __launch_bounds__(kRowThreads) void pkv_fp8_rows_kernel(RowsArgs a) {
-  static_assert(REPS * kRowThreads * E <= kMaxWidth, "longer than any row");
+// ALIGNED: whole 16-byte vectors everywhere.  THREADS: as many as a row takes with eight elements a thread, once or twice (kReps).  us, with the residual, 256 threads and
+// as often as it takes / this: 16384 x 1024 29.9 / 22.1 (5.3 TB/s; a copy reaches 4.8), 20000 x 200 29.9 / 13.5, 4096 x 4096 23.4, 2048 x 8192 25.8 / 23.1, 1 x 16384 8.3 / 5.4.
+template <bool NORM, bool BF16, bool ALIGNED, int THREADS>
+__global__ __launch_bounds__(THREADS) void pkv_fp8_rows_kernel(RowsArgs a) {
+  constexpr int kRowThreads = THREADS, kRowWaves = THREADS / PKV_WAVE;
   __shared__ double s_sum[kRowWaves];
   __shared__ uint32_t s_top[kRowWaves];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const char *const x = a.x + row * a.x_stride;
-  float v[REPS][E], w[NORM ? REPS : 1][E];
+  float v[kReps][E], w[NORM ? kReps : 1][E];
   double sum = 0.0;
   uint32_t top = 0;
 #pragma unroll
-  for (int r = 0; r < REPS; ++r) {
+  for (int r = 0; r < kReps; ++r) {
     const int at = (r * kRowThreads + tid) * E, left = a.width - at;
     if (left <= 0) continue;
     const char *const from = x + (int64_t)at * (BF16 ? 2 : 4);
@@ -104,14 +104,14 @@ __global__ __launch_bounds__(kRowThreads) void pkv_fp8_rows_kernel(RowsArgs a) {
     for (int i = 0; i < kRowWaves; ++i) sum += s_sum[i];
     const float inv = (float)(1.0 / sqrt(sum / (double)a.width + a.eps));
 #pragma unroll
-    for (int r = 0; r < REPS; ++r) {
+    for (int r = 0; r < kReps; ++r) {
       if ((r * kRowThreads + tid) * E >= a.width) continue;
 #pragma unroll
       for (int e = 0; e < E; ++e) v[r][e] = v[r][e] * inv * w[r][e];
     }
   }
 #pragma unroll
-  for (int r = 0; r < REPS; ++r) {
+  for (int r = 0; r < kReps; ++r) {
     if ((r * kRowThreads + tid) * E >= a.width) continue;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(kRowThreads) void pkv_fp8_rows_kernel(RowsArgs a) {
   const float shrink = fp8_pow2(-e2);
   uint8_t *const codes = a.codes + row * a.code_stride;
 #pragma unroll
-  for (int r = 0; r < REPS; ++r) {
+  for (int r = 0; r < kReps; ++r) {
     const int at = (r * kRowThreads + tid) * E;
     if (at >= a.width) continue;
     *(pkv_u32x2 *)(codes + at) = fp8_codes8(v[r], shrink);  // zeros behind the row's last element: a row holds whole chunks of 128
@@ -138,21 +138,26 @@ __global__ __launch_bounds__(kRowThreads) void pkv_fp8_rows_kernel(RowsArgs a) {
   if (tid == 0) a.scales[row] = fp8_pow2(e2);
 }
 
-template <bool NORM, bool BF16>
-int launch(const RowsArgs &a, int64_t rows, bool aligned, hipStream_t s) {
-#define PKV_ROWS(ALIGNED, REPS) \
-  hipLaunchKernelGGL((pkv_fp8_rows_kernel<NORM, BF16, ALIGNED, REPS>), dim3((unsigned)rows), dim3(kRowThreads), 0, s, a)
-  const bool shorter = a.width <= 2 * kRowThreads * E;
-  if (aligned) {
-    if (shorter) PKV_ROWS(true, 2);
-    else PKV_ROWS(true, 8);
-  } else {
-    if (shorter) PKV_ROWS(false, 2);
-    else PKV_ROWS(false, 8);
-  }
+template <bool NORM, bool BF16, bool ALIGNED>
+int launch_as(const RowsArgs &a, int64_t rows, hipStream_t s) {
+  // Few rows: eight elements a thread once, up to 512 threads.  us, with the residual, once / twice: 1 x 4096 3.4 / 3.8, 300 x 1024 3.6 / 4.0, 700 x 4096 7.5 / 7.2,
+  // 300 x 8192 8.1 / 7.0.
+  const int threads = (a.width + E - 1) / E, most = rows <= 512 && threads <= 512 ? threads : (threads + kReps - 1) / kReps;
+#define PKV_ROWS(THREADS) \
+  hipLaunchKernelGGL((pkv_fp8_rows_kernel<NORM, BF16, ALIGNED, THREADS>), dim3((unsigned)rows), dim3(THREADS), 0, s, a)
+  if (most <= 64) PKV_ROWS(64);
+  else if (most <= 128) PKV_ROWS(128);
+  else if (most <= 256) PKV_ROWS(256);
+  else if (most <= 512) PKV_ROWS(512);
+  else PKV_ROWS(1024);
 #undef PKV_ROWS
+  static_assert(1024 * E * kReps == kMaxWidth, "no wider row");
   PKV_LAUNCH_CHECK("pkv_fp8_rows_kernel");
   return PKV_OK;
+}
+template <bool NORM, bool BF16>
+int launch(const RowsArgs &a, int64_t rows, bool aligned, hipStream_t s) {
+  return aligned ? launch_as<NORM, BF16, true>(a, rows, s) : launch_as<NORM, BF16, false>(a, rows, s);
 }
 
 int shape_ok(const char *who, int64_t rows, int64_t width, const void *codes, int64_t code_stride, const void *scales) {
