@@ -76,19 +76,18 @@ template <bool MASKED, int PARTS>
 __device__ __forceinline__ void weights(Tile<PARTS> &w, const float (&s)[8], const float (&kx)[8], uint32_t bits, float (&p)[8]) {
   const int j = pkv_lane() >> 4;
   float x[8], top = -INFINITY;  // scores above use
-  auto above = [&] {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = !MASKED || ((bits >> e) & 1u) ? fmaf(s[e], kx[e], -w.use) : -INFINITY;
-  };
-  above();
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
+  for (int e = 0; e < 8; ++e) {
+    x[e] = !MASKED || ((bits >> e) & 1u) ? fmaf(s[e], kx[e], -w.use) : -INFINITY;
+    top = fmaxf(top, x[e]);
+  }
   if (__any(top > w.lim)) {
     top = pkv_pair_max<32>(pkv_pair_max<16>(top));
     const bool fresh = w.lim < 0.f, moves = top > -INFINITY && (fresh || top > 0.f);
-    const float next = moves ? w.use + top : w.use, corr = fresh ? 0.f : __builtin_amdgcn_exp2f(w.use - next);
+    const float next = moves ? w.use + top : w.use, down = w.use - next, corr = fresh ? 0.f : __builtin_amdgcn_exp2f(down);
     w.use = next, w.lim = moves ? 8.f : w.lim;
-    above();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] += down;
     float cr[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) cr[i] = __shfl(corr, 4 * j + i, PKV_WAVE);

@@ -639,6 +639,36 @@ def test_linear_splits(m, n, k, out_dtype):
     assert bool((err <= tol + HALF[out_dtype] * ref.abs() + 1e-30).all())
 
 
+def test_linear_splits_streams_graphs():
+    """Calls on two streams at once and in two captured graphs, whose sums are their own."""
+    ops, g = _ops(), _gen(34)
+    weight = ops.Fp8Weight.quantize(_rows(g, 300, 12288).to(DEV))
+    x = [_rows(g, 70, 12288).to(DEV) for _ in range(2)]
+    assert weight.ws_bytes(70) > 0
+    want = [ops.fp8_linear(a, weight) for a in x]
+    streams, got, graphs = [torch.cuda.Stream() for _ in x], [None, None], [torch.cuda.CUDAGraph() for _ in x]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = ops.fp8_linear(x[i], weight)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for i, s in enumerate(streams):
+        with torch.cuda.graph(graphs[i], stream=s):
+            got[i] = ops.fp8_linear(x[i], weight)
+    for _ in range(3):
+        for a in x:
+            a.copy_(_rows(g, 70, 12288))
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(b, ops.fp8_linear(a, weight)) for a, b in zip(x, got))
+
+
 def test_linear_blocks_rounded():
     """bf16 results of many rows: the instructions for e4m3 codes cut each of eight neighbouring products off below 2^-13 of the largest of
     them, so every group of eight loses at most 7 * 2^-13 of its largest."""
