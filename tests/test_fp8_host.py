@@ -300,6 +300,20 @@ def test_rows_and_product_entry_points():
         assert size(*bad) == 0, bad
 
 
+def test_fp8_cache_refuses():
+    from pariskv_amd.cache_hub.fp8_cache import fp8_cache
+
+    def make(heads=2, group=4, dim=128, dtype=BF, device="cuda:0", **kw):
+        return fp8_cache(0, 1, 2, 100, heads, heads * group, dim, dtype, {"0": device}, **kw)
+
+    for kw, kind in ((dict(dim=64), ValueError), (dict(dtype=torch.float16), ValueError), (dict(device="cpu"), RuntimeError), (dict(block=48), RuntimeError)):
+        with pytest.raises(kind) as e:
+            make(**kw)
+        assert "HIP" not in str(e.value)
+    with pytest.raises(ValueError, match="multiple"):
+        fp8_cache(0, 1, 2, 100, 3, 8, 128, BF, {"0": "cuda:0"})
+
+
 def test_struct_mirrors():
     for which, mirror in ((10, _lib.Fp8Kv), (11, _lib.Fp8AttnArgs)):
         assert _lib.lib().pkv_struct_bytes(which) == ctypes.sizeof(mirror) > 0
