@@ -90,11 +90,18 @@ __device__ __forceinline__ void put4(const LinearArgs &a, int64_t row, int64_t c
     for (int i = 0; i < 4; ++i) v[i] += pkv_bf16_bits_to_f32(a.bias[WHOLE || col + i < a.n ? col + i : col]);
   }
   const int64_t at = row * a.n + col;
-  if constexpr (WHOLE) {
-    if constexpr (F32) *(fp8_f32x4 *)((float *)a.y + at) = fp8_f32x4{v[0], v[1], v[2], v[3]};
-    else
-      *(pkv_u32x2 *)((uint16_t *)a.y + at) = pkv_u32x2{(uint32_t)pkv_f32_to_bf16_bits(v[0]) | ((uint32_t)pkv_f32_to_bf16_bits(v[1]) << 16),
-                                                       (uint32_t)pkv_f32_to_bf16_bits(v[2]) | ((uint32_t)pkv_f32_to_bf16_bits(v[3]) << 16)};
+  if (WHOLE || col + 4 <= a.n) {
+    struct __attribute__((packed)) Four {
+      uint32_t w[F32 ? 4 : 2];
+    } o;
+    if constexpr (F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o.w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) o.w[i] = (uint32_t)pkv_f32_to_bf16_bits(v[2 * i]) | ((uint32_t)pkv_f32_to_bf16_bits(v[2 * i + 1]) << 16);
+    }
+    __builtin_memcpy((char *)a.y + at * (F32 ? 4 : 2), &o, sizeof o);  // the memory takes it at any alignment
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -195,7 +202,7 @@ __global__ __launch_bounds__(kStreamWaves * PKV_WAVE) void pkv_fp8_stream_kernel
 // (16 KB 0.7 us a compute unit; 0.4).  Vector v of row r lies at v ^ (r mod 8) of the row, so that rows of an operand are on different banks.
 typedef const __attribute__((address_space(1))) void *fp8_global;
 typedef __attribute__((address_space(3))) void *fp8_lds;
-// A wave's results, rows m0 .., columns n0 .. of y, 32 rows at a time through a part of LDS of its own and out as whole rows of it: 16 bytes of each of
+// A wave's results, rows m0 .., columns n0 .. of y, past the caches, 32 rows at a time through a part of LDS of its own and out as whole rows of it: 16 bytes of each of
 // 32 rows, as they lie in the registers, would take 20 us of 256 x 256 where rows of y are a multiple of 4096 bytes.
 // RAW: as sums, to a split's part.
 template <int TM, int TN, bool F32, bool RAW>
@@ -238,7 +245,8 @@ __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x1
       const pkv_u32x4 v = *(const pkv_u32x4 *)(mine + r0 * kStep + vec * 16);
       if (at >= a.m || col >= left) continue;
       char *const to = y + (at * n + n0 + col) * kEs;
-      if (whole) *(pkv_u32x4 *)to = v;
+      if (whole) __builtin_nontemporal_store(v, (pkv_u32x4 *)to);
+      else if (col + 16 / kEs <= left) __builtin_memcpy(to, &v, 16);  // the memory takes it at any alignment
       else
 #pragma unroll
         for (int i = 0; i < 16 / kEs; ++i) {

@@ -46,7 +46,7 @@ __device__ __forceinline__ void load_any(const char *p, int left, float (&v)[E])
 }
 
 // ALIGNED: whole 16-byte vectors everywhere.  THREADS: as many as a row takes with eight elements a thread, once or twice (kReps).  us, with the residual, 256 threads and
-// as often as it takes / this: 16384 x 1024 29.9 / 22.1 (5.3 TB/s; a copy reaches 4.8), 20000 x 200 29.9 / 13.5, 4096 x 4096 23.4, 2048 x 8192 25.8 / 23.1, 1 x 16384 8.3 / 5.4.
+// as often as it takes / this: 16384 x 1024 29.9 / 22.1 (5.3 TB/s; a copy reaches 4.8), 20000 x 200 29.9 / 13.5, 4096 x 4096 22.9, 2048 x 8192 25.8 / 23.1, 1 x 16384 8.3 / 5.4.
 template <bool NORM, bool BF16, bool ALIGNED, int THREADS>
 __global__ __launch_bounds__(THREADS) void pkv_fp8_rows_kernel(RowsArgs a) {
   constexpr int kRowThreads = THREADS, kRowWaves = THREADS / PKV_WAVE;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(THREADS) void pkv_fp8_rows_kernel(RowsArgs a) {
 #pragma unroll
           for (int p = 0; p < 4; ++p) o[p] = (__float_as_uint(v[r][2 * p]) >> 16) | (__float_as_uint(v[r][2 * p + 1]) & 0xffff0000u);
           if constexpr (ALIGNED) {
-            *(pkv_u32x4 *)to = o;
+            __builtin_nontemporal_store(o, (pkv_u32x4 *)to);
           } else if (left >= E) {
             __builtin_memcpy(to, &o, sizeof o);
           } else {
