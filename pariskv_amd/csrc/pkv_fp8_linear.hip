@@ -245,7 +245,8 @@ __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x1
       const pkv_u32x4 v = *(const pkv_u32x4 *)(mine + r0 * kStep + vec * 16);
       if (at >= a.m || col >= left) continue;
       char *const to = y + (at * n + n0 + col) * kEs;
-      if (whole) __builtin_nontemporal_store(v, (pkv_u32x4 *)to);
+      if (RAW) *(pkv_u32x4 *)to = v;  // read again by the second launch
+      else if (whole) __builtin_nontemporal_store(v, (pkv_u32x4 *)to);
       else if (col + 16 / kEs <= left) __builtin_memcpy(to, &v, 16);  // the memory takes it at any alignment
       else
 #pragma unroll
