@@ -4,8 +4,8 @@
 // Codes become bf16 numbers in registers, exactly (two to an instruction), and go to bf16 matrix instructions, whose products of them
 // are exact and whose sums are fp32.  The instructions that take e4m3 codes themselves have twice the rate, but add eight neighbouring products
 // up with nothing below 2^-13 of the largest of them (2^16 + 4 is 2^16); the sums of eight are added in fp32.  Rows of normal numbers come out 1.5e-5 of
-// their norm off, a hundredth of what rounding to bf16 does.  So they are used where the results are bf16 and the matrix rate counts, many
-// rows, and nowhere else: 4096 rows x (6144 x 4096) 108 us, 193 with bf16 instructions.
+// their norm off, a hundredth of what rounding to bf16 does.  So they are used where the results are bf16 and rows go through LDS (17 or more), and nowhere else:
+// 4096 rows x (6144 x 4096) 100 us, 193 with bf16 instructions.
 // Which columns a lane has is free as long as both operands agree: lane (r, j) takes columns 16 j .. 16 j + 15 and 64 + 16 j .. of a chunk of 128,
 // so that the rows of x are read 64 bytes side by side.  The matrix is laid out once in tiles of 16 rows x 128 columns in the order of the lanes.
 #include "pkv_fp8.h"
