@@ -1308,6 +1308,15 @@ class Fp8Attention:
               "1..1024 query tokens, at most 8192 query rows a KV head")
         self.bs, self.H, self.G, self.max_tokens, self.max_keys = bs, n_kv_heads, group, max_tokens, max_keys
         self.device = torch.device(device)
+        self._ws = {}
+
+    def _ws_bytes(self, code, tokens, keys):
+        need = self._ws.get((code, tokens, keys))
+        if need is None:
+            if len(self._ws) >= 1024:
+                self._ws.clear()
+            need = self._ws[code, tokens, keys] = _lib.lib().pkv_fp8_attention_ws_bytes(code, self.bs, self.H, self.G, tokens, keys)
+        return need
 
     def run(self, queries: torch.Tensor, cache: Fp8KVCache, segments, row_keys: Optional[torch.Tensor] = None, scale: Optional[float] = None,
             out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -1362,12 +1371,11 @@ class Fp8Attention:
             out = queries.new_empty(*shape)
         elif out.shape != shape or out.dtype != dt or out.get_device() != at or not out.is_contiguous() or out.data_ptr() & 15:
             raise RuntimeError("out: contiguous, like queries")
-        lib = _lib.lib()
-        need = lib.pkv_fp8_attention_ws_bytes(code, bs, H, G, T, total)
+        need = self._ws_bytes(code, T, total)
         ws = queries.new_empty(need, dtype=torch.uint8) if need else None
         block = _FP8_ATTN_BLOCK.pack(q.data_ptr(), code, G, T, n_seg, qs[0], qs[1], *cache._fields, *segs, keys_at, _SCALE if scale is None else scale,
                                      out.data_ptr(), ws.data_ptr() if need else 0, need)
-        _launch(at, lib.pkv_fp8_attention, block, _stream(queries))
+        _launch(at, _lib.lib().pkv_fp8_attention, block, _stream(queries))
         return out
 
 
