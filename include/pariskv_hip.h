@@ -693,7 +693,7 @@ int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w, void *str
 
 /* y[m][n] = x_scales[m] scale[n] sum_k x[m][k] code[n][k] + bias[n] (no counterpart in the reference): x codes [rows], x_stride bytes apart
  * (16-byte multiples, 16-byte aligned), zeros past k up to the next multiple of 128, as pkv_fp8_rows leaves them; bias bf16 [n] or NULL; y [rows][n] contiguous of out_dtype.  Sums of codes in
- * fp32, then the scales (bf16 results of more than 16 rows: of eight neighbouring products what is below 2^-13 of the largest may be left out); at most 2^22 rows and 2^40 results.  ws: pkv_fp8_linear_ws_bytes(rows, n, k, out_dtype) bytes for the sums of columns that are split (0: none
+ * fp32, then the scales; at most 2^22 rows and 2^40 results.  ws: pkv_fp8_linear_ws_bytes(rows, n, k, out_dtype) bytes for the sums of columns that are split (0: none
  * needed). */
 size_t pkv_fp8_linear_ws_bytes(int64_t rows, int64_t n, int64_t k, int out_dtype);
 int pkv_fp8_linear(const uint8_t *x, int64_t x_stride, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,

@@ -2,10 +2,9 @@
 // codes e4m3.  (No counterpart in the reference, whose projections are bf16 GEMMs, model_hub/qwen.py:327-383.)
 //
 // Codes become bf16 numbers in registers, exactly (two to an instruction), and go to bf16 matrix instructions, whose products of them
-// are exact and whose sums are fp32.  The instructions that take e4m3 codes themselves have twice the rate, but add eight neighbouring products
-// up with nothing below 2^-13 of the largest of them (2^16 + 4 is 2^16); the sums of eight are added in fp32.  Rows of normal numbers come out 1.5e-5 of
-// their norm off, a hundredth of what rounding to bf16 does.  So they are used where the results are bf16 and rows go through LDS (17 or more), and nowhere else:
-// 4096 rows x (6144 x 4096) 100 us, 193 with bf16 instructions.
+// are exact and whose sums are fp32.  The instructions that take e4m3 codes themselves have twice the rate (4096 rows x (6144 x 4096) 100 us, 193 with bf16
+// instructions), but add eight neighbouring products up with nothing below 2^-13 of the largest of them (2^16 + 4 is 2^16): where large products
+// of eight cancel, what is left is lost.  They are not used.
 // Which columns a lane has is free as long as both operands agree: lane (r, j) takes columns 16 j .. 16 j + 15 and 64 + 16 j .. of a chunk of 128,
 // so that the rows of x are read 64 bytes side by side.  The matrix is laid out once in tiles of 16 rows x 128 columns in the order of the lanes.
 #include "pkv_fp8.h"
@@ -18,7 +17,6 @@ typedef float fp8_f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTileRows = 16, kTileCols = 128, kTileBytes = kTileRows * kTileCols;
 
-typedef int fp8_i32x8 __attribute__((ext_vector_type(8)));
 struct Codes {  // 32 codes of a lane
   pkv_u32x4 half[2];
   // a quarter of them as bf16 numbers
@@ -29,14 +27,6 @@ struct Codes {  // 32 codes of a lane
 };
 __device__ __forceinline__ fp8_f32x4 fp8_mfma_part(pkv_u32x4 a, pkv_u32x4 b, fp8_f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fp8_bf16x8, a), __builtin_bit_cast(fp8_bf16x8, b), c, 0, 0, 0);
-}
-// 32 x 32 x 64 codes, and 32 x 32 x 16 of them as bf16 numbers
-__device__ __forceinline__ fp8_f32x16 fp8_mfma32_codes(const Codes &a, const Codes &b, fp8_f32x16 c) {
-  const fp8_i32x8 x = {(int)a.half[0].x, (int)a.half[0].y, (int)a.half[0].z, (int)a.half[0].w,
-                       (int)a.half[1].x, (int)a.half[1].y, (int)a.half[1].z, (int)a.half[1].w};
-  const fp8_i32x8 y = {(int)b.half[0].x, (int)b.half[0].y, (int)b.half[0].z, (int)b.half[0].w,
-                       (int)b.half[1].x, (int)b.half[1].y, (int)b.half[1].z, (int)b.half[1].w};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
 }
 __device__ __forceinline__ fp8_f32x16 fp8_mfma32_part(pkv_u32x4 a, pkv_u32x4 b, fp8_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(fp8_bf16x8, a), __builtin_bit_cast(fp8_bf16x8, b), c, 0, 0, 0);
@@ -261,7 +251,7 @@ __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x1
   }
 }
 
-template <int TM, int TN, int DEPTH, bool E4M3>
+template <int TM, int TN, int DEPTH>
 __global__ __launch_bounds__(256, TM * TN > 4 ? 1 : 2) void pkv_fp8_block_kernel(LinearArgs a, int m_blocks, int n_blocks) {
   constexpr int kEach = TM + TN, kX = 4 * TM * kTileBytes, kBuffer = kX + 4 * TN * kTileBytes;  // pieces of 1 KB that a wave brings in, of x and of the matrix
   extern __shared__ uint8_t lds[];
@@ -325,23 +315,16 @@ __global__ __launch_bounds__(256, TM * TN > 4 ? 1 : 2) void pkv_fp8_block_kernel
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[r][t][i] = 0.f;
   auto product = [&](const Codes (&x)[TM], const Codes (&w)[TN]) {
-    if constexpr (E4M3) {
 #pragma unroll
-      for (int r = 0; r < TN; ++r)
+    for (int p = 0; p < 4; ++p) {
+      pkv_u32x4 xo[TM];
 #pragma unroll
-        for (int t = 0; t < TM; ++t) acc[r][t] = fp8_mfma32_codes(w[r], x[t], acc[r][t]);
-    } else {
+      for (int t = 0; t < TM; ++t) xo[t] = x[t].part(p);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        pkv_u32x4 xo[TM];
+      for (int r = 0; r < TN; ++r) {
+        const pkv_u32x4 wo = w[r].part(p);
 #pragma unroll
-        for (int t = 0; t < TM; ++t) xo[t] = x[t].part(p);
-#pragma unroll
-        for (int r = 0; r < TN; ++r) {
-          const pkv_u32x4 wo = w[r].part(p);
-#pragma unroll
-          for (int t = 0; t < TM; ++t) acc[r][t] = fp8_mfma32_part(wo, xo[t], acc[r][t]);
-        }
+        for (int t = 0; t < TM; ++t) acc[r][t] = fp8_mfma32_part(wo, xo[t], acc[r][t]);
       }
     }
   };
@@ -358,13 +341,13 @@ __global__ __launch_bounds__(256, TM * TN > 4 ? 1 : 2) void pkv_fp8_block_kernel
     const int next = now + 1 == DEPTH ? 0 : now + 1;
     read(now, 1, x[1], w[1]);
     product(x[0], w[0]);
-    fp8_mix<E4M3 ? TM * TN : 4 * TM * TN, 2 * (TM + TN), 0>();
+    fp8_mix<4 * TM * TN, 2 * (TM + TN), 0>();
     fp8_wait<(DEPTH - 2) * 2 * kEach>();  // chunk c + 1 is there, for this wave, and its reads of chunk c are done
     __builtin_amdgcn_s_barrier();         // ... for all
     fetch(c + DEPTH < last ? c + DEPTH : last, now);
     read(next, 0, x[0], w[0]);
     product(x[1], w[1]);
-    fp8_mix<E4M3 ? TM * TN : 4 * TM * TN, 2 * (TM + TN), 2 * kEach>();
+    fp8_mix<4 * TM * TN, 2 * (TM + TN), 2 * kEach>();
     __builtin_amdgcn_sched_barrier(0);
     now = next;
   }
@@ -392,22 +375,18 @@ void launch_stream(const LinearArgs &a, hipStream_t s) {
   hipLaunchKernelGGL((pkv_fp8_stream_kernel<MT, RT>), dim3((tiles + RT - 1) / RT, (unsigned)((a.m + 16 * MT - 1) / (16 * MT))), dim3(kStreamWaves * PKV_WAVE), 0, s, a);
 }
 
-template <int TM, int TN, int DEPTH, bool E4M3>
-int launch_block_as(const LinearArgs &a, hipStream_t s) {
+template <int TM, int TN, int DEPTH>
+int launch_block(const LinearArgs &a, hipStream_t s) {
   const int mb = (int)((a.m + 64 * TM - 1) / (64 * TM)), nb = (int)((a.n + 64 * TN - 1) / (64 * TN));
   const int lds = DEPTH * 4 * (TM + TN) * kTileBytes;
-  PKV_HIP(hipFuncSetAttribute((const void *)pkv_fp8_block_kernel<TM, TN, DEPTH, E4M3>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  hipLaunchKernelGGL((pkv_fp8_block_kernel<TM, TN, DEPTH, E4M3>), dim3((unsigned)((mb * (int64_t)nb + 7) / 8 * 8), (unsigned)a.splits), dim3(256), lds, s, a, mb, nb);
+  PKV_HIP(hipFuncSetAttribute((const void *)pkv_fp8_block_kernel<TM, TN, DEPTH>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL((pkv_fp8_block_kernel<TM, TN, DEPTH>), dim3((unsigned)((mb * (int64_t)nb + 7) / 8 * 8), (unsigned)a.splits), dim3(256), lds, s, a, mb, nb);
   PKV_LAUNCH_CHECK("pkv_fp8_block_kernel");
   if (a.splits > 1) {
     hipLaunchKernelGGL(pkv_fp8_sum_kernel, dim3((unsigned)((a.m * (a.part_n / 4) + 255) / 256)), dim3(256), 0, s, a);
     PKV_LAUNCH_CHECK("pkv_fp8_sum_kernel");
   }
   return PKV_OK;
-}
-template <int TM, int TN, int DEPTH>
-int launch_block(const LinearArgs &a, hipStream_t s) {
-  return a.f32 ? launch_block_as<TM, TN, DEPTH, false>(a, s) : launch_block_as<TM, TN, DEPTH, true>(a, s);
 }
 
 int64_t row_tiles(int64_t n) { return (n + kTileRows - 1) / kTileRows; }
@@ -424,24 +403,23 @@ struct Plan {
 
 // The shape and number of splits of the least estimate, in us: a start, and for each round of workgroups (one to a compute unit; of kBlock22Two two)
 // another one and what they read at what a compute unit takes in with that shape, or the matrix at what memory gives, whichever is longer and a tenth of the other; splits write their sums, read again by a
-// second launch.  Over 240 products of 1 .. 4096 rows with matrices of 64 .. 150 000 rows and 100 .. 16 384 columns its choice takes 3 % more than the best of
-// all shapes and splits (up to 16, of four chunks at least), 1.3 times at the worst.  us: 1 x (4096 x 4096), 16x16 / 16x64 stream 5.3 / 8.7; 22 x (9637 x 4096)
-// 19.5 / 20.0, 32x64 11.5; 294 x (1840 x 4096), 32x64 stream 21.9, 64x64 block 9.9; 256 x (28672 x 4096) 152 and 61, 128x128 44; 145 x (955 x 12288),
-// 64x64 block in 1 / 4 / 8 splits 24.1 / 12.3 / 14.2; 4096 x (6144 x 4096), 128x128 blocks, one to a compute unit with four buffers 137, two with two 105;
-// 1024 x (4096 x 4096) 22.6 and 28.7.
-Plan linear_plan(int64_t m, int64_t n, int64_t k, bool f32) {
+// second launch.  Over 180 products of 1 .. 4096 rows with matrices of 64 .. 150 000 rows and 100 .. 16 384 columns, half of them with bf16 results, its choice takes 3 % more
+// than the best of all shapes and splits (up to 16, of four chunks at least), 1.3 times at the worst.  us, bf16 results: 1 x (4096 x 4096), 16x16 / 16x64 stream 5.3 / 8.8;
+// 22 x (9637 x 4096) 18.7 / 19.0, 32x64 11.1; 294 x (1840 x 4096), 32x64 stream 22.3, 64x64 block 15.9, 16.8 in two splits; 256 x (28672 x 4096) 155 and 86, 64x128 69;
+// 145 x (955 x 12288), 64x64 block in 1 / 4 / 5 / 8 splits 35.8 / 16.1 / 14.8 / 15.9; 128x128 blocks, one to a compute unit with four buffers / two with two:
+// 4096 x (6144 x 4096) 206 / 176-190, 1024 x (4096 x 4096) 36.9 / 35.6.
+Plan linear_plan(int64_t m, int64_t n, int64_t k) {
   struct Kind {
     int bm, bn, at_once;
-    double start, each, rate[2];  // KB a us of a compute unit: codes to the matrix instructions, and as bf16 numbers
+    double start, each, rate;  // KB a us of a compute unit
   };
-  static const Kind kKinds[] = {{16, 16, 1, 2.4, 0.85, {43, 43}},  {16, 32, 1, 2.4, 0.85, {43, 43}}, {16, 64, 1, 2.4, 0.85, {43, 43}}, {32, 32, 1, 2.4, 0.85, {43, 43}},
-                                {32, 64, 1, 2.4, 0.85, {43, 43}},  {64, 64, 1, 4.5, 2.5, {100, 58}}, {64, 128, 1, 4.5, 3.5, {100, 57}}, {128, 64, 1, 4.5, 3.5, {92, 53}},
-                                {128, 128, 1, 4.5, 5.0, {75, 36}}, {128, 128, 2, 4.5, 5.0, {80, 44}}};
+  static const Kind kKinds[] = {{16, 16, 1, 2.4, 0.85, 43}, {16, 32, 1, 2.4, 0.85, 43}, {16, 64, 1, 2.4, 0.85, 43},   {32, 32, 1, 2.4, 0.85, 43}, {32, 64, 1, 2.4, 0.85, 43},
+                                {64, 64, 1, 4.5, 2.5, 58},  {64, 128, 1, 4.5, 3.5, 57},  {128, 64, 1, 4.5, 3.5, 53},  {128, 128, 1, 4.5, 5.0, 36}, {128, 128, 2, 4.5, 5.0, 44}};
   static_assert(sizeof kKinds / sizeof kKinds[0] == kBlock22Two + 1, "a row a shape");
   const int chunks = chunks_of(k);
   Plan best = {kStream11, 1};
   double least = 0;
-  // up to 16 rows, streams only: 16 x (3208 x 12288) 15.2 us, the best split block 14.2, but 3 x (363 x 12288) 7.9 and 9.8
+  // up to 16 rows, streams only: 16 x (3208 x 12288) 13.0 us, the best split block 16.1; 3 x (363 x 12288) 7.2 and 10.3
   for (int i = 0; i <= (m <= 16 ? kStream24 : kBlock22Two); ++i) {
     const Kind &q = kKinds[i];
     const int64_t groups = (m + q.bm - 1) / q.bm * ((n + q.bn - 1) / q.bn);
@@ -450,9 +428,9 @@ Plan linear_plan(int64_t m, int64_t n, int64_t k, bool f32) {
     for (int s = 1; s <= most && (s == 1 || groups * s <= 512); ++s) {
       const int64_t round = 256 * q.at_once, whole = (groups * s + round - 1) / round;
       // workgroups that the vector instructions bound, which make bf16 numbers of codes, end less in step
-      const double rounds = !f32 || whole == 1 ? (double)whole : 0.6 * (double)whole + 0.4 * (double)(groups * s) / (double)round;
+      const double rounds = whole == 1 ? 1.0 : 0.6 * (double)whole + 0.4 * (double)(groups * s) / (double)round;
       const double reads = 0.128 * ((chunks + s - 1) / s) * ((m < q.bm ? m : q.bm) + q.bn) * q.at_once;
-      const double units = rounds * (reads / q.rate[f32] + q.each), memory = (double)n * (double)k / 6e6;
+      const double units = rounds * (reads / q.rate + q.each), memory = (double)n * (double)k / 6e6;
       const double us = q.start + (units > memory ? units + 0.1 * memory : memory + 0.1 * units) + (s > 1 ? 1.25e-6 * s * (double)m * (double)n : 0.0);
       if ((i == 0 && s == 1) || us < least) best = {(Shape)i, s}, least = us;
     }
@@ -519,9 +497,9 @@ extern "C" int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w
   return PKV_OK;
 }
 
-extern "C" size_t pkv_fp8_linear_ws_bytes(int64_t rows, int64_t n, int64_t k, int out_dtype) {
+extern "C" size_t pkv_fp8_linear_ws_bytes(int64_t rows, int64_t n, int64_t k, int /*out_dtype: the same for all*/) {
   if (!rows_ok(rows, n, k)) return 0;
-  const int splits = linear_plan(rows, n, k, out_dtype == PKV_DTYPE_F32).splits;
+  const int splits = linear_plan(rows, n, k).splits;
   return splits == 1 ? 0 : (size_t)splits * rows * ((n + 3) / 4 * 4) * sizeof(float);
 }
 
@@ -536,7 +514,7 @@ extern "C" int pkv_fp8_linear(const uint8_t *x, int64_t x_stride, const float *x
   a.x = x, a.x_stride = x_stride, a.sx = x_scales, a.tiles = (const uint8_t *)packed, a.sw = (const float *)((const uint8_t *)packed + tile_bytes(n, k));
   a.bias = (const uint16_t *)bias, a.y = y, a.m = rows, a.n = n, a.chunks = chunks_of(k), a.f32 = out_dtype == PKV_DTYPE_F32;
   hipStream_t s = (hipStream_t)stream;
-  const Plan plan = linear_plan(rows, n, k, a.f32);
+  const Plan plan = linear_plan(rows, n, k);
   a.splits = plan.splits, a.part_n = (n + 3) / 4 * 4, a.part = (float *)ws;
   const size_t need = a.splits == 1 ? 0 : (size_t)a.splits * rows * a.part_n * sizeof(float);
   if (need && (!ws || ws_bytes < need || !pkv_aligned(ws, 16))) {

@@ -1535,8 +1535,7 @@ class Fp8Weight:
 
 def fp8_linear(x, weight: Fp8Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., k] times the transpose of an eight-bit matrix, plus ``bias`` (bf16 [n]): [..., n] in ``out_dtype`` (bf16, the default, or
-    fp32).  x: :class:`Fp8Rows`, or bf16 or fp32 rows, which :func:`fp8_rows` quantises first.  Sums in fp32, one rounding; for bf16 results of more than 16
-    rows, what is below 2^-13 of the largest of eight neighbouring products may be left out."""
+    fp32).  x: :class:`Fp8Rows`, or bf16 or fp32 rows, which :func:`fp8_rows` quantises first.  Sums in fp32, one rounding."""
     packed, n = weight.packed, weight.n
     at = packed.get_device()
     if isinstance(x, Fp8Rows):

@@ -1,0 +1,37 @@
+"""Operators in eight bits where their arithmetic is at its limits: products that cancel, scales at both ends of fp32, and what else only a particular
+input shows.  Inputs are made so that the definition's result is known to a few units in the last place; each bound stands at its test."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_fp8 import BF, DEV, F8, F32, F64, HALF, U8, _gen, _ops
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ products
+
+
+def _cancelling(g, rows, k, second):
+    """Codes [rows,k]: 448 in columns 8 i, `second` in columns 8 i + 1, and 1, 1.5, 2 or 3 in the others."""
+    codes = torch.tensor([0x38, 0x3c, 0x40, 0x44], dtype=U8)[torch.randint(0, 4, (rows, k), generator=g)]
+    codes[:, 0::8], codes[:, 1::8] = 0x7e, second
+    return codes.to(DEV)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 100, 300), (16, 2000, 1000), (17, 2000, 1000), (130, 20000, 384), (520, 9001, 1000), (520, 1536, 4096), (256, 6144, 4096), (1024, 4096, 4096),
+                                   (145, 955, 12288)])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+def test_linear_sums_cancel(m, n, k, out_dtype):
+    """Of eight neighbouring products two are +-448^2 and cancel.  All products are multiples of 2^-2, those that are left add up to less than 2^17, and a path through the sum holds at
+    most a few of the large ones (below 2^18 each) that have not met their opposites yet: every sum is a multiple of 2^-2 below 2^22, exact in
+    fp32, and the scales are 1.  Only the rounding to bf16 is left."""
+    ops, g = _ops(), _gen(m + n)
+    codes, wcodes = _cancelling(g, m, k, 0x7e), _cancelling(g, n, k, 0xfe)
+    one = lambda rows: torch.ones(rows, device=DEV)
+    y = ops.fp8_linear(ops.Fp8Rows.from_codes(codes, one(m)), ops.Fp8Weight.from_codes(wcodes, one(n)), out_dtype=out_dtype)
+    ref = codes.view(F8).to(F64) @ wcodes.view(F8).to(F64).t()
+    assert float(ref.abs().max()) < 2.0 ** 17
+    err = (y.to(F64) - ref).abs()
+    assert bool((err <= (HALF[out_dtype] * ref.abs() if out_dtype == BF else 0.0)).all()), float((err / ref.abs()).max())
