@@ -66,6 +66,15 @@ struct LinearArgs {
   int splits;
 };
 
+// Scales as m 2^e, |m| < 1: sums of codes are 0 or of 2^-18 to 2^38, so sum mx mw is far from fp32's ends whatever the scales are, and only the result
+// itself can pass them.  (sum sx sw overflows on the way for sx = 2^107, sw = 2^-25.)
+struct Scale {
+  float m;
+  int e;
+  __device__ __forceinline__ explicit Scale(float s) : m(__builtin_amdgcn_frexp_mantf(s)), e(__builtin_amdgcn_frexp_expf(s)) {}
+};
+__device__ __forceinline__ float scaled(float sum, const Scale &x, const Scale &w) { return __builtin_ldexpf(sum * x.m * w.m, x.e + w.e); }
+
 // Columns col .. col + 3 of a row of y, col a multiple of four.  WHOLE: rows of y are whole vectors.  The flags are chosen once for all of a
 // workgroup's results: asked for at each of the 64 a lane may have, they take longer than eight chunks of columns (20 us of 256 x 256).
 template <bool F32, bool BIAS, bool WHOLE>
@@ -74,7 +83,7 @@ __device__ __forceinline__ void put4(const LinearArgs &a, int64_t row, int64_t c
   const fp8_f32x4 sw = *(const fp8_f32x4 *)(a.sw + col);  // there are scales up to the next multiple of 16
   float v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = sum[i] * sx * sw[i];
+  for (int i = 0; i < 4; ++i) v[i] = scaled(sum[i], Scale(sx), Scale(sw[i]));
   if constexpr (BIAS) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] += pkv_bf16_bits_to_f32(a.bias[WHOLE || col + i < a.n ? col + i : col]);
@@ -208,7 +217,7 @@ __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x1
   const int vec = lane % kVecs, col = vec * (16 / kEs);
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
-    const float sx = a.sx[m0 + 32 * t + row < a.m ? m0 + 32 * t + row : a.m - 1];
+    const Scale sx(a.sx[m0 + 32 * t + row < a.m ? m0 + 32 * t + row : a.m - 1]);
 #pragma unroll
     for (int r = 0; r < TN; ++r)
 #pragma unroll
@@ -218,7 +227,7 @@ __device__ __forceinline__ void block_store(const LinearArgs &a, const fp8_f32x1
         const fp8_f32x4 sw = *(const fp8_f32x4 *)(a.sw + (in ? n0 + c : 0));  // there are scales up to the next multiple of 16
         fp8_f32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = RAW ? acc[r][t][4 * q + i] : acc[r][t][4 * q + i] * sx * sw[i];
+        for (int i = 0; i < 4; ++i) v[i] = RAW ? acc[r][t][4 * q + i] : scaled(acc[r][t][4 * q + i], sx, Scale(sw[i]));
         if (!RAW && a.bias) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] += pkv_bf16_bits_to_f32(a.bias[c + i < left ? n0 + c + i : 0]);

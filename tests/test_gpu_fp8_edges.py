@@ -35,3 +35,18 @@ def test_linear_sums_cancel(m, n, k, out_dtype):
     assert float(ref.abs().max()) < 2.0 ** 17
     err = (y.to(F64) - ref).abs()
     assert bool((err <= (HALF[out_dtype] * ref.abs() if out_dtype == BF else 0.0)).all()), float((err / ref.abs()).max())
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 100, 300), (60, 300, 300), (130, 20000, 384), (145, 955, 12288), (520, 1536, 4096)])
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+@pytest.mark.parametrize("sx,sw", [(2.0 ** 107, 2.0 ** -25), (2.0 ** -25, 2.0 ** 118), (-3e36, 1e-37), (1e-42, 1.7e37), (3e-39, -3e38), (2.0 ** -100, 2.0 ** 100)])
+def test_linear_scales(m, n, k, sx, sw, out_dtype):
+    """Scales of both ends of fp32, subnormal ones among them, whose results are in the middle of it.  Codes 1 to 3.75 of either sign: products are multiples of 2^-6, sums below 2^18,
+    exact; then two roundings for the scales, 2 u |y|, and that to the output's type."""
+    ops, g = _ops(), _gen(m + n)
+    codes, wcodes = ((torch.randint(0x38, 0x48, (r, k), generator=g) + 128 * torch.randint(0, 2, (r, k), generator=g)).to(U8).to(DEV) for r in (m, n))
+    sx, sw = torch.full((m,), sx, device=DEV), torch.full((n,), sw, device=DEV)
+    y = ops.fp8_linear(ops.Fp8Rows.from_codes(codes, sx), ops.Fp8Weight.from_codes(wcodes, sw), out_dtype=out_dtype)
+    ref = codes.view(F8).to(F64) @ wcodes.view(F8).to(F64).t() * (sx.to(F64).unsqueeze(1) * sw.to(F64))
+    err = (y.to(F64) - ref).abs()
+    assert bool((err <= (2 * 2.0 ** -24 + HALF[out_dtype]) * ref.abs()).all()), float((err / ref.abs()).max())
