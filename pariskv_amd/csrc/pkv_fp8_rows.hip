@@ -75,20 +75,20 @@ __global__ __launch_bounds__(THREADS) void pkv_fp8_rows_kernel(RowsArgs a) {
         else load_any<true>(res, left, add);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[r][e] = pkv_bf16_round(v[r][e] + add[e]);
-        if (a.out_sum) {
-          uint16_t *const to = a.out_sum + row * a.width + at;
-          pkv_u32x4 o;
+      }
+      if (a.out_sum) {
+        uint16_t *const to = a.out_sum + row * a.width + at;
+        pkv_u32x4 o;
 #pragma unroll
-          for (int p = 0; p < 4; ++p) o[p] = (__float_as_uint(v[r][2 * p]) >> 16) | (__float_as_uint(v[r][2 * p + 1]) & 0xffff0000u);
-          if constexpr (ALIGNED) {
-            __builtin_nontemporal_store(o, (pkv_u32x4 *)to);
-          } else if (left >= E) {
-            __builtin_memcpy(to, &o, sizeof o);
-          } else {
+        for (int p = 0; p < 4; ++p) o[p] = (__float_as_uint(v[r][2 * p]) >> 16) | (__float_as_uint(v[r][2 * p + 1]) & 0xffff0000u);
+        if constexpr (ALIGNED) {
+          __builtin_nontemporal_store(o, (pkv_u32x4 *)to);
+        } else if (left >= E) {
+          __builtin_memcpy(to, &o, sizeof o);
+        } else {
 #pragma unroll
-            for (int e = 0; e < E - 1; ++e)
-              if (e < left) to[e] = (uint16_t)(__float_as_uint(v[r][e]) >> 16);
-          }
+          for (int e = 0; e < E - 1; ++e)
+            if (e < left) to[e] = (uint16_t)(__float_as_uint(v[r][e]) >> 16);
         }
       }
 #pragma unroll

@@ -10,6 +10,23 @@ from test_gpu_fp8 import BF, DEV, F8, F32, F64, HALF, U8, _gen, _ops
 pytestmark = pytest.mark.gpu
 
 
+# ------------------------------------------------------------------ norms
+
+
+@pytest.mark.parametrize("width", [8, 101, 256, 4096, 4099])
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm_leaves_the_sum(width, residual):
+    """The entry point's out_sum: x + residual, or x where there is no residual."""
+    from pariskv_amd import _lib
+
+    g, rows, wide = _gen(width), 3, -(-width // 128) * 128
+    x, r, w = (torch.randn(n, width, generator=g).to(BF).to(DEV) for n in (rows, rows, 1))
+    total, codes, scales = torch.full_like(x, 7.0), torch.zeros(rows, wide, dtype=U8, device=DEV), torch.zeros(rows, device=DEV)
+    assert _lib.lib().pkv_add_rmsnorm_fp8(x.data_ptr(), r.data_ptr() if residual else None, w.data_ptr(), 1e-6, rows, width, total.data_ptr(), codes.data_ptr(), wide,
+                                          scales.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(total, (x.float() + r.float()).to(BF) if residual else x)
+
+
 # ------------------------------------------------------------------ products
 
 
