@@ -105,9 +105,10 @@ __global__ __launch_bounds__(THREADS) void pkv_fp8_rows_kernel(RowsArgs a) {
     const float inv = (float)(1.0 / sqrt(sum / (double)a.width + a.eps));
 #pragma unroll
     for (int r = 0; r < kReps; ++r) {
-      if ((r * kRowThreads + tid) * E >= a.width) continue;
+      const int left = a.width - (r * kRowThreads + tid) * E;
+      if (left <= 0) continue;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[r][e] = v[r][e] * inv * w[r][e];
+      for (int e = 0; e < E; ++e) v[r][e] = ALIGNED || e < left ? v[r][e] * inv * w[r][e] : 0.f;  // past the row zeros, also where inv is a NaN
     }
   }
 #pragma unroll

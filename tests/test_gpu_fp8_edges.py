@@ -27,6 +27,18 @@ def test_norm_leaves_the_sum(width, residual):
     assert torch.equal(total, (x.float() + r.float()).to(BF) if residual else x)
 
 
+@pytest.mark.parametrize("width", [1, 100, 101, 1021, 4099])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_norm_padding(width, bad):
+    """Zeros follow a row up to the next multiple of 128 columns, whatever is in it."""
+    ops, g = _ops(), _gen(width)
+    x = torch.randn(2, width, generator=g).to(BF)
+    x[1, width // 2] = bad
+    _, q = ops.add_rmsnorm_fp8(x.to(DEV), None, torch.ones(width, dtype=BF, device=DEV), 1e-6)
+    assert bool(q.codes.float().isnan().any(1).cpu()[1]) and not bool(q.codes.float().isnan().any(1).cpu()[0])
+    assert not bool(q.padded.view(U8)[:, width:].any())
+
+
 # ------------------------------------------------------------------ products
 
 
