@@ -621,7 +621,7 @@ typedef struct pkv_fp8_kv {
 /* Rows into a cache in eight bits (no counterpart in the reference; what pkv_append_kv and a prompt's copy are for bf16 caches).  Token t of
  * sequence b, heads h of k and v [bs][n_tokens][n_kv_heads][128] of `dtype` (strides in elements, 16-byte multiples; rows
  * contiguous), becomes row starts[b] + t (`start` + t where starts is NULL) for t < lengths[b] (NULL: all).  A block whose
- * first rows are there already, before starts[b], keeps them: its scale becomes the larger of the one it has and the one that the new rows
+ * first rows are there already, before starts[b], keeps them: its scale becomes the larger, in magnitude, of the one it has and the one that the new rows
  * need, and where it grows the older codes are rounded again.  Rows behind the written ones stay as they are, but where they share a
  * block with written ones they hold nothing that counts.  A sequence whose start is not a row of the cache, or whose length is <= 0, stores
  * nothing; rows past the capacity are left out. */

@@ -1,7 +1,7 @@
 // A K/V cache in eight bits: rows quantised as they are written, and read back.  (No counterpart in the reference, whose caches are bf16.)
 //
 // Row r of head h of sequence b is 128 e4m3 codes; the rows of a block of 16, 32, 64 or 128 share one scale each for K and for V
-// (pkv_fp8.h).  Rows written behind others in a block keep those: the scale is the larger of what stands there and what the new rows
+// (pkv_fp8.h).  Rows written behind others in a block keep those: the scale is the larger (in magnitude) of what stands there and what the new rows
 // need, and where it grows the older rows' codes are rounded again under it.  Rows from the block's first one on start it anew.
 #include "pkv_fp8.h"
 
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kStoreThreads) void pkv_fp8_store_kernel(StoreArgs 
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kStoreThreads / PKV_WAVE; ++w) top = s_top[w] > top ? s_top[w] : top;
-  const float need = fp8_pow2(fp8_exponent(top)), scale = was > need ? was : need;
+  const float need = fp8_pow2(fp8_exponent(top)), scale = fabsf(was) > need ? was : need;  // a scale that the caller set may be negative
   const float inv = 1.0f / scale;  // exact where the scale is a power of two, as it is unless the caller set it
 #pragma unroll
   for (int i = 0; i < kIter; ++i) {

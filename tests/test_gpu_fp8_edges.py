@@ -5,9 +5,39 @@ import math
 import pytest
 import torch
 
-from test_gpu_fp8 import BF, DEV, F8, F32, F64, HALF, U8, _gen, _ops
+from test_gpu_fp8 import BF, DEV, F8, F32, F64, HALF, U8, _exponent, _gen, _ops, _round, _top
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ the cache
+
+
+@pytest.mark.parametrize("was", [-4.0, 4.0, -0.02, 0.02, -3.7, 2.9, -(2.0 ** -12), 2.0 ** -120, -1e30, 0.0])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_store_behind_any_scale(was, dtype):
+    """Rows behind those of a block whose scale the caller set, negative or no power of two: the older rows stay.  The scale is the old one where that is the larger in
+    magnitude; then older codes are untouched, and a new one is that of x times fp32(1 / scale), off by 2 u of itself before it is rounded.  Else it is
+    the power of two that the new rows need, and an older code is rounded again, exactly as the oracle does where the old scale is a power of two, else after
+    a product off by u."""
+    ops, g = _ops(), _gen(17)
+    old = torch.randint(0, 0x78, (1, 2, 32, 128), generator=g).to(U8)
+    old[0, 0, 3:5] |= 0x80
+    scale = torch.full((1, 2, 2), was)
+    cache = ops.Fp8KVCache.from_codes(old.clone().to(DEV), scale.clone().to(DEV), old.clone().to(DEV), scale.clone().to(DEV), block=16)
+    x = torch.randn(1, 2, 2, 128, generator=g).to(dtype)
+    cache.store(x.to(DEV), x.to(DEV), 5)
+    need = torch.exp2(_exponent(_top(x.to(F64)).amax((1, 3))))  # [1, heads]
+    held = torch.tensor(was, dtype=F32).to(F64)
+    for codes, scales in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        codes, scales = codes.float().cpu().to(F64), scales.cpu().to(F64)
+        s = torch.where(held.abs() > need, held, need)
+        assert torch.equal(scales[:, :, 0], s) and torch.equal(scales[:, :, 1], held.expand(1, 2))
+        slack = torch.tensor([1 - 4 * 2.0 ** -24, 1 + 4 * 2.0 ** -24], dtype=F64).view(2, 1, 1, 1, 1)
+        for got, exact in ((codes[:, :, :5], old.view(F8).float().to(F64)[:, :, :5] * (held / s).view(1, 2, 1, 1)), (codes[:, :, 5:7], x.to(F64).transpose(1, 2) / s.view(1, 2, 1, 1))):
+            ends = _round(exact * slack)
+            assert bool((got >= ends.amin(0)).all()) and bool((got <= ends.amax(0)).all())
+        assert torch.equal(codes[:, :, 7:], old.view(F8).float().to(F64)[:, :, 7:])
 
 
 # ------------------------------------------------------------------ norms
