@@ -66,11 +66,16 @@ class fp8_cache(KV_Cache):
             self.context = n
         return k, v
 
+    def _rows_of(self, layer_idx):
+        """How many rows every sequence has in a layer."""
+        n, rows = self.current_seq_len[layer_idx], self._prefilled[layer_idx]
+        if rows.count(n) != self.batch_size:
+            raise RuntimeError("sequences of several lengths: every sample's prompt has to have as many rows")
+        return n
+
     def decode_update_kv_cache(self, key_states, value_states, layer_idx):
         """Rows [bs,T,Hkv,D] of the next tokens of every sequence, behind those that are there."""
-        n, T = self.current_seq_len[layer_idx], key_states.shape[1]
-        if any(rows != n for rows in self._prefilled[layer_idx]):
-            raise RuntimeError("sequences of several lengths: every sample's prompt has to have as many rows")
+        n, T = self._rows_of(layer_idx), key_states.shape[1]
         if n + T > self.max_length:
             raise RuntimeError(f"{n} + {T} rows in a cache of {self.max_length}")
         self.layers[layer_idx].store(key_states, value_states, n)
@@ -82,7 +87,7 @@ class fp8_cache(KV_Cache):
 
     def compute(self, queries, layer_idx):
         """Attention of the last T tokens, [bs,T,Hq,D] -> [bs,T,Hq,D]: each sees the rows up to its own."""
-        return self._attention.run(queries, self.layers[layer_idx], [(0, self.current_seq_len[layer_idx])])
+        return self._attention.run(queries, self.layers[layer_idx], [(0, self._rows_of(layer_idx))])
 
     def draft_attend(self, queries, key_states, value_states, layer_idx, mask=None):
         raise RuntimeError("drafted tokens: polar_cache attends to them")

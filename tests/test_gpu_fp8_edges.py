@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_fp8 import BF, DEV, F8, F32, F64, HALF, U8, _exponent, _gen, _ops, _round, _top
+from test_gpu_fp8 import BF, D, DEV, F8, F32, F64, HALF, U8, _exponent, _gen, _ops, _round, _top
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,27 @@ def test_linear_scales(m, n, k, sx, sw, out_dtype):
     ref = codes.view(F8).to(F64) @ wcodes.view(F8).to(F64).t() * (sx.to(F64).unsqueeze(1) * sw.to(F64))
     err = (y.to(F64) - ref).abs()
     assert bool((err <= (2 * 2.0 ** -24 + HALF[out_dtype]) * ref.abs()).all()), float((err / ref.abs()).max())
+
+
+# ------------------------------------------------------------------ the dense cache
+
+
+def test_dense_cache_lengths():
+    """Attention over sequences whose prompts differ in length is refused, as their next rows are: there is one length for all."""
+    from pariskv_amd.cache_hub.fp8_cache import fp8_cache
+
+    g, bs = _gen(3), 2
+    cache = fp8_cache(0, 2, bs, 40, 2, 4, D, BF, {"0": DEV, "1": DEV})
+    k, q = torch.randn(bs, 30, 2, D, generator=g).to(BF).to(DEV), torch.randn(bs, 1, 4, D, generator=g).to(BF).to(DEV)
+    cache.prefill_update_kv_cache(None, k[:1, :20], k[:1, :20], 0, 0)
+    for n in (None, 23):  # the other sample without a prompt, and with a longer one
+        if n:
+            cache.prefill_update_kv_cache(None, k[1:, :n], k[1:, :n], 0, 1)
+        with pytest.raises(RuntimeError, match="several lengths"):
+            cache.compute(q, 0)
+        with pytest.raises(RuntimeError, match="several lengths"):
+            cache.decode_update_kv_cache(k[:, :1], k[:, :1], 0)
+    cache.prefill_update_kv_cache(None, k[1:, :20], k[1:, :20], 0, 1)
+    want = cache.compute(q, 0)
+    cache.prefill_update_kv_cache(None, k[:, :20], k[:, :20], 1, 0)
+    assert torch.equal(cache.compute(q, 1), want)
