@@ -447,32 +447,33 @@ Plan linear_plan(int64_t m, int64_t n, int64_t k) {
   return best;
 }
 
-// Codes [n][k] into tiles and back: one 16-byte vector of a tile a thread.
+// Codes [n][k] into tiles, one 16-byte vector of a tile a thread at a time, and back, element by element.  A launch has fewer than 2^32 threads.
+constexpr int64_t kMostBlocks = (int64_t)1 << 23;
 __global__ __launch_bounds__(256) void pkv_fp8_pack_kernel(const uint8_t *__restrict__ codes, const float *__restrict__ scales, int64_t n, int64_t k,
                                                            int64_t stride, int chunks, int64_t vecs, uint8_t *__restrict__ tiles, float *__restrict__ sw) {
-  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t rows = (n + kTileRows - 1) / kTileRows * kTileRows;
-  if (v < rows) sw[v] = v < n ? scales[v] : 0.f;
-  if (v >= vecs) return;
-  const int lane = (int)(v & 63), h = (int)(v >> 6) & 1;
-  const int64_t tc = v >> 7, tile = tc / chunks, c = tc - tile * chunks;
-  const int64_t row = tile * 16 + (lane & 15), col = c * kTileCols + h * 64 + (lane >> 4) * 16;
-  uint8_t out[16];
+  for (int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x; v < vecs; v += kMostBlocks * 256) {
+    if (v < rows) sw[v] = v < n ? scales[v] : 0.f;  // there are more vectors than rows
+    const int lane = (int)(v & 63), h = (int)(v >> 6) & 1;
+    const int64_t tc = v >> 7, tile = tc / chunks, c = tc - tile * chunks;
+    const int64_t row = tile * 16 + (lane & 15), col = c * kTileCols + h * 64 + (lane >> 4) * 16;
+    uint8_t out[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) out[i] = row < n && col + i < k ? codes[row * stride + col + i] : (uint8_t)0;
-  pkv_u32x4 o;
-  memcpy(&o, out, 16);
-  *(pkv_u32x4 *)(tiles + v * 16) = o;
+    for (int i = 0; i < 16; ++i) out[i] = row < n && col + i < k ? codes[row * stride + col + i] : (uint8_t)0;
+    pkv_u32x4 o;
+    memcpy(&o, out, 16);
+    *(pkv_u32x4 *)(tiles + v * 16) = o;
+  }
 }
 
 __global__ __launch_bounds__(256) void pkv_fp8_unpack_kernel(const uint8_t *__restrict__ tiles, const float *__restrict__ sw, int64_t n, int64_t k,
                                                              int chunks, float *__restrict__ w) {
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= n * k) return;
-  const int64_t row = e / k, col = e - row * k;
-  const int in = (int)(col & 127);
-  const uint8_t code = tiles[((row >> 4) * chunks + (col >> 7)) * kTileBytes + (in >> 6) * 1024 + (((in & 63) >> 4) * 16 + (row & 15)) * 16 + (in & 15)];
-  w[e] = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false)[0] * sw[row];
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n * k; e += kMostBlocks * 256) {
+    const int64_t row = e / k, col = e - row * k;
+    const int in = (int)(col & 127);
+    const uint8_t code = tiles[((row >> 4) * chunks + (col >> 7)) * kTileBytes + (in >> 6) * 1024 + (((in & 63) >> 4) * 16 + (row & 15)) * 16 + (in & 15)];
+    w[e] = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false)[0] * sw[row];
+  }
 }
 
 bool matrix_ok(int64_t n, int64_t k) { return n > 0 && n < ((int64_t)1 << 31) - 16 && k > 0 && k <= ((int64_t)1 << 20); }
@@ -489,9 +490,8 @@ extern "C" int pkv_fp8_pack(const uint8_t *codes, int64_t row_stride, const floa
   PKV_REQUIRE(codes && scales && packed, "pkv_fp8_pack: null pointer");
   PKV_REQUIRE(matrix_ok(n, k) && row_stride >= k, "pkv_fp8_pack: bad matrix %lld x %lld", (long long)n, (long long)k);
   PKV_REQUIRE(pkv_aligned(packed, 16) && pkv_aligned(scales, 4), "pkv_fp8_pack: 16-byte aligned buffers required");
-  const int64_t vecs = (int64_t)(tile_bytes(n, k) / 16);
-  PKV_REQUIRE(vecs / 256 < ((int64_t)1 << 31), "pkv_fp8_pack: matrix too large");
-  hipLaunchKernelGGL(pkv_fp8_pack_kernel, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, (hipStream_t)stream, codes, scales, n, k, row_stride,
+  const int64_t vecs = (int64_t)(tile_bytes(n, k) / 16), blocks = (vecs + 255) / 256;
+  hipLaunchKernelGGL(pkv_fp8_pack_kernel, dim3((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks)), dim3(256), 0, (hipStream_t)stream, codes, scales, n, k, row_stride,
                      chunks_of(k), vecs, (uint8_t *)packed, (float *)((uint8_t *)packed + tile_bytes(n, k)));
   PKV_LAUNCH_CHECK("pkv_fp8_pack_kernel");
   return PKV_OK;
@@ -499,8 +499,9 @@ extern "C" int pkv_fp8_pack(const uint8_t *codes, int64_t row_stride, const floa
 
 extern "C" int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w, void *stream) {
   PKV_REQUIRE(packed && w, "pkv_fp8_unpack: null pointer");
-  PKV_REQUIRE(matrix_ok(n, k) && pkv_aligned(packed, 16) && n * k / 256 < ((int64_t)1 << 31), "pkv_fp8_unpack: bad matrix %lld x %lld", (long long)n, (long long)k);
-  hipLaunchKernelGGL(pkv_fp8_unpack_kernel, dim3((unsigned)((n * k + 255) / 256)), dim3(256), 0, (hipStream_t)stream, (const uint8_t *)packed,
+  PKV_REQUIRE(matrix_ok(n, k) && pkv_aligned(packed, 16), "pkv_fp8_unpack: bad matrix %lld x %lld", (long long)n, (long long)k);
+  const int64_t blocks = (n * k + 255) / 256;
+  hipLaunchKernelGGL(pkv_fp8_unpack_kernel, dim3((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks)), dim3(256), 0, (hipStream_t)stream, (const uint8_t *)packed,
                      (const float *)((const uint8_t *)packed + tile_bytes(n, k)), n, k, chunks_of(k), w);
   PKV_LAUNCH_CHECK("pkv_fp8_unpack_kernel");
   return PKV_OK;

@@ -157,8 +157,16 @@ int launch_as(const RowsArgs &a, int64_t rows, hipStream_t s) {
   return PKV_OK;
 }
 template <bool NORM, bool BF16>
-int launch(const RowsArgs &a, int64_t rows, bool aligned, hipStream_t s) {
-  return aligned ? launch_as<NORM, BF16, true>(a, rows, s) : launch_as<NORM, BF16, false>(a, rows, s);
+int launch(RowsArgs a, int64_t rows, bool aligned, hipStream_t s) {
+  constexpr int64_t kMost = (int64_t)1 << 21;  // rows of a launch, which has fewer than 2^32 threads; the next ones begin at a multiple of 16 bytes where these do
+  for (;;) {
+    const int64_t n = rows < kMost ? rows : kMost;
+    if (const int rc = aligned ? launch_as<NORM, BF16, true>(a, n, s) : launch_as<NORM, BF16, false>(a, n, s)) return rc;
+    if ((rows -= n) == 0) return PKV_OK;
+    a.x += n * a.x_stride, a.codes += n * a.code_stride, a.scales += n;
+    if (a.residual) a.residual += n * a.width;
+    if (a.out_sum) a.out_sum += n * a.width;
+  }
 }
 
 int shape_ok(const char *who, int64_t rows, int64_t width, const void *codes, int64_t code_stride, const void *scales) {

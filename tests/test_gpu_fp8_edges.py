@@ -69,7 +69,37 @@ def test_norm_padding(width, bad):
     assert not bool(q.padded.view(U8)[:, width:].any())
 
 
+def test_rows_more_than_2_to_26():
+    """More rows than a launch has waves, which has fewer than 2^32 threads."""
+    ops, g = _ops(), _gen(4)
+    few, times, rest = 4096, 1 << 14, 5
+    x = torch.randn(few, 8, generator=g).to(BF).to(DEV)
+    want = ops.fp8_rows(x)
+    q = ops.fp8_rows(torch.cat([x.repeat(times, 1), x[:rest]]))
+    ones = torch.ones(8, dtype=BF, device=DEV)
+    normed, norm = ops.add_rmsnorm_fp8(x, None, ones, 1e-6)[1], ops.add_rmsnorm_fp8(torch.cat([x.repeat(times, 1), x[:rest]]), None, ones, 1e-6)[1]
+    for got, ref in ((q, want), (norm, normed)):
+        codes, ref_codes, n = got.padded.view(U8), ref.padded.view(U8), few * times
+        assert torch.equal(got.scales[:n].view(times, few), ref.scales.expand(times, few)) and torch.equal(got.scales[n:], ref.scales[:rest])
+        for i in range(0, times, 1 << 12):
+            part = codes[i * few:(i + (1 << 12)) * few].view(1 << 12, few, 128)
+            assert bool((part == ref_codes).all())
+        assert torch.equal(codes[n:], ref_codes[:rest])
+
+
 # ------------------------------------------------------------------ products
+
+
+def test_matrix_of_more_than_2_to_32():
+    """A matrix of more elements than a launch has threads, there and back."""
+    ops, n, k = _ops(), (1 << 16) + 3, 1 << 16
+    row = torch.randint(0, 0x78, (1 << 10, k), generator=_gen(5)).to(U8).to(DEV)
+    codes = row.repeat(-(-n // (1 << 10)), 1)[:n]
+    scales = torch.exp2((torch.arange(n, device=DEV) % 7).float())
+    w = ops.Fp8Weight.from_codes(codes, scales).dequantize()
+    for i in range(0, n, 1 << 12):
+        assert torch.equal(w[i:i + (1 << 12)], codes[i:i + (1 << 12)].view(F8).float() * scales[i:i + (1 << 12)].unsqueeze(1))
+
 
 
 def _cancelling(g, rows, k, second):
