@@ -691,6 +691,10 @@ int pkv_fp8_pack(const uint8_t *codes, int64_t row_stride, const float *scales, 
 /* The matrix back from its stored form, fp32 [n][k] contiguous (no counterpart in the reference). */
 int pkv_fp8_unpack(const void *packed, int64_t n, int64_t k, float *w, void *stream);
 
+/* How a product of that size is dealt out (no counterpart in the reference; nothing is launched): plan[0] rows of x by plan[1] rows of the matrix a workgroup, plan[2]
+ * splits of the columns, plan[3] workgroups at once to a compute unit. */
+int pkv_fp8_linear_plan(int64_t rows, int64_t n, int64_t k, int *plan);
+
 /* y[m][n] = x_scales[m] scale[n] sum_k x[m][k] code[n][k] + bias[n] (no counterpart in the reference): x codes [rows], x_stride bytes apart
  * (16-byte multiples, 16-byte aligned), zeros past k up to the next multiple of 128, as pkv_fp8_rows leaves them; bias bf16 [n] or NULL; y [rows][n] contiguous of out_dtype.  Sums of codes in
  * fp32, then the scales; at most 2^22 rows and 2^40 results.  ws: pkv_fp8_linear_ws_bytes(rows, n, k, out_dtype) bytes for the sums of columns that are split (0: none

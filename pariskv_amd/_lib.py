@@ -219,6 +219,7 @@ PROTOTYPES = {
     "pkv_fp8_pack": (_i, [_vp, _i64, _vp, _i64, _i64, _vp, _vp]),
     "pkv_fp8_unpack": (_i, [_vp, _i64, _i64, _vp, _vp]),
     "pkv_fp8_linear_ws_bytes": (_sz, [_i64, _i64, _i64, _i]),
+    "pkv_fp8_linear_plan": (_i, [_i64, _i64, _i64, C.POINTER(_i)]),
     "pkv_fp8_linear": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i, _vp, _sz, _vp]),
     "pkv_w4_silu_mul": (_i, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i, _vp, _vp, _sz, _vp]),
     "pkv_decode_attention": (_i, [_vp, _i, _i, _i, _i, C.POINTER(AttnSegment), _i, _vp, C.c_float, _vp, _vp, _sz, _vp]),

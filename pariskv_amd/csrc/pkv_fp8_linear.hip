@@ -409,6 +409,13 @@ struct Plan {
   Shape shape;
   int splits;
 };
+struct Kind {
+  int bm, bn, at_once;
+  double start, each, rate;  // KB a us of a compute unit
+};
+const Kind kKinds[] = {{16, 16, 1, 2.4, 0.85, 43}, {16, 32, 1, 2.4, 0.85, 43}, {16, 64, 1, 2.4, 0.85, 43},   {32, 32, 1, 2.4, 0.85, 43}, {32, 64, 1, 2.4, 0.85, 43},
+                       {64, 64, 1, 4.5, 2.5, 58},  {64, 128, 1, 4.5, 3.5, 57},  {128, 64, 1, 4.5, 3.5, 53},  {128, 128, 1, 4.5, 5.0, 36}, {128, 128, 2, 4.5, 5.0, 44}};
+static_assert(sizeof kKinds / sizeof kKinds[0] == kBlock22Two + 1, "a row a shape");
 
 // The shape and number of splits of the least estimate, in us: a start, and for each round of workgroups (one to a compute unit; of kBlock22Two two)
 // another one and what they read at what a compute unit takes in with that shape, or the matrix at what memory gives, whichever is longer and a tenth of the other; splits write their sums, read again by a
@@ -418,13 +425,6 @@ struct Plan {
 // 145 x (955 x 12288), 64x64 block in 1 / 4 / 5 / 8 splits 35.8 / 16.1 / 14.8 / 15.9; 128x128 blocks, one to a compute unit with four buffers / two with two:
 // 4096 x (6144 x 4096) 206 / 176-190, 1024 x (4096 x 4096) 36.9 / 35.6.
 Plan linear_plan(int64_t m, int64_t n, int64_t k) {
-  struct Kind {
-    int bm, bn, at_once;
-    double start, each, rate;  // KB a us of a compute unit
-  };
-  static const Kind kKinds[] = {{16, 16, 1, 2.4, 0.85, 43}, {16, 32, 1, 2.4, 0.85, 43}, {16, 64, 1, 2.4, 0.85, 43},   {32, 32, 1, 2.4, 0.85, 43}, {32, 64, 1, 2.4, 0.85, 43},
-                                {64, 64, 1, 4.5, 2.5, 58},  {64, 128, 1, 4.5, 3.5, 57},  {128, 64, 1, 4.5, 3.5, 53},  {128, 128, 1, 4.5, 5.0, 36}, {128, 128, 2, 4.5, 5.0, 44}};
-  static_assert(sizeof kKinds / sizeof kKinds[0] == kBlock22Two + 1, "a row a shape");
   const int chunks = chunks_of(k);
   Plan best = {kStream11, 1};
   double least = 0;
@@ -511,6 +511,15 @@ extern "C" size_t pkv_fp8_linear_ws_bytes(int64_t rows, int64_t n, int64_t k, in
   if (!rows_ok(rows, n, k)) return 0;
   const int splits = linear_plan(rows, n, k).splits;
   return splits == 1 ? 0 : (size_t)splits * rows * ((n + 3) / 4 * 4) * sizeof(float);
+}
+
+extern "C" int pkv_fp8_linear_plan(int64_t rows, int64_t n, int64_t k, int *plan) {
+  PKV_REQUIRE(plan, "pkv_fp8_linear_plan: null pointer");
+  PKV_REQUIRE(rows_ok(rows, n, k), "pkv_fp8_linear_plan: bad shape %lld rows, %lld x %lld", (long long)rows, (long long)n, (long long)k);
+  const Plan p = linear_plan(rows, n, k);
+  const Kind &q = kKinds[p.shape];
+  plan[0] = q.bm, plan[1] = q.bn, plan[2] = p.splits, plan[3] = q.at_once;
+  return PKV_OK;
 }
 
 extern "C" int pkv_fp8_linear(const uint8_t *x, int64_t x_stride, const float *x_scales, int64_t rows, const void *packed, int64_t n, int64_t k, const void *bias,

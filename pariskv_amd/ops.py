@@ -1487,6 +1487,12 @@ class Fp8Weight:
         """Bytes of workspace that a product of ``rows`` rows takes."""
         return self._ws_bytes(rows, _dt(out_dtype))
 
+    def plan(self, rows: int):
+        """How a product of ``rows`` rows is dealt out: (rows of x, rows of the matrix) a workgroup, splits of the columns, workgroups at once to a compute unit."""
+        plan = (C.c_int * 4)()
+        _lib.check(_lib.lib().pkv_fp8_linear_plan(rows, self.n, self.k, plan))
+        return tuple(plan)
+
     def _ws_bytes(self, rows, code):
         need = self._ws.get((rows, code))
         if need is None:

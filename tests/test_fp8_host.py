@@ -318,3 +318,23 @@ def test_struct_mirrors():
     for which, mirror in ((10, _lib.Fp8Kv), (11, _lib.Fp8AttnArgs)):
         assert _lib.lib().pkv_struct_bytes(which) == ctypes.sizeof(mirror) > 0
     assert ops._FP8_ATTN_BLOCK.size == ctypes.sizeof(_lib.Fp8AttnArgs)
+
+
+def test_product_plan():
+    L, plan = _lib.lib(), (ctypes.c_int * 4)()
+    for bad in ((0, 955, 12288), (145, 0, 12288), (145, 955, 0), ((1 << 22) + 1, 955, 12288), (145, 1 << 31, 128)):
+        assert L.pkv_fp8_linear_plan(*bad, plan) == _lib.EINVAL, bad
+    assert L.pkv_fp8_linear_plan(145, 955, 12288, None) == _lib.EINVAL
+    for m, n, k in ((1, 1, 1), (16, 4096, 4096), (17, 4096, 4096), (145, 955, 12288), (4096, 6144, 4096), (1 << 22, 16, 128), (1 << 22, 1 << 15, 128), (1, 1 << 28, 128)):
+        assert L.pkv_fp8_linear_plan(m, n, k, plan) == 0
+        bm, bn, splits, at_once = plan
+        assert bm in (16, 32, 64, 128) and bn in (16, 32, 64, 128) and at_once in (1, 2) and 1 <= splits <= 16 and splits <= -(-k // 128)
+        # the workspace is that of these splits, and a launch's workgroups and threads are within its limits
+        for dtype in (_lib.DTYPE_BF16, _lib.DTYPE_F32):
+            assert L.pkv_fp8_linear_ws_bytes(m, n, k, dtype) == (0 if splits == 1 else splits * m * (-(-n // 4) * 4) * 4)
+        down, across, threads = -(-m // bm), -(-n // bn), 512 if bm * bn <= 2048 else 256
+        assert (down <= 65535 and across * threads < 1 << 32) if threads == 512 else down * across * threads < 1 << 32
+    weight = _weight()
+    assert weight.plan(3) == (16, 16, 1, 1)
+    with pytest.raises(RuntimeError):
+        weight.plan(0)

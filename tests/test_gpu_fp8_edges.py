@@ -126,6 +126,49 @@ def test_linear_sums_cancel(m, n, k, out_dtype):
     assert bool((err <= (HALF[out_dtype] * ref.abs() if out_dtype == BF else 0.0)).all()), float((err / ref.abs()).max())
 
 
+# (rows of x, rows of the matrix) a workgroup, split or not, workgroups at once to a compute unit: products that are dealt out so
+PLANS = {
+    (16, 16, False, 1): [(1, 17, 103), (15, 1003, 1185), (16, 512, 4096)],
+    (16, 32, False, 1): [(1, 4103, 101), (13, 8000, 640)],
+    (16, 64, False, 1): [(1, 8255, 101), (16, 20000, 256)],
+    (32, 32, False, 1): [(17, 4285, 105), (32, 5000, 512)],
+    (32, 64, False, 1): [(17, 8599, 101), (31, 12000, 384)],
+    (64, 64, False, 1): [(33, 10297, 1431), (520, 1536, 4096)],
+    (64, 64, True, 1): [(17, 17, 6173), (145, 955, 12288), (64, 512, 8192)],
+    (64, 128, False, 1): [(35, 31537, 293), (256, 6144, 4096), (64, 24576, 4096)],
+    (64, 128, True, 1): [(17, 8401, 5691), (256, 4096, 12288)],
+    (128, 64, False, 1): [(97, 16229, 267), (110, 16000, 640)],
+    (128, 64, True, 1): [(67, 1713, 6593), (78, 2448, 12288)],
+    (128, 128, False, 1): [(65, 32199, 137), (1024, 4096, 4096)],
+    (128, 128, True, 1): [(65, 9813, 6033), (68, 9360, 5760)],
+    (128, 128, False, 2): [(67, 38391, 105), (520, 9001, 1000), (4096, 6144, 512)],
+}
+
+
+@pytest.mark.parametrize("plan,m,n,k", [(plan, *case) for plan, cases in PLANS.items() for case in cases])
+def test_linear_every_kernel(plan, m, n, k):
+    """Every kernel that the rule for shapes picks, bf16 and fp32 results, with and without a bias, odd and whole sizes; the case is one of the kernel it stands for.
+    Codes 1 to 3.75 of either sign: products are multiples of 2^-6, sums below 2^18, exact in fp32; two roundings for the scales, one for the bias, one to
+    the output's type."""
+    ops, g = _ops(), _gen(m + n + k)
+    codes, wcodes = ((torch.randint(0x38, 0x48, (r, k), generator=g) + 128 * torch.randint(0, 2, (r, k), generator=g)).to(U8).to(DEV) for r in (m, n))
+    sx, sw = (torch.rand(m, generator=g) + 0.1).to(DEV), (torch.rand(n, generator=g) - 0.5).to(DEV)
+    weight, rows = ops.Fp8Weight.from_codes(wcodes, sw), ops.Fp8Rows.from_codes(codes, sx)
+    bm, bn, splits, at_once = weight.plan(m)
+    assert (bm, bn, splits > 1, at_once) == plan
+    ref = codes.view(F8).to(F64) @ wcodes.view(F8).to(F64).t() * sx.to(F64).unsqueeze(1) * sw.to(F64)
+    for bias in (None, torch.randn(n, generator=g).to(BF).to(DEV)):
+        want, tol = ref, 2 * 2.0 ** -24 * ref.abs()
+        if bias is not None:
+            want = ref + bias.to(F64)
+            tol = tol + 2.0 ** -24 * (want.abs() + tol)
+        for out_dtype in (BF, F32):
+            y = ops.fp8_linear(rows, weight, bias=bias, out_dtype=out_dtype)
+            assert y.dtype == out_dtype and (weight.ws_bytes(m, out_dtype) > 0) == (splits > 1)
+            err = (y.to(F64) - want).abs()
+            assert bool((err <= tol + (HALF[out_dtype] * (want.abs() + tol) if out_dtype == BF else 0.0) + 1e-30).all()), (out_dtype, float((err / want.abs()).max()))
+
+
 @pytest.mark.parametrize("m,n,k", [(5, 100, 300), (60, 300, 300), (130, 20000, 384), (145, 955, 12288), (520, 1536, 4096)])
 @pytest.mark.parametrize("out_dtype", [BF, F32])
 @pytest.mark.parametrize("sx,sw", [(2.0 ** 107, 2.0 ** -25), (2.0 ** -25, 2.0 ** 118), (-3e36, 1e-37), (1e-42, 1.7e37), (3e-39, -3e38), (2.0 ** -100, 2.0 ** 100)])
