@@ -40,6 +40,86 @@ def test_store_behind_any_scale(was, dtype):
         assert torch.equal(codes[:, :, 7:], old.view(F8).float().to(F64)[:, :, 7:])
 
 
+# ------------------------------------------------------------------ attention in fp32
+
+
+class Pinned:
+    """Inputs of fp32 attention whose result is known to a few units in the last place: q [bs,T,H*G,128], codes and scales of K and V (blocks of 16), the result in
+    64 bits and how far a number may be off, relative to itself.  ``cut(q)`` and ``cut(weights)`` stand for a kernel that holds fewer bits of them."""
+
+    def result(self, cut_q=lambda x: x, cut_weights=lambda x: x):
+        bs, H, n, _ = self.k.shape
+        T, G = self.q.shape[1], self.q.shape[2] // H
+        k, v = (c.view(F8).float().to(F64) for c in (self.k, self.v))
+        ks, vs = (s.to(F64).repeat_interleave(16, -1)[:, :, :n] for s in (self.k_scale, self.v_scale))
+        q = cut_q(self.q).to(F64).view(bs, T, H, G, D).permute(0, 2, 1, 3, 4)
+        z = (q.reshape(bs, H, T * G, D) @ k.transpose(2, 3)) * ks.unsqueeze(2) * self.scale
+        seen = torch.arange(n) < n - (T - 1 - torch.arange(T).repeat_interleave(G)).unsqueeze(1)
+        p = torch.softmax(z.masked_fill(~seen, -math.inf), -1)
+        top = p.amax(-1, keepdim=True)  # weights relative to the largest, as a kernel holds them
+        o = (cut_weights((p / top * vs.unsqueeze(2)).to(F32)).to(F64) @ v) * top
+        return o.view(bs, H, T, G, D).permute(0, 2, 1, 3, 4).reshape(bs, T, H * G, D)
+
+    def holds(self, out):
+        want = self.result()
+        return bool(((out.cpu().to(F64) - want).abs() <= self.bound * want.abs() + 1e-18).all())
+
+
+def pinned_weights(n, T, G, seed):
+    """All scores 0: weights are 1 and their sum is a whole number, exactly.  A dim has one value other than 0 among all keys, whose scale has 24 bits: a number out is code * scale / keys,
+    off by an addition of the parts' products, the division's two roundings and the joining of waves and splits: 8 steps, 16 u."""
+    c, g, bs, H = Pinned(), _gen(seed), 2, 2
+    blocks = -(-n // 16)
+    c.q = torch.zeros(bs, T, H * G, D)
+    c.k = torch.randint(0, 0x78, (bs, H, blocks * 16, D), generator=g).to(U8)[:, :, :n]
+    c.v = torch.zeros(bs, H, n, D, dtype=U8)
+    c.k_scale, c.v_scale = (torch.rand(bs, H, blocks, generator=g) + 1.0 for _ in range(2))
+    c.v_scale *= torch.exp2(torch.randint(-20, 20, (bs, H, blocks), generator=g).float())
+    for b in range(bs):
+        for h in range(H):
+            at = torch.randint(0, max(1, n - T + 1), (D,), generator=g)
+            c.v[b, h, at, torch.arange(D)] = torch.randint(0x30, 0x78, (D,), generator=g).to(U8)
+    c.scale, c.bound = 1 / math.sqrt(D), 16 * 2.0 ** -24
+    return c
+
+
+def pinned_scores(n, G, seed):
+    """A head has two keys with one code 1 each, at two dims of q, all others are 0: the scores are two numbers of q, of 24 bits, 64 to 128 and at most 2 apart, and 0, whose weight is nothing (n 2^-64).
+    A score in powers of two, S <= 186, is off by a rounding, u S, the base that a wave, and a split, subtracts by as much: 4 u S in a difference, which is as much of a weight times
+    log 2, and twice that in the ratio's denominator; the scale's rounding moves the difference by 2 u 3; exponentials, sums and the division are some 40 u."""
+    c, g, bs, H = Pinned(), _gen(seed), 2, 4
+    blocks = -(-n // 16)
+    a = 64 + torch.randint(0, 1 << 23, (bs, 1, H * G), generator=g).double() * 2.0 ** -17
+    b = (a + torch.randint(-(1 << 18), 1 << 18, a.shape, generator=g).double() * 2.0 ** -17).clamp(64, 128 - 2.0 ** -17)
+    c.q = torch.randn(bs, 1, H * G, D, generator=g)
+    c.k, c.v = torch.zeros(bs, H, n, D, dtype=U8), torch.zeros(bs, H, n, D, dtype=U8)
+    c.k_scale, c.v_scale = torch.ones(bs, H, blocks), torch.ones(bs, H, blocks)
+    for i in range(bs):
+        for h in range(H):
+            dims, keys = torch.randperm(D, generator=g)[:2], torch.randperm(n, generator=g)[:2]
+            c.q[i, 0, h * G:(h + 1) * G, dims[0]], c.q[i, 0, h * G:(h + 1) * G, dims[1]] = a[i, 0, h * G:(h + 1) * G].float(), b[i, 0, h * G:(h + 1) * G].float()
+            c.k[i, h, keys, dims] = 0x38
+            c.v[i, h, keys[0], :64], c.v[i, h, keys[1], 64:] = 0x38, 0x38
+    c.scale, c.bound = 1.0, (8 * 186 + 6 + 40) * 2.0 ** -24
+    return c
+
+
+PINNED = [(pinned_weights, a) for a in ((1, 1, 4, 1), (40, 1, 4, 2), (301, 1, 1, 3), (301, 5, 7, 4), (1000, 1, 16, 5), (5003, 2, 8, 6))] + [
+    (pinned_scores, a) for a in ((2, 4, 1), (33, 1, 2), (64, 16, 3), (300, 20, 4), (1000, 4, 5), (5003, 8, 6))]
+
+
+@pytest.mark.parametrize("make,a", PINNED)
+def test_attention_f32_holds_24_bits(make, a):
+    """q and the weights in all of fp32's bits: with 16 of them, or 8, the bound is missed (tests/test_fp8_precision_host.py)."""
+    ops, c = _ops(), make(*a)
+    bs, H, n, _ = c.k.shape
+    T, G, cap = c.q.shape[1], c.q.shape[2] // H, c.k_scale.shape[2] * 16
+    k, v = (torch.cat([t, t.new_full((bs, H, cap - n, D), 0x7f)], 2).to(DEV) for t in (c.k, c.v))
+    cache = ops.Fp8KVCache.from_codes(k, c.k_scale.to(DEV), v, c.v_scale.to(DEV), block=16)
+    out = ops.Fp8Attention(bs, H, G, T, n, DEV).run(c.q.to(DEV), cache, [(0, n)], scale=c.scale)
+    assert c.holds(out), float(((out.cpu().to(F64) - c.result()).abs() / c.result().abs().clamp(min=1e-18)).max() * 2.0 ** 24)
+
+
 # ------------------------------------------------------------------ norms
 
 
