@@ -43,7 +43,7 @@ class QwenConfig:
 class QwenLayer:
     """Weights of one decoder layer (reference ``QwenLayer``, qwen.py:14-70), random-initialised."""
 
-    def __init__(self, cfg: QwenConfig, device, dtype, gen: torch.Generator, pack=None, gate_apart: bool = False):
+    def __init__(self, cfg: QwenConfig, device, dtype, gen: torch.Generator, pack=None):
         h, q, kv, inter = cfg.hidden_size, cfg.num_heads * cfg.head_dim, cfg.num_key_value_heads * cfg.head_dim, cfg.intermediate_size
 
         def w(rows, cols):  # ~ N(0, 1/cols): activations keep unit scale through the layer
@@ -54,7 +54,7 @@ class QwenLayer:
         self.bqkv = None
         self.wo = pack(w(h, q))
         gate_up = w(2 * inter, h)
-        if gate_apart:  # two matrices to one call
+        if isinstance(self.wo, ops.W4Weight):  # two matrices to one call
             self.gate_up_proj, self.gate_proj, self.up_proj = None, pack(gate_up[:inter]), pack(gate_up[inter:])
         else:
             self.gate_up_proj = pack(gate_up)
@@ -88,7 +88,7 @@ class QwenModel:
         gen = torch.Generator(device=self.device).manual_seed(seed)
         pack = ops.Fp8Weight.quantize if fp8 else (lambda weight: ops.W4Weight.quantize(weight, weight_group)) if weight_bits == 4 else None
         self.fp8 = fp8
-        self.layers = [QwenLayer(cfg, self.device, dtype, gen, pack, gate_apart=weight_bits == 4) for _ in range(cfg.num_layers)]
+        self.layers = [QwenLayer(cfg, self.device, dtype, gen, pack) for _ in range(cfg.num_layers)]
         self.embed_tokens = (torch.randn(cfg.vocab_size, cfg.hidden_size, generator=gen, device=self.device,
                                          dtype=torch.float32)).to(dtype)
         self.lm_head = (torch.randn(cfg.vocab_size, cfg.hidden_size, generator=gen, device=self.device, dtype=torch.float32)

@@ -338,3 +338,17 @@ def test_product_plan():
     assert weight.plan(3) == (16, 16, 1, 1)
     with pytest.raises(RuntimeError):
         weight.plan(0)
+
+
+def test_layer_takes_any_packing():
+    """A layer whose weights are packed to 4 bits has the two matrices that the gated product takes; any other packing goes to both as one."""
+    from pariskv_amd.model_hub.qwen import QwenConfig, QwenLayer
+
+    cfg = QwenConfig(hidden_size=16, num_layers=1, num_heads=2, num_key_value_heads=1, intermediate_size=8, vocab_size=5)
+    layer = lambda pack: QwenLayer(cfg, "cpu", F32, torch.Generator().manual_seed(1), pack)
+    four = layer(lambda w: ops.W4Weight.__new__(ops.W4Weight))
+    assert four.gate_up_proj is None and isinstance(four.gate_proj, ops.W4Weight) and isinstance(four.up_proj, ops.W4Weight)
+    shapes = []
+    eight = layer(lambda w: shapes.append(tuple(w.shape)) or ops.Fp8Weight.__new__(ops.Fp8Weight))
+    assert isinstance(eight.gate_up_proj, ops.Fp8Weight) and (16, 16) in shapes and not hasattr(eight, "gate_proj")
+    assert tuple(layer(None).gate_up_proj.shape) == (16, 16)
