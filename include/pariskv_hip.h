@@ -604,7 +604,7 @@ int pkv_w4_silu_mul(const void *x, int64_t x_stride, int64_t rows, const void *g
 /* Values in eight bits, no counterpart in the reference (bf16 caches, activations and weights): e4m3 codes (OCP: sign, 4 exponent bits, 3
  * mantissa bits; largest 448) times a scale 2^e that a group of values shares, e the least whole number from -100 on with
  * |x| <= 448 2^e for every finite x of the group.  A code is the nearest one to x / 2^e (ties to even), of an infinity 448 with its sign, of a NaN
- * the NaN 0x7f.  Values of at most 10^38.
+ * a NaN (0x7f or 0xff).  Values of at most 10^38.
  *
  * A K/V cache in that form: k, v uint8 [bs][n_kv_heads][capacity][128], 16-byte aligned; k_scale, v_scale fp32
  * [bs][n_kv_heads][capacity / block], one for the rows block*i .. block*(i+1)-1 of a head; block 16, 32, 64 or 128, capacity a multiple of it and at
@@ -631,7 +631,7 @@ int pkv_fp8_store(const pkv_fp8_kv *cache, const void *k, const void *v, int dty
 
 /* Rows of a cache in eight bits as values of `dtype` (no counterpart in the reference; pkv_gather_hbm and pkv_gather_uva for such a cache, whose codes may lie
  * in mapped host memory): out[b][h][i] = row row0 + i, or row row0 + idx[(b*n_kv_heads + h)*idx_stride + i] where idx is
- * not NULL (a row that is not there: zeros), i < n_rows.  Output strides in elements, 16-byte multiples; rows contiguous. */
+ * not NULL (one below 0, or of a row past the capacity: zeros), i < n_rows.  Output strides in elements, 16-byte multiples; rows contiguous. */
 int pkv_fp8_read(const pkv_fp8_kv *cache, int64_t row0, int64_t n_rows, const int64_t *idx, int64_t idx_stride, int dtype, void *out_k,
                  void *out_v, int64_t ok_stride_b, int64_t ok_stride_h, int64_t ok_stride_row, int64_t ov_stride_b, int64_t ov_stride_h,
                  int64_t ov_stride_row, void *stream);
@@ -642,7 +642,8 @@ int pkv_fp8_read(const pkv_fp8_kv *cache, int64_t row0, int64_t n_rows, const in
  * L = min(row_keys[b*n_kv_heads + h], all) (NULL: all; none where it is <= 0).  Token t sees the keys j < L - (n_tokens - 1 - t): the
  * last key is the last token's own.
  *   out[b][t][hq] = sum_j softmax_j(scale q[b][t][hq] . k_j) v_j
- * A token that sees nothing gets zeros; what a token does not see does not touch it, NaN included.
+ * A token that sees nothing, or whose scores are all -infinity, gets zeros; what a token does not see does not touch it, NaN included.
+ * Products of q with codes are summed up before the scales come in: q of at most 10^33.
  * q [bs][n_tokens][n_kv_heads*group][128], heads side by side, of `dtype` (strides in elements, 16-byte multiples); out the same,
  * contiguous.  1 <= n_tokens <= 1024, n_tokens * group <= 8192, at most PKV_FP8_MAX_ROWS keys.  fp32 sums and statistics; bf16: weights are
  * rounded to bf16 for the product with V, and the normaliser is the sum of the rounded ones; fp32: no rounding but that of fp32.

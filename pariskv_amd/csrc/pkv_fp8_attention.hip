@@ -289,9 +289,10 @@ typedef const __attribute__((address_space(1))) void *global_at;
 typedef __attribute__((address_space(3))) void *lds_at;
 
 // A wave takes steps of 64 keys, dealt round the waves of all splits.  Rows go straight from memory to LDS, half a step at a time into a part of the
-// wave's own: a half is asked for as soon as the one before in its place has been used, and no registers wait for it.  4 x 8 heads x 65536 keys (541 MB): 106 us
-// with the join, of them 101 without any arithmetic and 51 without the loads (a plain read of as many bytes takes 77); rows kept by the caches 120;
-// straight to registers, half a step ahead, 115 to 125.  More than 16 query rows: two tiles of them a wave, which share the codes' conversion: 1 x 8 x 32768
+// wave's own: a half is asked for as soon as the one before in its place has been used, and no registers wait for it.  But the scales of the next step are multiplied with
+// scale log2 e where they are loaded, in front of the first half's products, and loads come back in order: a wave waits for both halves there, and has nothing under way while it
+// multiplies the first.  4 x 8 heads x 65536 keys (541 MB): 85 to 101 us and 4.6 the join; of 106 in all, 101 without any arithmetic and 51 without the loads (a plain read of
+// as many bytes takes 77); rows kept by the caches 120; straight to registers, half a step ahead, 115 to 125.  More than 16 query rows: two tiles of them a wave, which share the codes' conversion: 1 x 8 x 32768
 // keys, 256 rows 65 us, one tile 105.  Where several workgroups read a key, for their tiles of rows, the caches keep it: 65 and 74 us.
 template <bool BF16, int NT, bool INDEXED>
 __global__ __launch_bounds__(kWaves * PKV_WAVE, 2) void pkv_fp8_attention_kernel(Call a) {

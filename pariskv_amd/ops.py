@@ -1268,7 +1268,7 @@ class Fp8KVCache:
 
     def read(self, row0: int = 0, n: Optional[int] = None, idx: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16, out=None):
         """Rows as values: (K, V) [bs,Hkv,n,128] in ``dtype`` (bf16 or fp32).  Rows row0 .. row0+n-1 (n None: to the end), or rows
-        row0 + idx[b,h,:n] with idx int64 [bs,Hkv,>=n] on the GPU (n None: all of it; a row that is not there: zeros).  ``out``: two tensors of that
+        row0 + idx[b,h,:n] with idx int64 [bs,Hkv,>=n] on the GPU (n None: all of it; below 0, or past the cache: zeros).  ``out``: two tensors of that
         shape and type with contiguous rows to write to, for instance the rows behind a dense prefix."""
         bs, H, code = self.bs, self.n_kv_heads, _dt(dtype)
         idx_at, idx_stride = None, 0
