@@ -1232,7 +1232,7 @@ class Fp8KVCache:
         self._at = k_scale.get_device()
 
     def store(self, k: torch.Tensor, v: torch.Tensor, start=0, lengths: Optional[torch.Tensor] = None) -> None:
-        """Rows k, v [bs,S,Hkv,128] (bf16 or fp32, of at most 10^38; any strides) quantised into rows start .. of every sequence.  start: an integer, or
+        """Rows k, v [bs,S,Hkv,128] (S up to the capacity; bf16 or fp32, of at most 10^38; any strides) quantised into rows start .. of every sequence.  start: an integer, or
         int32 [bs] on the GPU (a sequence whose start is no row of the cache stores nothing, rows past the capacity are left out);
         lengths: int32 [bs] on the GPU, how many of its S rows a sequence has (None: all).  Rows that a block holds
         already, before the start, stay: its scale only grows, and their codes are rounded again when it does."""
@@ -1323,7 +1323,7 @@ class Fp8Attention:
         """queries [bs,T,Hq,128] (bf16 or fp32); segments: at most four (row0, n_rows) or (row0, n_rows, idx) of the cache, its keys in that order: rows
         row0 .. row0+n_rows-1, or rows row0 + idx[b,h,:n_rows] with idx int64 [bs,Hkv,>=n_rows] on the GPU (values outside the cache are clamped);
         row_keys int32 [bs,Hkv]: how many of these keys a row has (None: all; 0 or less: none).  The last key is the last token's
-        own: token t sees all but the last T-1-t.  Returns [bs,T,Hq,128]; a token that sees nothing gets zeros, and what a token does not see does not touch it."""
+        own: token t sees all but the last T-1-t.  Returns [bs,T,Hq,128]; a token that sees nothing gets zeros, and what a token does not see does not touch it.  Queries of at most 10^33."""
         bs, H, G = self.bs, self.H, self.G
         shape, dt, at = queries.shape, queries.dtype, queries.get_device()
         T = shape[1] if len(shape) == 4 else 0
